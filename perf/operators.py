@@ -200,9 +200,7 @@ def _token(state, t):
 def _plain(state):
     kind, dtype = state["kind"], state["dtype"]
     if kind == "quant":
-        x = state["x"]
-        # what is quantised is silu_and_mul's result in the input's type
-        return _quantised_values((_silu_and_mul(x).to(dtype) if state["silu"] else x).float()).to(dtype)
+        return _quantised_values(_silu_and_mul(state["x"]) if state["silu"] else state["x"].float()).to(dtype)
     if kind == "dequant":
         return _values(state["q"], state["s"]).to(dtype)
     if kind == "moe":
@@ -270,7 +268,6 @@ def exact(case, seed):
         if state["silu"]:
             half = x.shape[1] // 2
             x = x[:, :half] * torch.sigmoid(x[:, :half]) * x[:, half:]
-            x = x.to(state["dtype"]).double()
         return _exact_quantised(x)
     if kind == "dequant":
         return _exact_values(state["q"], state["s"])
