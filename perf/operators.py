@@ -245,7 +245,7 @@ def _exact_values(q, words):
     exponent, fraction = (c // 2) % 4, (c % 2).double()
     size = torch.where(exponent == 0, 0.5 * fraction, (1.0 + 0.5 * fraction) * 2.0 ** (exponent - 1).double())
     value = torch.where(c >= 8, -size, size)
-    byte = words.contiguous().view(torch.uint8)[..., : k // BLOCK].double()
+    byte = words.clone(memory_format=torch.contiguous_format).view(torch.uint8)[..., : k // BLOCK].double()
     return value * torch.repeat_interleave(2.0 ** (byte - 127.0), BLOCK, dim=-1)
 
 
