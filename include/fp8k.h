@@ -473,6 +473,59 @@ int fp8k_moe_fused_gate(const void* input, const void* bias, float* topk_weights
                         int64_t num_fused_shared_experts, double routed_scaling_factor,
                         int apply_routed_scaling_factor_on_output, int dtype, void* stream);
 
+/*
+ * MXFP4: 32 e2m1 values along K share one e8m0 scale 2^(byte - 127); byte 255 is NaN.  Codes: two to a byte, the even element in the
+ * low half, [rows, K/2].  Scales: int32 words of four bytes, blocks 4j .. 4j+3 of a row in word j (byte 0 first), ceil(K/128) words to
+ * a row at s[row * stride_row + word * stride_w] (strides in words; column-major with the rows padded to 4 is what the kernels read
+ * fastest and what fp8k_mxfp4_quant is handed by this package).  Bytes of a last word that no block has must not be 255.  K is a
+ * multiple of 32.  Rows of codes are 16-byte aligned.
+ *
+ * fp8k_mxfp4_quant: x [M, K] of in_dtype with row stride ldx elements (a multiple of 8) -> q [M, K/2] contiguous, s.  The scale's
+ * exponent is that of the block's largest magnitude rounded to one fraction bit, minus 2, at least -127; values are rounded to
+ * nearest, ties to the even code, and end at 6.  A block that holds an infinity or a NaN gets byte 255 and zero codes.
+ * fuse_silu_and_mul: x is [M, 2K], gate columns then up; silu(gate) * up is formed in float32 and quantised unrounded.
+ * Whole words are written, unused bytes zero; nothing behind row M.
+ */
+int fp8k_mxfp4_quant(const void* x, void* q, void* s, int64_t M, int64_t K, int64_t ldx, int64_t s_stride_m, int64_t s_stride_w,
+                     int in_dtype, int fuse_silu_and_mul, void* stream);
+
+/* Values of q [E, N, K/2], s -> out [E, N, K] contiguous of out_dtype: exact in float32, one rounding. */
+int fp8k_mxfp4_dequant(const void* q, const void* s, void* out, int64_t E, int64_t N, int64_t K, int64_t s_stride_e, int64_t s_stride_n,
+                       int64_t s_stride_w, int out_dtype, void* stream);
+
+/*
+ * C [M, N] = A . B^T (+ bias[n]): both operands MXFP4, scales applied by the matrix core, float32 sums, bias added in float32, one
+ * rounding to out_dtype (F16/BF16).  lda, ldb in bytes (multiples of 16), ldc in elements (a multiple of 4), N % 8 == 0.
+ * bias: NULL or [N] of bias_dtype, which is out_dtype or F32.
+ */
+int fp8k_mxfp4_gemm(const void* A, const void* B, const void* As, const void* Bs, const void* bias, void* C, int64_t M, int64_t N,
+                    int64_t K, int64_t lda, int64_t ldb, int64_t as_stride_m, int64_t as_stride_w, int64_t bs_stride_n,
+                    int64_t bs_stride_w, int64_t ldc, int out_dtype, int bias_dtype, void* stream);
+
+/*
+ * A whole linear on 16-bit activations x [M, K] (row stride ldx elements): fp8k_mxfp4_quant, then fp8k_mxfp4_gemm, whose results these
+ * are bit for bit.  Workspace: 256-byte aligned, fp8k_mxfp4_linear_workspace_bytes of it (0 possible), not initialised.
+ */
+int64_t fp8k_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int fp8k_mxfp4_linear(const void* x, const void* B, const void* Bs, const void* bias, void* C, int64_t M, int64_t N, int64_t K,
+                      int64_t ldx, int64_t ldb, int64_t bs_stride_n, int64_t bs_stride_w, int64_t ldc, int dtype, int bias_dtype,
+                      void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * A mixture-of-experts layer on MXFP4 weights for a few tokens (at most 128, and at most 1024 (token, choice) pairs), two launches.
+ * x [T, H] of dtype (F16/BF16), row stride ldx elements; w1 [E, 2I, H/2] (gate rows, then up rows), w2 [E, H, I/2], rows contiguous;
+ * topk_weights [T, topk], topk_ids [T, topk] int32 or int64; an id outside 0 .. E-1 contributes nothing.
+ *   h = round(act(x . gate^T) * (x . up^T));  out[t] = round(scaling * sum over k of weight[t, k] * h[t, k] . W2^T)
+ * with float32 sums; weight_on_input: the weight multiplies both products of the first stage instead.  activation: fp8k_activation_kind
+ * SILU or GELU.  out [T, H] contiguous may be x.  Workspace: 256-byte aligned, not initialised.
+ */
+int64_t fp8k_mxfp4_experts_workspace_bytes(int64_t T, int64_t topk, int64_t I);
+int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2, const void* s1, const void* s2, const float* topk_weights,
+                       const void* topk_ids, int ids_are_64bit, void* out, int64_t T, int64_t topk, int64_t E, int64_t H, int64_t I,
+                       int64_t ldx, int64_t w1_stride_e, int64_t w2_stride_e, int64_t s1_stride_e, int64_t s1_stride_n,
+                       int64_t s1_stride_w, int64_t s2_stride_e, int64_t s2_stride_n, int64_t s2_stride_w, int activation,
+                       int weight_on_input, float scaling, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -5,6 +5,7 @@ Modules:
   fp8_kernel  - ``sglang.srt.layers.quantization.fp8_kernel`` entry points
   fp8_utils   - ``sglang.srt.layers.quantization.fp8_utils`` entry points (linear apply)
   fused_moe   - block-FP8 fused-experts pipeline
+  mxfp4       - 4-bit (MXFP4) quantisation, products, linears, and an expert layer for a few tokens
 """
 import torch
 
@@ -20,4 +21,4 @@ def _check_host() -> None:
 
 _check_host()
 
-__all__ = ["sgl_kernel", "fp8_kernel", "fp8_utils", "fused_moe"]
+__all__ = ["sgl_kernel", "fp8_kernel", "fp8_utils", "fused_moe", "mxfp4"]

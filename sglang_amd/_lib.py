@@ -97,6 +97,15 @@ SIGNATURES = {
     "fp8k_activation": (_c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _c_ptr]),
     "fp8k_moe_sum_reduce": (_c_int, [_c_ptr, _c_ptr] + [_c_i64] * 6 + [_c_f32, _c_int, _c_ptr]),
     "fp8k_moe_sum": (_c_int, [_c_ptr, _c_ptr] + [_c_i64] * 6 + [_c_int, _c_ptr]),
+    "fp8k_mxfp4_quant": (_c_int, [_c_ptr] * 3 + [_c_i64] * 5 + [_c_int, _c_int, _c_ptr]),
+    "fp8k_mxfp4_dequant": (_c_int, [_c_ptr] * 3 + [_c_i64] * 6 + [_c_int, _c_ptr]),
+    "fp8k_mxfp4_gemm": (_c_int, [_c_ptr] * 6 + [_c_i64] * 10 + [_c_int, _c_int, _c_ptr]),
+    "fp8k_mxfp4_linear_workspace_bytes": (_c_i64, [_c_i64] * 3),
+    "fp8k_mxfp4_linear": (_c_int, [_c_ptr] * 5 + [_c_i64] * 8 + [_c_int, _c_int, _c_ptr, _c_i64, _c_ptr]),
+    "fp8k_mxfp4_experts_workspace_bytes": (_c_i64, [_c_i64] * 3),
+    "fp8k_mxfp4_experts": (
+        _c_int, [_c_ptr] * 7 + [_c_int, _c_ptr] + [_c_i64] * 14 + [_c_int, _c_int, _c_f32, _c_int, _c_ptr, _c_i64, _c_ptr],
+    ),
     "fp8k_moe_fused_gate": (
         _c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr] + [_c_i64] * 6 + [ctypes.c_double, _c_int, _c_int, _c_ptr],
     ),

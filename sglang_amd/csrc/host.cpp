@@ -632,6 +632,171 @@ PyObject* fused_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------------------------- MXFP4
+// codes uint8 [.., rows, K/2] with contiguous, 16-byte aligned rows, and their int32 scale words [.., rows, ceil(K/128)]
+bool mx_operand(const Tensor& q, const Tensor& s, int64_t dim, int device) {
+  if (!plain(q, device) || !plain(s, device) || q.scalar_type() != ScalarType::Byte || s.scalar_type() != ScalarType::Int) return false;
+  if (q.dim() != dim || s.dim() != dim || q.numel() == 0 || q.stride(-1) != 1 || q.size(-1) % 16 != 0 || !non_negative_strides(s)) return false;
+  if ((uintptr_t)q.data_ptr() % 16 != 0 || s.size(-1) != ceil_div(q.size(-1), 64)) return false;
+  for (int64_t d = 0; d + 1 < dim; ++d)
+    if (s.size(d) != q.size(d) || q.stride(d) % 16 != 0 || q.stride(d) < 0) return false;
+  return true;
+}
+
+// rows of 16-bit or 32-bit activations that the kernels read as they lie in memory
+bool mx_rows(const Tensor& x) {
+  return x.dim() == 2 && x.numel() > 0 && x.stride(1) == 1 && (uintptr_t)x.data_ptr() % 16 == 0 &&
+         (x.size(0) == 1 || (x.stride(0) >= x.size(1) && x.stride(0) % 8 == 0));
+}
+int64_t row_stride(const Tensor& x) { return x.size(0) > 1 ? x.stride(0) : x.size(1); }
+
+bool mx_bias(const Tensor& bias, int64_t N, ScalarType dt, int device) {
+  return plain(bias, device) && bias.numel() == N && bias.is_contiguous() && (bias.scalar_type() == dt || bias.scalar_type() == ScalarType::Float);
+}
+
+// mx_quant(x, fuse_silu_and_mul) -> (codes, scales) or None
+PyObject* mx_quant(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor x;
+  if (n != 2 || modes_active() || !tensor_arg(a[0], x) || !x.is_cuda() || !plain(x, x.get_device())) DECLINE;
+  const bool fuse = truth(a[1]);
+  const ScalarType dt = x.scalar_type();
+  if (!(is_half(dt) || dt == ScalarType::Float) || !mx_rows(x)) DECLINE;
+  const int64_t M = x.size(0), width = x.size(1), K = fuse ? width / 2 : width;
+  if (K == 0 || K % 32 != 0 || (fuse && width % 2 != 0)) DECLINE;
+  Tensor q, s;
+  {
+    Call c(x);
+    OBSERVED("mx_quant", x);
+    const int64_t ld = ceil_to(M, 4);
+    q = empty({M, K / 2}, ScalarType::Byte, x.device());
+    s = empty_column_major(M, ceil_div(K, 128), ld, ScalarType::Int, x.device());
+    check(fp8k_mxfp4_quant(x.data_ptr(), q.data_ptr(), s.data_ptr(), M, K, row_stride(x), 1, ld, code(dt), fuse ? 1 : 0, c.stream));
+  }
+  PyObject* out = PyTuple_New(2);
+  if (!out) return nullptr;
+  PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(q)));
+  PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(s)));
+  return out;
+  END_HANDLE_TH_ERRORS
+}
+
+// mx_dequant(q, s, dtype) -> values or None
+PyObject* mx_dequant(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, s;
+  if (n != 3 || modes_active() || !tensor_arg(a[0], q) || !tensor_arg(a[1], s) || !THPDtype_Check(a[2]) || !q.is_cuda()) DECLINE;
+  const ScalarType dt = reinterpret_cast<THPDtype*>(a[2])->scalar_type;
+  if (!(is_half(dt) || dt == ScalarType::Float) || (q.dim() != 2 && q.dim() != 3)) DECLINE;
+  if (!mx_operand(q, s, q.dim(), q.get_device()) || !q.is_contiguous()) DECLINE;
+  const int64_t E = q.dim() == 3 ? q.size(0) : 1, N = q.size(-2), K = q.size(-1) * 2;
+  Tensor out;
+  {
+    Call c(q);
+    OBSERVED("mx_dequant", q, s);
+    c10::SmallVector<int64_t, 5> shape(q.sizes().begin(), q.sizes().end());
+    shape.back() = K;
+    out = empty(shape, dt, q.device());
+    check(fp8k_mxfp4_dequant(q.data_ptr(), s.data_ptr(), out.data_ptr(), E, N, K, q.dim() == 3 ? s.stride(0) : 0, s.stride(-2), s.stride(-1),
+                             code(dt), c.stream));
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// mx_matmul(A, B, As, Bs, out_dtype, bias) -> C or None
+PyObject* mx_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor x, w, xs, ws, bias;
+  if (n != 6 || modes_active() || !tensor_arg(a[0], x) || !tensor_arg(a[1], w) || !tensor_arg(a[2], xs) || !tensor_arg(a[3], ws)) DECLINE;
+  if (!THPDtype_Check(a[4]) || !x.is_cuda()) DECLINE;
+  const int dev = x.get_device();
+  const ScalarType dt = reinterpret_cast<THPDtype*>(a[4])->scalar_type;
+  if (!is_half(dt) || !mx_operand(x, xs, 2, dev) || !mx_operand(w, ws, 2, dev) || x.size(1) != w.size(1) || w.size(0) % 8 != 0) DECLINE;
+  const int64_t M = x.size(0), N = w.size(0), K = x.size(1) * 2;
+  if (a[5] != Py_None && (!tensor_arg(a[5], bias) || !mx_bias(bias, N, dt, dev))) DECLINE;
+  Tensor out;
+  {
+    Call c(x);
+    OBSERVED("mx_matmul", x, w, xs, ws, bias);
+    out = empty({M, N}, dt, x.device());
+    check(fp8k_mxfp4_gemm(x.data_ptr(), w.data_ptr(), xs.data_ptr(), ws.data_ptr(), bias.defined() ? bias.data_ptr() : nullptr, out.data_ptr(),
+                          M, N, K, row_stride(x), row_stride(w), xs.stride(0), xs.stride(1), ws.stride(0), ws.stride(1), N, code(dt),
+                          bias.defined() ? code(bias.scalar_type()) : FP8K_F32, c.stream));
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// mx_linear(x, weight, weight_scale, bias) -> output or None: quantisation, product, bias
+PyObject* mx_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor x, w, ws, bias;
+  if (n != 4 || modes_active() || !tensor_arg(a[0], x) || !tensor_arg(a[1], w) || !tensor_arg(a[2], ws) || !x.is_cuda()) DECLINE;
+  const int dev = x.get_device();
+  const ScalarType dt = x.scalar_type();
+  if (!plain(x, dev) || !is_half(dt) || x.dim() < 1 || x.numel() == 0) DECLINE;
+  if (!(x.is_contiguous() || x.dim() == 2) || (x.dim() == 2 ? !mx_rows(x) : (uintptr_t)x.data_ptr() % 16 != 0)) DECLINE;
+  if (!mx_operand(w, ws, 2, dev) || w.size(1) * 2 != x.size(-1) || w.size(0) % 8 != 0) DECLINE;
+  const int64_t K = x.size(-1), M = x.numel() / K, N = w.size(0);
+  if (a[3] != Py_None && (!tensor_arg(a[3], bias) || !mx_bias(bias, N, dt, dev))) DECLINE;
+  Tensor out;
+  {
+    Call c(x);
+    OBSERVED("mx_linear", x, w, ws, bias);
+    c10::SmallVector<int64_t, 5> shape(x.sizes().begin(), x.sizes().end());
+    shape.back() = N;
+    out = empty(shape, dt, x.device());
+    const int64_t wsb = fp8k_mxfp4_linear_workspace_bytes(M, N, K);
+    Scratch mem(wsb, c.stream);
+    check(fp8k_mxfp4_linear(x.data_ptr(), w.data_ptr(), ws.data_ptr(), bias.defined() ? bias.data_ptr() : nullptr, out.data_ptr(), M, N, K,
+                            x.dim() == 2 ? row_stride(x) : K, row_stride(w), ws.stride(0), ws.stride(1), N, code(dt),
+                            bias.defined() ? code(bias.scalar_type()) : FP8K_F32, wsb ? mem.take(wsb) : nullptr, wsb, c.stream));
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// mx_experts(x, w1, w2, topk_weights, topk_ids, s1, s2, gelu, weight_on_input, scaling, inplace) -> output or None
+PyObject* mx_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor x, w1, w2, tw, ids, s1, s2;
+  if (n != 11 || modes_active() || !tensor_arg(a[0], x) || !tensor_arg(a[1], w1) || !tensor_arg(a[2], w2) || !tensor_arg(a[3], tw) ||
+      !tensor_arg(a[4], ids) || !tensor_arg(a[5], s1) || !tensor_arg(a[6], s2) || !x.is_cuda() || !PyFloat_Check(a[9]))
+    DECLINE;
+  const bool gelu = truth(a[7]), on_input = truth(a[8]), inplace = truth(a[10]);
+  const int dev = x.get_device();
+  const ScalarType dt = x.scalar_type();
+  if (!plain(x, dev) || !is_half(dt) || !mx_rows(x) || (inplace && !x.is_contiguous())) DECLINE;
+  if (!mx_operand(w1, s1, 3, dev) || !mx_operand(w2, s2, 3, dev) || !w1.is_contiguous() || !w2.is_contiguous()) DECLINE;
+  const int64_t T = x.size(0), H = x.size(1), E = w1.size(0), I = w1.size(1) / 2;
+  if (w1.size(2) * 2 != H || w1.size(1) % 2 != 0 || w2.size(0) != E || w2.size(1) != H || w2.size(2) * 2 != I) DECLINE;
+  if (!plain(tw, dev) || !plain(ids, dev) || tw.dim() != 2 || ids.dim() != 2 || tw.sizes() != ids.sizes() || ids.size(0) != T) DECLINE;
+  if (tw.scalar_type() != ScalarType::Float || !tw.is_contiguous() || !ids.is_contiguous()) DECLINE;
+  const bool ids64 = ids.scalar_type() == ScalarType::Long;
+  if ((!ids64 && ids.scalar_type() != ScalarType::Int) || ids.size(1) == 0) DECLINE;
+  const int64_t topk = ids.size(1);
+  const float scaling = (float)PyFloat_AS_DOUBLE(a[9]);
+  Tensor out;
+  {
+    Call c(x);
+    OBSERVED("mx_experts", x, w1, w2, tw, ids, s1, s2);
+    out = inplace ? x : empty({T, H}, dt, x.device());
+    const int64_t wsb = fp8k_mxfp4_experts_workspace_bytes(T, topk, I);
+    Scratch mem(wsb, c.stream);
+    check(fp8k_mxfp4_experts(x.data_ptr(), w1.data_ptr(), w2.data_ptr(), s1.data_ptr(), s2.data_ptr(), tw.data_ptr<float>(), ids.data_ptr(), ids64,
+                             out.data_ptr(), T, topk, E, H, I, row_stride(x), w1.stride(0), w2.stride(0), s1.stride(0), s1.stride(1), s1.stride(2),
+                             s2.stride(0), s2.stride(1), s2.stride(2), gelu ? FP8K_ACT_GELU : FP8K_ACT_SILU, on_input, scaling, code(dt),
+                             mem.take(wsb), wsb, c.stream));
+  }
+  if (inplace) {
+    Py_INCREF(a[0]);
+    return a[0];
+  }
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 // set_workspace(registry, grow): the per-stream GEMM workspaces of sgl_kernel
 PyObject* set_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 2 || !PyDict_Check(a[0]) || !PyCallable_Check(a[1])) {
@@ -647,7 +812,8 @@ PyObject* set_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 #define FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FN(group_quant), FN(block_linear), FN(block_matmul), FN(token_linear), FN(mla_quant),     FN(bmm),
-                         FN(fused_gate),  FN(fused_experts), FN(set_workspace), {nullptr, nullptr, 0, nullptr}};
+                         FN(fused_gate),  FN(fused_experts), FN(mx_quant),     FN(mx_dequant),   FN(mx_matmul),
+                         FN(mx_linear),   FN(mx_experts),    FN(set_workspace), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "native calls of the layer-level entry points", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 

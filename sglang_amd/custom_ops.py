@@ -170,6 +170,16 @@ _register(
     "-> (Tensor, Tensor)", _k.moe_fused_gate, _gate_fake,
 )
 
+# ---- MXFP4 (sgl_kernel.py, mxfp4.py)
+_register("mxfp4_quant(Tensor input, Tensor(a!) output_q, Tensor(b!) output_s, bool fuse_silu_and_mul=False) -> ()", _k.mxfp4_quant, _none)
+_register("mxfp4_dequant(Tensor q, Tensor s, Tensor(a!) out) -> ()", _k.mxfp4_dequant, _none)
+_register("mxfp4_scaled_mm(Tensor mat_a, Tensor mat_b, Tensor scales_a, Tensor scales_b, ScalarType out_dtype, Tensor? bias=None) -> Tensor",
+          _k.mxfp4_scaled_mm,
+          lambda mat_a, mat_b, scales_a, scales_b, out_dtype, bias=None: mat_a.new_empty((mat_a.shape[0], mat_b.shape[0]), dtype=out_dtype))
+_register("mxfp4_experts(Tensor hidden_states, Tensor w1, Tensor w2, Tensor topk_weights, Tensor topk_ids, Tensor w1_scale, "
+          "Tensor w2_scale, Tensor(a!) out, str activation, bool apply_router_weight_on_input, float routed_scaling_factor) -> ()",
+          _k.mxfp4_experts, _none)
+
 _ops = torch.ops.fp8k
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -307,3 +317,21 @@ def moe_fused_gate(input_tensor, bias, num_expert_group, topk_group, topk, num_f
                    routed_scaling_factor=0.0, apply_routed_scaling_factor_on_output=False) -> Tuple[torch.Tensor, torch.Tensor]:
     return _ops.moe_fused_gate(input_tensor, bias, num_expert_group, topk_group, topk, num_fused_shared_experts,
                                float(routed_scaling_factor), apply_routed_scaling_factor_on_output)
+
+
+def mxfp4_quant(input, output_q, output_s, fuse_silu_and_mul: bool = False) -> None:
+    _ops.mxfp4_quant(input, output_q, output_s, fuse_silu_and_mul)
+
+
+def mxfp4_dequant(q, s, out) -> None:
+    _ops.mxfp4_dequant(q, s, out)
+
+
+def mxfp4_scaled_mm(mat_a, mat_b, scales_a, scales_b, out_dtype, bias=None) -> torch.Tensor:
+    return _ops.mxfp4_scaled_mm(mat_a, mat_b, scales_a, scales_b, out_dtype, bias)
+
+
+def mxfp4_experts(hidden_states, w1, w2, topk_weights, topk_ids, w1_scale, w2_scale, out, activation="silu",
+                  apply_router_weight_on_input=False, routed_scaling_factor=1.0) -> None:
+    _ops.mxfp4_experts(hidden_states, w1, w2, topk_weights, topk_ids, w1_scale, w2_scale, out, activation,
+                       apply_router_weight_on_input, float(routed_scaling_factor))

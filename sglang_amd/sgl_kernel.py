@@ -979,3 +979,163 @@ def moe_fused_gate(
         )
     )
     return output, indices
+
+
+# --------------------------------------------------------------------------------------------
+# MXFP4: 4-bit operands with one e8m0 scale per 32 values
+# --------------------------------------------------------------------------------------------
+# Codes are uint8 [.., rows, K/2] (element 2i in the low half of byte i), scales int32 words [.., rows, ceil(K/128)] of four e8m0 bytes
+# (include/fp8k.h).  mxfp4.py makes and takes apart these layouts and holds the layer-level calls.
+
+
+def _mx_codes(t: torch.Tensor, what: str, dim: int = 2) -> None:
+    if t.dtype != torch.uint8 or t.dim() != dim:
+        raise RuntimeError("%s must be a %d-D uint8 tensor of packed codes" % (what, dim))
+    if t.shape[-1] % 16 != 0 or t.shape[-1] == 0:
+        raise RuntimeError("%s: K must be a positive multiple of 32" % what)
+    if t.stride(-1) != 1:
+        raise RuntimeError("%s must have contiguous rows" % what)
+
+
+def _mx_scales(s: torch.Tensor, codes: torch.Tensor, what: str) -> None:
+    words = (codes.shape[-1] * 2 + 127) // 128
+    if s.dtype != torch.int32 or tuple(s.shape) != tuple(codes.shape[:-1]) + (words,):
+        raise RuntimeError("%s must be int32 words of e8m0 scales, %s" % (what, tuple(codes.shape[:-1]) + (words,)))
+    if any(st < 0 for st in s.stride()):
+        raise RuntimeError("%s must have non-negative strides" % what)
+
+
+def _same_device(*tensors: Optional[torch.Tensor]) -> None:
+    require_cuda(*tensors)
+    if len({t.device for t in tensors if t is not None}) > 1:
+        raise RuntimeError("fp8k: tensors must live on one device")
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return t.data_ptr() if t is not None else None
+
+
+def mxfp4_quant(input: torch.Tensor, output_q: torch.Tensor, output_s: torch.Tensor, fuse_silu_and_mul: bool = False) -> None:
+    """input [M, K] float32 / float16 / bfloat16 with contiguous rows ([M, 2K] with fuse_silu_and_mul) -> output_q uint8 [M, K/2]
+    contiguous, output_s int32 [M, ceil(K/128)] in any strides.  Words are written whole, rows behind the last one stay as they are."""
+    _same_device(input, output_q, output_s)
+    if input.dim() != 2 or (input.shape[1] > 1 and input.stride(1) != 1):
+        raise RuntimeError("input must be 2-D with contiguous rows")
+    width = input.shape[1]
+    if fuse_silu_and_mul and width % 2 != 0:
+        raise RuntimeError("fuse_silu_and_mul needs an even last dimension")
+    M, K = input.shape[0], width // 2 if fuse_silu_and_mul else width
+    if K % 32 != 0 or K == 0:
+        raise RuntimeError("the last dimension must be a positive multiple of 32, got %d" % K)
+    _mx_codes(output_q, "output_q")
+    if tuple(output_q.shape) != (M, K // 2) or not output_q.is_contiguous():
+        raise RuntimeError("output_q must be contiguous uint8 [M, K/2]")
+    _mx_scales(output_s, output_q, "output_s")
+    if M == 0:
+        return
+    with torch.cuda.device(input.device):
+        check(lib.fp8k_mxfp4_quant(input.data_ptr(), output_q.data_ptr(), output_s.data_ptr(), M, K, input.stride(0) if M > 1 else width,
+                                   output_s.stride(0) if M > 1 else 1, output_s.stride(1) if output_s.shape[1] > 1 else 4,
+                                   dtype_code(input.dtype), 1 if fuse_silu_and_mul else 0, stream_ptr(input.device)))
+
+
+def mxfp4_dequant(q: torch.Tensor, s: torch.Tensor, out: torch.Tensor) -> None:
+    """Values of codes q uint8 [N, K/2] or [E, N, K/2] (contiguous) and their scale words into out [.., K] (contiguous)."""
+    _same_device(q, s, out)
+    if q.dim() not in (2, 3):
+        raise RuntimeError("q must be 2-D or 3-D")
+    _mx_codes(q, "q", q.dim())
+    _mx_scales(s, q, "s")
+    if tuple(out.shape) != tuple(q.shape[:-1]) + (q.shape[-1] * 2,) or not out.is_contiguous() or not q.is_contiguous():
+        raise RuntimeError("q and out must be contiguous, out [.., K]")
+    E, N = (q.shape[0], q.shape[1]) if q.dim() == 3 else (1, q.shape[0])
+    code = dtype_code(out.dtype)
+    if E * N == 0:
+        return
+    with torch.cuda.device(q.device):
+        check(lib.fp8k_mxfp4_dequant(q.data_ptr(), s.data_ptr(), out.data_ptr(), E, N, q.shape[-1] * 2, s.stride(0) if q.dim() == 3 else 0,
+                                     s.stride(-2), s.stride(-1), code, stream_ptr(q.device)))
+
+
+def mxfp4_scaled_mm(mat_a: torch.Tensor, mat_b: torch.Tensor, scales_a: torch.Tensor, scales_b: torch.Tensor, out_dtype: torch.dtype,
+                    bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """mat_a [M, K/2], mat_b [N, K/2] codes with contiguous, 16-byte aligned rows -> [M, N] = A . B^T (+ bias in float32, then one
+    rounding to out_dtype)."""
+    _same_device(mat_a, mat_b, scales_a, scales_b, bias)
+    _mx_codes(mat_a, "mat_a")
+    _mx_codes(mat_b, "mat_b")
+    if mat_a.shape[1] != mat_b.shape[1]:
+        raise RuntimeError("mat_a and mat_b shapes cannot be multiplied")
+    _mx_scales(scales_a, mat_a, "scales_a")
+    _mx_scales(scales_b, mat_b, "scales_b")
+    out_code = _out_code(out_dtype)
+    M, N, K = mat_a.shape[0], mat_b.shape[0], mat_a.shape[1] * 2
+    if N % 8 != 0 or N == 0:
+        raise RuntimeError("out must be multiple of 16 bytes for memory alignment")
+    bias_code = out_code
+    if bias is not None:
+        if bias.numel() != N or not bias.is_contiguous():
+            raise RuntimeError("bias must be contiguous with one value per column")
+        if bias.dtype not in (out_dtype, torch.float32):
+            raise RuntimeError("bias must have the result's type or be float32")
+        bias_code = dtype_code(bias.dtype)
+    out = torch.empty((M, N), dtype=out_dtype, device=mat_a.device)
+    if M == 0:
+        return out
+    with torch.cuda.device(mat_a.device):
+        check(lib.fp8k_mxfp4_gemm(mat_a.data_ptr(), mat_b.data_ptr(), scales_a.data_ptr(), scales_b.data_ptr(), _ptr(bias), out.data_ptr(),
+                                  M, N, K, mat_a.stride(0) if M > 1 else K // 2, mat_b.stride(0), scales_a.stride(0), scales_a.stride(1),
+                                  scales_b.stride(0), scales_b.stride(1), N, out_code, bias_code, stream_ptr(mat_a.device)))
+    return out
+
+
+MXFP4_EXPERTS_MAX_TOKENS = 128   # of a call of mxfp4_experts
+MXFP4_EXPERTS_MAX_SLOTS = 1024   # (token, choice) pairs
+
+
+def mxfp4_experts(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, topk_weights: torch.Tensor, topk_ids: torch.Tensor,
+                  w1_scale: torch.Tensor, w2_scale: torch.Tensor, out: torch.Tensor, activation: str = "silu",
+                  apply_router_weight_on_input: bool = False, routed_scaling_factor: float = 1.0) -> None:
+    """The gated experts of a few tokens in two launches (include/fp8k.h: fp8k_mxfp4_experts).  out may be hidden_states."""
+    _same_device(hidden_states, w1, w2, topk_weights, topk_ids, w1_scale, w2_scale, out)
+    if activation not in ("silu", "gelu"):
+        raise ValueError("Unsupported activation: %r" % (activation,))
+    if hidden_states.dim() != 2 or hidden_states.stride(1) != 1 or hidden_states.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError("hidden_states must be 2-D float16 or bfloat16 with contiguous rows")
+    _mx_codes(w1, "w1", 3)
+    _mx_codes(w2, "w2", 3)
+    T, H = hidden_states.shape
+    E, two_i = w1.shape[0], w1.shape[1]
+    if w1.shape[2] * 2 != H:
+        raise RuntimeError("Hidden size mismatch")
+    if two_i % 2 != 0 or E == 0 or tuple(w2.shape) != (E, H, two_i // 4):
+        raise RuntimeError("w1 [E, 2I, H/2] and w2 [E, H, I/2] do not belong together")
+    if not (w1.is_contiguous() and w2.is_contiguous()):
+        raise RuntimeError("expert weights must be contiguous")
+    _mx_scales(w1_scale, w1, "w1_scale")
+    _mx_scales(w2_scale, w2, "w2_scale")
+    if topk_ids.dim() != 2 or topk_weights.shape != topk_ids.shape or topk_ids.shape[0] != T or topk_ids.shape[1] == 0:
+        raise RuntimeError("topk shape mismatch")
+    if topk_weights.dtype != torch.float32 or topk_ids.dtype not in (torch.int32, torch.int64):
+        raise RuntimeError("topk_weights must be float32, topk_ids int32 or int64")
+    if not (topk_weights.is_contiguous() and topk_ids.is_contiguous()):
+        raise RuntimeError("topk_weights and topk_ids must be contiguous")
+    if tuple(out.shape) != (T, H) or out.dtype != hidden_states.dtype or not out.is_contiguous():
+        raise RuntimeError("out must be contiguous [tokens, hidden] of the activations' type")
+    topk = topk_ids.shape[1]
+    if T > MXFP4_EXPERTS_MAX_TOKENS or T * topk > MXFP4_EXPERTS_MAX_SLOTS:
+        raise RuntimeError("mxfp4_experts: built for at most %d tokens and %d (token, choice) pairs, got %d and %d"
+                           % (MXFP4_EXPERTS_MAX_TOKENS, MXFP4_EXPERTS_MAX_SLOTS, T, T * topk))
+    if T == 0:
+        return
+    I = two_i // 2
+    need = lib.fp8k_mxfp4_experts_workspace_bytes(T, topk, I)
+    with torch.cuda.device(hidden_states.device):
+        ws = torch.empty(need, dtype=torch.uint8, device=hidden_states.device)  # of the current stream: the allocator keeps it in order
+        check(lib.fp8k_mxfp4_experts(
+            hidden_states.data_ptr(), w1.data_ptr(), w2.data_ptr(), w1_scale.data_ptr(), w2_scale.data_ptr(), topk_weights.data_ptr(),
+            topk_ids.data_ptr(), 1 if topk_ids.dtype == torch.int64 else 0, out.data_ptr(), T, topk, E, H, I,
+            hidden_states.stride(0) if T > 1 else H, w1.stride(0), w2.stride(0), w1_scale.stride(0), w1_scale.stride(1), w1_scale.stride(2),
+            w2_scale.stride(0), w2_scale.stride(1), w2_scale.stride(2), 1 if activation == "gelu" else 0,
+            1 if apply_router_weight_on_input else 0, float(routed_scaling_factor), dtype_code(hidden_states.dtype), ws.data_ptr(), need,
+            stream_ptr(hidden_states.device)))
