@@ -38,6 +38,10 @@ __device__ __forceinline__ uint32_t buf_load_u16(rsrc_t r, uint32_t voff) {
   return (uint32_t)(u16)__builtin_amdgcn_raw_buffer_load_b16(r, (int)voff, 0, 0);
 }
 
+__device__ __forceinline__ uint32_t buf_load4(rsrc_t r, uint32_t voff) {
+  return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)voff, 0, 0);
+}
+
 struct MxArgs {
   const uint8_t* X;   // [M, K/2] codes of the activations
   const uint8_t* W;   // [N, K/2] codes of the weight
@@ -51,6 +55,10 @@ struct MxArgs {
   int64_t sx_m, sx_w, sw_n, sw_w;  // int32 words
   int nw;             // mx_stream_kernel: waves of a workgroup along n (1, 2, 4 or 8; the other 8 / nw cut K)
   int kb_per_wave;    // mx_stream_kernel: K blocks of a wave
+  int tiles_m, tiles_n;
+  int walkers;        // mx_tile256_kernel: workgroups [0, walkers) walk the whole tiles (a multiple of 8)
+  int tail_first;     // mx_tile256_kernel: tiles from here on are computed as two 128-row halves
+  int tail_shared;    // mx_tile256_kernel: half u belongs to workgroup u (after its walk), else to workgroup walkers + u
 };
 
 // descriptor of the scales of `rows` rows from row `row0` on, and the byte offset of the two scales that lane (row, kq) needs in K

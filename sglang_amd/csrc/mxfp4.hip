@@ -5,6 +5,7 @@
 #include "mx_common.h"
 #include "mx_gemm.h"
 #include "mx_moe.h"
+#include "mx_tile256.h"
 
 namespace fp8k {
 
@@ -163,7 +164,34 @@ int check_quant(const void* x, const void* q, int64_t M, int64_t K, int64_t ldx,
 }
 
 // ------------------------------------------------------------------------------------------------ product
+template <int O, int B>
+void launch_tile256(MxArgs p, hipStream_t st) {
+  p.tiles_m = (p.M + 255) / 256;
+  p.tiles_n = (p.N + 255) / 256;
+  const int tiles = p.tiles_m * p.tiles_n, cu = std::max(8, num_cu() / 8 * 8), rest = tiles % cu;
+  // the last, partial round over the chip: as halves, one workgroup each, where they fill at most the chip
+  p.tail_first = rest > 0 && 2 * rest <= cu ? tiles - rest : tiles;
+  const int units = (tiles - p.tail_first) * 2;
+  unsigned grid;
+  if (p.tail_first >= cu) {
+    p.walkers = cu;
+    p.tail_shared = 1;
+    grid = (unsigned)std::max(cu, units);
+  } else {
+    p.walkers = (p.tail_first + 7) / 8 * 8;
+    p.tail_shared = 0;
+    grid = (unsigned)(p.walkers + units);
+  }
+  if (p.K % kMxStep) mx_tile256_kernel<O, B, true><<<grid, 512, 0, st>>>(p);
+  else mx_tile256_kernel<O, B, false><<<grid, 512, 0, st>>>(p);
+}
+
 int launch_gemm(MxArgs p, int out_dtype, int bias_dtype, hipStream_t st) {
+  if (p.M > 128) {
+    if (out_dtype == FP8K_BF16) bias_dtype == FP8K_F32 ? launch_tile256<FP8K_BF16, FP8K_F32>(p, st) : launch_tile256<FP8K_BF16, FP8K_BF16>(p, st);
+    else bias_dtype == FP8K_F32 ? launch_tile256<FP8K_F16, FP8K_F32>(p, st) : launch_tile256<FP8K_F16, FP8K_F16>(p, st);
+    return check_launch("mxfp4 gemm");
+  }
   const int kbs = (p.K + kMxStep - 1) / kMxStep;
   const int ms = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
   const int m_blocks = (p.M + ms * 16 - 1) / (ms * 16);
