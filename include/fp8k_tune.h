@@ -29,6 +29,12 @@ extern "C" {
 void fp8k_tune_force_gemm_plan(int kind, int splits);
 
 /*
+ * Tuning and test aid: pins the kernel that MXFP4 products of the calling thread take.  -1: automatic (the default); 0: the weight
+ * stream; 1: 64x64 tiles; 2, 3: tiles of 128 weight rows and 64 or 128 activation rows; 4: 256x256 tiles.
+ */
+void fp8k_tune_force_mxfp4_plan(int kind);
+
+/*
  * Measurement aid (no counterpart in the reference): streams `bytes` of device memory at `src` once through the load
  * path of the weight-streaming kernels - one workgroup of 8 wavefronts per CU, 32 KB stages of 16-byte-per-lane loads
  * straight into LDS, two stages in flight, a workgroup barrier per stage - and drops the data.  Timed by the caller, it

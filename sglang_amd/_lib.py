@@ -77,6 +77,7 @@ SIGNATURES = {
     "fp8k_block_linear": (_c_int, [_c_ptr] * 5 + [_c_i64] * 7 + [_c_f32, _c_int, _c_ptr, _c_i64, _c_ptr]),
     "fp8k_token_linear": (_c_int, [_c_ptr] * 3 + [_c_i64, _c_ptr, _c_int, _c_ptr] + [_c_i64] * 5 + [_c_int, _c_ptr, _c_i64, _c_ptr]),
     "fp8k_tune_force_gemm_plan": (None, [_c_int, _c_int]),
+    "fp8k_tune_force_mxfp4_plan": (None, [_c_int]),
     "fp8k_tune_stream_read": (_c_int, [_c_ptr, _c_i64, _c_ptr]),
     "fp8k_tune_stream_read_tiles": (_c_int, [_c_ptr, _c_i64, _c_i64, _c_ptr]),
     "fp8k_tune_stream_read_write": (_c_int, [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_ptr]),

@@ -2,10 +2,13 @@
 // expert layer for a few tokens.  The format is described in mx_common.h.
 #include <algorithm>
 
+#include "../../include/fp8k_tune.h"
 #include "mx_common.h"
 #include "mx_gemm.h"
 #include "mx_moe.h"
+#include "mx_tile128.h"
 #include "mx_tile256.h"
+#include "mx_tile64.h"
 
 namespace fp8k {
 
@@ -186,12 +189,19 @@ void launch_tile256(MxArgs p, hipStream_t st) {
   else mx_tile256_kernel<O, B, false><<<grid, 512, 0, st>>>(p);
 }
 
-int launch_gemm(MxArgs p, int out_dtype, int bias_dtype, hipStream_t st) {
-  if (p.M > 128) {
-    if (out_dtype == FP8K_BF16) bias_dtype == FP8K_F32 ? launch_tile256<FP8K_BF16, FP8K_F32>(p, st) : launch_tile256<FP8K_BF16, FP8K_BF16>(p, st);
-    else bias_dtype == FP8K_F32 ? launch_tile256<FP8K_F16, FP8K_F32>(p, st) : launch_tile256<FP8K_F16, FP8K_F16>(p, st);
-    return check_launch("mxfp4 gemm");
-  }
+template <int O, int B>
+void launch_tile(MxArgs p, int tm, int tn, hipStream_t st) {
+  p.tiles_m = (p.M + tm - 1) / tm;
+  p.tiles_n = (p.N + tn - 1) / tn;
+  const unsigned grid = (unsigned)(((int64_t)p.tiles_m * p.tiles_n + 7) / 8 * 8);
+  const bool ragged = p.K % kMxStep != 0;
+  if (tn == 64) ragged ? mx_tile64_kernel<O, B, true><<<grid, 256, 0, st>>>(p) : mx_tile64_kernel<O, B, false><<<grid, 256, 0, st>>>(p);
+  else if (tm == 64) ragged ? mx_tile128_kernel<O, B, 64, true><<<grid, 512, 0, st>>>(p) : mx_tile128_kernel<O, B, 64, false><<<grid, 512, 0, st>>>(p);
+  else ragged ? mx_tile128_kernel<O, B, 128, true><<<grid, 512, 0, st>>>(p) : mx_tile128_kernel<O, B, 128, false><<<grid, 512, 0, st>>>(p);
+}
+
+template <int O, int B>
+void launch_stream(MxArgs p, hipStream_t st) {
   const int kbs = (p.K + kMxStep - 1) / kMxStep;
   const int ms = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
   const int m_blocks = (p.M + ms * 16 - 1) / (ms * 16);
@@ -202,21 +212,34 @@ int launch_gemm(MxArgs p, int out_dtype, int bias_dtype, hipStream_t st) {
   const int ks = 8 / nw;
   p.kb_per_wave = (kbs + ks - 1) / ks;
   const dim3 grid((unsigned)((p.N + nw * 16 - 1) / (nw * 16)), (unsigned)m_blocks);
-#define MX_STREAM(O, B)                                                   \
-  do {                                                                    \
-    if (ms == 1) mx_stream_kernel<1, O, B><<<grid, 512, 0, st>>>(p);      \
-    else if (ms == 2) mx_stream_kernel<2, O, B><<<grid, 512, 0, st>>>(p); \
-    else mx_stream_kernel<4, O, B><<<grid, 512, 0, st>>>(p);              \
-  } while (0)
-  if (out_dtype == FP8K_BF16) {
-    if (bias_dtype == FP8K_F32) MX_STREAM(FP8K_BF16, FP8K_F32);
-    else MX_STREAM(FP8K_BF16, FP8K_BF16);
-  } else {
-    if (bias_dtype == FP8K_F32) MX_STREAM(FP8K_F16, FP8K_F32);
-    else MX_STREAM(FP8K_F16, FP8K_F16);
+  if (ms == 1) mx_stream_kernel<1, O, B><<<grid, 512, 0, st>>>(p);
+  else if (ms == 2) mx_stream_kernel<2, O, B><<<grid, 512, 0, st>>>(p);
+  else mx_stream_kernel<4, O, B><<<grid, 512, 0, st>>>(p);
+}
+
+thread_local int g_force = -1;  // fp8k_tune_force_mxfp4_plan
+
+// which kernel a product takes: the tuning aid's numbers
+enum { kPlanStream = 0, kPlanTile64 = 1, kPlanTile128x64 = 2, kPlanTile128 = 3, kPlanTile256 = 4 };
+int plan_of(const MxArgs& p) {
+  if (g_force >= 0) return g_force;
+  return p.M <= 64 ? kPlanStream : p.M <= 128 ? kPlanTile64 : kPlanTile256;
+}
+
+template <int O, int B>
+int launch_gemm(const MxArgs& p, hipStream_t st) {
+  switch (plan_of(p)) {
+    case kPlanStream: launch_stream<O, B>(p, st); break;
+    case kPlanTile64: launch_tile<O, B>(p, 64, 64, st); break;
+    case kPlanTile128x64: launch_tile<O, B>(p, 64, 128, st); break;
+    case kPlanTile128: launch_tile<O, B>(p, 128, 128, st); break;
+    default: launch_tile256<O, B>(p, st);
   }
-#undef MX_STREAM
   return check_launch("mxfp4 gemm");
+}
+int launch_gemm(const MxArgs& p, int out_dtype, int bias_dtype, hipStream_t st) {
+  if (out_dtype == FP8K_BF16) return bias_dtype == FP8K_F32 ? launch_gemm<FP8K_BF16, FP8K_F32>(p, st) : launch_gemm<FP8K_BF16, FP8K_BF16>(p, st);
+  return bias_dtype == FP8K_F32 ? launch_gemm<FP8K_F16, FP8K_F32>(p, st) : launch_gemm<FP8K_F16, FP8K_F16>(p, st);
 }
 
 int check_gemm(const char* what, int64_t M, int64_t N, int64_t K, int64_t ldb, int64_t ldc, const void* B, const void* C, const void* bias,
@@ -241,6 +264,8 @@ int64_t experts_part(int64_t slots, int64_t I) { return up_to(slots * I * 2, 256
 }  // namespace fp8k
 
 using namespace fp8k;
+
+extern "C" void fp8k_tune_force_mxfp4_plan(int kind) { g_force = kind >= 0 && kind <= kPlanTile256 ? kind : -1; }
 
 extern "C" int fp8k_mxfp4_quant(const void* x, void* q, void* s, int64_t M, int64_t K, int64_t ldx, int64_t s_stride_m, int64_t s_stride_w,
                                 int in_dtype, int fuse_silu_and_mul, void* stream) {

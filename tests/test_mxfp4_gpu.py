@@ -152,8 +152,16 @@ SHAPES = [(1, 8, 32), (1, 16, 128), (3, 24, 96), (16, 64, 256), (17, 40, 288), (
           (513, 776, 1312), (1, 4096, 4096), (8, 1000, 7168), (5, 8, 18432), (1000, 1096, 768), (2050, 2056, 512)]
 
 
-@pytest.mark.parametrize("m,n,k", SHAPES)
-def test_matmul_is_exact(dev, m, n, k):
+@pytest.fixture
+def plan():
+    """Pins the kernel that products take."""
+    from sglang_amd._lib import lib
+
+    yield lib.fp8k_tune_force_mxfp4_plan
+    lib.fp8k_tune_force_mxfp4_plan(-1)
+
+
+def _exact(dev, m, n, k):
     rng = np.random.default_rng(m * 7 + n * 3 + k)
     for dtype, row_major in ((torch.bfloat16, False), (torch.float16, True)):
         spread = 1 if k <= 8192 else 0
@@ -168,6 +176,38 @@ def test_matmul_is_exact(dev, m, n, k):
             bias = torch.from_numpy(rng.integers(-64, 65, n) / 8.0).to(bias_type).to(dev)
             got = mxfp4.w4a4_mxfp4_matmul(a, b, sa, sb, dtype, bias=bias)
             assert torch.equal(got.cpu(), _rounded(ref + _np(bias), dtype)), (m, n, k, bias_type)
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+def test_matmul_is_exact(dev, m, n, k):
+    _exact(dev, m, n, k)
+
+
+@pytest.mark.parametrize("kind", range(5))
+@pytest.mark.parametrize("m,n,k", [(1, 8, 32), (15, 72, 256), (64, 64, 288), (65, 72, 512), (127, 136, 736), (129, 264, 1024), (130, 256, 1280), (200, 520, 1568),
+                                   (257, 248, 2048), (300, 1032, 2304), (520, 776, 4640)])
+def test_every_kernel_is_exact(dev, plan, kind, m, n, k):
+    """One, two, three .. K blocks, remainders of every unrolling, rows and columns around the edges of every tile."""
+    plan(kind)
+    _exact(dev, m, n, k)
+
+
+@pytest.mark.parametrize("kind", range(5))
+def test_every_kernel_stores_unaligned_rows(dev, plan, kind):
+    """Rows of the result that start at multiples of 8 bytes only, through the C interface; what lies between them stays."""
+    from sglang_amd import _lib
+
+    rng = np.random.default_rng(kind)
+    plan(kind)
+    m, n, k = 150, 328, 544
+    av, a, sa = _operand(rng, m, k, dev)
+    bv, b, sb = _operand(rng, n, k, dev)
+    wide = torch.full((m, n + 20), 7.0, dtype=torch.bfloat16, device=dev)
+    out = wide[:, 4:4 + n]
+    _lib.check(_lib.lib.fp8k_mxfp4_gemm(a.data_ptr(), b.data_ptr(), sa.data_ptr(), sb.data_ptr(), None, out.data_ptr(), m, n, k, k // 2, k // 2,
+                                        sa.stride(0), sa.stride(1), sb.stride(0), sb.stride(1), n + 20, _lib.BF16, _lib.F32, _lib.stream_ptr(dev)))
+    assert torch.equal(out.cpu(), _rounded(av @ bv.T, torch.bfloat16))
+    assert (wide[:, :4] == 7).all() and (wide[:, 4 + n:] == 7).all()
 
 
 @pytest.mark.parametrize("m,n,k", [(4, 64, 512), (40, 128, 288), (300, 264, 1056), (520, 512, 800)])
