@@ -38,6 +38,28 @@ __device__ __forceinline__ uint32_t buf_load_u16(rsrc_t r, uint32_t voff) {
   return (uint32_t)(u16)__builtin_amdgcn_raw_buffer_load_b16(r, (int)voff, 0, 0);
 }
 
+// Quantises the 8 values of each of four neighbouring lanes, which make a block: the lane's eight codes, and the block's scale byte.
+// The scale's exponent is that of the largest magnitude after a rounding to one fraction bit (the codes' own), minus the 2 of the
+// largest code 6 = 1.5 * 2^2: 3.5 <= |largest| / scale < 7, and what lies above 6 becomes 6.  The values times 2^-exponent (exact) are
+// rounded to nearest, ties to the even code, by v_cvt_scalef32_pk_fp4_f32.  An infinity or a NaN makes the byte 255 and the codes zero.
+__device__ __forceinline__ uint32_t mx_quant8(const float (&v)[8], uint32_t& byte) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);  // NaN above infinity above every number
+  m = dpp_umax<kDppXor1>(m);
+  m = dpp_umax<kDppXor2>(m);
+  const bool finite = m < 0x7f800000u;
+  const int e = min((int)((m + 0x200000u) >> 23), 254) - 2;
+  byte = finite ? (uint32_t)max(e, 0) : 255u;
+  const float to = finite ? __uint_as_float((254u - byte) << 23) : 0.f;  // 2^(127 - byte)
+  uint32_t codes = 0;
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[0] * to, v[1] * to, 1.0f, 0);
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[2] * to, v[3] * to, 1.0f, 1);
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[4] * to, v[5] * to, 1.0f, 2);
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[6] * to, v[7] * to, 1.0f, 3);
+  return finite ? codes : 0u;
+}
+
 __device__ __forceinline__ uint32_t buf_load4(rsrc_t r, uint32_t voff) {
   return (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(r, (int)voff, 0, 0);
 }
@@ -50,11 +72,9 @@ struct MxArgs {
   const void* bias;   // [N], may be null; added in float32 before the only rounding
   void* C;            // [M, N]
   int M, N, K;
-  int64_t ldx, ldw;   // bytes
+  int64_t ldx, ldw;   // bytes (16-bit activations: elements)
   int64_t ldc;        // elements
   int64_t sx_m, sx_w, sw_n, sw_w;  // int32 words
-  int nw;             // mx_stream_kernel: waves of a workgroup along n (1, 2, 4 or 8; the other 8 / nw cut K)
-  int kb_per_wave;    // mx_stream_kernel: K blocks of a wave
   int tiles_m, tiles_n;
   int walkers;        // mx_tile256_kernel: workgroups [0, walkers) walk the whole tiles (a multiple of 8)
   int tail_first;     // mx_tile256_kernel: tiles from here on are computed as two 128-row halves

@@ -21,13 +21,6 @@ namespace fp8k {
 // Memory bound: 2 bytes read and 17/32 written per 16-bit element.  A wave takes 512 columns of four rows, 8 values to a lane, four
 // lanes to a block and sixteen to a scale word; the words of four rows lie side by side in memory and leave as one 16-byte store.
 // ------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t abs_max8_bits(const float (&a)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(a[i]) & 0x7fffffffu);  // NaN above infinity above every number
-  return m;
-}
-
 template <int DT, bool FUSE>
 __global__ __launch_bounds__(256) void mx_quant_kernel(const void* x, uint8_t* q, int32_t* s, int M, int K, int64_t ldx, int64_t s_m, int64_t s_w) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
@@ -55,19 +48,8 @@ __global__ __launch_bounds__(256) void mx_quant_kernel(const void* x, uint8_t* q
 #pragma unroll
       for (int k = 0; k < 8; ++k) v[k] = silu_f32(v[k]) * u[k];
     }
-    uint32_t m = abs_max8_bits(v);
-    m = dpp_umax<kDppXor1>(m);
-    m = dpp_umax<kDppXor2>(m);
-    const bool finite = m < 0x7f800000u;
-    const int e = min((int)((m + 0x200000u) >> 23), 254) - 2;
-    const uint32_t byte = finite ? (uint32_t)max(e, 0) : 255u;
-    const float to = finite ? __uint_as_float((254u - byte) << 23) : 0.f;  // 2^(127 - byte)
-    uint32_t codes = 0;
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[0] * to, v[1] * to, 1.0f, 0);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[2] * to, v[3] * to, 1.0f, 1);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[4] * to, v[5] * to, 1.0f, 2);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, v[6] * to, v[7] * to, 1.0f, 3);
-    if (!finite) codes = 0;
+    uint32_t byte;
+    const uint32_t codes = mx_quant8(v, byte);
     if (in && m0 + i < M) *reinterpret_cast<uint32_t*>(q + (int64_t)(m0 + i) * (K >> 1) + (c >> 1)) = codes;
     // the four bytes of a word: one per quad of lanes; past the end of the row zero
     uint32_t word = in ? byte << (((lane >> 2) & 3) * 8) : 0u;
@@ -200,36 +182,60 @@ void launch_tile(MxArgs p, int tm, int tn, hipStream_t st) {
   else ragged ? mx_tile128_kernel<O, B, 128, true><<<grid, 512, 0, st>>>(p) : mx_tile128_kernel<O, B, 128, false><<<grid, 512, 0, st>>>(p);
 }
 
+// strips of 16 NS weight rows: as wide as leaves every CU two workgroups
+int strip_groups(int64_t N, int m_blocks, int most) {
+  int ns = 1;
+  while (ns < most && (N + 32 * ns - 1) / (32 * ns) * m_blocks >= 2 * num_cu()) ns *= 2;
+  return ns;
+}
+template <int MS, int NS, bool FUSE, int O, int B>
+void launch_strip(const MxArgs& p, hipStream_t st) {
+  const dim3 grid((unsigned)((p.N + 16 * NS - 1) / (16 * NS)), (unsigned)((p.M + 16 * MS - 1) / (16 * MS)));
+  if (p.K % kMxStep) mx_strip_kernel<MS, NS, FUSE, O, B, true><<<grid, 512, 0, st>>>(p);
+  else mx_strip_kernel<MS, NS, FUSE, O, B, false><<<grid, 512, 0, st>>>(p);
+}
 template <int O, int B>
-void launch_stream(MxArgs p, hipStream_t st) {
-  const int kbs = (p.K + kMxStep - 1) / kMxStep;
-  const int ms = p.M <= 16 ? 1 : p.M <= 32 ? 2 : 4;
-  const int m_blocks = (p.M + ms * 16 - 1) / (ms * 16);
-  // as many waves along n as leave every CU a workgroup, and no more K ranges than K blocks
-  int nw = 1;
-  while (nw < 8 && ((int64_t)(p.N + nw * 32 - 1) / (nw * 32) * m_blocks >= num_cu() || 8 / nw > kbs)) nw *= 2;
-  p.nw = nw;
-  const int ks = 8 / nw;
-  p.kb_per_wave = (kbs + ks - 1) / ks;
-  const dim3 grid((unsigned)((p.N + nw * 16 - 1) / (nw * 16)), (unsigned)m_blocks);
-  if (ms == 1) mx_stream_kernel<1, O, B><<<grid, 512, 0, st>>>(p);
-  else if (ms == 2) mx_stream_kernel<2, O, B><<<grid, 512, 0, st>>>(p);
-  else mx_stream_kernel<4, O, B><<<grid, 512, 0, st>>>(p);
+void launch_strips(const MxArgs& p, hipStream_t st) {
+  if (p.M <= 16) {
+    const int ns = strip_groups(p.N, 1, 4);
+    if (ns == 1) launch_strip<1, 1, false, O, B>(p, st);
+    else if (ns == 2) launch_strip<1, 2, false, O, B>(p, st);
+    else launch_strip<1, 4, false, O, B>(p, st);
+  } else if (p.M <= 32) {
+    if (strip_groups(p.N, 1, 2) == 1) launch_strip<2, 1, false, O, B>(p, st);
+    else launch_strip<2, 2, false, O, B>(p, st);
+  } else {
+    launch_strip<4, 1, false, O, B>(p, st);
+  }
+}
+// a whole linear of a few rows in one launch: p.X holds 16-bit activations, p.ldx their row stride in elements
+bool fuses_quant(int64_t M, int64_t K) {
+  if (M > 16 || M * K > kMxFuse) return false;
+  const int64_t kbs = (K + kMxStep - 1) / kMxStep;
+  return M * mx_fuse_stride((int)kbs) <= kMxFuseRows && M * kbs * 8 <= kMxFuseScales;
+}
+template <int O, int B>
+int launch_fused(const MxArgs& p, hipStream_t st) {
+  const int ns = strip_groups(p.N, 1, 4);
+  if (ns == 1) launch_strip<1, 1, true, O, B>(p, st);
+  else if (ns == 2) launch_strip<1, 2, true, O, B>(p, st);
+  else launch_strip<1, 4, true, O, B>(p, st);
+  return check_launch("mxfp4 linear");
 }
 
 thread_local int g_force = -1;  // fp8k_tune_force_mxfp4_plan
 
 // which kernel a product takes: the tuning aid's numbers
-enum { kPlanStream = 0, kPlanTile64 = 1, kPlanTile128x64 = 2, kPlanTile128 = 3, kPlanTile256 = 4 };
+enum { kPlanStrips = 0, kPlanTile64 = 1, kPlanTile128x64 = 2, kPlanTile128 = 3, kPlanTile256 = 4 };
 int plan_of(const MxArgs& p) {
   if (g_force >= 0) return g_force;
-  return p.M <= 64 ? kPlanStream : p.M <= 128 ? kPlanTile64 : kPlanTile256;
+  return p.M <= 64 ? kPlanStrips : p.M <= 128 ? kPlanTile64 : kPlanTile256;
 }
 
 template <int O, int B>
 int launch_gemm(const MxArgs& p, hipStream_t st) {
   switch (plan_of(p)) {
-    case kPlanStream: launch_stream<O, B>(p, st); break;
+    case kPlanStrips: launch_strips<O, B>(p, st); break;
     case kPlanTile64: launch_tile<O, B>(p, 64, 64, st); break;
     case kPlanTile128x64: launch_tile<O, B>(p, 64, 128, st); break;
     case kPlanTile128: launch_tile<O, B>(p, 128, 128, st); break;
@@ -316,7 +322,7 @@ extern "C" int fp8k_mxfp4_gemm(const void* A, const void* B, const void* As, con
 }
 
 extern "C" int64_t fp8k_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || fuses_quant(M, K)) return 0;
   return up_to(M * K / 2, 256) + up_to(words_of(K) * up_to(M, 4) * 4, 256);
 }
 
@@ -331,16 +337,27 @@ extern "C" int fp8k_mxfp4_linear(const void* x, const void* B, const void* Bs, c
   const int64_t need = fp8k_mxfp4_linear_workspace_bytes(M, N, K);
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
     return fail(FP8K_ERR_WORKSPACE, "mxfp4 linear: workspace of %lld bytes needed, 256-byte aligned", (long long)need);
+  MxArgs p{};
+  p.W = (const uint8_t*)B; p.sw = (const uint8_t*)Bs;
+  p.bias = bias; p.C = C; p.M = (int)M; p.N = (int)N; p.K = (int)K;
+  p.ldw = ldb; p.ldc = ldc;
+  p.sw_n = bs_stride_n; p.sw_w = bs_stride_w;
+  const hipStream_t st = (hipStream_t)stream;
+  const int bt = bias ? bias_dtype : FP8K_F32;
+  if (fuses_quant(M, K)) {
+    p.X = (const uint8_t*)x;
+    p.ldx = ldx;
+    if (dtype == FP8K_BF16) return bt == FP8K_F32 ? launch_fused<FP8K_BF16, FP8K_F32>(p, st) : launch_fused<FP8K_BF16, FP8K_BF16>(p, st);
+    return bt == FP8K_F32 ? launch_fused<FP8K_F16, FP8K_F32>(p, st) : launch_fused<FP8K_F16, FP8K_F16>(p, st);
+  }
   uint8_t* const q = (uint8_t*)workspace;
   uint8_t* const s = q + up_to(M * K / 2, 256);
   const int64_t ld = up_to(M, 4);
-  if (const int rc = quant(x, q, s, M, K, ldx, 1, ld, dtype, false, (hipStream_t)stream)) return rc;
-  MxArgs p{};
-  p.X = q; p.W = (const uint8_t*)B; p.sx = s; p.sw = (const uint8_t*)Bs;
-  p.bias = bias; p.C = C; p.M = (int)M; p.N = (int)N; p.K = (int)K;
-  p.ldx = K / 2; p.ldw = ldb; p.ldc = ldc;
-  p.sx_m = 1; p.sx_w = ld; p.sw_n = bs_stride_n; p.sw_w = bs_stride_w;
-  return launch_gemm(p, dtype, bias ? bias_dtype : FP8K_F32, (hipStream_t)stream);
+  if (const int rc = quant(x, q, s, M, K, ldx, 1, ld, dtype, false, st)) return rc;
+  p.X = q; p.sx = s;
+  p.ldx = K / 2;
+  p.sx_m = 1; p.sx_w = ld;
+  return launch_gemm(p, dtype, bt, st);
 }
 
 extern "C" int64_t fp8k_mxfp4_experts_workspace_bytes(int64_t T, int64_t topk, int64_t I) {
