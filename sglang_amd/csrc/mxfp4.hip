@@ -227,9 +227,30 @@ thread_local int g_force = -1;  // fp8k_tune_force_mxfp4_plan
 
 // which kernel a product takes: the tuning aid's numbers
 enum { kPlanStrips = 0, kPlanTile64 = 1, kPlanTile128x64 = 2, kPlanTile128 = 3, kPlanTile256 = 4 };
+// Up to 64 rows the strips, while they are one round over the chip or the rows are few; of the tiles the one with the shortest time
+// by rounds * (start and write-out + K blocks * time of a block), the times as measured on products of 128 .. 4096 rows (weights
+// out of HBM): 64x64 tiles 0.24 us a block, 128x64 0.385, 128x128 0.62, 256x256 1.1 while the tiles are computed in halves and 2.0 whole.
 int plan_of(const MxArgs& p) {
   if (g_force >= 0) return g_force;
-  return p.M <= 64 ? kPlanStrips : p.M <= 128 ? kPlanTile64 : kPlanTile256;
+  const int64_t cu = num_cu();
+  // 64 x 4096 x 4096: strips 6.5 us, 64x64 tiles 8.0; 64 x 4608 x 7168, a second round: 15.0 and 10.1
+  if (p.M <= 64 && p.N <= 16 * cu) return kPlanStrips;
+  // 24 x 7168 x 18432: strips 23.2, 64x64 tiles 26.3, 128x64 33.7; 32 x 28672 x 4096: 19.4, 19.7, 15.3; 16 rows: 16.8, 19.2, 15.0
+  if (p.M <= 32 && p.N <= 64 * cu) return kPlanStrips;
+  const double kbs = (p.K + kMxStep - 1) / kMxStep;
+  const auto time = [&](int tm, int tn, double tile, double block) {
+    const int64_t tiles = (int64_t)((p.M + tm - 1) / tm) * ((p.N + tn - 1) / tn);
+    return (double)((tiles + cu - 1) / cu) * (tile + kbs * block);
+  };
+  const int64_t big = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256), rest = big % cu;
+  const bool halves = rest > 0 && 2 * rest <= cu;
+  const double t[] = {time(64, 64, 1.2, 0.24), time(64, 128, 1.3, 0.385), time(128, 128, 1.6, 0.62),
+                      (double)((big + cu - 1) / cu - halves) * (4.0 + kbs * 2.0) + (halves ? 3.0 + kbs * 1.1 : 0.0)};
+  constexpr int kind[] = {kPlanTile64, kPlanTile128x64, kPlanTile128, kPlanTile256};
+  int best = 0;
+  for (int i = 1; i < 4; ++i)
+    if (t[i] < t[best]) best = i;
+  return kind[best];
 }
 
 template <int O, int B>
@@ -363,7 +384,7 @@ extern "C" int fp8k_mxfp4_linear(const void* x, const void* B, const void* Bs, c
 extern "C" int64_t fp8k_mxfp4_experts_workspace_bytes(int64_t T, int64_t topk, int64_t I) {
   if (T <= 0 || topk <= 0 || I <= 0) return 0;
   const int64_t slots = T * topk;
-  return experts_part(slots, I) + up_to(slots * 16, 256) + up_to(slots * 4, 256) + 256;
+  return experts_part(slots, I) + 3 * up_to(slots * 4, 256) + 256;
 }
 
 extern "C" int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2, const void* s1, const void* s2, const float* topk_weights,
@@ -376,7 +397,7 @@ extern "C" int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2,
   FP8K_REQUIRE(activation == FP8K_ACT_SILU || activation == FP8K_ACT_GELU, "mxfp4 experts: the activation must be silu or gelu");
   FP8K_REQUIRE(T >= 0 && topk > 0 && E > 0 && H > 0 && I > 0, "mxfp4 experts: bad sizes");
   FP8K_REQUIRE(H % kMxBlock == 0 && I % kMxBlock == 0, "mxfp4 experts: hidden and intermediate size must be multiples of 32");
-  FP8K_REQUIRE(H <= (1 << 20) && I <= (1 << 20) && E <= 65535, "mxfp4 experts: too large");
+  FP8K_REQUIRE(H <= (1 << 20) && I <= (1 << 20) && H * I < (1ll << 31) && E <= 65535, "mxfp4 experts: too large");
   FP8K_REQUIRE(T <= kMxMaxTokens && T * topk <= kMxMaxSlots, "mxfp4 experts: built for at most %d tokens and %d (token, choice) pairs, got %lld and %lld",
                kMxMaxTokens, kMxMaxSlots, (long long)T, (long long)(T * topk));
   if (T == 0) return FP8K_OK;
@@ -397,8 +418,9 @@ extern "C" int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2,
   p.topk_w = topk_weights; p.ids = topk_ids; p.out = out;
   uint8_t* at = (uint8_t*)workspace;
   p.h = at; at += experts_part(slots, I);
-  p.tiles = (int32_t*)at; at += up_to(slots * 16, 256);
+  p.tiles = (int32_t*)at; at += up_to(slots * 4, 256);
   p.order = (int32_t*)at; at += up_to(slots * 4, 256);
+  p.weights = (float*)at; at += up_to(slots * 4, 256);
   p.ntiles = (int32_t*)at;
   p.T = (int)T; p.topk = (int)topk; p.E = (int)E; p.H = (int)H; p.I = (int)I; p.slots = (int)slots;
   p.ids64 = ids_are_64bit != 0; p.on_input = weight_on_input != 0; p.ldx = ldx;
@@ -408,13 +430,17 @@ extern "C" int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2,
   p.scaling = scaling;
   const hipStream_t st = (hipStream_t)stream;
   const bool gelu = activation == FP8K_ACT_GELU;
-  const dim3 grid1((unsigned)((I + 15) / 16 + 1), (unsigned)std::min(slots, E)), grid2((unsigned)((H + 15) / 16));
+  // runs of strips: as long as leaves two workgroups for every CU, so that a workgroup's start - the list of its slots, its first lines -
+  // comes once for several strips
+  const int64_t units = std::min(slots, E), strips = I / 16;
+  p.run = (int)std::min<int64_t>(8, std::max<int64_t>(1, units * strips / (2 * num_cu())));
+  const dim3 grid1((unsigned)((strips + p.run - 1) / p.run + 1), (unsigned)units), grid2((unsigned)(H / 16));
 #define MX_EXPERTS(DT)                                                                       \
   do {                                                                                       \
     if (gelu) mx_experts_up_kernel<DT, true><<<grid1, 512, 0, st>>>(p);                      \
     else mx_experts_up_kernel<DT, false><<<grid1, 512, 0, st>>>(p);                          \
     if (const int rc = check_launch("mxfp4 experts")) return rc;                             \
-    if (T <= 16) mx_experts_down_kernel<DT, 16><<<grid2, 512, 0, st>>>(p);                   \
+    if (T <= 16 && slots <= mx_down_places(16)) mx_experts_down_kernel<DT, 16><<<grid2, 512, 0, st>>>(p);                   \
     else if (T <= 64) mx_experts_down_kernel<DT, 64><<<grid2, 512, 0, st>>>(p);              \
     else mx_experts_down_kernel<DT, kMxMaxTokens><<<grid2, 512, 0, st>>>(p);                 \
   } while (0)
