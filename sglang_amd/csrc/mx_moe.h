@@ -61,13 +61,14 @@ struct MxExpertArgs {
   const void* ids;      // [T, topk] int32 or int64
   void* out;            // [T, H]
   void* h;              // [slots, I] 16-bit: the workspace, as are the four arrays of the table
-  int32_t* tiles;       // [slots] tile t: up to 16 slots of one expert (mx_tile below)
+  int32_t* tiles;       // [slots] tile t: some slots of one expert (mx_tile below)
   int32_t* order;       // [slots] slots sorted by expert
   float* weights;       // [slots] their routed weights, in that order
   int32_t* ntiles;
   int T, topk, E, H, I, slots;
   int ids64, on_input;
   int run;              // mx_experts_up_kernel: strips of a workgroup
+  int tile;             // slots of a tile (4 or 16)
   int64_t ldx;          // elements
   int64_t w1_e, w2_e;   // bytes
   int64_t s1_e, s1_n, s1_w, s2_e, s2_n, s2_w;  // int32 words
@@ -89,23 +90,33 @@ struct MxCodes {
   __device__ __forceinline__ explicit MxCodes(int lane) : rd((uint32_t)((lane & 15) * kMxStepBytes + (lane >> 4) * 4)), key(((lane & 15) >> 1) & 7) {}
   __device__ __forceinline__ uint32_t get(const uint8_t* slot, int j) const { return *reinterpret_cast<const uint32_t*>(slot + rd + ((j ^ key) << 4)); }
 };
-__device__ __forceinline__ float mx_block_scale(uint32_t lo, uint32_t hi, int j) { return e8m0_f32(((j < 4 ? lo : hi) >> ((j & 3) * 8)) & 255u); }
+// the scale of block j, byte j & 3 of one of two words.  The conversion to bfloat16 takes a scale's exponent field as the e8m0 byte it is
+// (255, infinity's, makes NaN), which saves telling 0 and 255 apart.
+template <int DT>
+__device__ __forceinline__ float mx_block_scale(uint32_t lo, uint32_t hi, int j) {
+  const uint32_t word = j < 4 ? lo : hi;
+  if (DT != FP8K_BF16) return e8m0_f32((word >> ((j & 3) * 8)) & 255u);
+  const int up = 23 - (j & 3) * 8;
+  return __uint_as_float((up < 0 ? word >> 1 : word << (up < 0 ? 0 : up)) & 0x7f800000u);
+}
 
-// The table of the second launch: slots sorted by expert (and by their number within one), cut into tiles of up to 16 slots of one
-// expert.  One workgroup of 512 threads; keys: LDS for kMxMaxSlots words, aux: for 64.
+// The table of the second launch: slots sorted by expert (and by their number within one), cut into tiles of up to p.tile slots of one
+// expert.  One workgroup of 256 threads; keys, sorted: LDS for kMxMaxSlots words, aux: for 32.
 __device__ __forceinline__ void mx_sort_slots(const MxExpertArgs& p, int* keys, int* sorted, int* aux) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   constexpr int kNone = 0x7fffffff;
+  constexpr int NT = 256, J = kMxMaxSlots / NT;
   const int padded = (p.slots + 3) & ~3;
-  for (int s = tid; s < padded; s += 512) {
+  for (int s = tid; s < padded; s += NT) {
     const int e = s < p.slots ? mx_expert_of(p, s) : -1;
     keys[s] = e < 0 ? kNone : (e << 10) | s;
   }
+  if (tid < 16) aux[tid] = -1;
   __syncthreads();
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int s = j * 512 + tid;
-    const int key = s < p.slots ? keys[s] : kNone;
+  // a key's place is the number of smaller ones
+  int valid = 0;
+  for (int s = tid; s < padded; s += NT) {
+    const int key = keys[s];
     int at = 0;
 #pragma unroll 4
     for (int o = 0; o < padded; o += 4) {
@@ -118,68 +129,70 @@ __device__ __forceinline__ void mx_sort_slots(const MxExpertArgs& p, int* keys, 
       p.weights[at] = p.topk_w[s];
     }
   }
-  if (tid < 16) aux[tid] = -1;
-  int valid = 0;
 #pragma unroll 4
   for (int o = 0; o < padded; o += 4) {
     const int4 k = *reinterpret_cast<const int4*>(keys + o);
     valid += (k.x != kNone) + (k.y != kNone) + (k.z != kNone) + (k.w != kNone);
   }
   __syncthreads();
-  // places 64 (8 j + w) + lane: the first of an expert; a place's rank is its distance to the last of those at or before it
+  // places 64 (4 j + w) + lane: the first of an expert; a place's rank is its distance to the last of those at or before it
   const uint64_t upto = (2ull << lane) - 1;
-  int rank[2];
-  uint64_t starts[2];
+  uint64_t heads[J], starts[J];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int at = j * 512 + tid;
-    const uint64_t heads = __ballot(at < valid && (at == 0 || (sorted[at - 1] >> 10) != (sorted[at] >> 10)));
-    rank[j] = (heads & upto) ? 63 - __clzll((long long)(heads & upto)) : -1;
-    if (lane == 0 && heads) aux[j * 8 + w] = (j * 8 + w) * 64 + 63 - __clzll((long long)heads);
+  for (int j = 0; j < J; ++j) {
+    const int at = j * NT + tid, chunk = j * 4 + w;
+    heads[j] = __ballot(at < valid && (at == 0 || (sorted[at - 1] >> 10) != (sorted[at] >> 10)));
+    if (lane == 0 && heads[j]) aux[chunk] = chunk * 64 + 63 - __clzll((long long)heads[j]);
   }
   __syncthreads();
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int at = j * 512 + tid, chunk = j * 8 + w;
-    int head = rank[j] >= 0 ? chunk * 64 + rank[j] : -1;
-    for (int c = 0; c < 16; ++c)
-      if (rank[j] < 0 && c < chunk && aux[c] >= 0) head = aux[c];
-    starts[j] = __ballot(at < valid && (at - head) % 16 == 0);
+  for (int j = 0; j < J; ++j) {
+    const int at = j * NT + tid, chunk = j * 4 + w;
+    int head = -1;
+    for (int c = 0; c < chunk; ++c) head = max(head, aux[c]);
+    if (heads[j] & upto) head = chunk * 64 + 63 - __clzll((long long)(heads[j] & upto));
+    starts[j] = __ballot(at < valid && (at - head) % p.tile == 0);
     if (lane == 0) aux[16 + chunk] = __popcll(starts[j]);
   }
   __syncthreads();
-  int total = 0;
-  for (int c = 0; c < 16; ++c) total += aux[16 + c];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int at = j * 512 + tid, chunk = j * 8 + w;
+  for (int j = 0; j < J; ++j) {
+    const int at = j * NT + tid, chunk = j * 4 + w;
     if (!((starts[j] >> lane) & 1)) continue;
     int t = __popcll(starts[j] & (upto >> 1));
     for (int c = 0; c < chunk; ++c) t += aux[16 + c];
     int n = 1;
-    while (n < 16 && at + n < valid && (sorted[at + n] >> 10) == (sorted[at] >> 10)) ++n;
+    while (n < p.tile && at + n < valid && (sorted[at + n] >> 10) == (sorted[at] >> 10)) ++n;
     p.tiles[t] = mx_tile(sorted[at] >> 10, at, n);
   }
-  if (tid == 0) p.ntiles[0] = total;
+  if (tid == 0) {
+    int total = 0;
+    for (int c = 0; c < 16; ++c) total += aux[16 + c];
+    p.ntiles[0] = total;
+  }
 }
 
 // ------------------------------------------------------------------------------------------------
 // First launch.  Grid (runs of strips + 1, units).  Units are slots (the first slot of an expert does the work, the others end at once)
 // or experts, whichever are fewer; the workgroup behind the last run of unit 0 makes the table of the second launch.
 //
-// A workgroup takes a run of strips of 16 columns of h: 16 gate and 16 up rows, all of K, for the expert's slots, 16 at a time.  Its eight
-// waves take every eighth K block each.  A wave's requests - whole lines of its 32 rows straight to an LDS slot of its own and their scale
-// words two blocks ahead, the slots' activations to registers one block ahead - run on across the strips of the run.  The eight sums meet in LDS;
-// the last wave, which has the fewest blocks, adds them up, applies the activation and writes h, while the others go on.
-// Bound: the weights' bytes.  80 KB of LDS and 128 registers: two workgroups share a CU.
+// A workgroup takes a run of strips of 16 columns of h: 16 gate and 16 up rows, all of K, for the expert's slots, RX at a time.  Its four
+// waves take every fourth K block each.  What a block needs - the lines of 32 rows, their scale words, the slots' activations - goes
+// straight to an LDS slot of the wave, two blocks ahead and on across the strips of the run, and no other load stands in the loop.  The
+// four sums meet in LDS; the last wave, which has the fewest blocks, adds them up, applies the activation and writes h, while the
+// others go on.
+// Bound: the weights' bytes.  With RX = 4 two workgroups share a CU.
 // ------------------------------------------------------------------------------------------------
-template <int DT, bool GELU>
-__global__ __launch_bounds__(512, 4) void mx_experts_up_kernel(const MxExpertArgs p) {
-  constexpr int kSlot = 2 * 2048, kWave = 2 * kSlot;
-  constexpr int kOps = 4 + 4;  // loads of a wave per K block beside the activations: scale words, lines
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[8 * kWave];
-  __shared__ __attribute__((aligned(16))) v4f red[7][2][64];
+constexpr int mx_up_slot(int rx) { return 4096 + rx * 512 + 256; }
+
+template <int DT, bool GELU, int RX>
+__global__ __launch_bounds__(256, 2) void mx_experts_up_kernel(const MxExpertArgs p) {
+  constexpr int NW = 4, ST = 2, kSlot = mx_up_slot(RX), kWave = ST * kSlot, kX = 4096, kS = 4096 + RX * 512;
+  constexpr int kLoads = 5 + RX / 2;  // of a wave per K block
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[NW * kWave];
+  __shared__ __attribute__((aligned(16))) v4f red[NW - 1][2][64];
   __shared__ u16 list[kMxMaxSlots];
+  static_assert(sizeof(smem) >= (2 * kMxMaxSlots + 32) * 4, "the sort works where the slots are");
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -194,124 +207,124 @@ __global__ __launch_bounds__(512, 4) void mx_experts_up_kernel(const MxExpertArg
 
   // ---- the unit's expert and the list of its slots, ascending
   const bool by_slot = (int)gridDim.y == p.slots;
-  bool mine[2];
-  uint64_t masks[2];
   const int expert = __builtin_amdgcn_readfirstlane(by_slot ? mx_expert_of(p, blockIdx.y) : (int)blockIdx.y);
   if (expert < 0) return;
+  constexpr int J = kMxMaxSlots / 256;
+  uint64_t masks[J];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int s = j * 512 + tid;
-    mine[j] = s < p.slots && mx_expert_of(p, s) == expert;
-    masks[j] = __ballot(mine[j]);
-    if (lane == 0) scratch[j * 8 + w] = __popcll(masks[j]);
+  for (int j = 0; j < J; ++j) {
+    const int s = j * 256 + tid;
+    masks[j] = __ballot(s < p.slots && mx_expert_of(p, s) == expert);
+    if (lane == 0) scratch[j * 4 + w] = __popcll(masks[j]);
   }
   __syncthreads();
   int total = 0;
   for (int k = 0; k < 16; ++k) total += scratch[k];
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
+  for (int j = 0; j < J; ++j) {
     int at = __popcll(masks[j] & ((1ull << lane) - 1));
-    for (int k = 0; k < j * 8 + w; ++k) at += scratch[k];
-    if (mine[j]) list[at] = (u16)(j * 512 + tid);
+    for (int k = 0; k < j * 4 + w; ++k) at += scratch[k];
+    if ((masks[j] >> lane) & 1) list[at] = (u16)(j * 256 + tid);
   }
   total = __builtin_amdgcn_readfirstlane(total);
   __syncthreads();
   if (total == 0 || (by_slot && list[0] != (int)blockIdx.y)) return;
 
   const int row_bytes = p.H >> 1, words = (p.H + 127) >> 7, kbs = (p.H + kMxStep - 1) / kMxStep;
-  const int strip0 = blockIdx.x * p.run, nstrips = min(p.run, strips - strip0), ntiles = (total + 15) >> 4;
-  const int nb = kbs > w ? (kbs - w + 7) >> 3 : 0;  // blocks of the wave: w, w + 8, ..
+  const int strip0 = blockIdx.x * p.run, nstrips = min(p.run, strips - strip0), ntiles = (total + RX - 1) / RX;
+  const int nb = kbs > w ? (kbs - w + NW - 1) / NW : 0;  // blocks of the wave: w, w + 4, ..
   const rsrc_t rW = make_rsrc(p.w1 + (int64_t)expert * p.w1_e, (uint32_t)(2 * p.I * row_bytes));
   const rsrc_t rS = mx_scale_rsrc(p.s1 + (int64_t)expert * p.s1_e * 4, 0, 2 * p.I, words, p.s1_n, p.s1_w);
   const rsrc_t rX = make_rsrc(p.x, (uint32_t)(((p.T - 1) * p.ldx + p.H) * 2));
   const int rl = lane >> 3, cp = lane & 7;
   const uint32_t vo0 = (uint32_t)(rl * row_bytes + (cp ^ (rl >> 1)) * 16), vo1 = (uint32_t)((rl + 8) * row_bytes + (cp ^ (4 + (rl >> 1))) * 16);
-  const uint32_t voS = (uint32_t)(r * p.s1_n * 4), up_rows = (uint32_t)(p.I * row_bytes), up_scales = (uint32_t)(p.I * p.s1_n * 4);
+  const uint32_t up_rows = (uint32_t)(p.I * row_bytes);
+  // scale words of a block: lanes 0 .. 15 word 0 of the gate rows, then word 1, then those of the up rows
+  const uint32_t voS = (uint32_t)((r + (kq >> 1) * p.I) * p.s1_n * 4);
   uint8_t* const own = smem + w * kWave;
   const MxCodes codes(lane);
 
-  // a position in the wave's list of work: strips, tiles of a strip, blocks of a tile
-  struct At { int strip, tile, i; };
-  auto advance = [&](At& a) {
-    if (++a.i < nb) return;
-    a.i = 0;
-    if (++a.tile < ntiles) return;
-    a.tile = 0;
-    ++a.strip;
-  };
-  auto row_of = [&](int tile) -> uint32_t {  // byte offset of the activations of the lane's slot
-    const int k = tile * 16 + r;
-    return k < total ? (uint32_t)((list[k] / p.topk) * p.ldx * 2) + kq * 16 : kOutOfRange;
-  };
-  uint32_t sc[2][4];
-  v4i x[8];
-  At ahead{0, 0, 0}, now{0, 0, 0};
-  uint32_t xrow = row_of(0);
-  auto request_x = [&](const At& a, int j) __attribute__((always_inline)) {
-    const int k = (w + 8 * a.i) * kMxStep + j * 32;
-    x[j] = buf_load16(rX, xrow != kOutOfRange && k + kq * 8 < p.H ? xrow + (uint32_t)k * 2 : kOutOfRange);
-  };
-  auto request = [&](int slot) __attribute__((always_inline)) {  // what `ahead` stands at; behind the end nothing is in range
-    const bool in = ahead.strip < nstrips;
-    const int kb = w + 8 * ahead.i, c0 = (strip0 + ahead.strip) * 16;
-    const uint32_t ko = (uint32_t)kb * kMxStepBytes + (uint32_t)(c0 * row_bytes);
-    const uint32_t so = voS + (uint32_t)(c0 * p.s1_n * 4);
+  // ---- requests: the wave's blocks of a tile, the tiles of a strip, the strips of the run
+  int ri = 0, rtile = 0, rstrip = 0;
+  uint32_t xoff[RX / 2];  // of the activations that the lane fetches: two slots a load, 16-byte piece c of slot i at position c ^ (4 (i & 3))
+  auto rows_of = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const uint32_t wo = (uint32_t)min(2 * kb + j, words - 1) * (uint32_t)(p.s1_w * 4);
-      sc[slot][j] = buf_load4(rS, in ? so + wo : kOutOfRange);
-      sc[slot][2 + j] = buf_load4(rS, in ? so + up_scales + wo : kOutOfRange);
+    for (int i = 0; i < RX / 2; ++i) {
+      const int row = 2 * i + (lane >> 5), k = tile * RX + row;
+      xoff[i] = k < total ? (uint32_t)((list[k] / p.topk) * p.ldx * 2) + (((lane & 31) ^ ((row & 3) << 2)) << 4) : kOutOfRange;
     }
+  };
+  rows_of(0);
+  auto request = [&](int slot) __attribute__((always_inline)) {
+    const bool in = rstrip < nstrips;  // behind the end nothing is in range
+    const int kb = w + NW * ri, c0 = (strip0 + rstrip) * 16;
+    const uint32_t ko = in ? (uint32_t)kb * kMxStepBytes + (uint32_t)(c0 * row_bytes) : kOutOfRange;
     uint8_t* const to = own + slot * kSlot;
     buf_load16_to_lds<true>(rW, in ? vo0 + ko : kOutOfRange, 0, to);
     buf_load16_to_lds<true>(rW, in ? vo1 + ko : kOutOfRange, 0, to + 1024);
-    buf_load16_to_lds<true>(rW, in ? vo0 + ko + up_rows : kOutOfRange, 0, to + 2048);
-    buf_load16_to_lds<true>(rW, in ? vo1 + ko + up_rows : kOutOfRange, 0, to + 3072);
+    buf_load16_to_lds<true>(rW, in ? vo0 + (ko + up_rows) : kOutOfRange, 0, to + 2048);
+    buf_load16_to_lds<true>(rW, in ? vo1 + (ko + up_rows) : kOutOfRange, 0, to + 3072);
+#pragma unroll
+    for (int i = 0; i < RX / 2; ++i) {
+      const int row = 2 * i + (lane >> 5), k = kb * kMxStep + ((lane & 31) ^ ((row & 3) << 2)) * 8;
+      buf_load16_to_lds(rX, in && xoff[i] != kOutOfRange && k < p.H ? xoff[i] + (uint32_t)(kb * kMxStep * 2) : kOutOfRange, 0, to + kX + i * 1024);
+    }
+    buf_load4_to_lds(rS, in ? voS + (uint32_t)(c0 * p.s1_n * 4) + (uint32_t)min(2 * kb + (kq & 1), words - 1) * (uint32_t)(p.s1_w * 4) : kOutOfRange, 0, to + kS);
     SB();
-    if (in) advance(ahead);
+    if (++ri >= nb && in) {
+      ri = 0;
+      if (++rtile == ntiles) { rtile = 0; ++rstrip; }
+      if (ntiles > 1) rows_of(rtile);
+    }
   };
 
   v4f ag = {0.f, 0.f, 0.f, 0.f}, au = {0.f, 0.f, 0.f, 0.f};
+  const uint32_t xrd = (uint32_t)(kX + (r & (RX - 1)) * 512);
+  const int xkey = (r & 3) << 2;
   auto block = [&](int slot) __attribute__((always_inline)) {
-    wait_vm<kOps>();  // younger than the block's activations: the lines of the block behind this one
+    wait_vm<(ST - 1) * kLoads>();
     const uint8_t* const from = own + slot * kSlot;
-    uint32_t cg[8], cu[8];
+    uint32_t s[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) { cg[j] = codes.get(from, j); cu[j] = codes.get(from + 2048, j); }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every code is out of its slot
-    At next = now;
-    advance(next);
-    if (next.tile != now.tile) xrow = row_of(next.tile);
+    for (int k = 0; k < 4; ++k) s[k] = *reinterpret_cast<const uint32_t*>(from + kS + k * 64 + r * 4);
+    uint32_t cg[8], cu[8];
+    v4i x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      ag = mx_mac<DT>(ag, x[j], cg[j], mx_block_scale(sc[slot][0], sc[slot][1], j));
-      au = mx_mac<DT>(au, x[j], cu[j], mx_block_scale(sc[slot][2], sc[slot][3], j));
-      request_x(next, j);  // of the block behind this one
-      SB();
+      x[j] = *reinterpret_cast<const v4i*>(from + xrd + (((j * 4 + kq) ^ xkey) << 4));
+      cg[j] = codes.get(from, j);
+      cu[j] = codes.get(from + 2048, j);
     }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // everything is out of its slot
+    SB();
     request(slot);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      ag = mx_mac<DT>(ag, x[j], cg[j], mx_block_scale<DT>(s[0], s[1], j));
+      au = mx_mac<DT>(au, x[j], cu[j], mx_block_scale<DT>(s[2], s[3], j));
+      if (DT != FP8K_BF16) SB();
+    }
+    SB();
   };
   // the sums of a tile of a strip
-  auto finish = [&](int strip, int tile) {
-    if (w < 7) {
+  auto finish = [&](int strip, int tile) __attribute__((always_inline)) {
+    if (w < NW - 1) {
       red[w][0][lane] = ag;
       red[w][1][lane] = au;
     }
     lds_barrier();  // requests stay in flight
-    if (w == 7) {
+    if (w == NW - 1) {
       v4f g = red[0][0][lane], u = red[0][1][lane];
-#pragma unroll 1
-      for (int k = 1; k < 7; ++k) {
-        const v4f a = red[k][0][lane], b = red[k][1][lane];
+#pragma unroll
+      for (int k = 1; k < NW; ++k) {
+        const v4f a = k < NW - 1 ? red[k < NW - 1 ? k : 0][0][lane] : ag, b = k < NW - 1 ? red[k < NW - 1 ? k : 0][1][lane] : au;
 #pragma unroll
         for (int i = 0; i < 4; ++i) { g[i] += a[i]; u[i] += b[i]; }
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { g[i] += ag[i]; u[i] += au[i]; }
-#pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int k = tile * 16 + kq * 4 + i;
-        if (k >= total) continue;
+        const int row = kq * 4 + i, k = tile * RX + row;
+        if (row >= RX || k >= total) continue;
         const int s = list[k];
         if (p.on_input) {
           g[i] *= p.topk_w[s];
@@ -329,20 +342,20 @@ __global__ __launch_bounds__(512, 4) void mx_experts_up_kernel(const MxExpertArg
     for (int k = 0; k < nstrips * ntiles; ++k) finish(k / ntiles, k % ntiles);
     return;
   }
-  request(0);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) request_x(now, j);
-  SB();
-  request(1);
+  for (int s = 0; s < ST; ++s) request(s);
   const int all = nstrips * ntiles * nb;
-  for (int q = 0; q < all; q += 2) {
+  int ci = 0, ctile = 0, cstrip = 0;
+  for (int q = 0; q < all; q += ST) {
 #pragma unroll
-    for (int slot = 0; slot < 2; ++slot) {
+    for (int slot = 0; slot < ST; ++slot) {
       if (q + slot >= all) break;
-      const At at = now;
       block(slot);
-      advance(now);
-      if (now.i == 0) finish(at.strip, at.tile);
+      if (++ci == nb) {
+        finish(cstrip, ctile);
+        ci = 0;
+        if (++ctile == ntiles) { ctile = 0; ++cstrip; }
+      }
     }
   }
   wait_vm0();  // requests behind the end moved nothing, but still point at the slots
@@ -351,17 +364,29 @@ __global__ __launch_bounds__(512, 4) void mx_experts_up_kernel(const MxExpertArg
 // ------------------------------------------------------------------------------------------------
 // Second launch, grid H / 16: a workgroup owns 16 output columns and goes through all tiles of the table.  The K blocks of all tiles are
 // one list, which the waves share out in runs; a wave adds a tile's results, times the routed weights, to sums of its own in LDS ([T][16]
-// floats), and the eight sets are added in order at the end: no atomics between waves, so results do not depend on timing.
-// Lines go to LDS slots of the wave ST blocks ahead, the activations to registers two blocks ahead.
+// floats), and the sets are added in order at the end: no atomics between waves, so results do not depend on timing.
+//
+// Everything a K block needs - the lines of 16 weight rows, their scale words, the activations of the tile's RX slots - goes straight to
+// an LDS slot of the wave, ST blocks ahead, and no other load stands in the loop.  (Activations in operand form straight to registers:
+// eight loads a block of which a few lanes are used, 28 us against 62 MB; and as loads retire in order, waiting for them drained the
+// lines behind them.)
 // ------------------------------------------------------------------------------------------------
-constexpr int mx_down_slots(int tc) { return tc <= 16 ? 4 : 2; }       // K blocks in flight per wave
 constexpr int mx_down_places(int tc) { return tc <= 16 ? 512 : kMxMaxSlots; }  // (token, choice) pairs
+constexpr int mx_down_slot(int rx) { return 2048 + rx * 512 + 128; }
+constexpr int mx_down_fixed(int tc, int waves) { return waves * tc * 64 + mx_down_places(tc) * 10; }
+// K blocks in flight per wave: what 160 KB (eight waves) or half of it (four: two workgroups to a CU) have room for, four at most
+constexpr int mx_down_stages(int tc, int rx, int waves) {
+  const int st = (waves * 20480 - mx_down_fixed(tc, waves)) / (waves * mx_down_slot(rx));
+  return st > 4 ? 4 : st;
+}
 
-template <int DT, int TC>  // TC: tokens that the sums have room for
-__global__ __launch_bounds__(512, 4) void mx_experts_down_kernel(const MxExpertArgs p) {
-  constexpr int ST = mx_down_slots(TC), kWave = ST * 2048;
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[8 * kWave];
-  __shared__ __attribute__((aligned(16))) float sums[8 * TC * 16];  // [8][T][16]
+template <int DT, int TC, int RX, int NW>  // TC: tokens that the sums have room for; RX: slots of a tile; NW: waves
+__global__ __launch_bounds__(NW * 64, 2) void mx_experts_down_kernel(const MxExpertArgs p) {
+  constexpr int ST = mx_down_stages(TC, RX, NW), kSlot = mx_down_slot(RX), kWave = ST * kSlot, kX = 2048, kS = 2048 + RX * 512;
+  constexpr int kLoads = 3 + RX / 2;  // of a wave per K block
+  static_assert(ST >= 1, "no room");
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[NW * kWave];
+  __shared__ __attribute__((aligned(16))) float sums[NW * TC * 16];  // [NW][T][16]
   __shared__ int tiles[mx_down_places(TC)];
   __shared__ float weights[mx_down_places(TC)];
   __shared__ u16 order[mx_down_places(TC)];
@@ -373,7 +398,7 @@ __global__ __launch_bounds__(512, 4) void mx_experts_down_kernel(const MxExpertA
   float* const mine = sums + w * p.T * 16;
 
   const int ntiles = p.ntiles[0];
-  for (int i = tid; i < p.slots; i += 512) {  // what lies behind the tiles and valid slots is not read below
+  for (int i = tid; i < p.slots; i += NW * 64) {  // what lies behind the tiles and the valid slots is not used below
     tiles[i] = p.tiles[i];
     order[i] = (u16)p.order[i];
     weights[i] = p.on_input ? 1.f : p.weights[i];
@@ -382,8 +407,8 @@ __global__ __launch_bounds__(512, 4) void mx_experts_down_kernel(const MxExpertA
   __syncthreads();
 
   const int row_bytes = p.I >> 1, words = (p.I + 127) >> 7, kbs = (p.I + kMxStep - 1) / kMxStep;
-  const int all = ntiles * kbs, per = (all + 7) >> 3;
-  const int b0 = w * per, b1 = min(all, b0 + per);
+  const int all = ntiles * kbs, per = (all + NW - 1) / NW;
+  const int b0 = w * per, nb = max(min(all, b0 + per) - b0, 0);
   const rsrc_t rH = make_rsrc(p.h, (uint32_t)((int64_t)p.slots * p.I * 2));
   const int rl = lane >> 3, cp = lane & 7;
   const uint32_t vo0 = (uint32_t)((n0 + rl) * row_bytes + (cp ^ (rl >> 1)) * 16), vo1 = (uint32_t)((n0 + rl + 8) * row_bytes + (cp ^ (4 + (rl >> 1))) * 16);
@@ -391,93 +416,83 @@ __global__ __launch_bounds__(512, 4) void mx_experts_down_kernel(const MxExpertA
   uint8_t* const own = smem + w * kWave;
   const MxCodes codes(lane);
 
-  struct At { int tile, kb; };
-  auto entry = [&](int tile) { return __builtin_amdgcn_readfirstlane(tiles[min(tile, ntiles - 1)]); };
-  auto advance = [&](At& a) {
-    if (++a.kb == kbs) { a.kb = 0; ++a.tile; }
-  };
-  // lines of block `wa` into slot `slot`, its scale words into sc[slot]
-  uint32_t sc[ST][2];
-  auto request_w = [&](int slot, At& a, int left) __attribute__((always_inline)) {
-    const bool in = left > 0;
-    const int64_t e = entry(a.tile) >> 14;
-    const rsrc_t rW = make_rsrc(p.w2 + e * p.w2_e, (uint32_t)(p.H * row_bytes));
-    const rsrc_t rS = mx_scale_rsrc(p.s2 + e * p.s2_e * 4, 0, p.H, words, p.s2_n, p.s2_w);
-    const uint32_t ko = (uint32_t)a.kb * kMxStepBytes;
+  // ---- requests: block by block through the wave's run
+  int rt = 0, rkb = 0, left = nb;  // tile, its K block, blocks to come
+  auto request = [&](int slot) __attribute__((always_inline)) {
+    const int t = __builtin_amdgcn_readfirstlane(tiles[min(rt, ntiles - 1)]);
+    const int64_t e = t >> 14;
+    const int first = (t >> 4) & 1023, count = (t & 15) + 1;
+    const bool in = left > 0;  // behind the end nothing is in range
+    const rsrc_t rW = make_rsrc(p.w2 + e * p.w2_e, in ? (uint32_t)(p.H * row_bytes) : 0u);
+    const rsrc_t rS = mx_scale_rsrc(p.s2 + e * p.s2_e * 4, 0, in ? p.H : 0, words, p.s2_n, p.s2_w);
+    uint8_t* const to = own + slot * kSlot;
+    const uint32_t ko = (uint32_t)rkb * kMxStepBytes;
+    buf_load16_to_lds<true>(rW, vo0 + ko, 0, to);
+    buf_load16_to_lds<true>(rW, vo1 + ko, 0, to + 1024);
+    // activations: two slots' 256 values a load; 16-byte piece c of slot i at position c ^ (4 (i & 3)), so that the operand reads of
+    // different slots fall into different banks
 #pragma unroll
-    for (int j = 0; j < 2; ++j) sc[slot][j] = buf_load4(rS, in ? voS + (uint32_t)min(2 * a.kb + j, words - 1) * (uint32_t)(p.s2_w * 4) : kOutOfRange);
-    buf_load16_to_lds<true>(rW, in ? vo0 + ko : kOutOfRange, 0, own + slot * 2048);
-    buf_load16_to_lds<true>(rW, in ? vo1 + ko : kOutOfRange, 0, own + slot * 2048 + 1024);
-    SB();
-    advance(a);
-  };
-  v4i x[2][8];
-  auto request_x = [&](int slot, At& a, int left) __attribute__((always_inline)) {
-    const int t = entry(a.tile), first = (t >> 4) & 1023, count = left > 0 ? (t & 15) + 1 : 0;
-    const uint32_t row = r < count ? (uint32_t)order[first + r] * (uint32_t)(p.I * 2) + kq * 16 : kOutOfRange;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int k = a.kb * kMxStep + j * 32;
-      x[slot][j] = buf_load16(rH, r < count && k + kq * 8 < p.I ? row + (uint32_t)k * 2 : kOutOfRange);
+    for (int i = 0; i < RX; i += 2) {
+      const int row = i + (lane >> 5), piece = (lane & 31) ^ ((row & 3) << 2), k = rkb * kMxStep + piece * 8;
+      const uint32_t off = (uint32_t)order[min(first + row, p.slots - 1)] * (uint32_t)(p.I * 2) + (uint32_t)k * 2;
+      buf_load16_to_lds(rH, in && row < count && k < p.I ? off : kOutOfRange, 0, to + kX + i * 512);
     }
+    if (lane < 32)  // scale words 0 and 1 of the 16 rows
+      buf_load4_to_lds(rS, voS + (uint32_t)min(2 * rkb + kq, words - 1) * (uint32_t)(p.s2_w * 4), 0, to + kS);
     SB();
-    advance(a);
+    --left;
+    if (++rkb == kbs) { rkb = 0; ++rt; }
   };
+
   v4f acc = {0.f, 0.f, 0.f, 0.f};
-  At now{0, 0};
-  if (b0 < b1) {
-    now = At{b0 / kbs, b0 % kbs};
-    At wa = now, xa = now;
-    int wleft = b1 - b0, xleft = wleft;
-    // the order of the loop: a block's activations, then the lines of the block ST - 2 behind it
+  if (nb > 0) {
+    rt = b0 / kbs;
+    rkb = b0 - rt * kbs;
+    int ct = rt, ckb = rkb;
 #pragma unroll
-    for (int s = 0; s < ST - 2; ++s) request_w(s, wa, wleft--);
-    request_x(0, xa, xleft--);
-    request_w(ST - 2, wa, wleft--);
-    request_x(1, xa, xleft--);
-    request_w(ST - 1, wa, wleft--);
-    auto block = [&](int ws, int xs, bool last) __attribute__((always_inline)) {
-      // younger than the block's activations and lines: the next block's activations, and the lines behind the two
-      wait_vm<(ST > 2 ? 16 : 12)>();
-      const uint8_t* const from = own + ws * 2048;
-      uint32_t c[8];
+    for (int s = 0; s < ST; ++s) request(s);
+    const uint32_t xrd = (uint32_t)(kX + (r & (RX - 1)) * 512);
+    const int xkey = (r & 3) << 2;
+    for (int b = 0; b < nb; b += ST) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) c[j] = codes.get(from, j);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // every code is out of its slot
+      for (int s = 0; s < ST; ++s) {
+        if (b + s >= nb) break;
+        wait_vm<(ST - 1) * kLoads>();
+        const uint8_t* const from = own + s * kSlot;
+        uint32_t c[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        acc = mx_mac<DT>(acc, x[xs][j], c[j], mx_block_scale(sc[ws][0], sc[ws][1], j));
+        for (int j = 0; j < 8; ++j) c[j] = codes.get(from, j);
+        const uint32_t s0 = *reinterpret_cast<const uint32_t*>(from + kS + r * 4), s1 = *reinterpret_cast<const uint32_t*>(from + kS + 64 + r * 4);
+        v4i x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const v4i*>(from + xrd + (((j * 4 + kq) ^ xkey) << 4));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // everything is out of its slot
         SB();
-      }
-      request_x(xs, xa, xleft--);
-      request_w(ws, wa, wleft--);
-      const At at = now;
-      advance(now);
-      if (now.kb == 0 || last) {
-        const int t = entry(at.tile), first = (t >> 4) & 1023, count = (t & 15) + 1;
+        request(s);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = kq * 4 + i;
-          // two slots of a tile may be of one token: an LDS atomic, whose order within the wave is fixed
-          if (row < count) atomicAdd(&mine[(order[first + row] / p.topk) * 16 + r], acc[i] * weights[first + row]);
-          acc[i] = 0.f;
+        for (int j = 0; j < 8; ++j) acc = mx_mac<DT>(acc, x[j], c[j], mx_block_scale<DT>(s0, s1, j));
+        SB();
+        if (++ckb == kbs || b + s == nb - 1) {
+          const int t = __builtin_amdgcn_readfirstlane(tiles[ct]), first = (t >> 4) & 1023, count = (t & 15) + 1;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = kq * 4 + i;
+            // two slots of a tile may be of one token: an LDS atomic, whose order within the wave is fixed
+            if (row < count) atomicAdd(&mine[(order[first + row] / p.topk) * 16 + r], acc[i] * weights[first + row]);
+            acc[i] = 0.f;
+          }
+          ckb = 0;
+          ++ct;
         }
-      }
-    };
-    for (int b = b0; b < b1; b += ST) {
-#pragma unroll
-      for (int k = 0; k < ST; ++k) {
-        if (b + k >= b1) break;
-        block(k, k & 1, b + k == b1 - 1);
       }
     }
   }
   wait_vm0();
   __syncthreads();
-  for (int i = tid; i < p.T * 16; i += 512) {
+  for (int i = tid; i < p.T * 16; i += NW * 64) {
     float v = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v += sums[k * p.T * 16 + i];
+    for (int k = 0; k < NW; ++k) v += sums[k * p.T * 16 + i];
     v *= p.scaling;
     ((u16*)p.out)[(int64_t)(i >> 4) * p.H + n0 + (i & 15)] = (u16)(DT == FP8K_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v));
   }

@@ -435,17 +435,34 @@ extern "C" int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2,
   const int64_t units = std::min(slots, E), strips = I / 16;
   p.run = (int)std::min<int64_t>(8, std::max<int64_t>(1, units * strips / (2 * num_cu())));
   const dim3 grid1((unsigned)((strips + p.run - 1) / p.run + 1), (unsigned)units), grid2((unsigned)(H / 16));
-#define MX_EXPERTS(DT)                                                                       \
-  do {                                                                                       \
-    if (gelu) mx_experts_up_kernel<DT, true><<<grid1, 512, 0, st>>>(p);                      \
-    else mx_experts_up_kernel<DT, false><<<grid1, 512, 0, st>>>(p);                          \
-    if (const int rc = check_launch("mxfp4 experts")) return rc;                             \
-    if (T <= 16 && slots <= mx_down_places(16)) mx_experts_down_kernel<DT, 16><<<grid2, 512, 0, st>>>(p);                   \
-    else if (T <= 64) mx_experts_down_kernel<DT, 64><<<grid2, 512, 0, st>>>(p);              \
-    else mx_experts_down_kernel<DT, kMxMaxTokens><<<grid2, 512, 0, st>>>(p);                 \
+  // tiles of 4 slots while an expert has no more on average
+  p.tile = slots <= 4 * units ? 4 : 16;
+  // more strips than CUs: workgroups of four waves, two of which share a CU
+  const bool narrow = H > 16 * num_cu();
+#define MX_DOWN(DT, TC)                                                                                   \
+  do {                                                                                                    \
+    if (p.tile == 4 && narrow) mx_experts_down_kernel<DT, TC, 4, 4><<<grid2, 256, 0, st>>>(p);            \
+    else if (p.tile == 4) mx_experts_down_kernel<DT, TC, 4, 8><<<grid2, 512, 0, st>>>(p);                 \
+    else mx_experts_down_kernel<DT, TC, 16, 8><<<grid2, 512, 0, st>>>(p);                                 \
+  } while (0)
+#define MX_UP(DT, RX)                                                             \
+  do {                                                                            \
+    if (gelu) mx_experts_up_kernel<DT, true, RX><<<grid1, 256, 0, st>>>(p);       \
+    else mx_experts_up_kernel<DT, false, RX><<<grid1, 256, 0, st>>>(p);           \
+  } while (0)
+#define MX_EXPERTS(DT)                                                     \
+  do {                                                                     \
+    if (p.tile == 4) MX_UP(DT, 4);                                         \
+    else MX_UP(DT, 16);                                                    \
+    if (const int rc = check_launch("mxfp4 experts")) return rc;           \
+    if (T <= 16 && slots <= mx_down_places(16)) MX_DOWN(DT, 16);           \
+    else if (T <= 64) MX_DOWN(DT, 64);                                     \
+    else MX_DOWN(DT, kMxMaxTokens);                                        \
   } while (0)
   if (dtype == FP8K_BF16) MX_EXPERTS(FP8K_BF16);
   else MX_EXPERTS(FP8K_F16);
 #undef MX_EXPERTS
+#undef MX_UP
+#undef MX_DOWN
   return check_launch("mxfp4 experts");
 }
