@@ -101,7 +101,7 @@ __device__ __forceinline__ float mx_block_scale(uint32_t lo, uint32_t hi, int j)
 }
 
 // The table of the second launch: slots sorted by expert (and by their number within one), cut into tiles of up to p.tile slots of one
-// expert.  One workgroup of 256 threads; keys, sorted: LDS for kMxMaxSlots words, aux: for 32.
+// expert.  One workgroup of 256 threads; keys, sorted: LDS for kMxMaxSlots words, aux: for 33.
 __device__ __forceinline__ void mx_sort_slots(const MxExpertArgs& p, int* keys, int* sorted, int* aux) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   constexpr int kNone = 0x7fffffff;
@@ -112,9 +112,10 @@ __device__ __forceinline__ void mx_sort_slots(const MxExpertArgs& p, int* keys, 
     keys[s] = e < 0 ? kNone : (e << 10) | s;
   }
   if (tid < 16) aux[tid] = -1;
+  if (tid == 32) aux[tid] = 0;
   __syncthreads();
   // a key's place is the number of smaller ones
-  int valid = 0;
+  int own = 0;
   for (int s = tid; s < padded; s += NT) {
     const int key = keys[s];
     int at = 0;
@@ -124,17 +125,15 @@ __device__ __forceinline__ void mx_sort_slots(const MxExpertArgs& p, int* keys, 
       at += (k.x < key) + (k.y < key) + (k.z < key) + (k.w < key);
     }
     if (key != kNone) {
+      ++own;
       sorted[at] = key;
       p.order[at] = s;
       p.weights[at] = p.topk_w[s];
     }
   }
-#pragma unroll 4
-  for (int o = 0; o < padded; o += 4) {
-    const int4 k = *reinterpret_cast<const int4*>(keys + o);
-    valid += (k.x != kNone) + (k.y != kNone) + (k.z != kNone) + (k.w != kNone);
-  }
+  atomicAdd(&aux[32], own);
   __syncthreads();
+  const int valid = aux[32];
   // places 64 (4 j + w) + lane: the first of an expert; a place's rank is its distance to the last of those at or before it
   const uint64_t upto = (2ull << lane) - 1;
   uint64_t heads[J], starts[J];
@@ -178,21 +177,20 @@ __device__ __forceinline__ void mx_sort_slots(const MxExpertArgs& p, int* keys, 
 //
 // A workgroup takes a run of strips of 16 columns of h: 16 gate and 16 up rows, all of K, for the expert's slots, RX at a time.  Its four
 // waves take every fourth K block each.  What a block needs - the lines of 32 rows, their scale words, the slots' activations - goes
-// straight to an LDS slot of the wave, two blocks ahead and on across the strips of the run, and no other load stands in the loop.  The
-// four sums meet in LDS; the last wave, which has the fewest blocks, adds them up, applies the activation and writes h, while the
-// others go on.
-// Bound: the weights' bytes.  With RX = 4 two workgroups share a CU.
+// straight to an LDS slot of the wave, requested as soon as the operands of the block before are out of it and on across the strips of
+// the run, and no other load stands in the loop.  The four sums meet in LDS; the last wave, which has the fewest blocks, adds them up,
+// applies the activation and writes h, while the others go on.
+// Bound: the weights' bytes.  One slot to a wave and four workgroups to a CU (RX = 4) beat two slots and two workgroups: 626 against
+// 645 us (64 tokens, 256 experts of 7168 x 2048), 21.0 against 28 (13 tokens, 128 of 4096 x 256): the conversions of one wave run
+// while another waits.
 // ------------------------------------------------------------------------------------------------
-constexpr int mx_up_slot(int rx) { return 4096 + rx * 512 + 256; }
-
 template <int DT, bool GELU, int RX>
-__global__ __launch_bounds__(256, 2) void mx_experts_up_kernel(const MxExpertArgs p) {
-  constexpr int NW = 4, ST = 2, kSlot = mx_up_slot(RX), kWave = ST * kSlot, kX = 4096, kS = 4096 + RX * 512;
-  constexpr int kLoads = 5 + RX / 2;  // of a wave per K block
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[NW * kWave];
+__global__ __launch_bounds__(256, RX == 4 ? 4 : 2) void mx_experts_up_kernel(const MxExpertArgs p) {
+  constexpr int NW = 4, kSlot = 4096 + RX * 512 + 256, kX = 4096, kS = 4096 + RX * 512;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[NW * kSlot];
   __shared__ __attribute__((aligned(16))) v4f red[NW - 1][2][64];
   __shared__ u16 list[kMxMaxSlots];
-  static_assert(sizeof(smem) >= (2 * kMxMaxSlots + 32) * 4, "the sort works where the slots are");
+  static_assert(sizeof(smem) >= (2 * kMxMaxSlots + 33) * 4, "the sort works where the slots are");
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -241,7 +239,7 @@ __global__ __launch_bounds__(256, 2) void mx_experts_up_kernel(const MxExpertArg
   const uint32_t up_rows = (uint32_t)(p.I * row_bytes);
   // scale words of a block: lanes 0 .. 15 word 0 of the gate rows, then word 1, then those of the up rows
   const uint32_t voS = (uint32_t)((r + (kq >> 1) * p.I) * p.s1_n * 4);
-  uint8_t* const own = smem + w * kWave;
+  uint8_t* const own = smem + w * kSlot;
   const MxCodes codes(lane);
 
   // ---- requests: the wave's blocks of a tile, the tiles of a strip, the strips of the run
@@ -255,23 +253,21 @@ __global__ __launch_bounds__(256, 2) void mx_experts_up_kernel(const MxExpertArg
     }
   };
   rows_of(0);
-  auto request = [&](int slot) __attribute__((always_inline)) {
-    const bool in = rstrip < nstrips;  // behind the end nothing is in range
+  auto request = [&] __attribute__((always_inline)) {
     const int kb = w + NW * ri, c0 = (strip0 + rstrip) * 16;
-    const uint32_t ko = in ? (uint32_t)kb * kMxStepBytes + (uint32_t)(c0 * row_bytes) : kOutOfRange;
-    uint8_t* const to = own + slot * kSlot;
-    buf_load16_to_lds<true>(rW, in ? vo0 + ko : kOutOfRange, 0, to);
-    buf_load16_to_lds<true>(rW, in ? vo1 + ko : kOutOfRange, 0, to + 1024);
-    buf_load16_to_lds<true>(rW, in ? vo0 + (ko + up_rows) : kOutOfRange, 0, to + 2048);
-    buf_load16_to_lds<true>(rW, in ? vo1 + (ko + up_rows) : kOutOfRange, 0, to + 3072);
+    const uint32_t ko = (uint32_t)kb * kMxStepBytes + (uint32_t)(c0 * row_bytes);
+    buf_load16_to_lds<true>(rW, vo0 + ko, 0, own);
+    buf_load16_to_lds<true>(rW, vo1 + ko, 0, own + 1024);
+    buf_load16_to_lds<true>(rW, vo0 + (ko + up_rows), 0, own + 2048);
+    buf_load16_to_lds<true>(rW, vo1 + (ko + up_rows), 0, own + 3072);
 #pragma unroll
     for (int i = 0; i < RX / 2; ++i) {
       const int row = 2 * i + (lane >> 5), k = kb * kMxStep + ((lane & 31) ^ ((row & 3) << 2)) * 8;
-      buf_load16_to_lds(rX, in && xoff[i] != kOutOfRange && k < p.H ? xoff[i] + (uint32_t)(kb * kMxStep * 2) : kOutOfRange, 0, to + kX + i * 1024);
+      buf_load16_to_lds(rX, xoff[i] != kOutOfRange && k < p.H ? xoff[i] + (uint32_t)(kb * kMxStep * 2) : kOutOfRange, 0, own + kX + i * 1024);
     }
-    buf_load4_to_lds(rS, in ? voS + (uint32_t)(c0 * p.s1_n * 4) + (uint32_t)min(2 * kb + (kq & 1), words - 1) * (uint32_t)(p.s1_w * 4) : kOutOfRange, 0, to + kS);
+    buf_load4_to_lds(rS, voS + (uint32_t)(c0 * p.s1_n * 4) + (uint32_t)min(2 * kb + (kq & 1), words - 1) * (uint32_t)(p.s1_w * 4), 0, own + kS);
     SB();
-    if (++ri >= nb && in) {
+    if (++ri == nb) {
       ri = 0;
       if (++rtile == ntiles) { rtile = 0; ++rstrip; }
       if (ntiles > 1) rows_of(rtile);
@@ -281,23 +277,22 @@ __global__ __launch_bounds__(256, 2) void mx_experts_up_kernel(const MxExpertArg
   v4f ag = {0.f, 0.f, 0.f, 0.f}, au = {0.f, 0.f, 0.f, 0.f};
   const uint32_t xrd = (uint32_t)(kX + (r & (RX - 1)) * 512);
   const int xkey = (r & 3) << 2;
-  auto block = [&](int slot) __attribute__((always_inline)) {
-    wait_vm<(ST - 1) * kLoads>();
-    const uint8_t* const from = own + slot * kSlot;
+  auto block = [&](bool more) __attribute__((always_inline)) {
+    wait_vm<0>();
     uint32_t s[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) s[k] = *reinterpret_cast<const uint32_t*>(from + kS + k * 64 + r * 4);
+    for (int k = 0; k < 4; ++k) s[k] = *reinterpret_cast<const uint32_t*>(own + kS + k * 64 + r * 4);
     uint32_t cg[8], cu[8];
     v4i x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      x[j] = *reinterpret_cast<const v4i*>(from + xrd + (((j * 4 + kq) ^ xkey) << 4));
-      cg[j] = codes.get(from, j);
-      cu[j] = codes.get(from + 2048, j);
+      x[j] = *reinterpret_cast<const v4i*>(own + xrd + (((j * 4 + kq) ^ xkey) << 4));
+      cg[j] = codes.get(own, j);
+      cu[j] = codes.get(own + 2048, j);
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // everything is out of its slot
     SB();
-    request(slot);
+    if (more) request();
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       ag = mx_mac<DT>(ag, x[j], cg[j], mx_block_scale<DT>(s[0], s[1], j));
@@ -342,23 +337,17 @@ __global__ __launch_bounds__(256, 2) void mx_experts_up_kernel(const MxExpertArg
     for (int k = 0; k < nstrips * ntiles; ++k) finish(k / ntiles, k % ntiles);
     return;
   }
-#pragma unroll
-  for (int s = 0; s < ST; ++s) request(s);
+  request();
   const int all = nstrips * ntiles * nb;
   int ci = 0, ctile = 0, cstrip = 0;
-  for (int q = 0; q < all; q += ST) {
-#pragma unroll
-    for (int slot = 0; slot < ST; ++slot) {
-      if (q + slot >= all) break;
-      block(slot);
-      if (++ci == nb) {
-        finish(cstrip, ctile);
-        ci = 0;
-        if (++ctile == ntiles) { ctile = 0; ++cstrip; }
-      }
+  for (int q = 0; q < all; ++q) {
+    block(q + 1 < all);
+    if (++ci == nb) {
+      finish(cstrip, ctile);
+      ci = 0;
+      if (++ctile == ntiles) { ctile = 0; ++cstrip; }
     }
   }
-  wait_vm0();  // requests behind the end moved nothing, but still point at the slots
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -367,29 +356,24 @@ __global__ __launch_bounds__(256, 2) void mx_experts_up_kernel(const MxExpertArg
 // floats), and the sets are added in order at the end: no atomics between waves, so results do not depend on timing.
 //
 // Everything a K block needs - the lines of 16 weight rows, their scale words, the activations of the tile's RX slots - goes straight to
-// an LDS slot of the wave, ST blocks ahead, and no other load stands in the loop.  (Activations in operand form straight to registers:
-// eight loads a block of which a few lanes are used, 28 us against 62 MB; and as loads retire in order, waiting for them drained the
-// lines behind them.)
+// the wave's LDS slot, requested as soon as the operands of the block before are out of it, and no other load stands in the loop.
+// (Activations in operand form straight to registers, eight loads a block of which a few lanes are used, took 28 us for the 62 MB of one
+// token where this takes 15.)  Eight waves and two workgroups to a CU beat four waves with three slots each, 363 against 394 us with 64
+// tokens and 256 experts of 7168 x 2048; up to one strip per CU sixteen waves, 13.2 against 14.5 us (13 tokens, 128 of 4096 x 256).
+// Sums of several workgroups per strip, added up by the last one to come, cost more than they balance: a release to the whole device
+// writes its L2 back (13 tokens 16 -> 38 us).
 // ------------------------------------------------------------------------------------------------
 constexpr int mx_down_places(int tc) { return tc <= 16 ? 512 : kMxMaxSlots; }  // (token, choice) pairs
-constexpr int mx_down_slot(int rx) { return 2048 + rx * 512 + 128; }
-constexpr int mx_down_fixed(int tc, int waves) { return waves * tc * 64 + mx_down_places(tc) * 10; }
-// K blocks in flight per wave: what 160 KB (eight waves) or half of it (four: two workgroups to a CU) have room for, four at most
-constexpr int mx_down_stages(int tc, int rx, int waves) {
-  const int st = (waves * 20480 - mx_down_fixed(tc, waves)) / (waves * mx_down_slot(rx));
-  return st > 4 ? 4 : st;
-}
 
 template <int DT, int TC, int RX, int NW>  // TC: tokens that the sums have room for; RX: slots of a tile; NW: waves
-__global__ __launch_bounds__(NW * 64, 2) void mx_experts_down_kernel(const MxExpertArgs p) {
-  constexpr int ST = mx_down_stages(TC, RX, NW), kSlot = mx_down_slot(RX), kWave = ST * kSlot, kX = 2048, kS = 2048 + RX * 512;
-  constexpr int kLoads = 3 + RX / 2;  // of a wave per K block
-  static_assert(ST >= 1, "no room");
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[NW * kWave];
+__global__ __launch_bounds__(NW * 64, RX == 4 && TC <= 64 ? 4 : 2) void mx_experts_down_kernel(const MxExpertArgs p) {
+  constexpr int kSlot = 2048 + RX * 512 + 128, kX = 2048, kS = 2048 + RX * 512;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[NW * kSlot];
   __shared__ __attribute__((aligned(16))) float sums[NW * TC * 16];  // [NW][T][16]
   __shared__ int tiles[mx_down_places(TC)];
   __shared__ float weights[mx_down_places(TC)];
   __shared__ u16 order[mx_down_places(TC)];
+  __shared__ uint8_t token[mx_down_places(TC)];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -400,7 +384,9 @@ __global__ __launch_bounds__(NW * 64, 2) void mx_experts_down_kernel(const MxExp
   const int ntiles = p.ntiles[0];
   for (int i = tid; i < p.slots; i += NW * 64) {  // what lies behind the tiles and the valid slots is not used below
     tiles[i] = p.tiles[i];
-    order[i] = (u16)p.order[i];
+    const int slot = p.order[i];
+    order[i] = (u16)slot;
+    token[i] = (uint8_t)(slot / p.topk);
     weights[i] = p.on_input ? 1.f : p.weights[i];
   }
   for (int i = lane; i < p.T * 16; i += 64) mine[i] = 0.f;
@@ -413,81 +399,112 @@ __global__ __launch_bounds__(NW * 64, 2) void mx_experts_down_kernel(const MxExp
   const int rl = lane >> 3, cp = lane & 7;
   const uint32_t vo0 = (uint32_t)((n0 + rl) * row_bytes + (cp ^ (rl >> 1)) * 16), vo1 = (uint32_t)((n0 + rl + 8) * row_bytes + (cp ^ (4 + (rl >> 1))) * 16);
   const uint32_t voS = (uint32_t)((n0 + r) * p.s2_n * 4);
-  uint8_t* const own = smem + w * kWave;
+  uint8_t* const own = smem + w * kSlot;
   const MxCodes codes(lane);
 
-  // ---- requests: block by block through the wave's run
+  // ---- requests: block by block through the wave's run.  What a tile's requests need is formed when the run comes to it, from its entry
+  // and its slots, which were read from LDS one tile earlier (the entry two): a request never waits for LDS.
   int rt = 0, rkb = 0, left = nb;  // tile, its K block, blocks to come
-  auto request = [&](int slot) __attribute__((always_inline)) {
-    const int t = __builtin_amdgcn_readfirstlane(tiles[min(rt, ntiles - 1)]);
-    const int64_t e = t >> 14;
-    const int first = (t >> 4) & 1023, count = (t & 15) + 1;
-    const bool in = left > 0;  // behind the end nothing is in range
-    const rsrc_t rW = make_rsrc(p.w2 + e * p.w2_e, in ? (uint32_t)(p.H * row_bytes) : 0u);
-    const rsrc_t rS = mx_scale_rsrc(p.s2 + e * p.s2_e * 4, 0, in ? p.H : 0, words, p.s2_n, p.s2_w);
-    uint8_t* const to = own + slot * kSlot;
-    const uint32_t ko = (uint32_t)rkb * kMxStepBytes;
-    buf_load16_to_lds<true>(rW, vo0 + ko, 0, to);
-    buf_load16_to_lds<true>(rW, vo1 + ko, 0, to + 1024);
-    // activations: two slots' 256 values a load; 16-byte piece c of slot i at position c ^ (4 (i & 3)), so that the operand reads of
-    // different slots fall into different banks
+  rsrc_t rW = make_rsrc(p.w2, 0), rS = make_rsrc(p.s2, 0);
+  uint32_t xoff[RX / 2];           // of the activations that the lane fetches; 16-byte piece c of slot i lies at position c ^ (4 (i & 3)),
+  int count = 0;                   // so that the operand reads of different slots fall into different banks
+  int entry1 = 0, entry2 = 0;      // of tiles rt + 1 (here, when it becomes rt) and rt + 2
+  int slots1[RX / 2];
+  auto read_entry = [&](int t) { return tiles[min(t, ntiles - 1)]; };
+  auto read_slots = [&](int entry) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < RX; i += 2) {
-      const int row = i + (lane >> 5), piece = (lane & 31) ^ ((row & 3) << 2), k = rkb * kMxStep + piece * 8;
-      const uint32_t off = (uint32_t)order[min(first + row, p.slots - 1)] * (uint32_t)(p.I * 2) + (uint32_t)k * 2;
-      buf_load16_to_lds(rH, in && row < count && k < p.I ? off : kOutOfRange, 0, to + kX + i * 512);
+    for (int i = 0; i < RX / 2; ++i) slots1[i] = order[min(((entry >> 4) & 1023) + 2 * i + (lane >> 5), p.slots - 1)];
+  };
+  auto enter_tile = [&] __attribute__((always_inline)) {  // entry1 and slots1 are those of tile rt
+    const int t = __builtin_amdgcn_readfirstlane(entry1);
+    const int64_t e = t >> 14;
+    count = (t & 15) + 1;
+    rW = make_rsrc(p.w2 + e * p.w2_e, (uint32_t)(p.H * row_bytes));
+    rS = mx_scale_rsrc(p.s2 + e * p.s2_e * 4, 0, p.H, words, p.s2_n, p.s2_w);
+#pragma unroll
+    for (int i = 0; i < RX / 2; ++i) {
+      const int row = 2 * i + (lane >> 5);
+      xoff[i] = row < count ? (uint32_t)slots1[i] * (uint32_t)(p.I * 2) + (uint32_t)(((lane & 31) ^ ((row & 3) << 2)) * 16) : kOutOfRange;
+    }
+    entry1 = entry2;
+    read_slots(entry2);
+    entry2 = read_entry(rt + 2);
+  };
+  auto request = [&] __attribute__((always_inline)) {
+    const uint32_t ko = (uint32_t)rkb * kMxStepBytes;
+    buf_load16_to_lds<true>(rW, vo0 + ko, 0, own);
+    buf_load16_to_lds<true>(rW, vo1 + ko, 0, own + 1024);
+#pragma unroll
+    for (int i = 0; i < RX / 2; ++i) {
+      const int row = 2 * i + (lane >> 5), k = rkb * kMxStep + ((lane & 31) ^ ((row & 3) << 2)) * 8;
+      buf_load16_to_lds(rH, xoff[i] != kOutOfRange && k < p.I ? xoff[i] + (uint32_t)(rkb * kMxStep * 2) : kOutOfRange, 0, own + kX + i * 1024);
     }
     if (lane < 32)  // scale words 0 and 1 of the 16 rows
-      buf_load4_to_lds(rS, voS + (uint32_t)min(2 * rkb + kq, words - 1) * (uint32_t)(p.s2_w * 4), 0, to + kS);
+      buf_load4_to_lds(rS, voS + (uint32_t)min(2 * rkb + kq, words - 1) * (uint32_t)(p.s2_w * 4), 0, own + kS);
     SB();
     --left;
-    if (++rkb == kbs) { rkb = 0; ++rt; }
+    if (++rkb == kbs) {
+      rkb = 0;
+      ++rt;
+      if (left > 0) enter_tile();
+    }
   };
 
-  v4f acc = {0.f, 0.f, 0.f, 0.f};
+  v4f acc = {0.f, 0.f, 0.f, 0.f}, odd = acc;
   if (nb > 0) {
     rt = b0 / kbs;
     rkb = b0 - rt * kbs;
     int ct = rt, ckb = rkb;
-#pragma unroll
-    for (int s = 0; s < ST; ++s) request(s);
+    entry1 = read_entry(rt);
+    read_slots(entry1);
+    entry2 = read_entry(rt + 1);
+    enter_tile();
+    request();
     const uint32_t xrd = (uint32_t)(kX + (r & (RX - 1)) * 512);
     const int xkey = (r & 3) << 2;
-    for (int b = 0; b < nb; b += ST) {
+    for (int b = 0; b < nb; ++b) {
+      wait_vm<0>();
+      uint32_t c[8];
 #pragma unroll
-      for (int s = 0; s < ST; ++s) {
-        if (b + s >= nb) break;
-        wait_vm<(ST - 1) * kLoads>();
-        const uint8_t* const from = own + s * kSlot;
-        uint32_t c[8];
+      for (int j = 0; j < 8; ++j) c[j] = codes.get(own, j);
+      const uint32_t s0 = *reinterpret_cast<const uint32_t*>(own + kS + r * 4), s1 = *reinterpret_cast<const uint32_t*>(own + kS + 64 + r * 4);
+      v4i x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) c[j] = codes.get(from, j);
-        const uint32_t s0 = *reinterpret_cast<const uint32_t*>(from + kS + r * 4), s1 = *reinterpret_cast<const uint32_t*>(from + kS + 64 + r * 4);
-        v4i x[8];
+      for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const v4i*>(own + xrd + (((j * 4 + kq) ^ xkey) << 4));
+      SB();
+      // two chains of products: one result waits for the one before it
+      acc = mx_mac<DT>(acc, x[0], c[0], mx_block_scale<DT>(s0, s1, 0));
+      odd = mx_mac<DT>(odd, x[1], c[1], mx_block_scale<DT>(s0, s1, 1));
+      SB();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // everything is out of its slot
+      if (b + 1 < nb) request();
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const v4i*>(from + xrd + (((j * 4 + kq) ^ xkey) << 4));
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // everything is out of its slot
-        SB();
-        request(s);
+      for (int j = 2; j < 8; j += 2) {
+        acc = mx_mac<DT>(acc, x[j], c[j], mx_block_scale<DT>(s0, s1, j));
+        odd = mx_mac<DT>(odd, x[j + 1], c[j + 1], mx_block_scale<DT>(s0, s1, j + 1));
+      }
+      SB();
+      if (++ckb == kbs || b == nb - 1) {
+        const int t = __builtin_amdgcn_readfirstlane(tiles[ct]), first = (t >> 4) & 1023, count = (t & 15) + 1;
+        int to[4];
+        float by[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc = mx_mac<DT>(acc, x[j], c[j], mx_block_scale<DT>(s0, s1, j));
-        SB();
-        if (++ckb == kbs || b + s == nb - 1) {
-          const int t = __builtin_amdgcn_readfirstlane(tiles[ct]), first = (t >> 4) & 1023, count = (t & 15) + 1;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = kq * 4 + i;
-            // two slots of a tile may be of one token: an LDS atomic, whose order within the wave is fixed
-            if (row < count) atomicAdd(&mine[(order[first + row] / p.topk) * 16 + r], acc[i] * weights[first + row]);
-            acc[i] = 0.f;
-          }
-          ckb = 0;
-          ++ct;
+        for (int i = 0; i < 4; ++i) {
+          const int at = first + min(kq * 4 + i, count - 1);
+          to[i] = token[at] * 16 + r;
+          by[i] = weights[at];
         }
+        // two slots of a tile may be of one token: LDS atomics, whose order within the wave is fixed
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (kq * 4 + i < count) unsafeAtomicAdd(&mine[to[i]], (acc[i] + odd[i]) * by[i]);
+          acc[i] = odd[i] = 0.f;
+        }
+        ckb = 0;
+        ++ct;
       }
     }
   }
-  wait_vm0();
   __syncthreads();
   for (int i = tid; i < p.T * 16; i += NW * 64) {
     float v = 0.f;

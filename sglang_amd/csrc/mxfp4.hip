@@ -430,20 +430,20 @@ extern "C" int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2,
   p.scaling = scaling;
   const hipStream_t st = (hipStream_t)stream;
   const bool gelu = activation == FP8K_ACT_GELU;
-  // runs of strips: as long as leaves two workgroups for every CU, so that a workgroup's start - the list of its slots, its first lines -
-  // comes once for several strips
+  // runs of strips: as long as leaves four workgroups for every CU (they are on it together), so that a workgroup's start - the list of
+  // its slots, its first lines - comes once for several strips
   const int64_t units = std::min(slots, E), strips = I / 16;
-  p.run = (int)std::min<int64_t>(8, std::max<int64_t>(1, units * strips / (2 * num_cu())));
+  p.run = (int)std::min<int64_t>(8, std::max<int64_t>(1, units * strips / (4 * num_cu())));
   const dim3 grid1((unsigned)((strips + p.run - 1) / p.run + 1), (unsigned)units), grid2((unsigned)(H / 16));
   // tiles of 4 slots while an expert has no more on average
   p.tile = slots <= 4 * units ? 4 : 16;
-  // more strips than CUs: workgroups of four waves, two of which share a CU
-  const bool narrow = H > 16 * num_cu();
-#define MX_DOWN(DT, TC)                                                                                   \
-  do {                                                                                                    \
-    if (p.tile == 4 && narrow) mx_experts_down_kernel<DT, TC, 4, 4><<<grid2, 256, 0, st>>>(p);            \
-    else if (p.tile == 4) mx_experts_down_kernel<DT, TC, 4, 8><<<grid2, 512, 0, st>>>(p);                 \
-    else mx_experts_down_kernel<DT, TC, 16, 8><<<grid2, 512, 0, st>>>(p);                                 \
+  // up to one strip of columns per CU: sixteen waves to it, as far as their sums fit; else eight, two workgroups to a CU
+  const bool wide = H <= 16 * num_cu();
+#define MX_DOWN(DT, TC)                                                                                                          \
+  do {                                                                                                                           \
+    if (p.tile != 4) mx_experts_down_kernel<DT, TC, 16, 8><<<grid2, 512, 0, st>>>(p);                                            \
+    else if (wide && TC <= 64) mx_experts_down_kernel<DT, TC, 4, (TC <= 64 ? 16 : 8)><<<grid2, (TC <= 64 ? 16 : 8) * 64, 0, st>>>(p); \
+    else mx_experts_down_kernel<DT, TC, 4, 8><<<grid2, 512, 0, st>>>(p);                                                         \
   } while (0)
 #define MX_UP(DT, RX)                                                             \
   do {                                                                            \
