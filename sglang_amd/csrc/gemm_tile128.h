@@ -179,18 +179,21 @@ __global__ __launch_bounds__(512, 1) void gemm_tile128_kernel(const GemmArgs p) 
   // trip `it` (u = it % 4): block `it` has landed everywhere; its operands from LDS into `rd`, the MFMAs of block it-1 from `use`, and
   // the loads of block it + NST - 2 into the stage of block it-2.  Every wave has used that block's operands by now, so the barrier
   // does not have to wait for LDS reads: they run on across it.
-  auto trip = [&](auto u_c, int it, Operands& rd, const Operands& use) {
+  // `tail`: a trip behind the loop.  There is no further group, so it requests no scales and its wait counts none (a request whose result
+  // is never used is dropped by the compiler, and a wait that counted it would let block it's own loads pass).
+  auto trip = [&](auto u_c, auto tail_c, int it, Operands& rd, const Operands& use) {
     constexpr int u = decltype(u_c)::value;
+    constexpr bool tail = decltype(tail_c)::value;
     constexpr bool first = u == 1;  // block it-1 starts a group of scales
     // younger than block it's loads: those of the blocks behind it, and a group's scales if requested meanwhile
-    constexpr int back = NST - 3, scale_ops = MODE != kModeRow && ((u + 3) & 3) >= 1 && ((u + 3) & 3) <= back ? MT + 1 : 0;
+    constexpr int back = NST - 3, scale_ops = !tail && MODE != kModeRow && ((u + 3) & 3) >= 1 && ((u + 3) & 3) <= back ? MT + 1 : 0;
     const uint8_t* const st = smem + st_rd;
     const int kf = it + NST - 2, fill = st_fill;
     SB();  // the MFMAs issued before stay in front of this wait
     vm_barrier<back * LPB + scale_ops>();
     if (first) {
       take_scales(it >> 2);
-      request_scales((it >> 2) + 1);
+      if (!tail) request_scales((it >> 2) + 1);
       SB();
     }
     compute(std::integral_constant<int, (u + 3) & 3>{}, use, [&](int i) {
@@ -200,6 +203,8 @@ __global__ __launch_bounds__(512, 1) void gemm_tile128_kernel(const GemmArgs p) 
     st_rd = next(st_rd);
     st_fill = next(st_fill);
   };
+  const std::false_type loop{};
+  const std::true_type tail{};
   const std::integral_constant<int, 0> c0{};
   const std::integral_constant<int, 1> c1{};
   const std::integral_constant<int, 2> c2{};
@@ -224,24 +229,24 @@ __global__ __launch_bounds__(512, 1) void gemm_tile128_kernel(const GemmArgs p) 
   auto nothing = [](int) {};
   int it = 1;
   for (; it + 3 < nkb; it += 4) {
-    trip(c1, it, ob, oa);
-    trip(c2, it + 1, oa, ob);
-    trip(c3, it + 2, ob, oa);
-    trip(c0, it + 3, oa, ob);
+    trip(c1, loop, it, ob, oa);
+    trip(c2, loop, it + 1, oa, ob);
+    trip(c3, loop, it + 2, ob, oa);
+    trip(c0, loop, it + 3, oa, ob);
   }
   if (it >= nkb) {
     take_scales(it >> 2);
     compute(c0, oa, nothing);
   } else {
-    trip(c1, it, ob, oa);
+    trip(c1, tail, it, ob, oa);
     if (it + 1 >= nkb) {
       compute(c1, ob, nothing);
     } else {
-      trip(c2, it + 1, oa, ob);
+      trip(c2, tail, it + 1, oa, ob);
       if (it + 2 >= nkb) {
         compute(c2, oa, nothing);
       } else {
-        trip(c3, it + 2, ob, oa);
+        trip(c3, tail, it + 2, ob, oa);
         compute(c3, ob, nothing);
       }
     }

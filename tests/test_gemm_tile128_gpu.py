@@ -232,3 +232,30 @@ def test_every_count_of_k_runs_exact(dev, tile128, M, N, splits):
     got = fp8_scaled_mm(fp8_tensor(xq, dev), fp8_tensor(wq, dev).t(), torch.from_numpy(sa).to(dev), torch.from_numpy(sb).to(dev),
                         torch.bfloat16, torch.from_numpy(bias).to(dev)).float().cpu().numpy()
     np.testing.assert_array_equal(got, O.fp8_scaled_mm(xq, wq, sa, sb, out_dtype="bf16", bias=bias))
+
+
+@pytest.mark.parametrize("tile_rows", [64, 128])
+@pytest.mark.parametrize("splits", [1, 2])
+@pytest.mark.parametrize("kb", [2, 3, 4, 6, 7, 8, 11])
+def test_operands_from_memory_arrive_in_time(dev, tile128, tile_rows, splits, kb):
+    """Integers with power-of-two scales and operands that no cache holds, at every remainder of the unrolled loop: a wait that lets a
+    block's loads pass shows as rows of stale operands."""
+    from sglang_amd.fp8_kernel import w8a8_block_fp8_matmul
+
+    M, N, K = 130, 1032, kb * 128
+    gen = torch.Generator(device=dev).manual_seed(kb)
+    flush = torch.empty(1 << 27, dtype=torch.float32, device=dev)
+
+    def operand(rows, scale_rows):
+        v = torch.randint(-4, 5, (rows, K), device=dev, generator=gen).float()
+        return v, v.to(torch.float8_e4m3fn), 2.0 ** torch.randint(-2, 3, (scale_rows, kb), device=dev, generator=gen).float()
+
+    tile128((256 if tile_rows == 64 else 0) + splits)
+    for _ in range(6):
+        (xv, xq, xs), (wv, wq, ws) = operand(M, M), operand(N, (N + 127) // 128)
+        x = (xv.view(M, kb, 128) * xs[:, :, None]).view(M, K).double()
+        w = (wv.view(N, kb, 128) * ws.repeat_interleave(128, 0)[:N, :, None]).view(N, K).double()
+        ref = (x @ w.t()).bfloat16()  # terms are multiples of 1/16 and at most 256: float32 sums are exact
+        for _ in range(3):
+            flush.zero_()
+            assert torch.equal(w8a8_block_fp8_matmul(xq, wq, xs, ws, [128, 128], output_dtype=torch.bfloat16), ref)
