@@ -128,26 +128,31 @@ __global__ __launch_bounds__(512, 1) void mx_tile128_kernel(const MxArgs p) {
   int st_rd = 0, st_fill = (NST - 2) * kStage;  // stage of block `it`, stage that block it + NST - 2 goes to
   auto next = [&](int st) { return st == (NST - 1) * kStage ? 0 : st + kStage; };
   // trip `it` (u = it % 4): block `it` has landed everywhere; its operands from LDS into `rd`, the products of block it-1 from `use`, and the
-  // loads of block it + 3 into the stage of block it-2, whose operands every wave has used by now
-  auto trip = [&](auto u_c, int it, Operands& rd, const Operands& use) {
+  // loads of block it + 3 into the stage of block it-2, whose operands every wave has used by now.  The trips behind the loop (u = 1 .. 3)
+  // request nothing and count the operand loads alone: a request whose result is never used is dropped by the compiler, and a wait that
+  // counted it would let a block's own loads pass.
+  auto trip = [&](auto u_c, auto tail_c, int it, Operands& rd, const Operands& use) {
     constexpr int u = decltype(u_c)::value;
+    constexpr bool tail = decltype(tail_c)::value;
     const uint8_t* const st = smem + st_rd;
     const int kf = it + NST - 2, fill = st_fill;
     SB();
-    vm_barrier<(NST - 3) * (LPB + SL)>();  // younger than block it's loads: those of the two blocks behind it
+    vm_barrier<tail ? (NST - 2 - u) * LPB : (NST - 3) * (LPB + SL)>();  // younger than block it's loads: those of the two blocks behind it
     take_scales(ring[(u + 3) & 3]);
     SB();
-    request_scales(ring[(u + 3) & 3], kf);  // kf % 4 == (it - 1) % 4
+    if (!tail) request_scales(ring[(u + 3) & 3], kf);  // kf % 4 == (it - 1) % 4
     SB();
     compute(use, [&](int i) {
 #pragma unroll
       for (int f = 0; f < FPP; ++f)
         if (i * FPP + f < NF) read_frag(rd, st, i * FPP + f);
-      if (i >= NP / 2 && i - NP / 2 < LPB) load_block(fill, kf, i - NP / 2);
+      if (!tail && i >= NP / 2 && i - NP / 2 < LPB) load_block(fill, kf, i - NP / 2);
     });
     st_rd = next(st_rd);
     st_fill = next(st_fill);
   };
+  const std::false_type loop{};
+  const std::true_type tail{};
   const std::integral_constant<int, 0> c0{};
   const std::integral_constant<int, 1> c1{};
   const std::integral_constant<int, 2> c2{};
@@ -175,26 +180,26 @@ __global__ __launch_bounds__(512, 1) void mx_tile128_kernel(const MxArgs p) {
   auto nothing = [](int) {};
   int it = 1;
   for (; it + 3 < nkb; it += 4) {
-    trip(c1, it, ob, oa);
-    trip(c2, it + 1, oa, ob);
-    trip(c3, it + 2, ob, oa);
-    trip(c0, it + 3, oa, ob);
+    trip(c1, loop, it, ob, oa);
+    trip(c2, loop, it + 1, oa, ob);
+    trip(c3, loop, it + 2, ob, oa);
+    trip(c0, loop, it + 3, oa, ob);
   }
   if (it >= nkb) {
     take_scales(ring[0]);
     compute(oa, nothing);
   } else {
-    trip(c1, it, ob, oa);
+    trip(c1, tail, it, ob, oa);
     if (it + 1 >= nkb) {
       take_scales(ring[1]);
       compute(ob, nothing);
     } else {
-      trip(c2, it + 1, oa, ob);
+      trip(c2, tail, it + 1, oa, ob);
       if (it + 2 >= nkb) {
         take_scales(ring[2]);
         compute(oa, nothing);
       } else {
-        trip(c3, it + 2, ob, oa);
+        trip(c3, tail, it + 2, ob, oa);
         take_scales(ring[3]);
         compute(ob, nothing);
       }

@@ -192,6 +192,30 @@ def test_every_kernel_is_exact(dev, plan, kind, m, n, k):
     _exact(dev, m, n, k)
 
 
+@pytest.mark.parametrize("kind", range(1, 5))
+@pytest.mark.parametrize("blocks", range(1, 12))
+def test_operands_from_memory_arrive_in_time(dev, plan, kind, blocks):
+    """Every count of K blocks with operands that no cache holds: a wait that lets a block's loads pass shows as rows of stale operands."""
+    k, gen = blocks * 256, torch.Generator(device=dev).manual_seed(blocks)
+
+    def operand(rows):
+        q = torch.randint(0, 256, (rows, k // 2), dtype=torch.uint8, device=dev, generator=gen)
+        byte = torch.randint(126, 128, (rows, k // 32), dtype=torch.uint8, device=dev, generator=gen)
+        return q, mxfp4.pack_mxfp4_scales(byte)
+
+    def values(q, s):
+        return mxfp4.mxfp4_dequant(q, s, torch.float32)
+
+    flush = torch.empty(1 << 27, dtype=torch.float32, device=dev)
+    plan(kind)
+    for _ in range(6):
+        (a, sa), (b, sb) = operand(130), operand(1032)
+        ref = (values(a, sa).double() @ values(b, sb).double().t()).bfloat16()  # terms are multiples of 1/16 and at most 36: float32 sums are exact
+        for _ in range(3):
+            flush.zero_()
+            assert torch.equal(mxfp4.w4a4_mxfp4_matmul(a, b, sa, sb), ref)
+
+
 @pytest.mark.parametrize("kind", range(5))
 def test_every_kernel_stores_unaligned_rows(dev, plan, kind):
     """Rows of the result that start at multiples of 8 bytes only, through the C interface; what lies between them stays."""
