@@ -503,8 +503,8 @@ int fp8k_mxfp4_gemm(const void* A, const void* B, const void* As, const void* Bs
                     int64_t bs_stride_w, int64_t ldc, int out_dtype, int bias_dtype, void* stream);
 
 /*
- * A whole linear on 16-bit activations x [M, K] (row stride ldx elements): fp8k_mxfp4_quant, then fp8k_mxfp4_gemm, whose results these
- * are bit for bit.  Workspace: 256-byte aligned, fp8k_mxfp4_linear_workspace_bytes of it (0 possible), not initialised.
+ * A whole linear on 16-bit activations x [M, K] (row stride ldx elements): fp8k_mxfp4_quant, then fp8k_mxfp4_gemm, in one launch for a
+ * few rows (float32 sums in another order then, if fp8k_mxfp4_gemm would not take the weight-streaming kernel).  Workspace: 256-byte aligned, fp8k_mxfp4_linear_workspace_bytes of it (0 possible), not initialised.
  */
 int64_t fp8k_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int fp8k_mxfp4_linear(const void* x, const void* B, const void* Bs, const void* bias, void* C, int64_t M, int64_t N, int64_t K,

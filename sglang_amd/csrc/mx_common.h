@@ -81,8 +81,7 @@ struct MxArgs {
   int tail_shared;    // mx_tile256_kernel: half u belongs to workgroup u (after its walk), else to workgroup walkers + u
 };
 
-// descriptor of the scales of `rows` rows from row `row0` on, and the byte offset of the two scales that lane (row, kq) needs in K
-// block kb: a lane of a product works on bytes 32 kq .. 32 kq + 31 of a 128-byte line, which are blocks 2 kq and 2 kq + 1
+// descriptor of the scale words of `rows` rows from row `row0` on
 __device__ __forceinline__ rsrc_t mx_scale_rsrc(const uint8_t* s, int64_t row0, int rows, int words, int64_t s_row, int64_t s_word) {
   return make_rsrc(s + row0 * s_row * 4, rows > 0 ? (uint32_t)(((rows - 1) * s_row + (words - 1) * s_word + 1) * 4) : 0u);
 }

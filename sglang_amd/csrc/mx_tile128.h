@@ -12,7 +12,6 @@
 // RAGGED: K is no multiple of 256; chunks of the activations past the end of a row arrive as zeros.
 #pragma once
 
-#include "gemm_tile128.h"
 #include "mx_common.h"
 
 namespace fp8k {

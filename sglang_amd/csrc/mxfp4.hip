@@ -309,7 +309,7 @@ extern "C" int fp8k_mxfp4_dequant(const void* q, const void* s, void* out, int64
   clear_error();
   FP8K_REQUIRE(is_float_type(out_dtype), "mxfp4 dequant: float32, float16 or bfloat16 output expected");
   FP8K_REQUIRE(E >= 0 && N >= 0 && K > 0 && K % kMxBlock == 0, "mxfp4 dequant: K must be a positive multiple of 32");
-  FP8K_REQUIRE(E <= 65535 && N <= (1 << 20) && K <= (1 << 24), "mxfp4 dequant: too large");
+  FP8K_REQUIRE(E <= 65535 && N <= (1 << 19) && K <= (1 << 24), "mxfp4 dequant: too large");
   if (E == 0 || N == 0) return FP8K_OK;
   FP8K_REQUIRE(q && out && aligned(q, 16) && aligned(out, 16), "mxfp4 dequant: operands must be 16-byte aligned");
   if (const int rc = check_scales("mxfp4 dequant", s, N, words_of(K), s_stride_n, s_stride_w)) return rc;
@@ -374,6 +374,7 @@ extern "C" int fp8k_mxfp4_linear(const void* x, const void* B, const void* Bs, c
   uint8_t* const q = (uint8_t*)workspace;
   uint8_t* const s = q + up_to(M * K / 2, 256);
   const int64_t ld = up_to(M, 4);
+  FP8K_REQUIRE(scales_fit(M, words_of(K), 1, ld), "mxfp4 linear: too many activations");
   if (const int rc = quant(x, q, s, M, K, ldx, 1, ld, dtype, false, st)) return rc;
   p.X = q; p.sx = s;
   p.ldx = K / 2;

@@ -91,7 +91,8 @@ def quant_weight_mxfp4(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor
 
 
 def mxfp4_dequant(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """Values [.., N, K] of codes [.., N, K/2] and their scales: exact in float32, rounded once to `dtype` (float32, float16, bfloat16)."""
+    """Values [N, K] of codes [N, K/2] and their scales, or [E, N, K] of a stack: exact in float32, rounded once to `dtype` (float32,
+    float16, bfloat16)."""
     if not torch.compiler.is_compiling():
         out = _host.mx_dequant(q, s, dtype)
         if out is not None:

@@ -103,6 +103,7 @@ def test_dequant_arguments(mem):
     _refused(f(p, p, p, 1, 4, 128, 0, -1, 4, _lib.BF16, None), b"strides")
     _refused(f(p, p, p, 1, 4, 128, -1, 1, 4, _lib.BF16, None), b"strides")
     _refused(f(p, p, p, 70000, 4, 128, 0, 1, 4, _lib.BF16, None), b"too large")
+    _refused(f(p, p, p, 1, 1 << 20, 128, 0, 1, 1 << 20, _lib.BF16, None), b"too large")
     assert f(None, None, None, 0, 4, 128, 0, 1, 4, _lib.BF16, None) == 0
 
 
@@ -126,6 +127,8 @@ def test_gemm_arguments(mem):
     _refused(lin(p, p, p, None, p, 300, 16, 128, 128, 64, 1, 16, 16, B, F, p, need - 1, None), b"workspace")
     _refused(lin(p, p, p, None, p, 300, 16, 128, 128, 64, 1, 16, 16, B, F, p + 16, need, None), b"workspace")
     _refused(lin(p, p, p, None, p, 300, 16, 128, 100, 64, 1, 16, 16, B, F, p, need, None), b"row stride")
+    # the scale words of the activations are addressed in 32 bits
+    _refused(lin(p, p, p, None, p, 1 << 17, 16, 1 << 20, 1 << 20, 1 << 19, 1, 16, 16, B, F, p, 1 << 60, None), b"too many activations")
 
 
 def test_experts_arguments(mem):

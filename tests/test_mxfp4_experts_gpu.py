@@ -109,6 +109,29 @@ def test_experts_of_other_ranks_and_repeated_ones(dev, t, topk):
     assert not none.any() and none.isfinite().all()
 
 
+def test_what_no_expert_takes_is_never_multiplied(dev):
+    """NaN and infinity in the weights of masked choices, and in tokens all of whose choices are masked."""
+    layer = _layer(5, 160, 96)
+    (w1, s1), (w2, s2) = layer
+    for t in (1, 6, 50):
+        x, weights, ids = _inputs(t, 160, 5, 3, torch.float16, t)
+        ids[:, 1] = -1
+        if t > 1:
+            ids[t // 2] = 5
+        zero = weights.clone()
+        zero[(ids < 0) | (ids > 4)] = 0
+        clean = mxfp4.fused_experts_mxfp4(x, w1, w2, zero, ids, s1, s2)
+        bad, dirty = weights.clone(), x.clone()
+        bad[(ids < 0) | (ids > 4)] = float("nan")
+        if t > 1:
+            bad[t // 2] = float("inf")
+            dirty[t // 2] = float("nan")
+            assert not clean[t // 2].any()
+        for on_input in (False, True):
+            want = clean if not on_input else mxfp4.fused_experts_mxfp4(x, w1, w2, zero, ids, s1, s2, apply_router_weight_on_input=True)
+            assert torch.equal(mxfp4.fused_experts_mxfp4(dirty, w1, w2, bad, ids, s1, s2, apply_router_weight_on_input=on_input), want)
+
+
 def test_a_token_that_is_not_finite_stays_alone(dev):
     layer = _layer(4, 160, 64)
     (w1, s1), (w2, s2) = layer
