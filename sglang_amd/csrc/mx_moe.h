@@ -183,7 +183,8 @@ __device__ __forceinline__ void mx_sort_slots(const MxExpertArgs& p, int* keys, 
 // applies the activation and writes h, while the others go on.
 // Bound: the weights' bytes.  One slot to a wave and four workgroups to a CU (RX = 4) beat two slots and two workgroups: 626 against
 // 645 us (64 tokens, 256 experts of 7168 x 2048), 21.0 against 28 (13 tokens, 128 of 4096 x 256): the conversions of one wave run
-// while another waits.
+// while another waits.  Weights that several tiles read stay in the caches, those that one reads go past them: 166 -> 151 us with 32
+// slots to an expert (64 tokens, 16 experts of 7168 x 2048), 85 -> 80 with 4 (128 of 4096 x 512); for all, 4 % slower with one tile.
 // ------------------------------------------------------------------------------------------------
 template <int DT, bool GELU, int RX>
 __global__ __launch_bounds__(256, RX == 4 ? 4 : 2) void mx_experts_up_kernel(const MxExpertArgs p) {
@@ -257,10 +258,14 @@ __global__ __launch_bounds__(256, RX == 4 ? 4 : 2) void mx_experts_up_kernel(con
   auto request = [&] __attribute__((always_inline)) {
     const int kb = w + NW * ri, c0 = (strip0 + rstrip) * 16;
     const uint32_t ko = (uint32_t)kb * kMxStepBytes + (uint32_t)(c0 * row_bytes);
-    buf_load16_to_lds<true>(rW, vo0 + ko, 0, own);
-    buf_load16_to_lds<true>(rW, vo1 + ko, 0, own + 1024);
-    buf_load16_to_lds<true>(rW, vo0 + (ko + up_rows), 0, own + 2048);
-    buf_load16_to_lds<true>(rW, vo1 + (ko + up_rows), 0, own + 3072);
+    const auto lines = [&](auto once) __attribute__((always_inline)) {
+      buf_load16_to_lds<once.value>(rW, vo0 + ko, 0, own);
+      buf_load16_to_lds<once.value>(rW, vo1 + ko, 0, own + 1024);
+      buf_load16_to_lds<once.value>(rW, vo0 + (ko + up_rows), 0, own + 2048);
+      buf_load16_to_lds<once.value>(rW, vo1 + (ko + up_rows), 0, own + 3072);
+    };
+    if (ntiles == 1) lines(std::true_type{});
+    else lines(std::false_type{});  // the next tile reads them again
 #pragma unroll
     for (int i = 0; i < RX / 2; ++i) {
       const int row = 2 * i + (lane >> 5), k = kb * kMxStep + ((lane & 31) ^ ((row & 3) << 2)) * 8;
