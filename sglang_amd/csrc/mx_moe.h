@@ -69,7 +69,7 @@ struct MxExpertArgs {
   int T, topk, E, H, I, slots;
   int ids64, on_input;
   int run;              // mx_experts_up_kernel: strips of a workgroup
-  int tile;             // slots of a tile (4 or 16)
+  int tile;             // slots of a tile of the second launch (4, 8 or 16)
   int64_t ldx;          // elements
   int64_t w1_e, w2_e;   // bytes
   int64_t s1_e, s1_n, s1_w, s2_e, s2_n, s2_w;  // int32 words
@@ -366,13 +366,16 @@ __global__ __launch_bounds__(256, RX == 4 ? 4 : 2) void mx_experts_up_kernel(con
 // (Activations in operand form straight to registers, eight loads a block of which a few lanes are used, took 28 us for the 62 MB of one
 // token where this takes 15.)  Eight waves and two workgroups to a CU beat four waves with three slots each, 363 against 394 us with 64
 // tokens and 256 experts of 7168 x 2048; up to one strip per CU sixteen waves, 13.2 against 14.5 us (13 tokens, 128 of 4096 x 256).
+// Tiles of 8 slots, with twelve waves where the sums of 64 tokens leave room for one workgroup only, against 16 and eight waves: 158 - 161
+// against 182 us with 6 slots to an expert (48 tokens, 64 of 7168 x 2048), 24 against 29 (12 tokens, 16 of 7168 x 1024); with 32 to one
+// (64 tokens, 16 of 7168 x 2048) 163 against 130.
 // Sums of several workgroups per strip, added up by the last one to come, cost more than they balance: a release to the whole device
 // writes its L2 back (13 tokens 16 -> 38 us).
 // ------------------------------------------------------------------------------------------------
 constexpr int mx_down_places(int tc) { return tc <= 16 ? 512 : kMxMaxSlots; }  // (token, choice) pairs
 
 template <int DT, int TC, int RX, int NW>  // TC: tokens that the sums have room for; RX: slots of a tile; NW: waves
-__global__ __launch_bounds__(NW * 64, RX == 4 && TC <= 64 ? 4 : 2) void mx_experts_down_kernel(const MxExpertArgs p) {
+__global__ __launch_bounds__(NW * 64, RX == 4 && TC <= 64 ? 4 : NW == 12 ? 3 : 2) void mx_experts_down_kernel(const MxExpertArgs p) {
   constexpr int kSlot = 2048 + RX * 512 + 128, kX = 2048, kS = 2048 + RX * 512;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[NW * kSlot];
   __shared__ __attribute__((aligned(16))) float sums[NW * TC * 16];  // [NW][T][16]

@@ -436,13 +436,16 @@ extern "C" int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2,
   const int64_t units = std::min(slots, E), strips = I / 16;
   p.run = (int)std::min<int64_t>(8, std::max<int64_t>(1, units * strips / (4 * num_cu())));
   const dim3 grid1((unsigned)((strips + p.run - 1) / p.run + 1), (unsigned)units), grid2((unsigned)(H / 16));
-  // tiles of 4 slots while an expert has no more on average
-  p.tile = slots <= 4 * units ? 4 : 16;
+  // slots that a workgroup of the first launch takes at a time, and of a tile of the second: what an expert has on average, rounded up.
+  // (The first with 8, 64 experts of 7168 x 2048 and 6 slots to one: 280 us, with 16 246.)
+  const bool few = slots <= 4 * units;
+  p.tile = few ? 4 : slots <= 8 * units ? 8 : 16;
   // up to one strip of columns per CU: sixteen waves to it, as far as their sums fit; else eight, two workgroups to a CU
   const bool wide = H <= 16 * num_cu();
 #define MX_DOWN(DT, TC)                                                                                                          \
   do {                                                                                                                           \
-    if (p.tile != 4) mx_experts_down_kernel<DT, TC, 16, 8><<<grid2, 512, 0, st>>>(p);                                            \
+    if (p.tile == 16) mx_experts_down_kernel<DT, TC, 16, 8><<<grid2, 512, 0, st>>>(p);                                           \
+    else if (p.tile == 8) mx_experts_down_kernel<DT, TC, 8, (TC == 64 ? 12 : 8)><<<grid2, (TC == 64 ? 12 : 8) * 64, 0, st>>>(p); \
     else if (wide && TC <= 64) mx_experts_down_kernel<DT, TC, 4, (TC <= 64 ? 16 : 8)><<<grid2, (TC <= 64 ? 16 : 8) * 64, 0, st>>>(p); \
     else mx_experts_down_kernel<DT, TC, 4, 8><<<grid2, 512, 0, st>>>(p);                                                         \
   } while (0)
@@ -453,7 +456,7 @@ extern "C" int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2,
   } while (0)
 #define MX_EXPERTS(DT)                                                     \
   do {                                                                     \
-    if (p.tile == 4) MX_UP(DT, 4);                                         \
+    if (few) MX_UP(DT, 4);                                                 \
     else MX_UP(DT, 16);                                                    \
     if (const int rc = check_launch("mxfp4 experts")) return rc;           \
     if (T <= 16 && slots <= mx_down_places(16)) MX_DOWN(DT, 16);           \

@@ -109,6 +109,19 @@ def test_experts_of_other_ranks_and_repeated_ones(dev, t, topk):
     assert not none.any() and none.isfinite().all()
 
 
+@pytest.mark.parametrize("t,e,topk,h,i", [(5, 4, 4, 288, 544), (16, 10, 4, 544, 288), (20, 20, 5, 160, 96), (64, 64, 8, 256, 96), (60, 32, 3, 4128, 64),
+                                          (100, 16, 1, 128, 288), (128, 64, 4, 160, 512)])
+def test_five_to_eight_slots_to_an_expert(dev, t, e, topk, h, i):
+    """Between the few-slot tiles and the large ones, with experts that have more than one tile and experts that have none."""
+    layer = _layer(e, h, i, t)
+    x, weights, ids = _inputs(t, h, e, topk, torch.bfloat16, e)
+    ids[: t // 2] = ids[: t // 2].clamp(max=e // 2)
+    (w1, s1), (w2, s2) = layer
+    out = mxfp4.fused_experts_mxfp4(x, w1, w2, weights, ids, s1, s2)
+    _check(out, x, layer, weights, ids)
+    assert torch.equal(out, mxfp4.fused_experts_mxfp4(x, w1, w2, weights, ids, s1, s2))
+
+
 def test_what_no_expert_takes_is_never_multiplied(dev):
     """NaN and infinity in the weights of masked choices, and in tokens all of whose choices are masked."""
     layer = _layer(5, 160, 96)
