@@ -504,7 +504,8 @@ int fp8k_mxfp4_gemm(const void* A, const void* B, const void* As, const void* Bs
 
 /*
  * A whole linear on 16-bit activations x [M, K] (row stride ldx elements): fp8k_mxfp4_quant, then fp8k_mxfp4_gemm, in one launch for a
- * few rows (float32 sums in another order then, if fp8k_mxfp4_gemm would not take the weight-streaming kernel).  Workspace: 256-byte aligned, fp8k_mxfp4_linear_workspace_bytes of it (0 possible), not initialised.
+ * few rows (float32 sums in another order then, if fp8k_mxfp4_gemm would not take the weight-streaming kernel).  Workspace: 256-byte
+ * aligned, fp8k_mxfp4_linear_workspace_bytes of it (0 possible), not initialised.
  */
 int64_t fp8k_mxfp4_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int fp8k_mxfp4_linear(const void* x, const void* B, const void* Bs, const void* bias, void* C, int64_t M, int64_t N, int64_t K,
@@ -515,8 +516,8 @@ int fp8k_mxfp4_linear(const void* x, const void* B, const void* Bs, const void* 
  * A mixture-of-experts layer on MXFP4 weights for a few tokens (at most 128, and at most 1024 (token, choice) pairs), two launches.
  * x [T, H] of dtype (F16/BF16), row stride ldx elements; w1 [E, 2I, H/2] (gate rows, then up rows), w2 [E, H, I/2], rows contiguous;
  * topk_weights [T, topk], topk_ids [T, topk] int32 or int64; an id outside 0 .. E-1 contributes nothing.
- *   h = round(act(x . gate^T) * (x . up^T));  out[t] = round(scaling * sum over k of weight[t, k] * h[t, k] . W2^T)
- * with float32 sums; weight_on_input: the weight multiplies both products of the first stage instead.  activation: fp8k_activation_kind
+ *   h = act(x . gate^T) * (x . up^T);  out[t] = round(scaling * sum over k of weight[t, k] * h[t, k] . W2^T)
+ * with float32 sums; h is held as the sum of two bfloat16 numbers.  weight_on_input: the weight multiplies both products of the first stage instead.  activation: fp8k_activation_kind
  * SILU or GELU.  out [T, H] contiguous may be x.  Workspace: 256-byte aligned, not initialised.
  */
 int64_t fp8k_mxfp4_experts_workspace_bytes(int64_t T, int64_t topk, int64_t I);

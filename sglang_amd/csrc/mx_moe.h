@@ -1,11 +1,12 @@
 // A whole mixture-of-experts layer on MXFP4 weights for a few tokens, in two launches (gfx950).
 //
-//   h[slot]  = round16(act(g) * u),  (g, u) = x[token] . W1[expert]^T        mx_experts_up_kernel
+//   h[slot]  = act(g) * u,  (g, u) = x[token] . W1[expert]^T                 mx_experts_up_kernel
 //   y[token] = round16(f * sum over its slots of weight * h[slot] . W2[expert]^T)   mx_experts_down_kernel
 //
 // A slot is one (token, choice) pair.  With few tokens the layer is a stream of the chosen experts' weights, so activations stay in 16
-// bits: quantising them would move no byte less.  h is rounded to the activations' type because the second product takes 16-bit
-// operands, as every layer of this library rounds between its products; all sums, the routed weights and the last sum are float32.  The
+// bits: quantising them would move no byte less.  All sums, the routed weights and the last sum are float32.  The second product takes
+// 16-bit operands, so h travels as a pair of bfloat16, rounded and what the rounding left, whose products are added: one 16-bit h would be
+// an error as large as the result's own rounding (1.4 times the whole error), the pair is off by 2^-16 and has float32's range.  The
 // codes become exact 16-bit floats in registers (v_cvt_scalef32_pk_*_fp4, two a instruction), and a product of 32 along K is one block
 // of the scales.
 //
@@ -30,23 +31,29 @@ __device__ __forceinline__ v4f mfma16(v4i a, v4i b, v4f c) {
   if (DT == FP8K_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
-// acc += a . (codes of a weight row * scale), 32 values along K that share the scale.  Eight codes to a lane become eight 16-bit floats.
-// bfloat16 has float32's exponents, so that code * scale is exact and the products add up in place.  float16 does not: its codes stay
-// unscaled, and the result of the 32 is multiplied (four more multiplications per product).
+// Eight codes become eight 16-bit floats, for bfloat16 times their scale: it has float32's exponents, so that code * scale is exact.
 template <int DT>
-__device__ __forceinline__ v4f mx_mac(v4f acc, v4i a, uint32_t c, float scale) {
+__device__ __forceinline__ v4i mx_floats(uint32_t c, float scale) {
   v4i b;
   if (DT == FP8K_BF16) {
     b[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0));
     b[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 1));
     b[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2));
     b[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3));
-    return mfma16<DT>(a, b, acc);
+  } else {
+    b[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, 1.0f, 0));
+    b[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, 1.0f, 1));
+    b[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, 1.0f, 2));
+    b[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, 1.0f, 3));
   }
-  b[0] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, 1.0f, 0));
-  b[1] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, 1.0f, 1));
-  b[2] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, 1.0f, 2));
-  b[3] = __builtin_bit_cast(int, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, 1.0f, 3));
+  return b;
+}
+// acc += a . (codes of a weight row * scale), 32 values along K that share the scale.  bfloat16 adds up in place.  float16's codes are
+// unscaled, and the result of the 32 is multiplied (four more multiplications per product).
+template <int DT>
+__device__ __forceinline__ v4f mx_mac(v4f acc, v4i a, uint32_t c, float scale) {
+  const v4i b = mx_floats<DT>(c, scale);
+  if (DT == FP8K_BF16) return mfma16<DT>(a, b, acc);
   const v4f part = mfma16<DT>(a, b, v4f{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i] = __builtin_fmaf(part[i], scale, acc[i]);
@@ -62,7 +69,7 @@ struct MxExpertArgs {
   const float* topk_w;  // [T, topk]
   const void* ids;      // [T, topk] int32 or int64
   void* out;            // [T, H]
-  void* h;              // [slots, I] 16-bit: the workspace, as are the four arrays of the table
+  void* h;              // [slots, 2, I] bfloat16, the pairs' first and second parts: the workspace, as are the four arrays of the table
   int32_t* tiles;       // [slots] tile t: some slots of one expert (mx_tile below)
   int32_t* order;       // [slots] slots sorted by expert
   float* weights;       // [slots] their routed weights, in that order
@@ -70,7 +77,7 @@ struct MxExpertArgs {
   int T, topk, E, H, I, slots;
   int ids64, on_input;
   int run;              // mx_experts_up_kernel: strips of a workgroup
-  int tile;             // slots of a tile of the second launch (4, 8 or 16)
+  int tile;             // slots of a tile of the second launch (4 or 8)
   int64_t ldx;          // elements
   int64_t w1_e, w2_e;   // bytes
   int64_t s1_e, s1_n, s1_w, s2_e, s2_n, s2_w;  // int32 words
@@ -333,7 +340,13 @@ __global__ __launch_bounds__(256, RX == 4 ? 4 : 2) void mx_experts_up_kernel(con
           u[i] *= p.topk_w[s];
         }
         const float v = (GELU ? gelu_f32(g[i]) : silu_f32(g[i])) * u[i];
-        ((u16*)p.h)[(int64_t)s * p.I + (strip0 + strip) * 16 + r] = (u16)(DT == FP8K_BF16 ? f32_to_bf16_bits(v) : f32_to_f16_bits(v));
+        // the first part stays finite, so that an infinity is left to the second
+        constexpr float kMost = 3.3895313892515355e38f;
+        const u16 hi = (u16)f32_to_bf16_bits(v > kMost ? kMost : v < -kMost ? -kMost : v);
+        const float left = v - __uint_as_float((uint32_t)hi << 16);
+        u16* const to = (u16*)p.h + (int64_t)s * 2 * p.I + (strip0 + strip) * 16 + r;
+        to[0] = hi;
+        to[p.I] = (u16)f32_to_bf16_bits(left);
       }
     }
     lds_barrier();
@@ -365,19 +378,24 @@ __global__ __launch_bounds__(256, RX == 4 ? 4 : 2) void mx_experts_up_kernel(con
 // Everything a K block needs - the lines of 16 weight rows, their scale words, the activations of the tile's RX slots - goes straight to
 // the wave's LDS slot, requested as soon as the operands of the block before are out of it, and no other load stands in the loop.
 // (Activations in operand form straight to registers, eight loads a block of which a few lanes are used, took 28 us for the 62 MB of one
-// token where this takes 15.)  Eight waves and two workgroups to a CU beat four waves with three slots each, 363 against 394 us with 64
-// tokens and 256 experts of 7168 x 2048; up to one strip per CU sixteen waves, 13.2 against 14.5 us (13 tokens, 128 of 4096 x 256).
-// Tiles of 8 slots, with twelve waves where the sums of 64 tokens leave room for one workgroup only, against 16 and eight waves: 158 - 161
-// against 182 us with 6 slots to an expert (48 tokens, 64 of 7168 x 2048), 24 against 29 (12 tokens, 16 of 7168 x 1024); with 32 to one
-// (64 tokens, 16 of 7168 x 2048) 163 against 130.
+// token where this takes 15.)  A slot's pair is two neighbouring rows of the operand, of whose sixteen few are used anyway: it costs LDS and
+// the fetch, no product.  As many waves as there is room for, one LDS slot each: eight and two workgroups to a CU beat four waves with three
+// slots each, 363 against 394 us (64 tokens, 256 experts of 7168 x 2048, h not in pairs); fourteen of one workgroup take 400 there, twelve 408;
+// up to one strip per CU sixteen waves, 13.0 against 14.5 us (13 tokens, 128 of 4096 x 256).
 // Sums of several workgroups per strip, added up by the last one to come, cost more than they balance: a release to the whole device
 // writes its L2 back (13 tokens 16 -> 38 us).
 // ------------------------------------------------------------------------------------------------
+// waves of a workgroup: as many as the LDS has room for, up to one strip per CU (`wide`); else two workgroups to a CU if they fit
+constexpr int mx_down_waves(int rx, int tc, bool wide) {
+  if (tc > 64) return 8;
+  if (tc > 32) return rx == 8 ? 10 : 14;
+  return rx == 8 ? 12 : wide ? 16 : 8;
+}
 constexpr int mx_down_places(int tc) { return tc <= 16 ? 512 : kMxMaxSlots; }  // (token, choice) pairs
 
-template <int DT, int TC, int RX, int NW>  // TC: tokens that the sums have room for; RX: slots of a tile; NW: waves
-__global__ __launch_bounds__(NW * 64, RX == 4 && TC <= 64 ? 4 : NW == 12 ? 3 : 2) void mx_experts_down_kernel(const MxExpertArgs p) {
-  constexpr int kSlot = 2048 + RX * 512 + 128, kX = 2048, kS = 2048 + RX * 512;
+template <int DT, int TC, int RX, int NW>  // DT: of the result; TC: tokens that the sums have room for; RX: slots of a tile; NW: waves
+__global__ __launch_bounds__(NW * 64, RX == 4 && TC <= 32 ? 4 : (NW + 3) / 4) void mx_experts_down_kernel(const MxExpertArgs p) {
+  constexpr int kSlot = 2048 + RX * 1024 + 128, kX = 2048, kS = 2048 + RX * 1024;
   __shared__ __attribute__((aligned(1024))) uint8_t smem[NW * kSlot];
   __shared__ __attribute__((aligned(16))) float sums[NW * TC * 16];  // [NW][T][16]
   __shared__ int tiles[mx_down_places(TC)];
@@ -405,7 +423,7 @@ __global__ __launch_bounds__(NW * 64, RX == 4 && TC <= 64 ? 4 : NW == 12 ? 3 : 2
   const int row_bytes = p.I >> 1, words = (p.I + 127) >> 7, kbs = (p.I + kMxStep - 1) / kMxStep;
   const int all = ntiles * kbs, per = (all + NW - 1) / NW;
   const int b0 = w * per, nb = max(min(all, b0 + per) - b0, 0);
-  const rsrc_t rH = make_rsrc(p.h, (uint32_t)((int64_t)p.slots * p.I * 2));
+  const rsrc_t rH = make_rsrc(p.h, (uint32_t)((int64_t)p.slots * p.I * 4));
   const int rl = lane >> 3, cp = lane & 7;
   const uint32_t vo0 = (uint32_t)((n0 + rl) * row_bytes + (cp ^ (rl >> 1)) * 16), vo1 = (uint32_t)((n0 + rl + 8) * row_bytes + (cp ^ (4 + (rl >> 1))) * 16);
   const uint32_t voS = (uint32_t)((n0 + r) * p.s2_n * 4);
@@ -416,14 +434,14 @@ __global__ __launch_bounds__(NW * 64, RX == 4 && TC <= 64 ? 4 : NW == 12 ? 3 : 2
   // and its slots, which were read from LDS one tile earlier (the entry two): a request never waits for LDS.
   int rt = 0, rkb = 0, left = nb;  // tile, its K block, blocks to come
   rsrc_t rW = make_rsrc(p.w2, 0), rS = make_rsrc(p.s2, 0);
-  uint32_t xoff[RX / 2];           // of the activations that the lane fetches; 16-byte piece c of slot i lies at position c ^ (4 (i & 3)),
-  int count = 0;                   // so that the operand reads of different slots fall into different banks
+  uint32_t xoff[RX];               // of the activations that the lane fetches: a load brings slot i's pair, rows 2 i and 2 i + 1 of the
+  int count = 0;                   // operand; 16-byte piece c of row m lies at position c ^ (4 (m & 3)), so that reads spread over the banks
   int entry1 = 0, entry2 = 0;      // of tiles rt + 1 (here, when it becomes rt) and rt + 2
-  int slots1[RX / 2];
+  int slots1[RX];
   auto read_entry = [&](int t) { return tiles[min(t, ntiles - 1)]; };
   auto read_slots = [&](int entry) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < RX / 2; ++i) slots1[i] = order[min(((entry >> 4) & 1023) + 2 * i + (lane >> 5), p.slots - 1)];
+    for (int i = 0; i < RX; ++i) slots1[i] = order[min(((entry >> 4) & 1023) + i, p.slots - 1)];
   };
   auto enter_tile = [&] __attribute__((always_inline)) {  // entry1 and slots1 are those of tile rt
     const int t = __builtin_amdgcn_readfirstlane(entry1);
@@ -432,10 +450,8 @@ __global__ __launch_bounds__(NW * 64, RX == 4 && TC <= 64 ? 4 : NW == 12 ? 3 : 2
     rW = make_rsrc(p.w2 + e * p.w2_e, (uint32_t)(p.H * row_bytes));
     rS = mx_scale_rsrc(p.s2 + e * p.s2_e * 4, 0, p.H, words, p.s2_n, p.s2_w);
 #pragma unroll
-    for (int i = 0; i < RX / 2; ++i) {
-      const int row = 2 * i + (lane >> 5);
-      xoff[i] = row < count ? (uint32_t)slots1[i] * (uint32_t)(p.I * 2) + (uint32_t)(((lane & 31) ^ ((row & 3) << 2)) * 16) : kOutOfRange;
-    }
+    for (int i = 0; i < RX; ++i)
+      xoff[i] = (uint32_t)(slots1[i] * 2 + (lane >> 5)) * (uint32_t)(p.I * 2) + (uint32_t)(((lane & 31) ^ (((2 * i + (lane >> 5)) & 3) << 2)) * 16);
     entry1 = entry2;
     read_slots(entry2);
     entry2 = read_entry(rt + 2);
@@ -445,9 +461,10 @@ __global__ __launch_bounds__(NW * 64, RX == 4 && TC <= 64 ? 4 : NW == 12 ? 3 : 2
     buf_load16_to_lds<true>(rW, vo0 + ko, 0, own);
     buf_load16_to_lds<true>(rW, vo1 + ko, 0, own + 1024);
 #pragma unroll
-    for (int i = 0; i < RX / 2; ++i) {
-      const int row = 2 * i + (lane >> 5), k = rkb * kMxStep + ((lane & 31) ^ ((row & 3) << 2)) * 8;
-      buf_load16_to_lds(rH, xoff[i] != kOutOfRange && k < p.I ? xoff[i] + (uint32_t)(rkb * kMxStep * 2) : kOutOfRange, 0, own + kX + i * 1024);
+    for (int i = 0; i < RX; ++i) {
+      if (i >= count) break;  // what is left in the rows behind makes results that nobody takes
+      const int k = rkb * kMxStep + ((lane & 31) ^ (((2 * i + (lane >> 5)) & 3) << 2)) * 8;
+      buf_load16_to_lds(rH, k < p.I ? xoff[i] + (uint32_t)(rkb * kMxStep * 2) : kOutOfRange, 0, own + kX + i * 1024);
     }
     if (lane < 32)  // scale words 0 and 1 of the 16 rows
       buf_load4_to_lds(rS, voS + (uint32_t)min(2 * rkb + kq, words - 1) * (uint32_t)(p.s2_w * 4), 0, own + kS);
@@ -470,7 +487,7 @@ __global__ __launch_bounds__(NW * 64, RX == 4 && TC <= 64 ? 4 : NW == 12 ? 3 : 2
     entry2 = read_entry(rt + 1);
     enter_tile();
     request();
-    const uint32_t xrd = (uint32_t)(kX + (r & (RX - 1)) * 512);
+    const uint32_t xrd = (uint32_t)(kX + (r & (2 * RX - 1)) * 512);
     const int xkey = (r & 3) << 2;
     for (int b = 0; b < nb; ++b) {
       wait_vm<0>();
@@ -483,33 +500,33 @@ __global__ __launch_bounds__(NW * 64, RX == 4 && TC <= 64 ? 4 : NW == 12 ? 3 : 2
       for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const v4i*>(own + xrd + (((j * 4 + kq) ^ xkey) << 4));
       SB();
       // two chains of products: one result waits for the one before it
-      acc = mx_mac<DT>(acc, x[0], c[0], mx_block_scale<DT>(s0, s1, 0));
-      odd = mx_mac<DT>(odd, x[1], c[1], mx_block_scale<DT>(s0, s1, 1));
+      acc = mx_mac<FP8K_BF16>(acc, x[0], c[0], mx_block_scale<FP8K_BF16>(s0, s1, 0));
+      odd = mx_mac<FP8K_BF16>(odd, x[1], c[1], mx_block_scale<FP8K_BF16>(s0, s1, 1));
       SB();
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // everything is out of its slot
       if (b + 1 < nb) request();
 #pragma unroll
       for (int j = 2; j < 8; j += 2) {
-        acc = mx_mac<DT>(acc, x[j], c[j], mx_block_scale<DT>(s0, s1, j));
-        odd = mx_mac<DT>(odd, x[j + 1], c[j + 1], mx_block_scale<DT>(s0, s1, j + 1));
+        acc = mx_mac<FP8K_BF16>(acc, x[j], c[j], mx_block_scale<FP8K_BF16>(s0, s1, j));
+        odd = mx_mac<FP8K_BF16>(odd, x[j + 1], c[j + 1], mx_block_scale<FP8K_BF16>(s0, s1, j + 1));
       }
       SB();
       if (++ckb == kbs || b == nb - 1) {
         const int t = __builtin_amdgcn_readfirstlane(tiles[ct]), first = (t >> 4) & 1023, count = (t & 15) + 1;
-        int to[4];
-        float by[4];
+        int to[2];
+        float by[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int at = first + min(kq * 4 + i, count - 1);
+        for (int i = 0; i < 2; ++i) {
+          const int at = first + min(kq * 2 + i, count - 1);
           to[i] = token[at] * 16 + r;
           by[i] = weights[at];
         }
-        // two slots of a tile may be of one token: LDS atomics, whose order within the wave is fixed
+        // the lane's rows are the pairs of two slots.  Two slots of a tile may be of one token: LDS atomics, whose order within the wave
+        // is fixed.
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if (kq * 4 + i < count) unsafeAtomicAdd(&mine[to[i]], (acc[i] + odd[i]) * by[i]);
-          acc[i] = odd[i] = 0.f;
-        }
+        for (int i = 0; i < 2; ++i)
+          if (kq * 2 + i < count) unsafeAtomicAdd(&mine[to[i]], (acc[2 * i] + odd[2 * i] + (acc[2 * i + 1] + odd[2 * i + 1])) * by[i]);
+        acc = odd = v4f{0.f, 0.f, 0.f, 0.f};
         ckb = 0;
         ++ct;
       }

@@ -287,7 +287,7 @@ int check_gemm(const char* what, int64_t M, int64_t N, int64_t K, int64_t ldb, i
   return FP8K_OK;
 }
 
-int64_t experts_part(int64_t slots, int64_t I) { return up_to(slots * I * 2, 256); }
+int64_t experts_part(int64_t slots, int64_t I) { return up_to(slots * I * 4, 256); }
 
 }  // namespace
 }  // namespace fp8k
@@ -400,7 +400,7 @@ extern "C" int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2,
   FP8K_REQUIRE(activation == FP8K_ACT_SILU || activation == FP8K_ACT_GELU, "mxfp4 experts: the activation must be silu or gelu");
   FP8K_REQUIRE(T >= 0 && topk > 0 && E > 0 && H > 0 && I > 0, "mxfp4 experts: bad sizes");
   FP8K_REQUIRE(H % kMxBlock == 0 && I % kMxBlock == 0, "mxfp4 experts: hidden and intermediate size must be multiples of 32");
-  FP8K_REQUIRE(H <= (1 << 20) && I <= (1 << 20) && H * I < (1ll << 31) && E <= 65535, "mxfp4 experts: too large");
+  FP8K_REQUIRE(H <= (1 << 20) && I <= (1 << 19) && H * I < (1ll << 31) && E <= 65535, "mxfp4 experts: too large");
   FP8K_REQUIRE(T <= kMxMaxTokens && T * topk <= kMxMaxSlots, "mxfp4 experts: built for at most %d tokens and %d (token, choice) pairs, got %lld and %lld",
                kMxMaxTokens, kMxMaxSlots, (long long)T, (long long)(T * topk));
   if (T == 0) return FP8K_OK;
@@ -438,18 +438,18 @@ extern "C" int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2,
   const int64_t units = std::min(slots, E), strips = I / 16;
   p.run = (int)std::min<int64_t>(8, std::max<int64_t>(1, units * strips / (4 * num_cu())));
   const dim3 grid1((unsigned)((strips + p.run - 1) / p.run + 1), (unsigned)units), grid2((unsigned)(H / 16));
-  // slots that a workgroup of the first launch takes at a time, and of a tile of the second: what an expert has on average, rounded up.
-  // (The first with 8, 64 experts of 7168 x 2048 and 6 slots to one: 280 us, with 16 246.)
+  // slots that a workgroup of the first launch takes at a time (4 or 16), and those of a tile of the second (4 or 8: the operand has 16 rows):
+  // few while an expert has no more on average.  (The first with 8, 64 experts of 7168 x 2048 and 6 slots to one: 280 us, with 16 246.)
   const bool few = slots <= 4 * units;
-  p.tile = few ? 4 : slots <= 8 * units ? 8 : 16;
+  p.tile = few ? 4 : 8;
   // up to one strip of columns per CU: sixteen waves to it, as far as their sums fit; else eight, two workgroups to a CU
   const bool wide = H <= 16 * num_cu();
-#define MX_DOWN(DT, TC)                                                                                                          \
-  do {                                                                                                                           \
-    if (p.tile == 16) mx_experts_down_kernel<DT, TC, 16, 8><<<grid2, 512, 0, st>>>(p);                                           \
-    else if (p.tile == 8) mx_experts_down_kernel<DT, TC, 8, (TC == 64 ? 12 : 8)><<<grid2, (TC == 64 ? 12 : 8) * 64, 0, st>>>(p); \
-    else if (wide && TC <= 64) mx_experts_down_kernel<DT, TC, 4, (TC <= 64 ? 16 : 8)><<<grid2, (TC <= 64 ? 16 : 8) * 64, 0, st>>>(p); \
-    else mx_experts_down_kernel<DT, TC, 4, 8><<<grid2, 512, 0, st>>>(p);                                                         \
+#define MX_DOWN(DT, TC)                                                                                                        \
+  do {                                                                                                                         \
+    constexpr int kMany = mx_down_waves(8, TC, false), kFew = mx_down_waves(4, TC, false), kWide = mx_down_waves(4, TC, true); \
+    if (!few) mx_experts_down_kernel<DT, TC, 8, kMany><<<grid2, kMany * 64, 0, st>>>(p);                                       \
+    else if (wide) mx_experts_down_kernel<DT, TC, 4, kWide><<<grid2, kWide * 64, 0, st>>>(p);                                  \
+    else mx_experts_down_kernel<DT, TC, 4, kFew><<<grid2, kFew * 64, 0, st>>>(p);                                              \
   } while (0)
 #define MX_UP(DT, RX)                                                             \
   do {                                                                            \
@@ -462,6 +462,7 @@ extern "C" int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2,
     else MX_UP(DT, 16);                                                    \
     if (const int rc = check_launch("mxfp4 experts")) return rc;           \
     if (T <= 16 && slots <= mx_down_places(16)) MX_DOWN(DT, 16);           \
+    else if (T <= 32) MX_DOWN(DT, 32);                                     \
     else if (T <= 64) MX_DOWN(DT, 64);                                     \
     else MX_DOWN(DT, kMxMaxTokens);                                        \
   } while (0)

@@ -162,7 +162,9 @@ def fused_experts_mxfp4(
     and topk_ids [T, k] as the routers of fused_moe return them; an id that is not 0 .. E-1 (-1: an expert of another rank)
     contributes nothing.  Activations stay in 16 bits: with few tokens the layer is bound by the weights' bytes.
 
-      h = round(act(x . gate^T) * (x . up^T)), out = round(routed_scaling_factor * sum of weight * h . w2^T), sums in float32
+      h = act(x . gate^T) * (x . up^T), out = round(routed_scaling_factor * sum of weight * h . w2^T), sums in float32
+
+    h is held as the sum of two bfloat16 numbers, so that the rounding of the result is the only one that counts.
 
     apply_router_weight_on_input: the weight multiplies both products of the first stage instead.  activation: "silu" or "gelu"."""
     scaling = 1.0 if routed_scaling_factor is None else float(routed_scaling_factor)

@@ -21,6 +21,10 @@ def _layer(e, h, i, seed=0, scale=0.1):
     return out
 
 
+def _np(t):
+    return t.double().cpu().numpy()
+
+
 def _values(q, s):
     return O.values(O.unpack(q.cpu().numpy()), mxfp4.unpack_mxfp4_scales(s.cpu(), q.shape[-1] * 2).numpy())
 
@@ -120,6 +124,36 @@ def test_five_to_eight_slots_to_an_expert(dev, t, e, topk, h, i):
     out = mxfp4.fused_experts_mxfp4(x, w1, w2, weights, ids, s1, s2)
     _check(out, x, layer, weights, ids)
     assert torch.equal(out, mxfp4.fused_experts_mxfp4(x, w1, w2, weights, ids, s1, s2))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,e,topk,h,i", [(1, 8, 4, 512, 288), (9, 16, 4, 1024, 256), (40, 6, 2, 256, 544), (70, 64, 4, 256, 96)])
+def test_the_intermediate_costs_no_precision(dev, t, e, topk, h, i, dtype):
+    """The whole error is that of the result's rounding, 2^-8 or 2^-11 at most and some 0.4 of it in the norm.  The pairs of the intermediate
+    are off by 2^-16 of a term at most, float32 sums by (h + i) * 2^-24 and the activation by 2^-18; the roundings of different terms are
+    independent, so that in the norm they add up like the terms themselves do, whose sizes add up to under 32 times the result (checked)
+    and their squares' root to a few times it: a tenth of float16's 0.4 * 2^-11, whose square is within the 1.1."""
+    layer = _layer(e, h, i, t)
+    (w1, s1), (w2, s2) = layer
+    x, weights, ids = _inputs(t, h, e, topk, dtype, e)
+    out = mxfp4.fused_experts_mxfp4(x, w1, w2, weights, ids, s1, s2)
+    ref, size = O.experts(x.double().cpu().numpy(), _values(w1, s1), _values(w2, s2), weights.double().cpu().numpy(), ids.cpu().numpy(), "silu", False, 1.0)
+    assert np.linalg.norm(size) < 32 * np.linalg.norm(ref)
+    rounded = torch.from_numpy(ref).to(dtype).double().numpy()
+    assert np.linalg.norm(_np(out) - ref) <= 1.1 * np.linalg.norm(rounded - ref)
+
+
+def test_intermediate_beyond_float16(dev):
+    """gate * up above 65504 with results that float16 holds."""
+    layer = [mxfp4.quant_weight_mxfp4((torch.randn((3, n, k), generator=torch.Generator().manual_seed(n)) * c).cuda()) for n, k, c in
+             ((192, 128, 3.0), (128, 96, 2.0**-12))]
+    (w1, s1), (w2, s2) = layer
+    x, weights, ids = _inputs(5, 128, 3, 2, torch.float16)
+    x = x * 20
+    v1 = _values(w1, s1)
+    products = np.einsum("tk,enk->ten", x.double().cpu().numpy(), v1)
+    assert (products[..., :96] * products[..., 96:]).max() > 2 * 65504
+    _check(mxfp4.fused_experts_mxfp4(x, w1, w2, weights, ids, s1, s2), x, layer, weights, ids)
 
 
 def test_what_no_expert_takes_is_never_multiplied(dev):
