@@ -270,7 +270,7 @@ __global__ __launch_bounds__(256, RX == 4 ? 4 : 2) void mx_experts_up_kernel(con
       buf_load16_to_lds<once.value>(rW, vo0 + ko, 0, own);
       buf_load16_to_lds<once.value>(rW, vo1 + ko, 0, own + 1024);
       buf_load16_to_lds<once.value>(rW, vo0 + (ko + up_rows), 0, own + 2048);
-      buf_load16_to_lds<once.value>(rW, vo1 + (ko + up_rows), 0, own + 3072);
+      buf_load16_to_lds<once.value>(rW, vo1 + (ko + up_rows), 0, own + 3 * 1024);
     };
     if (ntiles == 1) lines(std::true_type{});
     else lines(std::false_type{});  // the next tile reads them again
