@@ -31,7 +31,9 @@ __device__ __forceinline__ v4f mfma16(v4i a, v4i b, v4f c) {
   if (DT == FP8K_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
-// Eight codes become eight 16-bit floats, for bfloat16 times their scale: it has float32's exponents, so that code * scale is exact.
+// Eight codes become eight 16-bit floats, for bfloat16 times their scale: it has float32's exponents (subnormal ones too), so that code *
+// scale is exact wherever float32 holds it - with every scale up to 2^125, the largest that quantisation makes.  4 and 6 times 2^126 and
+// 2 to 6 times 2^127 are infinite, as mxfp4_dequant gives them.
 template <int DT>
 __device__ __forceinline__ v4i mx_floats(uint32_t c, float scale) {
   v4i b;
@@ -107,6 +109,14 @@ __device__ __forceinline__ float mx_block_scale(uint32_t lo, uint32_t hi, int j)
   if (DT != FP8K_BF16) return e8m0_f32((word >> ((j & 3) * 8)) & 255u);
   const int up = 23 - (j & 3) * 8;
   return __uint_as_float((up < 0 ? word >> 1 : word << (up < 0 ? 0 : up)) & 0x7f800000u);
+}
+
+// Mask of the two scale words of K block kb that leaves out the bytes of blocks at or past the end of the rows.  A row's last word stands
+// in place of one behind it, and the codes there are those of the next row: their product must not meet the zeros of the activations as
+// an infinity.
+__device__ __forceinline__ uint64_t mx_scales_there(int k, int kb) {
+  const int have = (k >> 5) - kb * (kMxStep / kMxBlock);
+  return have >= 8 ? ~0ull : (1ull << (8 * have)) - 1;
 }
 
 // The table of the second launch: slots sorted by expert (and by their number within one), cut into tiles of up to p.tile slots of one
@@ -291,7 +301,7 @@ __global__ __launch_bounds__(256, RX == 4 ? 4 : 2) void mx_experts_up_kernel(con
   v4f ag = {0.f, 0.f, 0.f, 0.f}, au = {0.f, 0.f, 0.f, 0.f};
   const uint32_t xrd = (uint32_t)(kX + (r & (RX - 1)) * 512);
   const int xkey = (r & 3) << 2;
-  auto block = [&](bool more) __attribute__((always_inline)) {
+  auto block = [&](int kb, bool more) __attribute__((always_inline)) {
     wait_vm<0>();
     uint32_t s[4];
 #pragma unroll
@@ -307,6 +317,9 @@ __global__ __launch_bounds__(256, RX == 4 ? 4 : 2) void mx_experts_up_kernel(con
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // everything is out of its slot
     SB();
     if (more) request();
+    const uint64_t there = mx_scales_there(p.H, kb);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) s[k] &= (uint32_t)(there >> (32 * (k & 1)));
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       ag = mx_mac<DT>(ag, x[j], cg[j], mx_block_scale<DT>(s[0], s[1], j));
@@ -361,7 +374,7 @@ __global__ __launch_bounds__(256, RX == 4 ? 4 : 2) void mx_experts_up_kernel(con
   const int all = nstrips * ntiles * nb;
   int ci = 0, ctile = 0, cstrip = 0;
   for (int q = 0; q < all; ++q) {
-    block(q + 1 < all);
+    block(w + NW * ci, q + 1 < all);
     if (++ci == nb) {
       finish(cstrip, ctile);
       ci = 0;
@@ -494,11 +507,14 @@ __global__ __launch_bounds__(NW * 64, RX == 4 && TC <= 32 ? 4 : (NW + 3) / 4) vo
       uint32_t c[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) c[j] = codes.get(own, j);
-      const uint32_t s0 = *reinterpret_cast<const uint32_t*>(own + kS + r * 4), s1 = *reinterpret_cast<const uint32_t*>(own + kS + 64 + r * 4);
+      uint32_t s0 = *reinterpret_cast<const uint32_t*>(own + kS + r * 4), s1 = *reinterpret_cast<const uint32_t*>(own + kS + 64 + r * 4);
       v4i x[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const v4i*>(own + xrd + (((j * 4 + kq) ^ xkey) << 4));
       SB();
+      const uint64_t there = mx_scales_there(p.I, ckb);
+      s0 &= (uint32_t)there;
+      s1 &= (uint32_t)(there >> 32);
       // two chains of products: one result waits for the one before it
       acc = mx_mac<FP8K_BF16>(acc, x[0], c[0], mx_block_scale<FP8K_BF16>(s0, s1, 0));
       odd = mx_mac<FP8K_BF16>(odd, x[1], c[1], mx_block_scale<FP8K_BF16>(s0, s1, 1));
