@@ -640,7 +640,7 @@ bool mx_operand(const Tensor& q, const Tensor& s, int64_t dim, int device) {
   if ((uintptr_t)q.data_ptr() % 16 != 0 || s.size(-1) != ceil_div(q.size(-1), 64)) return false;
   for (int64_t d = 0; d + 1 < dim; ++d)
     if (s.size(d) != q.size(d) || q.stride(d) % 16 != 0 || q.stride(d) < 0) return false;
-  return true;
+  return q.size(-2) == 1 || q.stride(-2) >= q.size(-1);  // rows that overlap (an expanded one) are the dispatcher path's to copy
 }
 
 // rows of 16-bit or 32-bit activations that the kernels read as they lie in memory
