@@ -171,14 +171,28 @@ _register(
 )
 
 # ---- MXFP4 (sgl_kernel.py, mxfp4.py)
-_register("mxfp4_quant(Tensor input, Tensor(a!) output_q, Tensor(b!) output_s, bool fuse_silu_and_mul=False) -> ()", _k.mxfp4_quant, _none)
-_register("mxfp4_dequant(Tensor q, Tensor s, Tensor(a!) out) -> ()", _k.mxfp4_dequant, _none)
+def _mx_rows(t: torch.Tensor, step: int) -> torch.Tensor:
+    """t [rows, n] as it is where the kernels can read it - contiguous rows that start at multiples of 16 bytes, `step` elements - else a
+    copy.  Made inside the operators, where a traced call has its address too."""
+    if t.dim() == 2 and t.numel() > 0 and (t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % step != 0 or t.stride(0) < t.shape[1]))):
+        t = t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 else t
+
+
+_register(
+    "mxfp4_quant(Tensor input, Tensor(a!) output_q, Tensor(b!) output_s, bool fuse_silu_and_mul=False) -> ()",
+    lambda input, output_q, output_s, fuse_silu_and_mul=False: _k.mxfp4_quant(_mx_rows(input, 8), output_q, output_s, fuse_silu_and_mul),
+    _none,
+)
+_register("mxfp4_dequant(Tensor q, Tensor s, Tensor(a!) out) -> ()",
+          lambda q, s, out: _k.mxfp4_dequant(_mx_rows(q.contiguous(), 16), s, out), _none)
 _register("mxfp4_scaled_mm(Tensor mat_a, Tensor mat_b, Tensor scales_a, Tensor scales_b, ScalarType out_dtype, Tensor? bias=None) -> Tensor",
-          _k.mxfp4_scaled_mm,
+          lambda mat_a, mat_b, scales_a, scales_b, out_dtype, bias=None: _k.mxfp4_scaled_mm(_mx_rows(mat_a, 16), _mx_rows(mat_b, 16), scales_a,
+                                                                                           scales_b, out_dtype, bias),
           lambda mat_a, mat_b, scales_a, scales_b, out_dtype, bias=None: mat_a.new_empty((mat_a.shape[0], mat_b.shape[0]), dtype=out_dtype))
 _register("mxfp4_experts(Tensor hidden_states, Tensor w1, Tensor w2, Tensor topk_weights, Tensor topk_ids, Tensor w1_scale, "
           "Tensor w2_scale, Tensor(a!) out, str activation, bool apply_router_weight_on_input, float routed_scaling_factor) -> ()",
-          _k.mxfp4_experts, _none)
+          lambda hidden_states, *args: _k.mxfp4_experts(_mx_rows(hidden_states, 8), *args), _none)
 
 _ops = torch.ops.fp8k
 

@@ -72,7 +72,7 @@ def per_token_group_quant_mxfp4(x: torch.Tensor, fuse_silu_and_mul: bool = False
     m, k = x.shape[0], x.shape[1] // 2 if fuse_silu_and_mul else x.shape[1]
     q = torch.empty((m, k // 2), dtype=torch.uint8, device=x.device)
     s = create_mxfp4_scales((m, k), x.device)
-    _ops.mxfp4_quant(_aligned_rows(x, 8), q, s, fuse_silu_and_mul)
+    _ops.mxfp4_quant(x, q, s, fuse_silu_and_mul)
     return q, s
 
 
@@ -86,7 +86,7 @@ def quant_weight_mxfp4(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor
     q = torch.empty((e, n, k // 2), dtype=torch.uint8, device=weight.device)
     s = create_mxfp4_scales((e, n, k), weight.device)
     for i in range(e):
-        _ops.mxfp4_quant(_aligned_rows(weight[i], 8), q[i], s[i])
+        _ops.mxfp4_quant(weight[i], q[i], s[i])
     return q, s
 
 
@@ -98,17 +98,8 @@ def mxfp4_dequant(q: torch.Tensor, s: torch.Tensor, dtype: torch.dtype) -> torch
         if out is not None:
             return out
     out = torch.empty(q.shape[:-1] + (q.shape[-1] * 2,), dtype=dtype, device=q.device)
-    _ops.mxfp4_dequant(q.contiguous(), s, out)
+    _ops.mxfp4_dequant(q, s, out)
     return out
-
-
-def _aligned_rows(t: torch.Tensor, step: int) -> torch.Tensor:
-    """t [rows, n] as it is where the kernels can read it - contiguous rows that start at multiples of 16 bytes - else a copy."""
-    if t.dim() == 2 and t.numel() > 0 and (t.stride(1) != 1 or (t.shape[0] > 1 and (t.stride(0) % step != 0 or t.stride(0) < t.shape[1]))):
-        return t.contiguous()
-    if not torch.compiler.is_compiling() and t.is_cuda and not isinstance(t, torch._subclasses.fake_tensor.FakeTensor) and t.data_ptr() % 16:
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
 
 
 def w4a4_mxfp4_matmul(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs: torch.Tensor, output_dtype: torch.dtype = torch.bfloat16,
@@ -119,7 +110,7 @@ def w4a4_mxfp4_matmul(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs: to
         out = _host.mx_matmul(A, B, As, Bs, output_dtype, bias)
         if out is not None:
             return out
-    return _ops.mxfp4_scaled_mm(_aligned_rows(A, 16), _aligned_rows(B, 16), As, Bs, output_dtype, bias)
+    return _ops.mxfp4_scaled_mm(A, B, As, Bs, output_dtype, bias)
 
 
 def w4a4_mxfp4_linear(input: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, input_scale: Optional[torch.Tensor] = None,
@@ -176,6 +167,6 @@ def fused_experts_mxfp4(
         if out is not None:
             return out
     out = torch.empty(hidden_states.shape, dtype=hidden_states.dtype, device=hidden_states.device)
-    _ops.mxfp4_experts(_aligned_rows(hidden_states, 8), w1, w2, topk_weights.contiguous(), topk_ids.contiguous(), w1_scale, w2_scale, out,
+    _ops.mxfp4_experts(hidden_states, w1, w2, topk_weights.contiguous(), topk_ids.contiguous(), w1_scale, w2_scale, out,
                        activation, apply_router_weight_on_input, scaling)
     return hidden_states.copy_(out) if inplace else out

@@ -24,3 +24,75 @@ def test_expanded_operands(dev):
     for rows in (x, x[:1], x.expand(3, 5, 288), x[:1].expand(4, 288)):
         got = mxfp4.w4a4_mxfp4_linear(rows, w[:1].expand(16, -1), ws[:1].expand(16, -1))
         assert torch.equal(got, mxfp4.w4a4_mxfp4_linear(rows.contiguous(), w[:1].repeat(16, 1), ws[:1].repeat(16, 1)))
+
+
+def _shifted(t, elements):
+    """t's values in rows that start `elements` elements behind a multiple of 16 bytes, a multiple of 16 bytes apart."""
+    wide = torch.zeros((t.shape[0], t.shape[1] + 64), dtype=t.dtype, device=t.device)
+    wide[:, elements:elements + t.shape[1]] = t
+    view = wide[:, elements:elements + t.shape[1]]
+    assert view.data_ptr() % 16 != 0 and view.stride(0) * view.element_size() % 16 == 0
+    return view
+
+
+def _experts(e, h, i):
+    (w1, s1), (w2, s2) = mxfp4.quant_weight_mxfp4(_random((e, 2 * i, h), seed=3) * 0.1), mxfp4.quant_weight_mxfp4(_random((e, h, i), seed=4) * 0.1)
+    return w1, w2, s1, s2
+
+
+# 20 rows: both ways of a linear are a quantisation and a product then
+X, W, E = (20, 288), (72, 288), (5, 288, 96)
+
+
+def _calls(place):
+    """Every entry point, its operand laid out by `place`."""
+    w, ws = mxfp4.quant_weight_mxfp4(_random(W, seed=1))
+    q, s = mxfp4.per_token_group_quant_mxfp4(_random(X))
+    w1, w2, s1, s2 = _experts(*E)
+    weights, ids = torch.rand((X[0], 2), generator=torch.Generator().manual_seed(5)).cuda(), (torch.arange(2 * X[0], device="cuda") % E[0]).view(X[0], 2)
+    x, gate_up = _random(X), _random((X[0], 2 * X[1]), torch.float16, seed=6)
+    return [("quant", lambda t: mxfp4.per_token_group_quant_mxfp4(t), place(x)), ("quant32", lambda t: mxfp4.per_token_group_quant_mxfp4(t), place(x.float())),
+            ("silu", lambda t: mxfp4.per_token_group_quant_mxfp4(t, True), place(gate_up)),
+            ("dequant", lambda t: mxfp4.mxfp4_dequant(t, s, torch.float16), place(q)),
+            ("matmul", lambda t: mxfp4.w4a4_mxfp4_matmul(t, w, s, ws), place(q)), ("weight", lambda t: mxfp4.w4a4_mxfp4_matmul(q, t, s, ws), place(w)),
+            ("linear", lambda t: mxfp4.w4a4_mxfp4_linear(t, w, ws), place(x)),
+            ("experts", lambda t: mxfp4.fused_experts_mxfp4(t, w1, w2, weights, ids, s1, s2), place(x))]
+
+
+def _equal(a, b):
+    a, b = (t if isinstance(t, tuple) else (t,) for t in (a, b))
+    return len(a) == len(b) and all(torch.equal(t, u) for t, u in zip(a, b))
+
+
+@pytest.mark.parametrize("name", ["quant", "quant32", "silu", "dequant", "matmul", "weight", "linear", "experts"])
+def test_rows_that_start_anywhere(dev, name):
+    """Operands that do not start at a multiple of 16 bytes: a view of other rows, and contiguous memory; eager and traced."""
+    want, got = [], []
+    for place in (lambda t: t, lambda t: _shifted(t, 3), lambda t: _shifted(t.flatten()[None], 1).view(t.shape)):
+        fn, t = next((f, t) for n, f, t in _calls(place) if n == name)
+        want.append(fn(t))
+        torch._dynamo.reset()
+        got.append(torch.compile(fn, backend="aot_eager", fullgraph=True)(t))
+    assert all(_equal(w, want[0]) for w in want), "eager"
+    assert all(_equal(g, want[0]) for g in got), "traced"
+
+
+def test_traced_once_for_both_alignments(dev):
+    """One trace serves operands of the same shape and strides at any address."""
+    w, ws = mxfp4.quant_weight_mxfp4(_random(W, seed=1))
+    x = _random(X)
+    wide = torch.zeros((X[0], X[1] + 64), dtype=x.dtype, device=dev)
+    fn = torch.compile(lambda t: mxfp4.w4a4_mxfp4_linear(t, w, ws), backend="aot_eager", fullgraph=True)
+    for at in (0, 8, 5, 16, 1):
+        wide[:, at:at + X[1]] = x
+        assert torch.equal(fn(wide[:, at:at + X[1]]), mxfp4.w4a4_mxfp4_linear(x, w, ws)), at
+
+
+def test_inplace_experts_of_a_view(dev):
+    w1, w2, s1, s2 = _experts(*E)
+    x = _random(X)
+    weights, ids = torch.rand((X[0], 2), generator=torch.Generator().manual_seed(5)).cuda(), (torch.arange(2 * X[0], device="cuda") % E[0]).view(X[0], 2)
+    want = mxfp4.fused_experts_mxfp4(x, w1, w2, weights, ids, s1, s2)
+    view = _shifted(x, 3)
+    got = mxfp4.fused_experts_mxfp4(view, w1, w2, weights, ids, s1, s2, inplace=True)
+    assert got.data_ptr() == view.data_ptr() and torch.equal(view, want)
