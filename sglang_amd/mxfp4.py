@@ -77,16 +77,21 @@ def per_token_group_quant_mxfp4(x: torch.Tensor, fuse_silu_and_mul: bool = False
 
 
 def quant_weight_mxfp4(weight: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
-    """A weight [.., N, K] of any float type -> (codes, scales), once after loading; expert stacks [E, N, K] matrix by matrix."""
-    if weight.dim() == 2:
-        return per_token_group_quant_mxfp4(weight)
-    if weight.dim() != 3:
+    """A weight [.., N, K] of any float type -> (codes, scales), once after loading; expert stacks [E, N, K] matrix by matrix.  Types other
+    than float32, float16 and bfloat16 are taken as their float32 values."""
+    if weight.dim() not in (2, 3):
         raise RuntimeError("quant_weight_mxfp4: [N, K] or [E, N, K] expected")
+
+    def readable(w: torch.Tensor) -> torch.Tensor:
+        return w.float() if w.is_floating_point() and w.dtype not in (torch.float32, torch.float16, torch.bfloat16) else w
+
+    if weight.dim() == 2:
+        return per_token_group_quant_mxfp4(readable(weight))
     e, n, k = weight.shape
     q = torch.empty((e, n, k // 2), dtype=torch.uint8, device=weight.device)
     s = create_mxfp4_scales((e, n, k), weight.device)
     for i in range(e):
-        _ops.mxfp4_quant(weight[i], q[i], s[i])
+        _ops.mxfp4_quant(readable(weight[i]), q[i], s[i])
     return q, s
 
 

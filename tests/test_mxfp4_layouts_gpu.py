@@ -96,3 +96,14 @@ def test_inplace_experts_of_a_view(dev):
     view = _shifted(x, 3)
     got = mxfp4.fused_experts_mxfp4(view, w1, w2, weights, ids, s1, s2, inplace=True)
     assert got.data_ptr() == view.data_ptr() and torch.equal(view, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float64, torch.float32, torch.float16, torch.float8_e4m3fn, torch.float8_e5m2])
+def test_weights_of_any_float_type(dev, dtype):
+    """What the kernel does not read itself goes through float32, which holds every 8-bit value."""
+    w = (_random((3, 40, 96), torch.float32) * 3).to(dtype)
+    for t in (w, w[1]):
+        got, want = mxfp4.quant_weight_mxfp4(t), mxfp4.quant_weight_mxfp4(t.float())
+        assert _equal(got, want)
+    with pytest.raises(RuntimeError):
+        mxfp4.quant_weight_mxfp4(torch.zeros((8, 32), dtype=torch.int32, device=dev))
