@@ -44,6 +44,25 @@ def _as_near_as_its_rounding(out, x, layer, weights, ids, kind="silu", on_input=
     assert np.linalg.norm(_np(out) - ref) <= 1.1 * np.linalg.norm(rounded - ref)
 
 
+# one slot to an expert, a few, five to eight (two tiles of 8 or one), many; over 16, 32 and 64 tokens, and K blocks that end early
+SHAPES = [(1, 8, 4, 512, 288), (9, 6, 2, 160, 96), (20, 20, 5, 288, 160), (40, 32, 5, 256, 96), (60, 32, 3, 544, 64), (64, 64, 8, 256, 96),
+          (70, 6, 2, 256, 288), (100, 16, 1, 128, 288), (128, 64, 4, 160, 96)]
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("kind,on_input", [("silu", False), ("gelu", False), ("silu", True), ("gelu", True)])
+@pytest.mark.parametrize("t,e,topk,h,i", SHAPES)
+def test_every_form_costs_one_rounding(dev, t, e, topk, h, i, kind, on_input, dtype):
+    layer = _layer(e, h, i, t)
+    (w1, s1), (w2, s2) = layer
+    x, weights, ids = _inputs(t, h, e, topk, dtype, e)
+    if on_input:
+        weights = weights + 0.5  # or the activation sees next to nothing
+    ids[:, topk // 2] = torch.where(torch.arange(t, device=dev) % 3 == 1, torch.tensor(-1, dtype=torch.int32, device=dev), ids[:, topk // 2])
+    out = mxfp4.fused_experts_mxfp4(x, w1, w2, weights, ids, s1, s2, activation=kind, apply_router_weight_on_input=on_input, routed_scaling_factor=1.5)
+    _as_near_as_its_rounding(out, x, layer, weights, ids, kind, on_input, 1.5)
+
+
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("t,e,topk", [(1, 4, 2), (6, 4, 2), (40, 4, 2)])
 @pytest.mark.parametrize("h,i", [(32, 32), (128, 96), (160, 128), (224, 160), (256, 256), (288, 224), (416, 288)])
