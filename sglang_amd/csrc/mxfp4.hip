@@ -184,7 +184,9 @@ void launch_tile(MxArgs p, int tm, int tn, hipStream_t st) {
   else ragged ? mx_tile128_kernel<O, B, 128, true><<<grid, 512, 0, st>>>(p) : mx_tile128_kernel<O, B, 128, false><<<grid, 512, 0, st>>>(p);
 }
 
-// strips of 16 NS weight rows: as wide as leaves every CU two workgroups
+// strips of 16 NS weight rows: wider while that leaves two or more for every CU.  Products that are quantised already reach 16 columns a
+// strip up to N = 16352 and 32 from there to the 16384 that plan_of gives them: 16 x 16384 x 7168 13.0 us (16 columns 17.2), 32 rows 15.1 (21.2).
+// Their LDS (96 .. 160 KB) has room for one workgroup on a CU at a time; the quantising form's for two up to 32 columns, for one with 64.
 int strip_groups(int64_t N, int m_blocks, int most) {
   int ns = 1;
   while (ns < most && (N + 32 * ns - 1) / (32 * ns) * m_blocks >= 2 * num_cu()) ns *= 2;
@@ -199,10 +201,8 @@ void launch_strip(const MxArgs& p, hipStream_t st) {
 template <int O, int B>
 void launch_strips(const MxArgs& p, hipStream_t st) {
   if (p.M <= 16) {
-    const int ns = strip_groups(p.N, 1, 4);
-    if (ns == 1) launch_strip<1, 1, false, O, B>(p, st);
-    else if (ns == 2) launch_strip<1, 2, false, O, B>(p, st);
-    else launch_strip<1, 4, false, O, B>(p, st);
+    if (strip_groups(p.N, 1, 2) == 1) launch_strip<1, 1, false, O, B>(p, st);
+    else launch_strip<1, 2, false, O, B>(p, st);
   } else if (p.M <= 32) {
     if (strip_groups(p.N, 1, 2) == 1) launch_strip<2, 1, false, O, B>(p, st);
     else launch_strip<2, 2, false, O, B>(p, st);
