@@ -107,3 +107,48 @@ def test_weights_of_any_float_type(dev, dtype):
         assert _equal(got, want)
     with pytest.raises(RuntimeError):
         mxfp4.quant_weight_mxfp4(torch.zeros((8, 32), dtype=torch.int32, device=dev))
+
+
+@pytest.mark.parametrize("m", [1, 5, 21, 70])
+def test_traced_feed_forward_with_odd_rows(dev, m):
+    """Scale words of a number of rows that is no multiple of four are a view of a padded buffer; tracing hands it from call to call."""
+    up, ups = mxfp4.quant_weight_mxfp4(_random((2 * 96, 288), seed=1))
+    down, downs = mxfp4.quant_weight_mxfp4(_random((288, 96), seed=2))
+
+    def forward(x):
+        q, s = mxfp4.per_token_group_quant_mxfp4(x)
+        h = mxfp4.w4a4_mxfp4_matmul(q, up, s, ups)
+        q, s = mxfp4.per_token_group_quant_mxfp4(h, fuse_silu_and_mul=True)
+        return mxfp4.w4a4_mxfp4_linear(q, down, downs, input_scale=s), mxfp4.mxfp4_dequant(q, s, torch.float32)
+
+    x = _random((m, 288), seed=m)
+    torch._dynamo.reset()
+    for got, want in zip(torch.compile(forward, backend="aot_eager", fullgraph=True)(x), forward(x)):
+        assert torch.equal(got, want)
+
+
+def test_operands_that_want_gradients(dev):
+    """There are none: the results are those of detached operands and require no gradient."""
+    w, ws = mxfp4.quant_weight_mxfp4(_random(W, seed=1))
+    w1, w2, s1, s2 = _experts(*E)
+    x = _random(X)
+    weights, ids = torch.rand((X[0], 2), generator=torch.Generator().manual_seed(5)).cuda(), (torch.arange(2 * X[0], device="cuda") % E[0]).view(X[0], 2)
+    wants = x.clone().requires_grad_()
+    for fn in (lambda t: mxfp4.per_token_group_quant_mxfp4(t)[0], lambda t: mxfp4.w4a4_mxfp4_linear(t, w, ws),
+               lambda t: mxfp4.fused_experts_mxfp4(t, w1, w2, weights, ids, s1, s2)):
+        got = fn(wants)
+        assert torch.equal(got, fn(x)) and not got.requires_grad
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k", [(2, 288), (4, 4096), (16, 160), (20, 288), (70, 1056)])
+def test_rows_that_are_not_finite_stay_alone_in_a_linear(dev, m, k, dtype):
+    """Quantised inside (up to 16 rows) or in front of the product."""
+    w, ws = mxfp4.quant_weight_mxfp4(_random((72, k), seed=1))
+    x = _random((m, k), dtype)
+    clean = mxfp4.w4a4_mxfp4_linear(x, w, ws)
+    bad = x.clone()
+    bad[1, k - 1], bad[m // 2, 0] = float("nan"), float("-inf")
+    got = mxfp4.w4a4_mxfp4_linear(bad, w, ws)
+    rest = torch.tensor([r not in (1, m // 2) for r in range(m)], device=dev)
+    assert torch.equal(got[rest], clean[rest]) and got[1].isnan().all() and got[m // 2].isnan().all()
