@@ -111,12 +111,14 @@ __device__ __forceinline__ float mx_block_scale(uint32_t lo, uint32_t hi, int j)
   return __uint_as_float((up < 0 ? word >> 1 : word << (up < 0 ? 0 : up)) & 0x7f800000u);
 }
 
-// Mask of the two scale words of K block kb that leaves out the bytes of blocks at or past the end of the rows.  A row's last word stands
-// in place of one behind it, and the codes there are those of the next row: their product must not meet the zeros of the activations as
-// an infinity.
-__device__ __forceinline__ uint64_t mx_scales_there(int k, int kb) {
-  const int have = (k >> 5) - kb * (kMxStep / kMxBlock);
-  return have >= 8 ? ~0ull : (1ull << (8 * have)) - 1;
+// Takes the bytes of blocks at or past the end of the rows out of the two scale words of K block kb, the last one of rows of k values.  A
+// row's last word stands in place of one behind it, and the codes there are those of the next row: their product must not meet the zeros
+// of the activations as an infinity.  A branch, kept one by the empty statement: masking every block took 1 % of the layer.
+__device__ __forceinline__ void mx_scales_there(uint32_t& lo, uint32_t& hi, int k, int kb) {
+  const uint64_t there = (1ull << (8 * ((k >> 5) - kb * (kMxStep / kMxBlock)))) - 1;
+  lo &= (uint32_t)there;
+  hi &= (uint32_t)(there >> 32);
+  asm volatile("" : "+v"(lo), "+v"(hi));
 }
 
 // The table of the second launch: slots sorted by expert (and by their number within one), cut into tiles of up to p.tile slots of one
@@ -317,9 +319,10 @@ __global__ __launch_bounds__(256, RX == 4 ? 4 : 2) void mx_experts_up_kernel(con
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // everything is out of its slot
     SB();
     if (more) request();
-    const uint64_t there = mx_scales_there(p.H, kb);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) s[k] &= (uint32_t)(there >> (32 * (k & 1)));
+    if (kb * kMxStep + kMxStep > p.H) {
+      mx_scales_there(s[0], s[1], p.H, kb);
+      mx_scales_there(s[2], s[3], p.H, kb);
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       ag = mx_mac<DT>(ag, x[j], cg[j], mx_block_scale<DT>(s[0], s[1], j));
@@ -512,9 +515,7 @@ __global__ __launch_bounds__(NW * 64, RX == 4 && TC <= 32 ? 4 : (NW + 3) / 4) vo
 #pragma unroll
       for (int j = 0; j < 8; ++j) x[j] = *reinterpret_cast<const v4i*>(own + xrd + (((j * 4 + kq) ^ xkey) << 4));
       SB();
-      const uint64_t there = mx_scales_there(p.I, ckb);
-      s0 &= (uint32_t)there;
-      s1 &= (uint32_t)(there >> 32);
+      if (ckb * kMxStep + kMxStep > p.I) mx_scales_there(s0, s1, p.I, ckb);
       // two chains of products: one result waits for the one before it
       acc = mx_mac<FP8K_BF16>(acc, x[0], c[0], mx_block_scale<FP8K_BF16>(s0, s1, 0));
       odd = mx_mac<FP8K_BF16>(odd, x[1], c[1], mx_block_scale<FP8K_BF16>(s0, s1, 1));
