@@ -517,8 +517,9 @@ int fp8k_mxfp4_linear(const void* x, const void* B, const void* Bs, const void* 
  * x [T, H] of dtype (F16/BF16), row stride ldx elements; w1 [E, 2I, H/2] (gate rows, then up rows), w2 [E, H, I/2], rows contiguous;
  * topk_weights [T, topk], topk_ids [T, topk] int32 or int64; an id outside 0 .. E-1 contributes nothing.
  *   h = act(x . gate^T) * (x . up^T);  out[t] = round(scaling * sum over k of weight[t, k] * h[t, k] . W2^T)
- * with float32 sums; h is held as the sum of two bfloat16 numbers.  weight_on_input: the weight multiplies both products of the first stage instead.  activation: fp8k_activation_kind
- * SILU or GELU.  out [T, H] contiguous may be x.  Workspace: 256-byte aligned, not initialised.
+ * with float32 sums; h is held as the sum of two bfloat16 numbers.  Weights beyond float32's range (4 and 6 times 2^126, 2 to 6 times
+ * 2^127) may count as infinite.  weight_on_input: the weight multiplies both products of the first stage instead.  activation:
+ * fp8k_activation_kind SILU or GELU.  out [T, H] contiguous may be x.  Workspace: 256-byte aligned, not initialised.
  */
 int64_t fp8k_mxfp4_experts_workspace_bytes(int64_t T, int64_t topk, int64_t I);
 int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2, const void* s1, const void* s2, const float* topk_weights,

@@ -200,7 +200,7 @@ __device__ __forceinline__ void mx_sort_slots(const MxExpertArgs& p, int* keys, 
 // waves take every fourth K block each.  What a block needs - the lines of 32 rows, their scale words, the slots' activations - goes
 // straight to an LDS slot of the wave, requested as soon as the operands of the block before are out of it and on across the strips of
 // the run, and no other load stands in the loop.  The four sums meet in LDS; the last wave, which has the fewest blocks, adds them up,
-// applies the activation and writes h, while the others go on.
+// applies the activation and writes h; the others wait for it at a barrier, with their next requests on the way.
 // Bound: the weights' bytes.  One slot to a wave and four workgroups to a CU (RX = 4) beat two slots and two workgroups: 626 against
 // 645 us (64 tokens, 256 experts of 7168 x 2048), 21.0 against 28 (13 tokens, 128 of 4096 x 256): the conversions of one wave run
 // while another waits.  Weights that several tiles read stay in the caches, those that one reads go past them: 166 -> 151 us with 32

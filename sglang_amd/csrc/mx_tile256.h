@@ -1,9 +1,11 @@
 // 256(n) x 256(m) x 256(k) workgroup tiles of the MXFP4 product for large batches, gfx950: 8 wavefronts (2 along n x 4 along m), wave tile
 // 128 x 64 = 8 x 4 products of 16 x 16, a K block being one 128-byte line of a row (256 values, two products of 128).
 //
-// Bound: the matrix cores under the chip's power limit.  A bare loop of e2m1 products on quantised normal data reaches 6.2 PFLOP/s here
-// (8.8 on zeros; the data sheet's rate is 10).  4096 x 18432 x 7168: 252 us, 4.3 PFLOP/s (zeros: 208 us), at 1.77 GHz and with the matrix cores
-// 58 % busy; moving the activation requests of a block apart changed nothing.
+// Bound: issue, at a clock that the power limit sets.  4096 x 18432 x 7168: 252 - 262 us, 4.1 - 4.3 PFLOP/s; the same 455 thousand clocks take 208 -
+// 217 us on zeros, the data lowers the clock from 2.3 to 1.9 GHz.  The matrix cores are 57 % busy in either; a wave issues in 39 % of its
+// clocks, waits for an issue slot in 34 % and at barriers or for memory in 26 % (two waves to a SIMD).  The LDS is busy with reads in 24 %,
+// 4 % of those in bank conflicts.  (A bare loop of e2m1 products reaches 6.2 PFLOP/s on quantised normal data, 8.8 on zeros.)  Moving the
+// activation requests of a block apart changed nothing.
 //
 // Stages, walk and write-out are those of gemm_tile256_kernel: three weight stages and two activation stages of 256 rows x 128 B, filled
 // by buffer_load ... lds with the whole offset in the range-checked per-lane operand, 16-byte chunk c of row r at position

@@ -2,9 +2,11 @@
 //
 // The structure is gemm_tile64_kernel's: one workgroup of four waves per tile, each on every fourth K block (a 128-byte line of every
 // row, 256 values) of the whole tile, its loads going to two LDS slots that nobody else touches; no barrier stands in the K loop, and
-// the four sums meet in LDS at the end, in ascending order.  A block is 32 products of 16x16x128 for 16 KB of operands: bound by the
-// CU's load path (64 B/clk).  128 x 7168 x 16384: 16.5 us (224 tiles, 62 MB of weights; 10.2 at 6.4 TB/s), 64 x 4608 x 7168 10.1.  Eight waves
-// with one slot each were no faster: there 10.1 -> 10.2 us, with 1 GB of weights in turn 18.2 -> 19.7, 64 x 64 x 16384 12.3 -> 14.0.
+// the four sums meet in LDS at the end, in ascending order.  A block is 32 products of 16x16x128 for 16 KB of operands.  Bound: the one
+// wave of a SIMD.  128 x 7168 x 16384: 16.5 us (224 tiles, 62 MB of weights; 10.2 at 6.4 TB/s), in which a wave issues in 46 % of its clocks,
+// waits for an issue slot in 31 % and for memory in 23 %; the matrix cores are 24 % busy.
+// 64 x 4608 x 7168 takes 10.1.  Eight waves with one slot each were no faster: there 10.1 -> 10.2 us, with 1 GB of weights in turn 18.2 ->
+// 19.7, 64 x 64 x 16384 12.3 -> 14.0.
 //
 // Scales: one load each of the two words of a block for 64 weight rows and 64 activation rows (lane = row), handed to the lanes of a row
 // by lane swaps, a byte permute picking those of the lane's chunks kq and 4 + kq.

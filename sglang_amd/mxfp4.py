@@ -160,7 +160,9 @@ def fused_experts_mxfp4(
 
       h = act(x . gate^T) * (x . up^T), out = round(routed_scaling_factor * sum of weight * h . w2^T), sums in float32
 
-    h is held as the sum of two bfloat16 numbers, so that the rounding of the result is the only one that counts.
+    h is held as the sum of two bfloat16 numbers, so that the rounding of the result is the only one that counts.  Weights beyond
+    float32's range (4 and 6 times 2^126, 2 to 6 times 2^127) may count as infinite, as mxfp4_dequant gives them.
+    More tokens are refused: dequantise the experts (mxfp4_dequant) for a grouped product in 16 bits, or call in pieces of 128.
 
     apply_router_weight_on_input: the weight multiplies both products of the first stage instead.  activation: "silu" or "gelu"."""
     scaling = 1.0 if routed_scaling_factor is None else float(routed_scaling_factor)
