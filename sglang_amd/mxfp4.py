@@ -12,7 +12,9 @@ K is a multiple of 32, the number of weight rows of a product a multiple of 8.
 
 Entry points: ``per_token_group_quant_mxfp4`` and ``mxfp4_dequant``; ``w4a4_mxfp4_matmul`` and ``w4a4_mxfp4_linear`` on 4-bit
 activations; ``fused_experts_mxfp4``, a whole expert layer for a few tokens, whose activations stay in 16 bits.  All launch on the
-current stream of their operands' device, never synchronise, and may be captured into a graph.  They compute no gradients.
+current stream of their operands' device, never synchronise, and may be captured into a graph.  They compute no gradients.  Activations and
+codes whose rows the kernels cannot read as they lie (not contiguous, overlapping, not at multiples of 16 bytes) are copied first; stacks of
+expert weights are not.
 """
 from __future__ import annotations
 
@@ -121,7 +123,8 @@ def w4a4_mxfp4_matmul(A: torch.Tensor, B: torch.Tensor, As: torch.Tensor, Bs: to
 def w4a4_mxfp4_linear(input: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, input_scale: Optional[torch.Tensor] = None,
                       bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """input [.., K] float16 / bfloat16, weight codes [N, K/2] -> [.., N] of the input's type: the activations are quantised as
-    per_token_group_quant_mxfp4 does, then multiplied.  With input_scale the input holds codes [.., K/2] already (quantised upstream,
+    per_token_group_quant_mxfp4 does, then multiplied: for a few rows in one launch, traced by torch.compile in two (float32 sums may
+    differ in order).  With input_scale the input holds codes [.., K/2] already (quantised upstream,
     scales [tokens, ceil(K/128)]) and the result is bfloat16."""
     if input_scale is None and not torch.compiler.is_compiling():
         output = _host.mx_linear(input, weight, weight_scale, bias)
@@ -154,7 +157,7 @@ def fused_experts_mxfp4(
 ) -> torch.Tensor:
     """The gated experts of a few tokens - at most 128, and at most 1024 (token, choice) pairs - in two launches.
 
-    hidden_states [T, H] float16 / bfloat16; w1 codes [E, 2I, H/2] (gate rows, then up rows), w2 codes [E, H, I/2]; topk_weights [T, k]
+    hidden_states [T, H] float16 / bfloat16; w1 codes [E, 2I, H/2] (gate rows, then up rows), w2 codes [E, H, I/2], contiguous; topk_weights [T, k]
     and topk_ids [T, k] as the routers of fused_moe return them; an id that is not 0 .. E-1 (-1: an expert of another rank)
     contributes nothing.  Activations stay in 16 bits: with few tokens the layer is bound by the weights' bytes.
 
