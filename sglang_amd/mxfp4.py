@@ -13,8 +13,8 @@ K is a multiple of 32, the number of weight rows of a product a multiple of 8.
 Entry points: ``per_token_group_quant_mxfp4`` and ``mxfp4_dequant``; ``w4a4_mxfp4_matmul`` and ``w4a4_mxfp4_linear`` on 4-bit
 activations; ``fused_experts_mxfp4``, a whole expert layer for a few tokens, whose activations stay in 16 bits.  All launch on the
 current stream of their operands' device, never synchronise, and may be captured into a graph.  They compute no gradients.  Activations and
-codes whose rows the kernels cannot read as they lie (not contiguous, overlapping, not at multiples of 16 bytes) are copied first; stacks of
-expert weights are not.
+codes whose rows the kernels cannot read as they lie (not contiguous, overlapping, not at multiples of 16 bytes) are copied first; the weights
+of the expert layer are not.
 """
 from __future__ import annotations
 

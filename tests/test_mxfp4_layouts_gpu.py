@@ -152,3 +152,35 @@ def test_rows_that_are_not_finite_stay_alone_in_a_linear(dev, m, k, dtype):
     got = mxfp4.w4a4_mxfp4_linear(bad, w, ws)
     rest = torch.tensor([r not in (1, m // 2) for r in range(m)], device=dev)
     assert torch.equal(got[rest], clean[rest]) and got[1].isnan().all() and got[m // 2].isnan().all()
+
+
+def test_threads_and_streams_at_once(dev):
+    """Four threads, each on a stream of its own, through the calls that take scratch memory."""
+    import threading
+
+    w, ws = mxfp4.quant_weight_mxfp4(_random(W, seed=1))
+    w1, w2, s1, s2 = _experts(*E)
+    xs = [_random((21 + 10 * j, X[1]), seed=10 + j) for j in range(4)]
+    weights = [torch.rand((x.shape[0], 2), generator=torch.Generator().manual_seed(5)).cuda() for x in xs]
+    ids = [(torch.arange(2 * x.shape[0], device=dev) % E[0]).view(-1, 2) for x in xs]
+
+    def step(j):
+        return mxfp4.w4a4_mxfp4_linear(xs[j], w, ws), mxfp4.fused_experts_mxfp4(xs[j], w1, w2, weights[j], ids[j], s1, s2)
+
+    want = [step(j) for j in range(4)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(j):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got = [step(j) for _ in range(50)]
+        stream.synchronize()
+        wrong.extend((j, i) for i, g in enumerate(got) if not _equal(g, want[j]))
+
+    threads = [threading.Thread(target=work, args=(j,)) for j in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
