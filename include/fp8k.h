@@ -528,6 +528,68 @@ int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2, const void
                        int64_t s1_stride_w, int64_t s2_stride_e, int64_t s2_stride_n, int64_t s2_stride_w, int activation,
                        int weight_on_input, float scaling, int dtype, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------------------------------ latent attention
+ * A token's keys and values are one row of 576 numbers: a latent of 512, then a position part of 64.  The cache holds rows, in the 16-bit
+ * type of the operands or (cache_is_fp8) in e4m3 with one device-resident scale (NULL: 1): value = code * scale.  It is [pages, page_size, 576],
+ * contiguous; a page table int32 [B, width] (row stride table_stride) names a request's pages in the order of its tokens.  Entries that
+ * are no page of the cache are read as the nearest one.  dtype: F16/BF16.  Strides in elements, multiples of 8; pointers 16-byte aligned.
+ *
+ * fp8k_mla_write_cache: for every token t, latent[t] (row stride ld_latent) goes to row slots[t] (int32 or int64) of the num_slots rows of the
+ * cache; a slot that is none of them (-1: a padded batch) is skipped.  Slots are distinct.  norm_weight (NULL: no norm; of dtype or F32): the latent
+ * becomes x / sqrt(mean(x^2) + eps) * weight.  cos_sin (NULL: no rotation), float32 [max_pos, 64], 32 cosines then 32 sines, row
+ * positions[t] (int32 or int64, held within the table): the position part is rotated, pairs of neighbours, or (neox) of numbers 32 apart.
+ * q_pe (NULL: none) [T, H, 64]: rotated likewise into q_out, which may be q_pe itself.  Float32 throughout, one rounding; e4m3 by
+ * x / scale, to nearest, at most 448 (NaN stays NaN).
+ */
+int fp8k_mla_write_cache(const void* latent, int64_t ld_latent, void* cache, const void* slots, int slots_are_64bit,
+                         const void* norm_weight, int norm_weight_dtype, float eps, const float* cos_sin, int64_t max_pos,
+                         const void* positions, int positions_are_64bit, int neox, const void* q_pe, int64_t q_stride_t,
+                         int64_t q_stride_h, void* q_out, int64_t o_stride_t, int64_t o_stride_h, const float* scale, int64_t T,
+                         int64_t H, int64_t num_slots, int dtype, int cache_is_fp8, void* stream);
+
+/*
+ * Row cu_seqlens[b] + i of out (row stride ld_out) becomes token starts[b] + i (starts NULL: i) of request b, for the rows up to
+ * cu_seqlens[b + 1] (int32 [B + 1], not decreasing) and num_tokens, which out has; rows of no request stay as they are.  Tokens are held within the page table.
+ */
+int fp8k_mla_gather_cache(const void* cache, const int32_t* page_table, int64_t table_stride, int64_t table_width,
+                          const int32_t* cu_seqlens, const int32_t* starts, const float* scale, void* out, int64_t ld_out, int64_t B,
+                          int64_t num_tokens, int64_t pages, int64_t page_size, int dtype, int cache_is_fp8, void* stream);
+
+/*
+ * Absorbed attention of the last n tokens of each request over its seq_lens[b] tokens (int32 [B], held within the page table; the new ones
+ * among them): with row = the cached row, query i of head h
+ *   s[r] = sm_scale * (q_nope[b, i, h] . row[:512] + q_pe[b, i, h] . row[512:]),  r < seq_lens[b] - (n - 1 - i)
+ *   out[b, i, h] = softmax(s) . row[:512],  lse[b, i, h] = log(sum exp(s))   (lse: NULL or float32)
+ * Float32 sums; the exponentials are rounded to dtype for their product with the rows.  A query that sees nothing gets 0 and -inf.
+ * out [B, n, H, 512], lse [B, n, H] contiguous.  sm_scale > 0; B <= 65535, n * H <= 65536.  Workspace: 256-byte aligned,
+ * fp8k_mla_decode_workspace_bytes of it (max_len: table_width * page_size), not initialised.
+ */
+int64_t fp8k_mla_decode_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t max_len);
+int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t qn_stride_n, int64_t qn_stride_h, const void* q_pe,
+                    int64_t qp_stride_b, int64_t qp_stride_n, int64_t qp_stride_h, const void* cache, const int32_t* page_table,
+                    int64_t table_stride, int64_t table_width, const int32_t* seq_lens, const float* scale, void* out, float* lse,
+                    int64_t B, int64_t n, int64_t H, int64_t pages, int64_t page_size, float sm_scale, int dtype, int cache_is_fp8,
+                    void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
+ * Expanded attention over ragged sequences: sequence b has queries cu_seqlens_q[b] .. [b + 1] of q [Tq, H, 192] and keys cu_seqlens_k[b] .. [b + 1]
+ * of k_nope [Tk, H, 128], k_pe [Tk, 64] (all heads') and v [Tk, H, 128] (int32 [B + 1], not decreasing).  Query i of its lq sees (causal) keys j <= i + lk - lq, else all.
+ * out [Tq, H, 128] and lse (NULL or float32 [Tq, H]) contiguous; a query that sees nothing gets 0 and -inf, queries of no sequence
+ * stay as they are.  max_seqlen_q: at least the longest lq.  Keys that a sequence has must be finite; whatever lies outside it may be anything.
+ */
+int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_nope, int64_t kn_stride_t,
+                     int64_t kn_stride_h, const void* k_pe, int64_t kp_stride_t, const void* v, int64_t v_stride_t,
+                     int64_t v_stride_h, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, void* out, float* lse, int64_t B,
+                     int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q, float sm_scale, int causal, int dtype, void* stream);
+
+/*
+ * Two attentions over disjoint keys as one: out = (exp(lse_a) out_a + exp(lse_b) out_b) / (exp(lse_a) + exp(lse_b)), lse = log(exp(lse_a) + exp(lse_b)),
+ * over rows x D numbers of dtype (F16/BF16/F32), D a multiple of 8, all contiguous; out may be out_a or out_b, lse likewise.  A part
+ * with an lse of -inf counts nothing, whatever its row holds; two of them give 0 and -inf.
+ */
+int fp8k_merge_attention_states(const void* out_a, const float* lse_a, const void* out_b, const float* lse_b, void* out, float* lse,
+                                int64_t rows, int64_t D, int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

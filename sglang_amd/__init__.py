@@ -6,6 +6,7 @@ Modules:
   fp8_utils   - ``sglang.srt.layers.quantization.fp8_utils`` entry points (linear apply)
   fused_moe   - block-FP8 fused-experts pipeline
   mxfp4       - 4-bit (MXFP4) quantisation, products, linears, and an expert layer for a few tokens
+  mla         - latent attention: the paged cache, absorbed attention of new tokens, expanded attention of prompts, their join
 """
 import torch
 
@@ -21,4 +22,4 @@ def _check_host() -> None:
 
 _check_host()
 
-__all__ = ["sgl_kernel", "fp8_kernel", "fp8_utils", "fused_moe", "mxfp4"]
+__all__ = ["sgl_kernel", "fp8_kernel", "fp8_utils", "fused_moe", "mxfp4", "mla"]

@@ -107,6 +107,23 @@ SIGNATURES = {
     "fp8k_mxfp4_experts": (
         _c_int, [_c_ptr] * 7 + [_c_int, _c_ptr] + [_c_i64] * 14 + [_c_int, _c_int, _c_f32, _c_int, _c_ptr, _c_i64, _c_ptr],
     ),
+    "fp8k_mla_write_cache": (
+        _c_int, [_c_ptr, _c_i64, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_f32, _c_ptr, _c_i64, _c_ptr, _c_int, _c_int, _c_ptr, _c_i64, _c_i64,
+                 _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _c_ptr],
+    ),
+    "fp8k_mla_gather_cache": (
+        _c_int, [_c_ptr, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr] + [_c_i64] * 5 + [_c_int, _c_int, _c_ptr],
+    ),
+    "fp8k_mla_decode_workspace_bytes": (_c_i64, [_c_i64] * 4),
+    "fp8k_mla_decode": (
+        _c_int, [_c_ptr] + [_c_i64] * 3 + [_c_ptr] + [_c_i64] * 3 + [_c_ptr, _c_ptr, _c_i64, _c_i64] + [_c_ptr] * 4 + [_c_i64] * 5
+        + [_c_f32, _c_int, _c_int, _c_ptr, _c_i64, _c_ptr],
+    ),
+    "fp8k_mla_prefill": (
+        _c_int, [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i64] + [_c_ptr] * 4 + [_c_i64] * 5
+        + [_c_f32, _c_int, _c_int, _c_ptr],
+    ),
+    "fp8k_merge_attention_states": (_c_int, [_c_ptr] * 6 + [_c_i64, _c_i64, _c_int, _c_ptr]),
     "fp8k_moe_fused_gate": (
         _c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr] + [_c_i64] * 6 + [ctypes.c_double, _c_int, _c_int, _c_ptr],
     ),

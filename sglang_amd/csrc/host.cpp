@@ -797,6 +797,227 @@ PyObject* mx_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------------------------- latent attention
+constexpr int64_t kMlaLatent = 512, kMlaRope = 64, kMlaRow = kMlaLatent + kMlaRope, kMlaNope = 128, kMlaValue = 128;
+
+bool aligned16(const Tensor& t) { return (uintptr_t)t.data_ptr() % 16 == 0; }
+
+// rows that the kernels read as they lie: a contiguous last dimension, the others at multiples of 16 bytes
+bool mla_rows(const Tensor& t, int64_t dim, int64_t last, ScalarType dt, int device) {
+  if (!plain(t, device) || t.dim() != dim || t.scalar_type() != dt || t.size(-1) != last || t.stride(-1) != 1 || !aligned16(t)) return false;
+  for (int64_t d = 0; d + 1 < dim; ++d)
+    if (t.stride(d) % 8 != 0 || t.stride(d) < 0) return false;
+  return true;
+}
+
+// a cache [pages, page_size, 576], and one float32 or nothing for its scale
+bool mla_cache(const Tensor& cache, PyObject* so, Tensor& scale, ScalarType dt, int device) {
+  if (!plain(cache, device) || cache.dim() != 3 || cache.size(2) != kMlaRow || cache.numel() == 0 || !cache.is_contiguous() || !aligned16(cache)) return false;
+  if (cache.scalar_type() != dt && !is_fp8(cache)) return false;
+  if (so == Py_None) return true;
+  return is_fp8(cache) && tensor_arg(so, scale) && plain(scale, device) && scale.scalar_type() == ScalarType::Float && scale.numel() == 1;
+}
+
+bool ints(const Tensor& t, int64_t n, int device) {
+  return plain(t, device) && t.dim() == 1 && t.size(0) == n && t.scalar_type() == ScalarType::Int && t.is_contiguous();
+}
+bool int_or_long(const Tensor& t, int64_t n, int device) {
+  return plain(t, device) && t.dim() == 1 && t.size(0) == n && t.is_contiguous() && (t.scalar_type() == ScalarType::Int || t.scalar_type() == ScalarType::Long);
+}
+bool mla_table(const Tensor& t, int64_t rows, int device) {
+  return plain(t, device) && t.dim() == 2 && t.size(0) == rows && t.scalar_type() == ScalarType::Int && t.size(1) > 0 && t.stride(1) == 1 && t.stride(0) >= 0;
+}
+
+float* float_or_null(const Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+
+PyObject* pair(PyObject* first, PyObject* second) {  // takes both
+  PyObject* const out = first && second ? PyTuple_New(2) : nullptr;
+  if (!out) {
+    Py_XDECREF(first);
+    Py_XDECREF(second);
+    return nullptr;
+  }
+  PyTuple_SET_ITEM(out, 0, first);
+  PyTuple_SET_ITEM(out, 1, second);
+  return out;
+}
+PyObject* same(PyObject* o) {
+  Py_INCREF(o);
+  return o;
+}
+
+// mla_write(latent, cache, slots, norm_weight, eps, cos_sin, positions, neox, q_pe, scale, q_out) -> (done, rotated queries or None)
+PyObject* mla_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+#define NOT_DONE                                    \
+  do {                                              \
+    PyErr_Clear();                                  \
+    return pair(same(Py_False), same(Py_None));     \
+  } while (0)
+  Tensor x, cache, slots, weight, table, pos, q, scale, qo;
+  if (n != 11 || modes_active() || !tensor_arg(a[0], x) || !tensor_arg(a[1], cache) || !tensor_arg(a[2], slots) || !PyFloat_Check(a[4]) || !x.is_cuda()) NOT_DONE;
+  const int dev = x.get_device();
+  const ScalarType dt = x.scalar_type();
+  if (!is_half(dt) || !mla_rows(x, 2, kMlaRow, dt, dev) || x.size(0) == 0 || !mla_cache(cache, a[9], scale, dt, dev)) NOT_DONE;
+  const int64_t T = x.size(0);
+  if ((T > 1 && x.stride(0) < kMlaRow) || !int_or_long(slots, T, dev)) NOT_DONE;
+  if (a[3] != Py_None) {
+    if (!tensor_arg(a[3], weight) || !plain(weight, dev) || weight.dim() != 1 || weight.size(0) != kMlaLatent || !weight.is_contiguous() ||
+        !aligned16(weight) || (weight.scalar_type() != dt && weight.scalar_type() != ScalarType::Float))
+      NOT_DONE;
+  }
+  int64_t H = 0;
+  if (a[5] != Py_None) {
+    if (!tensor_arg(a[5], table) || !plain(table, dev) || table.scalar_type() != ScalarType::Float || table.dim() != 2 || table.size(0) == 0 ||
+        table.size(1) != kMlaRope || !table.is_contiguous() || !aligned16(table) || !tensor_arg(a[6], pos) || !int_or_long(pos, T, dev))
+      NOT_DONE;
+    if (a[8] != Py_None) {
+      if (!tensor_arg(a[8], q) || !mla_rows(q, 3, kMlaRope, dt, dev) || q.size(0) != T || q.size(1) == 0) NOT_DONE;
+      if (a[10] != Py_None && (!tensor_arg(a[10], qo) || !mla_rows(qo, 3, kMlaRope, dt, dev) || qo.sizes() != q.sizes())) NOT_DONE;
+      H = q.size(1);
+    } else if (a[10] != Py_None) NOT_DONE;
+  } else if (a[6] != Py_None || a[8] != Py_None || a[10] != Py_None) NOT_DONE;
+#undef NOT_DONE
+  const float eps = (float)PyFloat_AS_DOUBLE(a[4]);
+  const bool neox = truth(a[7]), fresh = H > 0 && !qo.defined();
+  {
+    Call c(x);
+    OBSERVED("mla_write", x, cache, slots, weight, table, pos, q);
+    if (fresh) qo = empty(q.sizes(), dt, x.device());
+    check(fp8k_mla_write_cache(x.data_ptr(), T > 1 ? x.stride(0) : kMlaRow, cache.data_ptr(), slots.data_ptr(), slots.scalar_type() == ScalarType::Long,
+                               weight.defined() ? weight.data_ptr() : nullptr, weight.defined() ? code(weight.scalar_type()) : FP8K_F32, eps,
+                               float_or_null(table), table.defined() ? table.size(0) : 0, pos.defined() ? pos.data_ptr() : nullptr,
+                               pos.defined() && pos.scalar_type() == ScalarType::Long, neox, H ? q.data_ptr() : nullptr, H ? q.stride(0) : 0,
+                               H ? q.stride(1) : 0, H ? qo.data_ptr() : nullptr, H ? qo.stride(0) : 0, H ? qo.stride(1) : 0, float_or_null(scale), T,
+                               H, cache.numel() / kMlaRow, code(dt), is_fp8(cache), c.stream));
+  }
+  return pair(same(Py_True), H == 0 ? same(Py_None) : fresh ? THPVariable_Wrap(std::move(qo)) : same(a[10]));
+  END_HANDLE_TH_ERRORS
+}
+
+// mla_gather(cache, page_table, cu_seqlens, num_tokens, starts, dtype, scale, out) -> rows or None
+PyObject* mla_gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor cache, table, cu, starts, scale, out;
+  if (n != 8 || modes_active() || !tensor_arg(a[0], cache) || !tensor_arg(a[1], table) || !tensor_arg(a[2], cu) || !PyLong_Check(a[3]) ||
+      !THPDtype_Check(a[5]) || !cache.is_cuda())
+    DECLINE;
+  const int dev = cache.get_device();
+  const ScalarType dt = reinterpret_cast<THPDtype*>(a[5])->scalar_type;
+  const int64_t tokens = PyLong_AsLongLong(a[3]);
+  if (PyErr_Occurred() || tokens <= 0 || !is_half(dt) || !mla_cache(cache, a[6], scale, dt, dev) || cu.dim() != 1 || cu.size(0) < 2) DECLINE;
+  const int64_t B = cu.size(0) - 1;
+  if (!ints(cu, B + 1, dev) || !mla_table(table, B, dev)) DECLINE;
+  if (a[4] != Py_None && (!tensor_arg(a[4], starts) || !ints(starts, B, dev))) DECLINE;
+  const bool fresh = a[7] == Py_None;
+  if (!fresh && (!tensor_arg(a[7], out) || !mla_rows(out, 2, kMlaRow, dt, dev) || out.size(0) != tokens || (tokens > 1 && out.stride(0) < kMlaRow))) DECLINE;
+  {
+    Call c(cache);
+    OBSERVED("mla_gather", cache, table, cu);
+    if (fresh) out = empty({tokens, kMlaRow}, dt, cache.device());
+    check(fp8k_mla_gather_cache(cache.data_ptr(), table.data_ptr<int32_t>(), table.stride(0), table.size(1), cu.data_ptr<int32_t>(),
+                                starts.defined() ? starts.data_ptr<int32_t>() : nullptr, float_or_null(scale), out.data_ptr(),
+                                tokens > 1 ? out.stride(0) : kMlaRow, B, tokens, cache.size(0), cache.size(1), code(dt), is_fp8(cache), c.stream));
+  }
+  return fresh ? THPVariable_Wrap(std::move(out)) : same(a[7]);
+  END_HANDLE_TH_ERRORS
+}
+
+// mla_decode(q_nope, q_pe, cache, page_table, seq_lens, sm_scale, scale, return_lse, out) -> output, (output, lse) or None
+PyObject* mla_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, qp, cache, table, lens, scale, out, lse;
+  if (n != 9 || modes_active() || !tensor_arg(a[0], q) || !tensor_arg(a[1], qp) || !tensor_arg(a[2], cache) || !tensor_arg(a[3], table) ||
+      !tensor_arg(a[4], lens) || !PyFloat_Check(a[5]) || !q.is_cuda())
+    DECLINE;
+  const int dev = q.get_device();
+  const ScalarType dt = q.scalar_type();
+  const int64_t dim = q.dim();
+  if (!is_half(dt) || (dim != 3 && dim != 4) || !mla_rows(q, dim, kMlaLatent, dt, dev) || !mla_rows(qp, dim, kMlaRope, dt, dev) || q.numel() == 0) DECLINE;
+  const int64_t B = q.size(0), N = dim == 4 ? q.size(1) : 1, H = q.size(dim - 2);
+  if (qp.size(0) != B || qp.size(dim - 2) != H || (dim == 4 && qp.size(1) != N)) DECLINE;
+  if (!mla_cache(cache, a[6], scale, dt, dev) || !mla_table(table, B, dev) || !ints(lens, B, dev)) DECLINE;
+  const double sm_scale = PyFloat_AS_DOUBLE(a[5]);
+  if (!((float)sm_scale > 0.0f)) DECLINE;
+  const bool want_lse = truth(a[7]), fresh = a[8] == Py_None;
+  if (!fresh && (!tensor_arg(a[8], out) || !plain(out, dev) || out.scalar_type() != dt || out.sizes() != q.sizes() || !out.is_contiguous() || !aligned16(out))) DECLINE;
+  {
+    Call c(q);
+    OBSERVED("mla_decode", q, qp, cache, table, lens);
+    if (fresh) out = empty(q.sizes(), dt, q.device());
+    if (want_lse) lse = empty(q.sizes().slice(0, dim - 1), ScalarType::Float, q.device());
+    const int64_t wsb = fp8k_mla_decode_workspace_bytes(B, N, H, table.size(1) * cache.size(1));
+    Scratch mem(wsb, c.stream);
+    check(fp8k_mla_decode(q.data_ptr(), q.stride(0), dim == 4 ? q.stride(1) : 0, q.stride(dim - 2), qp.data_ptr(), qp.stride(0),
+                          dim == 4 ? qp.stride(1) : 0, qp.stride(dim - 2), cache.data_ptr(), table.data_ptr<int32_t>(), table.stride(0), table.size(1),
+                          lens.data_ptr<int32_t>(), float_or_null(scale), out.data_ptr(), float_or_null(lse), B, N, H, cache.size(0), cache.size(1),
+                          (float)sm_scale, code(dt), is_fp8(cache), mem.take(wsb), wsb, c.stream));
+  }
+  PyObject* const result = fresh ? THPVariable_Wrap(std::move(out)) : same(a[8]);
+  return want_lse ? pair(result, THPVariable_Wrap(std::move(lse))) : result;
+  END_HANDLE_TH_ERRORS
+}
+
+// mla_prefill(q, k_nope, k_pe, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, sm_scale, causal, return_lse, out) -> output, (output, lse) or None
+PyObject* mla_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, kn, kp, v, cu_q, cu_k, out, lse;
+  if (n != 11 || modes_active() || !tensor_arg(a[0], q) || !tensor_arg(a[1], kn) || !tensor_arg(a[2], kp) || !tensor_arg(a[3], v) ||
+      !tensor_arg(a[4], cu_q) || !tensor_arg(a[5], cu_k) || !PyLong_Check(a[6]) || !PyFloat_Check(a[7]) || !q.is_cuda())
+    DECLINE;
+  const int dev = q.get_device();
+  const ScalarType dt = q.scalar_type();
+  if (!is_half(dt) || !mla_rows(q, 3, kMlaNope + kMlaRope, dt, dev) || q.numel() == 0 || !mla_rows(kn, 3, kMlaNope, dt, dev) ||
+      !mla_rows(v, 3, kMlaValue, dt, dev) || !mla_rows(kp, 2, kMlaRope, dt, dev))
+    DECLINE;
+  const int64_t Tq = q.size(0), H = q.size(1), Tk = kn.size(0);
+  if (Tk == 0 || kn.size(1) != H || v.size(0) != Tk || v.size(1) != H || kp.size(0) != Tk || cu_q.dim() != 1 || cu_q.size(0) < 2) DECLINE;
+  const int64_t B = cu_q.size(0) - 1, most = PyLong_AsLongLong(a[6]);
+  if (PyErr_Occurred() || most < 0 || !ints(cu_q, B + 1, dev) || !ints(cu_k, B + 1, dev)) DECLINE;
+  const double sm_scale = PyFloat_AS_DOUBLE(a[7]);
+  if (!((float)sm_scale > 0.0f)) DECLINE;
+  const bool causal = truth(a[8]), want_lse = truth(a[9]), fresh = a[10] == Py_None;
+  if (!fresh && (!tensor_arg(a[10], out) || !plain(out, dev) || out.scalar_type() != dt || out.dim() != 3 || out.size(0) != Tq || out.size(1) != H ||
+                 out.size(2) != kMlaValue || !out.is_contiguous() || !aligned16(out)))
+    DECLINE;
+  {
+    Call c(q);
+    OBSERVED("mla_prefill", q, kn, kp, v, cu_q, cu_k);
+    if (fresh) out = empty({Tq, H, kMlaValue}, dt, q.device());
+    if (want_lse) lse = empty({Tq, H}, ScalarType::Float, q.device());
+    check(fp8k_mla_prefill(q.data_ptr(), q.stride(0), q.stride(1), kn.data_ptr(), kn.stride(0), kn.stride(1), kp.data_ptr(), kp.stride(0), v.data_ptr(),
+                           v.stride(0), v.stride(1), cu_q.data_ptr<int32_t>(), cu_k.data_ptr<int32_t>(), out.data_ptr(), float_or_null(lse), B, H, Tq,
+                           Tk, most, (float)sm_scale, causal, code(dt), c.stream));
+  }
+  PyObject* const result = fresh ? THPVariable_Wrap(std::move(out)) : same(a[10]);
+  return want_lse ? pair(result, THPVariable_Wrap(std::move(lse))) : result;
+  END_HANDLE_TH_ERRORS
+}
+
+// merge_states(out_a, lse_a, out_b, lse_b) -> (out, lse) or None
+PyObject* merge_states(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor x, sx, y, sy, out, lse;
+  if (n != 4 || modes_active() || !tensor_arg(a[0], x) || !tensor_arg(a[1], sx) || !tensor_arg(a[2], y) || !tensor_arg(a[3], sy) || !x.is_cuda()) DECLINE;
+  const int dev = x.get_device();
+  const ScalarType dt = x.scalar_type();
+  if (!plain(x, dev) || !plain(y, dev) || !(is_half(dt) || dt == ScalarType::Float) || y.scalar_type() != dt || x.dim() < 1 || x.numel() == 0 ||
+      x.sizes() != y.sizes() || !x.is_contiguous() || !y.is_contiguous() || !aligned16(x) || !aligned16(y) || x.size(-1) % 8 != 0)
+    DECLINE;
+  for (const Tensor* s : {&sx, &sy})
+    if (!plain(*s, dev) || s->scalar_type() != ScalarType::Float || !s->is_contiguous() || s->sizes() != x.sizes().slice(0, x.dim() - 1)) DECLINE;
+  {
+    Call c(x);
+    OBSERVED("merge_states", x, sx, y, sy);
+    out = empty(x.sizes(), dt, x.device());
+    lse = empty(sx.sizes(), ScalarType::Float, x.device());
+    check(fp8k_merge_attention_states(x.data_ptr(), sx.data_ptr<float>(), y.data_ptr(), sy.data_ptr<float>(), out.data_ptr(), lse.data_ptr<float>(),
+                                      sx.numel(), x.size(-1), code(dt), c.stream));
+  }
+  return pair(THPVariable_Wrap(std::move(out)), THPVariable_Wrap(std::move(lse)));
+  END_HANDLE_TH_ERRORS
+}
+
 // set_workspace(registry, grow): the per-stream GEMM workspaces of sgl_kernel
 PyObject* set_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 2 || !PyDict_Check(a[0]) || !PyCallable_Check(a[1])) {
@@ -813,7 +1034,8 @@ PyObject* set_workspace(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define FN(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FN(group_quant), FN(block_linear), FN(block_matmul), FN(token_linear), FN(mla_quant),     FN(bmm),
                          FN(fused_gate),  FN(fused_experts), FN(mx_quant),     FN(mx_dequant),   FN(mx_matmul),
-                         FN(mx_linear),   FN(mx_experts),    FN(set_workspace), {nullptr, nullptr, 0, nullptr}};
+                         FN(mx_linear),   FN(mx_experts),    FN(mla_write),    FN(mla_gather),    FN(mla_decode),
+                         FN(mla_prefill), FN(merge_states),  FN(set_workspace), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "native calls of the layer-level entry points", -1, methods,
                       nullptr, nullptr, nullptr, nullptr};
 

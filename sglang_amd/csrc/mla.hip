@@ -1,0 +1,427 @@
+// Latent attention: C entry points, the cache's writer and reader, and the join of two attentions.  The attention kernels are in
+// mla_decode.h and mla_prefill.h.
+#include <algorithm>
+
+#include "mla_decode.h"
+#include "mla_prefill.h"
+
+namespace fp8k {
+namespace {
+
+bool is_half_type(int dtype) { return dtype == FP8K_BF16 || dtype == FP8K_F16; }
+
+// ---------------------------------------------------------------------------------------------- cache
+struct MlaWriteArgs {
+  const u16 *latent, *q_pe;
+  void* cache;
+  u16* q_out;
+  const void *slots, *norm_weight, *positions;
+  const float *cos_sin, *scale;
+  int64_t ld_latent, q_t, q_h, o_t, o_h, num_slots, max_pos;
+  int T, H, row_blocks;
+  bool slots64, positions64, weight_f32, neox;
+  float eps;
+};
+
+// 16 numbers of a position part, eight pairs, rotated: pairs of neighbours (x the 16 numbers from 16 part on), or (neox) of numbers that lie
+// 32 apart (x the eight from 8 part on, then the eight from 32 + 8 part on).  table: 32 cosines, 32 sines.
+__device__ __forceinline__ void rotate16(float* x, const float* table, int part, bool neox) {
+  v4f co[2], si[2];
+  co[0] = *(const v4f*)(table + 8 * part);
+  co[1] = *(const v4f*)(table + 8 * part + 4);
+  si[0] = *(const v4f*)(table + 32 + 8 * part);
+  si[1] = *(const v4f*)(table + 32 + 8 * part + 4);
+  if (neox) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float cs = co[i >> 2][i & 3], sn = si[i >> 2][i & 3], a = x[i], b = x[8 + i];
+      x[i] = a * cs - b * sn;
+      x[8 + i] = b * cs + a * sn;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float cs = co[i >> 2][i & 3], sn = si[i >> 2][i & 3], a = x[2 * i], b = x[2 * i + 1];
+      x[2 * i] = a * cs - b * sn;
+      x[2 * i + 1] = b * cs + a * sn;
+    }
+  }
+}
+
+template <int DT>
+__device__ __forceinline__ void load8(const u16* p, float* x) {
+  const v4i v = *(const v4i*)p;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const v2f f = unpack2<DT>((uint32_t)v[i]);
+    x[2 * i] = f[0];
+    x[2 * i + 1] = f[1];
+  }
+}
+template <int DT>
+__device__ __forceinline__ void store8(u16* p, const float* x) {
+  *(v4i*)p = v4i{(int)pack2<DT>(x[0], x[1]), (int)pack2<DT>(x[2], x[3]), (int)pack2<DT>(x[4], x[5]), (int)pack2<DT>(x[6], x[7])};
+}
+// x / scale to e4m3: nearest, ties to even, at most 448; NaN stays NaN
+__device__ __forceinline__ float to_fp8_range(float x, float scale) {
+  const float v = x / scale;
+  return v != v ? v : fminf(fmaxf(v, -kFp8Max), kFp8Max);
+}
+__device__ __forceinline__ void store8_fp8(uint8_t* p, const float* x, float scale) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = to_fp8_range(x[i], scale);
+  *(v2i*)p = v2i{(int)cvt4_fp8(v[0], v[1], v[2], v[3]), (int)cvt4_fp8(v[4], v[5], v[6], v[7])};
+}
+
+// One wave to a token's row, then four threads to the position part of a token's head.  Bound by the bytes, or by the launch.
+template <int DT, bool FP8>
+__global__ __launch_bounds__(256) void mla_write_kernel(const MlaWriteArgs p) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  auto table_of = [&](int t) {
+    const int64_t pos = p.positions64 ? ((const int64_t*)p.positions)[t] : ((const int32_t*)p.positions)[t];
+    return p.cos_sin + min(max(pos, (int64_t)0), p.max_pos - 1) * kRope;
+  };
+  if ((int)blockIdx.x >= p.row_blocks) {
+    const int64_t i = (int64_t)(blockIdx.x - p.row_blocks) * 256 + tid;
+    const int part = (int)(i & 3);
+    const int64_t th = i >> 2;
+    if (th >= (int64_t)p.T * p.H) return;
+    const int t = (int)(th / p.H), h = (int)(th - (int64_t)t * p.H);
+    const int first = p.neox ? 8 * part : 16 * part, second = p.neox ? 32 + 8 * part : 16 * part + 8;
+    const u16* const from = p.q_pe + t * p.q_t + h * p.q_h;
+    u16* const to = p.q_out + t * p.o_t + h * p.o_h;
+    float x[16];
+    load8<DT>(from + first, x);
+    load8<DT>(from + second, x + 8);
+    rotate16(x, table_of(t), part, p.neox);
+    store8<DT>(to + first, x);
+    store8<DT>(to + second, x + 8);
+    return;
+  }
+  const int t = (int)blockIdx.x * 4 + (tid >> 6);
+  if (t >= p.T) return;
+  const int64_t slot = p.slots64 ? ((const int64_t*)p.slots)[t] : ((const int32_t*)p.slots)[t];
+  if (slot < 0 || slot >= p.num_slots) return;
+  const u16* const from = p.latent + t * p.ld_latent;
+  float x[8];
+  load8<DT>(from + 8 * lane, x);
+  if (p.norm_weight) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+    const float f = 1.0f / sqrtf(sum * (1.0f / kLatent) + p.eps);
+    float weight[8];
+    if (p.weight_f32) {
+      *(v4f*)weight = *(const v4f*)((const float*)p.norm_weight + 8 * lane);
+      *(v4f*)(weight + 4) = *(const v4f*)((const float*)p.norm_weight + 8 * lane + 4);
+    } else load8<DT>((const u16*)p.norm_weight + 8 * lane, weight);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * f * weight[i];
+  }
+  const float scale = FP8 && p.scale ? *p.scale : 1.0f;
+  auto store = [&](int at, const float* v) {
+    if (FP8) store8_fp8((uint8_t*)p.cache + slot * kLatentRow + at, v, scale);
+    else store8<DT>((u16*)p.cache + slot * kLatentRow + at, v);
+  };
+  store(8 * lane, x);
+  if (lane < 4) {
+    const int first = p.neox ? 8 * lane : 16 * lane, second = p.neox ? 32 + 8 * lane : 16 * lane + 8;
+    float y[16];
+    load8<DT>(from + kLatent + first, y);
+    load8<DT>(from + kLatent + second, y + 8);
+    if (p.cos_sin) rotate16(y, table_of(t), lane, p.neox);
+    store(kLatent + first, y);
+    store(kLatent + second, y + 8);
+  }
+}
+
+struct MlaGatherArgs {
+  const uint8_t* cache;
+  const int32_t *table, *cu, *starts;
+  const float* scale;
+  u16* out;
+  int64_t table_stride, ld_out;
+  int B, tokens, pages, page_size, table_width;
+};
+
+// One wave to a row at a time: 72 (8-bit: 36) chunks of 16 bytes.  Bound by the bytes.
+template <int DT, bool FP8>
+__global__ __launch_bounds__(256) void mla_gather_kernel(const MlaGatherArgs p) {
+  const int lane = threadIdx.x & 63;
+  const int i = (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6);
+  if (i >= p.tokens || i >= p.cu[p.B] || i < p.cu[0]) return;
+  // the last request that begins at or before row i and is not empty
+  int lo = 0, hi = p.B;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (p.cu[mid] <= i) lo = mid;
+    else hi = mid;
+  }
+  const int64_t tok = min(max((int64_t)i - p.cu[lo] + (p.starts ? p.starts[lo] : 0), (int64_t)0), (int64_t)p.table_width * p.page_size - 1);
+  const int page = (int)(tok / p.page_size);
+  const int64_t e = min(max(p.table[lo * p.table_stride + page], 0), p.pages - 1);
+  const int64_t row = e * p.page_size + (tok - (int64_t)page * p.page_size);
+  u16* const to = p.out + (int64_t)i * p.ld_out;
+  if (FP8) {
+    const float scale = p.scale ? *p.scale : 1.0f;
+    if (lane < 36) {
+      const v4i raw = *(const v4i*)(p.cache + row * kLatentRow + lane * 16);
+      float x[16];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const v2f a = __builtin_amdgcn_cvt_pk_f32_fp8(raw[k], false), b = __builtin_amdgcn_cvt_pk_f32_fp8(raw[k], true);
+        x[4 * k] = a[0] * scale;
+        x[4 * k + 1] = a[1] * scale;
+        x[4 * k + 2] = b[0] * scale;
+        x[4 * k + 3] = b[1] * scale;
+      }
+      store8<DT>(to + lane * 16, x);
+      store8<DT>(to + lane * 16 + 8, x + 8);
+    }
+  } else {
+    const v4i* const from = (const v4i*)(p.cache + row * (2 * kLatentRow));
+    const v4i a = from[lane];
+    ((v4i*)to)[lane] = a;
+    if (lane < 8) ((v4i*)to)[64 + lane] = from[64 + lane];
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- merge
+// out = (e^la a + e^lb b) / (e^la + e^lb), a row of D numbers, eight to a thread.  Bound by the bytes.
+template <int DT>
+__global__ __launch_bounds__(256) void mla_merge_kernel(const void* a, const float* la, const void* b, const float* lb, void* out, float* lse,
+                                                        int64_t rows, int D8) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = i / D8;
+  if (row >= rows) return;
+  const float x = la[row], y = lb[row], top = fmaxf(x, y), shift = shift_of(top);
+  const float ex = __builtin_amdgcn_exp2f((x - shift) * kLog2e), ey = __builtin_amdgcn_exp2f((y - shift) * kLog2e), sum = ex + ey;
+  const float f = sum == 0.0f ? 0.0f : 1.0f / sum, fx = ex * f, fy = ey * f;
+  if (i - row * D8 == 0) lse[row] = sum == 0.0f ? -INFINITY : __builtin_amdgcn_logf(sum) * kLn2 + shift;
+  float u[8], v[8];
+  if constexpr (DT == FP8K_F32) {
+    *(v4f*)u = ((const v4f*)a)[2 * i];
+    *(v4f*)(u + 4) = ((const v4f*)a)[2 * i + 1];
+    *(v4f*)v = ((const v4f*)b)[2 * i];
+    *(v4f*)(v + 4) = ((const v4f*)b)[2 * i + 1];
+  } else {
+    load8<DT>((const u16*)a + 8 * i, u);
+    load8<DT>((const u16*)b + 8 * i, v);
+  }
+  // a part that holds nothing counts nothing, whatever stands in its rows
+#pragma unroll
+  for (int k = 0; k < 8; ++k) u[k] = (x == -INFINITY ? 0.0f : u[k] * fx) + (y == -INFINITY ? 0.0f : v[k] * fy);
+  if constexpr (DT == FP8K_F32) {
+    ((v4f*)out)[2 * i] = *(v4f*)u;
+    ((v4f*)out)[2 * i + 1] = *(v4f*)(u + 4);
+  } else store8<DT>((u16*)out + 8 * i, u);
+}
+
+int64_t up_to(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+// How a decode call is cut: rows of a workgroup (16, 32, 64 or 128), and runs of tiles.  `walkers` workgroups to a block of rows, one
+// workgroup to a CU.  Fewer rows to a workgroup read the cache more often and cut it into fewer runs, whose partials are joined.
+struct DecodePlan {
+  int rows, mblocks, walkers;
+};
+DecodePlan decode_plan(int64_t B, int64_t M, int64_t max_len) {
+  DecodePlan d;
+  d.rows = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : 128;
+  // tiles that the lengths allow, as a table of pages bounds them: with less than two for every CU, more CUs to a tile
+  const int64_t tiles = B * ((max_len + kMlaTile - 1) / kMlaTile);
+  while (d.rows > 32 && tiles * ((M + d.rows - 1) / d.rows) < 2 * num_cu()) d.rows /= 2;
+  d.mblocks = (int)((M + d.rows - 1) / d.rows);
+  d.walkers = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(num_cu(), 256) / d.mblocks, tiles));
+  return d;
+}
+
+}  // namespace
+}  // namespace fp8k
+
+using namespace fp8k;
+
+extern "C" int fp8k_mla_write_cache(const void* latent, int64_t ld_latent, void* cache, const void* slots, int slots_are_64bit,
+                                    const void* norm_weight, int norm_weight_dtype, float eps, const float* cos_sin, int64_t max_pos,
+                                    const void* positions, int positions_are_64bit, int neox, const void* q_pe, int64_t q_stride_t,
+                                    int64_t q_stride_h, void* q_out, int64_t o_stride_t, int64_t o_stride_h, const float* scale, int64_t T,
+                                    int64_t H, int64_t num_slots, int dtype, int cache_is_fp8, void* stream) {
+  clear_error();
+  FP8K_REQUIRE(is_half_type(dtype), "mla write: Half or BFloat16 rows expected");
+  FP8K_REQUIRE(T >= 0 && T < (1ll << 30) && num_slots >= 0 && H >= 0 && H <= (1 << 16), "mla write: bad sizes");
+  if (T == 0) return FP8K_OK;
+  FP8K_REQUIRE(latent && cache && slots, "mla write: null pointer");
+  FP8K_REQUIRE(aligned(latent, 16) && aligned(cache, 16) && ld_latent % 8 == 0 && ld_latent >= kLatentRow, "mla write: rows must be 16-byte aligned");
+  FP8K_REQUIRE(aligned(slots, slots_are_64bit ? 8 : 4), "mla write: misaligned slots");
+  FP8K_REQUIRE(!norm_weight || ((norm_weight_dtype == dtype || norm_weight_dtype == FP8K_F32) && aligned(norm_weight, 16)),
+               "mla write: the norm's weight must be of the rows' type or float32, 16-byte aligned");
+  FP8K_REQUIRE(!cos_sin || (positions && max_pos > 0 && aligned(cos_sin, 16) && aligned(positions, positions_are_64bit ? 8 : 4)),
+               "mla write: the rotation needs positions and a 16-byte aligned table");
+  FP8K_REQUIRE(!q_pe || (cos_sin && q_out && H > 0), "mla write: queries need a table of cosines and sines, and a place");
+  if (q_pe) {
+    FP8K_REQUIRE(aligned(q_pe, 16) && aligned(q_out, 16) && q_stride_t % 8 == 0 && q_stride_h % 8 == 0 && o_stride_t % 8 == 0 && o_stride_h % 8 == 0,
+                 "mla write: queries must be 16-byte aligned");
+    FP8K_REQUIRE(q_stride_t >= 0 && q_stride_h >= 0 && o_stride_t >= 0 && o_stride_h >= 0, "mla write: negative stride");
+  }
+  MlaWriteArgs p{};
+  p.latent = (const u16*)latent; p.q_pe = (const u16*)q_pe; p.cache = cache; p.q_out = (u16*)q_out;
+  p.slots = slots; p.norm_weight = norm_weight; p.positions = positions; p.cos_sin = cos_sin; p.scale = scale;
+  p.ld_latent = ld_latent; p.q_t = q_stride_t; p.q_h = q_stride_h; p.o_t = o_stride_t; p.o_h = o_stride_h;
+  p.num_slots = num_slots; p.max_pos = max_pos; p.T = (int)T; p.H = (int)H;
+  p.row_blocks = (int)((T + 3) / 4);
+  p.slots64 = slots_are_64bit != 0; p.positions64 = positions_are_64bit != 0; p.weight_f32 = norm_weight_dtype == FP8K_F32; p.neox = neox != 0;
+  p.eps = eps;
+  const int64_t q_blocks = q_pe ? (T * H * 4 + 255) / 256 : 0;
+  FP8K_REQUIRE(p.row_blocks + q_blocks < (1ll << 31), "mla write: too large");
+  const dim3 grid((unsigned)(p.row_blocks + q_blocks));
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == FP8K_BF16) {
+    if (cache_is_fp8) mla_write_kernel<FP8K_BF16, true><<<grid, 256, 0, st>>>(p);
+    else mla_write_kernel<FP8K_BF16, false><<<grid, 256, 0, st>>>(p);
+  } else {
+    if (cache_is_fp8) mla_write_kernel<FP8K_F16, true><<<grid, 256, 0, st>>>(p);
+    else mla_write_kernel<FP8K_F16, false><<<grid, 256, 0, st>>>(p);
+  }
+  return check_launch("mla write");
+}
+
+extern "C" int fp8k_mla_gather_cache(const void* cache, const int32_t* page_table, int64_t table_stride, int64_t table_width,
+                                     const int32_t* cu_seqlens, const int32_t* starts, const float* scale, void* out, int64_t ld_out, int64_t B,
+                                     int64_t num_tokens, int64_t pages, int64_t page_size, int dtype, int cache_is_fp8, void* stream) {
+  clear_error();
+  FP8K_REQUIRE(is_half_type(dtype), "mla gather: Half or BFloat16 rows expected");
+  FP8K_REQUIRE(B >= 0 && B < (1 << 24) && num_tokens >= 0 && num_tokens < (1ll << 31), "mla gather: bad sizes");
+  if (B == 0 || num_tokens == 0) return FP8K_OK;
+  FP8K_REQUIRE(pages > 0 && pages < (1ll << 31) && page_size > 0 && page_size < (1ll << 31) && table_width > 0 && table_width < (1ll << 31) && table_stride >= 0,
+               "mla gather: bad sizes of the cache or the page table");
+  FP8K_REQUIRE(cache && page_table && cu_seqlens && out, "mla gather: null pointer");
+  FP8K_REQUIRE(aligned(cache, 16) && aligned(out, 16) && ld_out % 8 == 0 && ld_out >= kLatentRow, "mla gather: rows must be 16-byte aligned");
+  MlaGatherArgs p{};
+  p.cache = (const uint8_t*)cache; p.table = page_table; p.cu = cu_seqlens; p.starts = starts; p.scale = scale; p.out = (u16*)out;
+  p.table_stride = table_stride; p.ld_out = ld_out;
+  p.B = (int)B; p.tokens = (int)num_tokens; p.pages = (int)pages; p.page_size = (int)page_size; p.table_width = (int)table_width;
+  const dim3 grid((unsigned)((num_tokens + 3) / 4));
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == FP8K_BF16) {
+    if (cache_is_fp8) mla_gather_kernel<FP8K_BF16, true><<<grid, 256, 0, st>>>(p);
+    else mla_gather_kernel<FP8K_BF16, false><<<grid, 256, 0, st>>>(p);
+  } else {
+    if (cache_is_fp8) mla_gather_kernel<FP8K_F16, true><<<grid, 256, 0, st>>>(p);
+    else mla_gather_kernel<FP8K_F16, false><<<grid, 256, 0, st>>>(p);
+  }
+  return check_launch("mla gather");
+}
+
+extern "C" int64_t fp8k_mla_decode_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t max_len) {
+  if (B <= 0 || n <= 0 || H <= 0 || max_len <= 0) return 0;
+  const int64_t M = n * H, slots = decode_plan(B, M, max_len).walkers + B;
+  return up_to(slots * M * kLatent * 4, 256) + up_to(slots * M * 4, 256);
+}
+
+extern "C" int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t qn_stride_n, int64_t qn_stride_h, const void* q_pe,
+                               int64_t qp_stride_b, int64_t qp_stride_n, int64_t qp_stride_h, const void* cache, const int32_t* page_table,
+                               int64_t table_stride, int64_t table_width, const int32_t* seq_lens, const float* scale, void* out, float* lse,
+                               int64_t B, int64_t n, int64_t H, int64_t pages, int64_t page_size, float sm_scale, int dtype, int cache_is_fp8,
+                               void* workspace, int64_t workspace_bytes, void* stream) {
+  clear_error();
+  FP8K_REQUIRE(is_half_type(dtype), "mla decode: Half or BFloat16 queries expected");
+  FP8K_REQUIRE(B >= 0 && B <= 65535 && n > 0 && H > 0 && n * H <= (1 << 16), "mla decode: bad sizes");
+  FP8K_REQUIRE(sm_scale > 0.0f && sm_scale < INFINITY, "mla decode: the scale of the scores must be positive and finite");
+  if (B == 0) return FP8K_OK;
+  FP8K_REQUIRE(pages > 0 && pages < (1ll << 31) && page_size > 0 && page_size < (1ll << 31) && table_width > 0 && table_stride >= 0,
+               "mla decode: bad sizes of the cache or the page table");
+  FP8K_REQUIRE(q_nope && q_pe && cache && page_table && seq_lens && out, "mla decode: null pointer");
+  FP8K_REQUIRE(aligned(q_nope, 16) && aligned(q_pe, 16) && aligned(cache, 16) && aligned(out, 16), "mla decode: operands must be 16-byte aligned");
+  FP8K_REQUIRE((qn_stride_b | qn_stride_n | qn_stride_h | qp_stride_b | qp_stride_n | qp_stride_h) % 8 == 0, "mla decode: queries must be 16-byte aligned");
+  FP8K_REQUIRE(qn_stride_b >= 0 && qn_stride_n >= 0 && qn_stride_h >= 0 && qp_stride_b >= 0 && qp_stride_n >= 0 && qp_stride_h >= 0,
+               "mla decode: negative stride");
+  const int64_t max_len = table_width * page_size;
+  FP8K_REQUIRE(table_width < (1ll << 31) && max_len < (1ll << 31) - kMlaTile && B * (max_len / kMlaTile + 1) < (1ll << 31),
+               "mla decode: the page table holds more tokens than 32 bits count");
+  const int64_t need = fp8k_mla_decode_workspace_bytes(B, n, H, max_len);
+  if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
+    return fail(FP8K_ERR_WORKSPACE, "mla decode: workspace of %lld bytes needed, 256-byte aligned", (long long)need);
+  const int64_t M = n * H;
+  const DecodePlan d = decode_plan(B, M, max_len);
+  MlaDecodeArgs p{};
+  p.q_nope = q_nope; p.q_pe = q_pe;
+  p.qn_b = qn_stride_b; p.qn_n = qn_stride_n; p.qn_h = qn_stride_h;
+  p.qp_b = qp_stride_b; p.qp_n = qp_stride_n; p.qp_h = qp_stride_h;
+  p.cache = (const uint8_t*)cache; p.table = page_table; p.table_stride = table_stride; p.lens = seq_lens; p.scale = scale;
+  p.out = out; p.lse = lse;
+  p.part = (float*)workspace;
+  p.part_lse = (float*)((uint8_t*)workspace + up_to((d.walkers + B) * M * kLatent * 4, 256));
+  p.B = (int)B; p.n = (int)n; p.H = (int)H; p.M = (int)M;
+  p.page_size = (int)page_size; p.pages = (int)pages; p.max_len = (int)max_len;
+  p.walkers = d.walkers; p.mblocks = d.mblocks; p.sm_scale = sm_scale;
+  const hipStream_t st = (hipStream_t)stream;
+  const dim3 grid((unsigned)((d.walkers + 7) / 8 * 8 * d.mblocks));
+#define MLA_DECODE(DT, FP8)                                                          \
+  do {                                                                               \
+    if (d.rows == 16) mla_decode_kernel<DT, FP8, 1><<<grid, 256, 0, st>>>(p);        \
+    else if (d.rows == 32) mla_decode_kernel<DT, FP8, 2><<<grid, 512, 0, st>>>(p);   \
+    else if (d.rows == 64) mla_decode_kernel<DT, FP8, 4><<<grid, 512, 0, st>>>(p);   \
+    else mla_decode_kernel<DT, FP8, 8><<<grid, 512, 0, st>>>(p);                     \
+    if (const int rc = check_launch("mla decode")) return rc;                        \
+    mla_join_kernel<DT><<<dim3((unsigned)M, (unsigned)B), 256, 0, st>>>(p);          \
+  } while (0)
+  if (dtype == FP8K_BF16) {
+    if (cache_is_fp8) MLA_DECODE(FP8K_BF16, true);
+    else MLA_DECODE(FP8K_BF16, false);
+  } else {
+    if (cache_is_fp8) MLA_DECODE(FP8K_F16, true);
+    else MLA_DECODE(FP8K_F16, false);
+  }
+#undef MLA_DECODE
+  return check_launch("mla decode");
+}
+
+extern "C" int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_nope, int64_t kn_stride_t,
+                                int64_t kn_stride_h, const void* k_pe, int64_t kp_stride_t, const void* v, int64_t v_stride_t,
+                                int64_t v_stride_h, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, void* out, float* lse, int64_t B,
+                                int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q, float sm_scale, int causal, int dtype, void* stream) {
+  clear_error();
+  FP8K_REQUIRE(is_half_type(dtype), "mla prefill: Half or BFloat16 operands expected");
+  FP8K_REQUIRE(B >= 0 && H > 0 && B < (1 << 24) && H <= (1 << 16) && Tq >= 0 && Tk >= 0 && Tq < (1ll << 31) - 1024 && Tk < (1ll << 31) - 1024 && max_seqlen_q >= 0,
+               "mla prefill: bad sizes");
+  FP8K_REQUIRE(sm_scale > 0.0f && sm_scale < INFINITY, "mla prefill: the scale of the scores must be positive and finite");
+  if (B == 0 || Tq == 0 || max_seqlen_q == 0) return FP8K_OK;
+  FP8K_REQUIRE(q && cu_seqlens_q && cu_seqlens_k && out && (Tk == 0 || (k_nope && k_pe && v)), "mla prefill: null pointer");
+  FP8K_REQUIRE(aligned(q, 16) && aligned(k_nope, 16) && aligned(k_pe, 16) && aligned(v, 16) && aligned(out, 16) &&
+                   (q_stride_t | q_stride_h | kn_stride_t | kn_stride_h | kp_stride_t | v_stride_t | v_stride_h) % 8 == 0,
+               "mla prefill: operands must be 16-byte aligned");
+  FP8K_REQUIRE(q_stride_t >= 0 && q_stride_h >= 0 && kn_stride_t >= 0 && kn_stride_h >= 0 && kp_stride_t >= 0 && v_stride_t >= 0 && v_stride_h >= 0,
+               "mla prefill: negative stride");
+  const int64_t blocks = (std::min(max_seqlen_q, Tq) + kPreRows - 1) / kPreRows, units = up_to(B * H, 8);
+  FP8K_REQUIRE(units * blocks < (1ll << 31), "mla prefill: too many blocks of queries");
+  MlaPrefillArgs p{};
+  p.q = q; p.k_nope = k_nope; p.k_pe = k_pe; p.v = v;
+  p.q_t = q_stride_t; p.q_h = q_stride_h; p.kn_t = kn_stride_t; p.kn_h = kn_stride_h; p.kp_t = kp_stride_t; p.v_t = v_stride_t; p.v_h = v_stride_h;
+  p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.out = out; p.lse = lse;
+  p.B = (int)B; p.H = (int)H; p.Tq = (int)Tq; p.Tk = (int)Tk; p.blocks = (int)blocks; p.causal = causal != 0; p.sm_scale = sm_scale;
+  const dim3 grid((unsigned)(units * blocks));
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == FP8K_BF16) mla_prefill_kernel<FP8K_BF16><<<grid, 256, 0, st>>>(p);
+  else mla_prefill_kernel<FP8K_F16><<<grid, 256, 0, st>>>(p);
+  return check_launch("mla prefill");
+}
+
+extern "C" int fp8k_merge_attention_states(const void* out_a, const float* lse_a, const void* out_b, const float* lse_b, void* out, float* lse,
+                                           int64_t rows, int64_t D, int dtype, void* stream) {
+  clear_error();
+  FP8K_REQUIRE(is_half_type(dtype) || dtype == FP8K_F32, "merge states: float32, Half or BFloat16 expected");
+  FP8K_REQUIRE(rows >= 0 && D > 0 && D % 8 == 0 && D <= (1 << 16), "merge states: the last dimension must be a multiple of 8, at most 65536");
+  if (rows == 0) return FP8K_OK;
+  FP8K_REQUIRE(out_a && lse_a && out_b && lse_b && out && lse, "merge states: null pointer");
+  FP8K_REQUIRE(aligned(out_a, 16) && aligned(out_b, 16) && aligned(out, 16), "merge states: operands must be 16-byte aligned");
+  const int64_t blocks = (rows * (D / 8) + 255) / 256;
+  FP8K_REQUIRE(rows < (1ll << 40) && blocks < (1ll << 31), "merge states: too large");
+  const dim3 grid((unsigned)blocks);
+  const hipStream_t st = (hipStream_t)stream;
+  if (dtype == FP8K_BF16) mla_merge_kernel<FP8K_BF16><<<grid, 256, 0, st>>>(out_a, lse_a, out_b, lse_b, out, lse, rows, (int)(D / 8));
+  else if (dtype == FP8K_F16) mla_merge_kernel<FP8K_F16><<<grid, 256, 0, st>>>(out_a, lse_a, out_b, lse_b, out, lse, rows, (int)(D / 8));
+  else mla_merge_kernel<FP8K_F32><<<grid, 256, 0, st>>>(out_a, lse_a, out_b, lse_b, out, lse, rows, (int)(D / 8));
+  return check_launch("merge states");
+}

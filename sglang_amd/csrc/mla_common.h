@@ -1,0 +1,116 @@
+// Shared pieces of the latent-attention kernels (gfx950): matrix products of 16-bit operands, transposed LDS reads, LDS fills, lane
+// exchange, and the softmax's elementary steps.
+#pragma once
+
+#include "fp8k_common.h"
+
+namespace fp8k {
+
+constexpr int kLatent = 512, kRope = 64, kLatentRow = kLatent + kRope;  // numbers of a cached row
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4v __attribute__((__vector_size__(8)));
+
+// D += A . B, A [16, 32] with lane l holding row l % 16, columns 8 (l / 16) .. + 7; B [32, 16] likewise by columns; D [16, 16] with lane l
+// holding rows 4 (l / 16) .. + 3 of column l % 16
+template <int DT>
+__device__ __forceinline__ v4f mfma16(v4i a, v4i b, v4f c) {
+  if constexpr (DT == FP8K_BF16) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// the same over 16 columns of A: lane l holds columns 4 (l / 16) .. + 3
+template <int DT>
+__device__ __forceinline__ v4f mfma16_half(v2i a, v2i b, v4f c) {
+  if constexpr (DT == FP8K_BF16) return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+}
+// D += A . B, A [32, 16]: lane l holds row l % 32, columns 8 (l / 32) .. + 7; D [32, 32]: element i of lane l is row 8 (i / 4) + 4 (l / 32) + i % 4
+// of column l % 32
+template <int DT>
+__device__ __forceinline__ v16f mfma32(v4i a, v4i b, v16f c) {
+  if constexpr (DT == FP8K_BF16) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (DT == FP8K_BF16) return pack_bf16x2(lo, hi);
+  else {
+    const v2f v = {lo, hi};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+  }
+}
+// the two halves of a word of 16-bit numbers
+template <int DT>
+__device__ __forceinline__ v2f unpack2(uint32_t w) {
+  if constexpr (DT == FP8K_BF16) return v2f{bf16_lo(w), bf16_hi(w)};
+  else return v2f{f16_bits_to_f32(w & 0xffffu), f16_bits_to_f32(w >> 16)};
+}
+// two e4m3 bytes (the low or high half of w) as 16-bit numbers: exact in either type
+template <int DT, bool HIGH>
+__device__ __forceinline__ uint32_t fp8_to_16bit(uint32_t w) {
+  if constexpr (DT == FP8K_BF16) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HIGH));
+}
+
+typedef __attribute__((address_space(3))) void* mla_lds_ptr;
+// 16 bytes from every lane's own address to LDS at base + 16 * lane
+__device__ __forceinline__ void load16_to_lds(const void* p, void* lds_base) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (mla_lds_ptr)lds_base, 16, 0, 0);
+}
+// FIRST .. LAST - 1 of a row of such loads: the lanes' addresses p + STEP * j to base + TO_STEP * j + 16 * lane.  The instruction's offset
+// counts on both sides.
+template <int STEP, int TO_STEP, int FIRST, int LAST>
+__device__ __forceinline__ void load_blocks_to_lds(const uint8_t* p, uint8_t* lds_base) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (mla_lds_ptr)(lds_base + (TO_STEP - STEP) * FIRST), 16, STEP * FIRST, 0);
+  if constexpr (FIRST + 1 < LAST) load_blocks_to_lds<STEP, TO_STEP, FIRST + 1, LAST>(p, lds_base);
+}
+// Transposed read: within 16 lanes, lane i names the 8 bytes of row i / 4, numbers 4 (i % 4) .. + 3, of a block of 4 rows x 16 16-bit
+// numbers, and receives the four rows' number i.
+__device__ __forceinline__ v2i lds_read_transposed(const uint8_t* p) {
+  return __builtin_bit_cast(v2i, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4v*)p));
+}
+
+// v of lane l ^ 32, l ^ 16 combined with one's own
+__device__ __forceinline__ float max_across32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_across16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_across32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float sum_across16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// What an exponent is shifted by: the running maximum, or 0 while a row has seen nothing (-inf minus -inf is no number).
+__device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.0f : m; }
+
+// A row's maximum is raised (and what has been summed rescaled) only when a score passes it by more than this, in powers of two: up to
+// there the exponentials stay below 2^8, which float32 sums and 16-bit weights hold as exactly as those below 1.
+constexpr float kMaxSlack = 8.0f;
+
+// all of the wave's LDS reads and writes, and its loads to LDS, are done
+__device__ __forceinline__ void wait_all() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_all_barrier() {
+  wait_all();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+}  // namespace fp8k

@@ -194,6 +194,60 @@ _register("mxfp4_experts(Tensor hidden_states, Tensor w1, Tensor w2, Tensor topk
           "Tensor w2_scale, Tensor(a!) out, str activation, bool apply_router_weight_on_input, float routed_scaling_factor) -> ()",
           lambda hidden_states, *args: _k.mxfp4_experts(_mx_rows(hidden_states, 8), *args), _none)
 
+# ---- latent attention (sgl_kernel.py, mla.py)
+def _mla_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """t as it is where the kernels can read it - a contiguous last dimension, its rows at multiples of 16 bytes - else a copy."""
+    if t is None or t.numel() == 0:
+        return t
+    if t.stride(-1) != 1 or any(s % 8 != 0 or s < 0 for s in t.stride()[:-1]) or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _mla_latent(t: torch.Tensor) -> torch.Tensor:
+    return t.clone(memory_format=torch.contiguous_format) if t.dim() == 2 and t.shape[0] > 1 and t.stride(0) < t.shape[1] else _mla_rows(t)
+
+
+def _aligned(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t.clone() if t is not None and t.data_ptr() % 16 else t
+
+
+def _mla_write_impl(latent, cache, slots, norm_weight, eps, cos_sin, positions, neox, q_pe, q_out, scale) -> None:
+    place = q_out
+    if q_pe is not None and q_out is not None and q_out.numel() > 0 and _mla_rows(q_out) is not q_out:
+        place = torch.empty(q_out.shape, dtype=q_out.dtype, device=q_out.device)
+    _k.mla_write_cache(_mla_latent(latent), cache, slots.contiguous(), _aligned(norm_weight), eps, _aligned(cos_sin),
+                       positions.contiguous() if positions is not None else None, neox, _mla_rows(q_pe), place, scale)
+    if place is not q_out:
+        q_out.copy_(place)
+
+
+_register("mla_write_cache(Tensor latent, Tensor(a!) cache, Tensor slots, Tensor? norm_weight, float eps, Tensor? cos_sin, "
+          "Tensor? positions, bool neox, Tensor? q_pe, Tensor(b!)? q_out, Tensor? scale) -> ()", _mla_write_impl, _none)
+
+
+def _mla_gather_impl(cache, page_table, cu_seqlens, starts, scale, out) -> None:
+    readable = out.numel() == 0 or (out.stride(-1) == 1 and out.stride(0) % 8 == 0 and out.data_ptr() % 16 == 0)
+    place = out if readable else out.clone(memory_format=torch.contiguous_format)
+    _k.mla_gather_cache(cache, page_table.contiguous(), cu_seqlens.contiguous(), starts.contiguous() if starts is not None else None, scale, place)
+    if place is not out:
+        out.copy_(place)
+
+
+_register("mla_gather_cache(Tensor cache, Tensor page_table, Tensor cu_seqlens, Tensor? starts, Tensor? scale, Tensor(a!) out) -> ()",
+          _mla_gather_impl, _none)
+_register("mla_decode_attention(Tensor q_nope, Tensor q_pe, Tensor cache, Tensor page_table, Tensor seq_lens, float sm_scale, "
+          "Tensor? scale, Tensor(a!) out, Tensor(b!)? lse) -> ()",
+          lambda q_nope, q_pe, cache, page_table, seq_lens, sm_scale, scale, out, lse: _k.mla_decode_attention(
+              _mla_rows(q_nope), _mla_rows(q_pe), cache, page_table.contiguous(), seq_lens.contiguous(), sm_scale, scale, out, lse), _none)
+_register("mla_prefill_attention(Tensor q, Tensor k_nope, Tensor k_pe, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, int max_seqlen_q, "
+          "float sm_scale, bool causal, Tensor(a!) out, Tensor(b!)? lse) -> ()",
+          lambda q, k_nope, k_pe, v, cu_seqlens_q, cu_seqlens_k, *args: _k.mla_prefill_attention(
+              _mla_rows(q), _mla_rows(k_nope), _mla_rows(k_pe), _mla_rows(v), cu_seqlens_q.contiguous(), cu_seqlens_k.contiguous(), *args), _none)
+_register("merge_attention_states(Tensor out_a, Tensor lse_a, Tensor out_b, Tensor lse_b, Tensor(a!) out, Tensor(b!) lse) -> ()",
+          lambda out_a, lse_a, out_b, lse_b, out, lse: _k.merge_attention_states(
+              _aligned(out_a.contiguous()), lse_a.contiguous(), _aligned(out_b.contiguous()), lse_b.contiguous(), out, lse), _none)
+
 _ops = torch.ops.fp8k
 
 # ---------------------------------------------------------------------------------------------------------------
@@ -349,3 +403,23 @@ def mxfp4_experts(hidden_states, w1, w2, topk_weights, topk_ids, w1_scale, w2_sc
                   apply_router_weight_on_input=False, routed_scaling_factor=1.0) -> None:
     _ops.mxfp4_experts(hidden_states, w1, w2, topk_weights, topk_ids, w1_scale, w2_scale, out, activation,
                        apply_router_weight_on_input, float(routed_scaling_factor))
+
+
+def mla_write_cache(latent, cache, slots, norm_weight, eps: float, cos_sin, positions, neox: bool, q_pe, q_out, scale) -> None:
+    _ops.mla_write_cache(latent, cache, slots, norm_weight, float(eps), cos_sin, positions, bool(neox), q_pe, q_out, scale)
+
+
+def mla_gather_cache(cache, page_table, cu_seqlens, starts, scale, out) -> None:
+    _ops.mla_gather_cache(cache, page_table, cu_seqlens, starts, scale, out)
+
+
+def mla_decode_attention(q_nope, q_pe, cache, page_table, seq_lens, sm_scale: float, scale, out, lse) -> None:
+    _ops.mla_decode_attention(q_nope, q_pe, cache, page_table, seq_lens, float(sm_scale), scale, out, lse)
+
+
+def mla_prefill_attention(q, k_nope, k_pe, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q: int, sm_scale: float, causal: bool, out, lse) -> None:
+    _ops.mla_prefill_attention(q, k_nope, k_pe, v, cu_seqlens_q, cu_seqlens_k, int(max_seqlen_q), float(sm_scale), bool(causal), out, lse)
+
+
+def merge_attention_states(out_a, lse_a, out_b, lse_b, out, lse) -> None:
+    _ops.merge_attention_states(out_a, lse_a, out_b, lse_b, out, lse)

@@ -1139,3 +1139,204 @@ def mxfp4_experts(hidden_states: torch.Tensor, w1: torch.Tensor, w2: torch.Tenso
             w2_scale.stride(0), w2_scale.stride(1), w2_scale.stride(2), 1 if activation == "gelu" else 0,
             1 if apply_router_weight_on_input else 0, float(routed_scaling_factor), dtype_code(hidden_states.dtype), ws.data_ptr(), need,
             stream_ptr(hidden_states.device)))
+
+
+# --------------------------------------------------------------------------------------------
+# latent attention (mla.py has the entry points with fresh outputs)
+# --------------------------------------------------------------------------------------------
+
+MLA_LATENT, MLA_ROPE, MLA_ROW = 512, 64, 576   # numbers of a cached row: a latent, then a position part
+MLA_NOPE, MLA_VALUE = 128, 128                 # of a head's expanded key (beside the position part) and value
+_HALVES = (torch.float16, torch.bfloat16)
+
+
+def _mla_cache(cache: torch.Tensor, dtype: torch.dtype, scale: Optional[torch.Tensor]) -> bool:
+    """Checks a cache [pages, page_size, 576] (or [pages, page_size, 1, 576]) and its scale; whether it is 8-bit."""
+    if cache.dim() not in (3, 4) or cache.shape[-1] != MLA_ROW or (cache.dim() == 4 and cache.shape[2] != 1) or not cache.is_contiguous():
+        raise RuntimeError("cache must be contiguous [pages, page_size, 576]")
+    fp8 = cache.dtype == FP8_DTYPE
+    if not fp8 and cache.dtype != dtype:
+        raise RuntimeError("cache must be of the operands' type or float8_e4m3fn")
+    if scale is not None and (not fp8 or scale.dtype != torch.float32 or scale.numel() != 1):
+        raise RuntimeError("scale must be one float32, for a float8_e4m3fn cache")
+    return fp8
+
+
+def _mla_table(page_table: torch.Tensor, rows: int, what: str = "page_table") -> None:
+    if page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != rows or page_table.stride(1) != 1 and page_table.shape[1] > 1:
+        raise RuntimeError("%s must be int32 [requests, pages] with contiguous rows" % what)
+    if page_table.shape[0] > 1 and page_table.stride(0) < 0:
+        raise RuntimeError("%s has a negative stride" % what)
+
+
+def _ints(t: torch.Tensor, shape: tuple, what: str, types=(torch.int32,)) -> None:
+    if t.dtype not in types or tuple(t.shape) != shape or not t.is_contiguous():
+        raise RuntimeError("%s must be contiguous %s %s" % (what, " or ".join(str(x).split(".")[1] for x in types), list(shape)))
+
+
+def mla_write_cache(latent: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor, norm_weight: Optional[torch.Tensor], eps: float,
+                    cos_sin: Optional[torch.Tensor], positions: Optional[torch.Tensor], neox: bool, q_pe: Optional[torch.Tensor],
+                    q_out: Optional[torch.Tensor], scale: Optional[torch.Tensor]) -> None:
+    """Norm, rotation and store of tokens' rows (include/fp8k.h: fp8k_mla_write_cache).  q_out may be q_pe."""
+    _same_device(latent, cache, slots, norm_weight, cos_sin, positions, q_pe, q_out, scale)
+    if latent.dtype not in _HALVES or latent.dim() != 2 or latent.shape[1] != MLA_ROW or latent.stride(1) != 1:
+        raise RuntimeError("latent must be float16 or bfloat16 [tokens, 576] with contiguous rows")
+    T = latent.shape[0]
+    fp8 = _mla_cache(cache, latent.dtype, scale)
+    _ints(slots, (T,), "slots", (torch.int32, torch.int64))
+    if norm_weight is not None and (norm_weight.dtype not in (latent.dtype, torch.float32) or tuple(norm_weight.shape) != (MLA_LATENT,)
+                                    or not norm_weight.is_contiguous()):
+        raise RuntimeError("norm_weight must be contiguous [512] of the rows' type or float32")
+    if cos_sin is None:
+        if positions is not None or q_pe is not None:
+            raise RuntimeError("positions and q_pe need cos_sin")
+    else:
+        if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != MLA_ROPE or cos_sin.shape[0] == 0 or not cos_sin.is_contiguous():
+            raise RuntimeError("cos_sin must be contiguous float32 [positions, 64]")
+        if positions is None:
+            raise RuntimeError("cos_sin needs positions")
+        _ints(positions, (T,), "positions", (torch.int32, torch.int64))
+    H = 0
+    if q_pe is not None:
+        if q_pe.dtype != latent.dtype or q_pe.dim() != 3 or q_pe.shape[0] != T or q_pe.shape[2] != MLA_ROPE or q_pe.stride(2) != 1:
+            raise RuntimeError("q_pe must be [tokens, heads, 64] of the rows' type with a contiguous last dimension")
+        if q_out is None or q_out.dtype != q_pe.dtype or q_out.shape != q_pe.shape or q_out.stride(2) != 1:
+            raise RuntimeError("q_out must be of q_pe's type and shape with a contiguous last dimension")
+        H = q_pe.shape[1]
+    elif q_out is not None:
+        raise RuntimeError("q_out needs q_pe")
+    if T == 0:
+        return
+    if H == 0:
+        q_pe = q_out = None
+    with torch.cuda.device(latent.device):
+        check(lib.fp8k_mla_write_cache(
+            latent.data_ptr(), latent.stride(0) if T > 1 else MLA_ROW, cache.data_ptr(), slots.data_ptr(), 1 if slots.dtype == torch.int64 else 0,
+            _ptr(norm_weight), dtype_code(norm_weight.dtype) if norm_weight is not None else 0, float(eps), _ptr(cos_sin),
+            cos_sin.shape[0] if cos_sin is not None else 0, _ptr(positions), 1 if positions is not None and positions.dtype == torch.int64 else 0,
+            1 if neox else 0, _ptr(q_pe), q_pe.stride(0) if H else 0, q_pe.stride(1) if H else 0, _ptr(q_out), q_out.stride(0) if H else 0,
+            q_out.stride(1) if H else 0, _ptr(scale), T, H, cache.numel() // MLA_ROW, dtype_code(latent.dtype), 1 if fp8 else 0,
+            stream_ptr(latent.device)))
+
+
+def mla_gather_cache(cache: torch.Tensor, page_table: torch.Tensor, cu_seqlens: torch.Tensor, starts: Optional[torch.Tensor],
+                     scale: Optional[torch.Tensor], out: torch.Tensor) -> None:
+    """Rows of cached prefixes, one after the other (include/fp8k.h: fp8k_mla_gather_cache)."""
+    _same_device(cache, page_table, cu_seqlens, starts, scale, out)
+    if out.dtype not in _HALVES or out.dim() != 2 or out.shape[1] != MLA_ROW or out.stride(1) != 1:
+        raise RuntimeError("out must be float16 or bfloat16 [tokens, 576] with contiguous rows")
+    fp8 = _mla_cache(cache, out.dtype, scale)
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] == 0:
+        raise RuntimeError("cu_seqlens must be int32 [requests + 1]")
+    B, tokens = cu_seqlens.shape[0] - 1, out.shape[0]
+    _ints(cu_seqlens, (B + 1,), "cu_seqlens")
+    _mla_table(page_table, B)
+    if starts is not None:
+        _ints(starts, (B,), "starts")
+    if B == 0 or tokens == 0:
+        return
+    if cache.numel() == 0 or page_table.shape[1] == 0:
+        raise RuntimeError("tokens expected of a cache or a page table without pages")
+    with torch.cuda.device(cache.device):
+        check(lib.fp8k_mla_gather_cache(
+            cache.data_ptr(), page_table.data_ptr(), page_table.stride(0) if B > 1 else page_table.shape[1], page_table.shape[1], cu_seqlens.data_ptr(),
+            _ptr(starts), _ptr(scale), out.data_ptr(), out.stride(0) if tokens > 1 else MLA_ROW, B, tokens, cache.shape[0], cache.shape[1],
+            dtype_code(out.dtype), 1 if fp8 else 0, stream_ptr(cache.device)))
+
+
+def mla_decode_attention(q_nope: torch.Tensor, q_pe: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                         sm_scale: float, scale: Optional[torch.Tensor], out: torch.Tensor, lse: Optional[torch.Tensor]) -> None:
+    """Absorbed attention of the last n tokens of each request (include/fp8k.h: fp8k_mla_decode)."""
+    _same_device(q_nope, q_pe, cache, page_table, seq_lens, scale, out, lse)
+    if q_nope.dtype not in _HALVES or q_nope.dim() != 4 or q_nope.shape[3] != MLA_LATENT:
+        raise RuntimeError("q_nope must be float16 or bfloat16 [requests, tokens, heads, 512]")
+    B, n, H, _ = q_nope.shape
+    if q_pe.dtype != q_nope.dtype or tuple(q_pe.shape) != (B, n, H, MLA_ROPE):
+        raise RuntimeError("q_pe must be [requests, tokens, heads, 64] of q_nope's type")
+    if q_nope.stride(3) != 1 or q_pe.stride(3) != 1:
+        raise RuntimeError("q_nope and q_pe must have a contiguous last dimension")
+    fp8 = _mla_cache(cache, q_nope.dtype, scale)
+    _mla_table(page_table, B)
+    _ints(seq_lens, (B,), "seq_lens")
+    if out.dtype != q_nope.dtype or out.shape != q_nope.shape or not out.is_contiguous():
+        raise RuntimeError("out must be contiguous, of q_nope's type and shape")
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (B, n, H) or not lse.is_contiguous()):
+        raise RuntimeError("lse must be contiguous float32 [requests, tokens, heads]")
+    if not 0.0 < sm_scale < float("inf"):
+        raise RuntimeError("sm_scale must be positive and finite")
+    if out.numel() == 0:
+        return
+    width = page_table.shape[1]
+    if cache.numel() == 0 or width == 0:
+        out.zero_()
+        if lse is not None:
+            lse.fill_(float("-inf"))
+        return
+    need = lib.fp8k_mla_decode_workspace_bytes(B, n, H, width * cache.shape[1])
+    with torch.cuda.device(cache.device):
+        ws = torch.empty(need, dtype=torch.uint8, device=cache.device)  # of the current stream: the allocator keeps it in order
+        check(lib.fp8k_mla_decode(
+            q_nope.data_ptr(), q_nope.stride(0), q_nope.stride(1), q_nope.stride(2), q_pe.data_ptr(), q_pe.stride(0), q_pe.stride(1), q_pe.stride(2),
+            cache.data_ptr(), page_table.data_ptr(), page_table.stride(0) if B > 1 else width, width, seq_lens.data_ptr(), _ptr(scale),
+            out.data_ptr(), _ptr(lse), B, n, H, cache.shape[0], cache.shape[1], float(sm_scale), dtype_code(q_nope.dtype), 1 if fp8 else 0,
+            ws.data_ptr(), need, stream_ptr(cache.device)))
+
+
+def mla_prefill_attention(q: torch.Tensor, k_nope: torch.Tensor, k_pe: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
+                          cu_seqlens_k: torch.Tensor, max_seqlen_q: int, sm_scale: float, causal: bool, out: torch.Tensor,
+                          lse: Optional[torch.Tensor]) -> None:
+    """Expanded attention over ragged sequences (include/fp8k.h: fp8k_mla_prefill)."""
+    _same_device(q, k_nope, k_pe, v, cu_seqlens_q, cu_seqlens_k, out, lse)
+    if q.dtype not in _HALVES or q.dim() != 3 or q.shape[2] != MLA_NOPE + MLA_ROPE or q.shape[1] == 0:
+        raise RuntimeError("q must be float16 or bfloat16 [tokens, heads, 192]")
+    Tq, H, _ = q.shape
+    Tk = k_nope.shape[0]
+    if k_nope.dtype != q.dtype or v.dtype != q.dtype or k_pe.dtype != q.dtype:
+        raise RuntimeError("q, k_nope, k_pe and v must be of one type")
+    if tuple(k_nope.shape) != (Tk, H, MLA_NOPE) or tuple(v.shape) != (Tk, H, MLA_VALUE) or tuple(k_pe.shape) != (Tk, MLA_ROPE):
+        raise RuntimeError("k_nope and v must be [keys, heads, 128], k_pe [keys, 64]")
+    if q.stride(2) != 1 or k_nope.stride(2) != 1 or v.stride(2) != 1 or k_pe.stride(1) != 1:
+        raise RuntimeError("q, k_nope, k_pe and v must have a contiguous last dimension")
+    if cu_seqlens_q.dim() != 1 or cu_seqlens_q.shape[0] == 0:
+        raise RuntimeError("cu_seqlens_q must be int32 [sequences + 1]")
+    B = cu_seqlens_q.shape[0] - 1
+    _ints(cu_seqlens_q, (B + 1,), "cu_seqlens_q")
+    _ints(cu_seqlens_k, (B + 1,), "cu_seqlens_k")
+    if out.dtype != q.dtype or tuple(out.shape) != (Tq, H, MLA_VALUE) or not out.is_contiguous():
+        raise RuntimeError("out must be contiguous [tokens, heads, 128] of q's type")
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (Tq, H) or not lse.is_contiguous()):
+        raise RuntimeError("lse must be contiguous float32 [tokens, heads]")
+    if max_seqlen_q < 0:
+        raise RuntimeError("max_seqlen_q must not be negative")
+    if not 0.0 < sm_scale < float("inf"):
+        raise RuntimeError("sm_scale must be positive and finite")
+    if B == 0 or Tq == 0:
+        return
+    with torch.cuda.device(q.device):
+        check(lib.fp8k_mla_prefill(
+            q.data_ptr(), q.stride(0), q.stride(1), k_nope.data_ptr(), k_nope.stride(0), k_nope.stride(1), k_pe.data_ptr(), k_pe.stride(0),
+            v.data_ptr(), v.stride(0), v.stride(1), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), out.data_ptr(), _ptr(lse), B, H, Tq, Tk,
+            int(max_seqlen_q), float(sm_scale), 1 if causal else 0, dtype_code(q.dtype), stream_ptr(q.device)))
+
+
+def merge_attention_states(out_a: torch.Tensor, lse_a: torch.Tensor, out_b: torch.Tensor, lse_b: torch.Tensor, out: torch.Tensor,
+                           lse: torch.Tensor) -> None:
+    """Two attentions over disjoint keys as one (include/fp8k.h: fp8k_merge_attention_states)."""
+    _same_device(out_a, lse_a, out_b, lse_b, out, lse)
+    if out_a.dtype not in _HALVES + (torch.float32,) or out_a.dim() < 1:
+        raise RuntimeError("out_a must be float32, float16 or bfloat16")
+    if out_b.dtype != out_a.dtype or out_b.shape != out_a.shape or out.dtype != out_a.dtype or out.shape != out_a.shape:
+        raise RuntimeError("out_a, out_b and out must be of one type and shape")
+    D = out_a.shape[-1]
+    if D == 0 or D % 8 != 0:
+        raise RuntimeError("the last dimension must be a multiple of 8")
+    for t in (lse_a, lse_b, lse):
+        if t.dtype != torch.float32 or t.shape != out_a.shape[:-1]:
+            raise RuntimeError("lse_a, lse_b and lse must be float32, out_a's shape without the last dimension")
+    if not all(t.is_contiguous() for t in (out_a, lse_a, out_b, lse_b, out, lse)):
+        raise RuntimeError("operands must be contiguous")
+    if out_a.numel() == 0:
+        return
+    with torch.cuda.device(out_a.device):
+        check(lib.fp8k_merge_attention_states(out_a.data_ptr(), lse_a.data_ptr(), out_b.data_ptr(), lse_b.data_ptr(), out.data_ptr(), lse.data_ptr(),
+                                              out_a.numel() // D, D, dtype_code(out_a.dtype), stream_ptr(out_a.device)))
