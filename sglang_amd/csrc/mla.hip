@@ -317,7 +317,7 @@ extern "C" int fp8k_mla_gather_cache(const void* cache, const int32_t* page_tabl
 extern "C" int64_t fp8k_mla_decode_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t max_len) {
   if (B <= 0 || n <= 0 || H <= 0 || max_len <= 0) return 0;
   const int64_t M = n * H, slots = decode_plan(B, M, max_len).walkers + B;
-  return up_to(slots * M * kLatent * 4, 256) + up_to(slots * M * 4, 256);
+  return up_to(slots * M * kLatent * 4, 256) + up_to(slots * M * 4, 256) + up_to(B * 8, 256);
 }
 
 extern "C" int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t qn_stride_n, int64_t qn_stride_h, const void* q_pe,
@@ -330,7 +330,7 @@ extern "C" int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t 
   FP8K_REQUIRE(B >= 0 && B <= 65535 && n > 0 && H > 0 && n * H <= (1 << 16), "mla decode: bad sizes");
   FP8K_REQUIRE(sm_scale > 0.0f && sm_scale < INFINITY, "mla decode: the scale of the scores must be positive and finite");
   if (B == 0) return FP8K_OK;
-  FP8K_REQUIRE(pages > 0 && pages < (1ll << 31) && page_size > 0 && page_size < (1ll << 31) && table_width > 0 && table_stride >= 0,
+  FP8K_REQUIRE(pages > 0 && pages < (1ll << 31) && page_size > 0 && page_size <= (1 << 20) && table_width > 0 && table_stride >= 0,
                "mla decode: bad sizes of the cache or the page table");
   FP8K_REQUIRE(q_nope && q_pe && cache && page_table && seq_lens && out, "mla decode: null pointer");
   FP8K_REQUIRE(aligned(q_nope, 16) && aligned(q_pe, 16) && aligned(cache, 16) && aligned(out, 16), "mla decode: operands must be 16-byte aligned");
@@ -353,11 +353,13 @@ extern "C" int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t 
   p.out = out; p.lse = lse;
   p.part = (float*)workspace;
   p.part_lse = (float*)((uint8_t*)workspace + up_to((d.walkers + B) * M * kLatent * 4, 256));
+  p.spans = (v2i*)((uint8_t*)p.part_lse + up_to((d.walkers + B) * M * 4, 256));
   p.B = (int)B; p.n = (int)n; p.H = (int)H; p.M = (int)M;
   p.page_size = (int)page_size; p.pages = (int)pages; p.max_len = (int)max_len;
   p.walkers = d.walkers; p.mblocks = d.mblocks; p.sm_scale = sm_scale;
   const hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)((d.walkers + 7) / 8 * 8 * d.mblocks));
+  const bool few = B * M <= 4096;  // rows to join: a CU's worth of waves for four of them
 #define MLA_DECODE(DT, FP8)                                                          \
   do {                                                                               \
     if (d.rows == 16) mla_decode_kernel<DT, FP8, 1><<<grid, 256, 0, st>>>(p);        \
@@ -365,7 +367,8 @@ extern "C" int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t 
     else if (d.rows == 64) mla_decode_kernel<DT, FP8, 4><<<grid, 512, 0, st>>>(p);   \
     else mla_decode_kernel<DT, FP8, 8><<<grid, 512, 0, st>>>(p);                     \
     if (const int rc = check_launch("mla decode")) return rc;                        \
-    mla_join_kernel<DT><<<dim3((unsigned)M, (unsigned)B), 256, 0, st>>>(p);          \
+    if (few) mla_join_kernel<DT, 4><<<dim3((unsigned)M, (unsigned)B), 256, 0, st>>>(p);             \
+    else mla_join_kernel<DT, 1><<<dim3((unsigned)((M + 3) / 4), (unsigned)B), 256, 0, st>>>(p);     \
   } while (0)
   if (dtype == FP8K_BF16) {
     if (cache_is_fp8) MLA_DECODE(FP8K_BF16, true);

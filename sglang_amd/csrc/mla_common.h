@@ -58,17 +58,23 @@ __device__ __forceinline__ uint32_t fp8_to_16bit(uint32_t w) {
   else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HIGH));
 }
 
-typedef __attribute__((address_space(3))) void* mla_lds_ptr;
-// 16 bytes from every lane's own address to LDS at base + 16 * lane
-__device__ __forceinline__ void load16_to_lds(const void* p, void* lds_base) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (mla_lds_ptr)lds_base, 16, 0, 0);
+__device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
+// 16 bytes from every lane's own address p + OFFSET to LDS at `to` + 16 * lane (to: the wave's, one value).  In assembly, as the compiler
+// waits for all such loads that it knows of before any transposed read; this one writes no register, and whoever reads the LDS waits
+// for vmcnt himself.  The instruction's offset counts on both sides, hence the subtraction.
+template <int OFFSET = 0>
+__device__ __forceinline__ void load16_to_lds(const void* p, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(p), "s"(to - OFFSET), "n"(OFFSET) : "memory");
 }
-// FIRST .. LAST - 1 of a row of such loads: the lanes' addresses p + STEP * j to base + TO_STEP * j + 16 * lane.  The instruction's offset
-// counts on both sides.
+// 4 bytes likewise, to `to` + 4 * lane
+__device__ __forceinline__ void load4_to_lds(const void* p, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(to) : "memory");
+}
+// FIRST .. LAST - 1 of a row of such loads: the lanes' addresses p + STEP * j to `to` + TO_STEP * j + 16 * lane
 template <int STEP, int TO_STEP, int FIRST, int LAST>
-__device__ __forceinline__ void load_blocks_to_lds(const uint8_t* p, uint8_t* lds_base) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)p, (mla_lds_ptr)(lds_base + (TO_STEP - STEP) * FIRST), 16, STEP * FIRST, 0);
-  if constexpr (FIRST + 1 < LAST) load_blocks_to_lds<STEP, TO_STEP, FIRST + 1, LAST>(p, lds_base);
+__device__ __forceinline__ void load_blocks_to_lds(const uint8_t* p, uint32_t to) {
+  load16_to_lds<STEP * FIRST>(p, to + TO_STEP * FIRST);
+  if constexpr (FIRST + 1 < LAST) load_blocks_to_lds<STEP, TO_STEP, FIRST + 1, LAST>(p, to);
 }
 // Transposed read: within 16 lanes, lane i names the 8 bytes of row i / 4, numbers 4 (i % 4) .. + 3, of a block of 4 rows x 16 16-bit
 // numbers, and receives the four rows' number i.
@@ -101,14 +107,22 @@ __device__ __forceinline__ float shift_of(float m) { return m == -INFINITY ? 0.0
 // there the exponentials stay below 2^8, which float32 sums and 16-bit weights hold as exactly as those below 1.
 constexpr float kMaxSlack = 8.0f;
 
-// all of the wave's LDS reads and writes, and its loads to LDS, are done
-__device__ __forceinline__ void wait_all() {
+// The wave's LDS reads and writes are done, and all but the youngest N of its vector loads.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N < 64, "vmcnt is a 6-bit counter");
   asm volatile("" ::: "memory");
-  __builtin_amdgcn_s_waitcnt(0x0070);
+  __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | ((N >> 4) << 14));
   asm volatile("" ::: "memory");
 }
-__device__ __forceinline__ void wait_all_barrier() {
-  wait_all();
+__device__ __forceinline__ void wait_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+}
+// All waves of the workgroup have come here; their LDS traffic before it is done, their loads go on.
+__device__ __forceinline__ void lds_only_barrier() {
+  wait_lds();
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }

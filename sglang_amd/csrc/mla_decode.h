@@ -38,6 +38,7 @@ struct MlaDecodeArgs {
   void* out;           // [B, n, H, 512]
   float* lse;          // [B, n, H] or null
   float *part, *part_lse;  // [walkers + B, M, 512], [walkers + B, M]
+  v2i* spans;              // [B]: the first run that holds tokens of a request, and how many do
   int B, n, H, M;
   int page_size, pages, max_len;
   int walkers, mblocks;
@@ -45,7 +46,6 @@ struct MlaDecodeArgs {
 };
 
 constexpr int kMlaTile = 64;         // tokens of a tile
-constexpr int kMlaBlock = kMlaTile * 128;  // bytes of a block of 64 numbers of a tile in LDS
 constexpr int kMlaMinRun = 2;        // tiles that a run has at least
 
 __device__ __forceinline__ int mla_len(const MlaDecodeArgs& p, int b) { return min(max(p.lens[b], 0), p.max_len); }
@@ -54,9 +54,9 @@ __device__ __forceinline__ int mla_tiles(int len) { return (len + kMlaTile - 1) 
 __device__ __forceinline__ int mla_run(int total, int walkers) { return max((total + walkers - 1) / walkers, kMlaMinRun); }
 
 // Tiles of all requests, by a workgroup of NW waves; every thread returns the total.  Thread t counts requests [t * per, + per): `before`
-// is what lies in front of them.
+// is what lies in front of them, `mine` their own.
 template <int NW>
-__device__ __forceinline__ int mla_scan(const MlaDecodeArgs& p, int per, int& before, int* lds) {
+__device__ __forceinline__ int mla_scan(const MlaDecodeArgs& p, int per, int& before, int& mine, int* lds) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   int sum = 0;
   for (int b = tid * per; b < min((tid + 1) * per, p.B); ++b) sum += mla_tiles(mla_len(p, b));
@@ -67,7 +67,7 @@ __device__ __forceinline__ int mla_scan(const MlaDecodeArgs& p, int per, int& be
     if (lane >= d) run += v;
   }
   if (lane == 63) lds[w] = run;
-  __syncthreads();
+  lds_only_barrier();
   int total = 0, base = 0;
 #pragma unroll
   for (int i = 0; i < NW; ++i) {
@@ -75,6 +75,7 @@ __device__ __forceinline__ int mla_scan(const MlaDecodeArgs& p, int per, int& be
     total += lds[i];
   }
   before = base + run - sum;
+  mine = sum;
   return total;
 }
 
@@ -83,15 +84,27 @@ __device__ __forceinline__ int mla_scan(const MlaDecodeArgs& p, int per, int& be
 // does as well for the first alone, its rotation has half the rate there).
 __device__ __forceinline__ int mla_swizzle(int r) { return ((r & 2) ? 6 : 0) ^ ((r & 4) ? 5 : 0) ^ ((r & 8) ? 4 : 0); }
 
+template <int N>
+struct Const {
+  static constexpr int value = N;
+};
+
 template <int DT, bool FP8, int WM>
 __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const MlaDecodeArgs p) {
-  constexpr int NW = WM == 1 ? 4 : 8, WT = NW / WM, R = 16 * WM, NT = 4 / WT;  // NT: 16-token tiles of a wave
-  constexpr int kTileBytes = 9 * kMlaBlock, kStageBytes = FP8 ? kTileBytes / 2 : kTileBytes;
+  constexpr int NW = WM == 1 ? 4 : 8, WT = NW / WM, R = 16 * WM;
+  constexpr int TT = WM >= 4 ? 32 : 64, NT = TT / WT / 16;  // tokens of a step of the loop, 16-token tiles of a wave
+  constexpr bool kDeep = TT == 32;
+  constexpr int kBlock = TT * 128;                         // bytes of a block of 64 numbers of a step's rows
+  constexpr int kTileBytes = 9 * kBlock, kStageBytes = FP8 ? kTileBytes / 2 : kTileBytes;
+  constexpr int kTiles = FP8 ? (kDeep ? 2 : 1) : 0;        // 16-bit tiles beside the stages, for 8-bit rows
+  constexpr int kStageCount = kDeep ? 4 : 2;
   constexpr int kRow = FP8 ? kLatentRow : 2 * kLatentRow;  // bytes of a cached row
-  constexpr int kRowsOfLane = FP8 || NW == 8 ? 1 : 2;       // that a lane fetches from
-  // 16-bit: two tiles.  8-bit: a tile, then two stages of raw rows.
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[FP8 ? kTileBytes + 2 * kStageBytes : 2 * kTileBytes];
-  __shared__ int found[2], scan[NW];
+  // A wave fetches from kRowsOfWave rows, kRowsOfLane to a lane; kSharers waves share rows, by blocks: kMost of them the first, kLeast the others.
+  constexpr int kRowsOfWave = FP8 || NW == 4 ? 16 : 8, kRowsOfLane = !FP8 && NW == 4 ? 2 : 1;
+  constexpr int kSharers = NW * kRowsOfWave / TT, kLeast = 9 / kSharers, kMost = 9 - (kSharers - 1) * kLeast;
+  constexpr int kPageSlots = 8;
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[kTiles * kTileBytes + kStageCount * kStageBytes];
+  __shared__ int found[3], scan[NW], pages[kPageSlots][NW][16];
   __shared__ float join_m[NW][16], join_l[NW][16];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -102,38 +115,37 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
   if (walker >= p.walkers) return;
 
   const int per = (p.B + NW * 64 - 1) / (NW * 64);
-  int before;
-  const int total = mla_scan<NW>(p, per, before, scan);
+  int before, mine;
+  const int total = mla_scan<NW>(p, per, before, mine, scan);
   const int run = mla_run(total, p.walkers);
   if ((int64_t)walker * run >= total) return;
   const int first = walker * run, last = min(first + run, total);
-  {
-    int at = before;
-    for (int b = tid * per; b < min((tid + 1) * per, p.B); ++b) {
-      const int t = mla_tiles(mla_len(p, b));
-      if (first >= at && first < at + t) {
-        found[0] = b;
-        found[1] = at;
-      }
+  if (first >= before && first < before + mine) {  // this thread counted the request that the run begins in
+    int b = tid * per, at = before, len = mla_len(p, b);
+    for (int t = mla_tiles(len); per > 1 && first >= at + t; t = mla_tiles(len)) {
       at += t;
+      len = mla_len(p, ++b);
     }
+    found[0] = b;
+    found[1] = at;
+    found[2] = len;
   }
-  __syncthreads();
-  int b = __builtin_amdgcn_readfirstlane(found[0]), at = __builtin_amdgcn_readfirstlane(found[1]);
+  lds_only_barrier();
+  int b = __builtin_amdgcn_readfirstlane(found[0]), at = __builtin_amdgcn_readfirstlane(found[1]), len = __builtin_amdgcn_readfirstlane(found[2]);
 
-  const float kscale = FP8 && p.scale ? *p.scale : 1.0f;
+  const float kscale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(FP8 && p.scale ? *p.scale : 1.0f)));
   const float c = p.sm_scale * kLog2e * kscale;
 
   const int row = mblk * R + wm * 16 + l15;  // this lane's, of the M of a request
 
-  // LDS offsets: operand reads of K (row l15 of a 16-token tile, chunk 4 ks + g), transposed reads of V
-  const int k_off = (wt * NT * 16 + l15) * 128 + ((g ^ mla_swizzle(l15)) << 4);
-  const int v_row = 4 * g + (l15 >> 2);
-  const int v_off = (wt * NT * 16 + v_row) * 128 + ((((l15 & 3) >> 1) ^ mla_swizzle(v_row)) << 4) + ((l15 & 1) << 3);
+  // Waves w and w + 4 share a SIMD.  With the first one's instructions in front, it runs ahead of the other within a tile, and its softmax beside the
+  // other's products.
+  if (NW == 8 && w < 4) __builtin_amdgcn_s_setprio(1);
 
-  for (int pos = first; pos < last; ++b) {
-    const int len = mla_len(p, b), tiles = mla_tiles(len);
-    const int t_begin = pos - at, t_end = min(last - at, tiles);
+  for (int pos = first, next_len; pos < last; ++b, len = next_len) {
+    next_len = b + 1 < p.B ? mla_len(p, b + 1) : 0;
+    const int tiles = mla_tiles(len), t_begin = pos - at, t_end = min(last - at, tiles);
+    if (t_begin == 0 && mblk == 0 && tid == 0 && tiles > 0) p.spans[b] = v2i{walker, (at + tiles - 1) / run - walker + 1};
     at += tiles;
     if (t_begin >= t_end) continue;
     pos += t_end - t_begin;
@@ -156,103 +168,204 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
     for (int dt = 0; dt < 32; ++dt) o[dt] = v4f{0, 0, 0, 0};
     float m = -INFINITY, l = 0.0f;
 
-    // ---- fetching.  Tokens past the end are the last one's row again (masked).  16 bits: a wave has 8 rows of a tile (four waves: 16).  8 bits:
-    // wave w has 16 rows, from row 16 (w % 4) on; of eight waves, two share them, by blocks.
-    struct Rows {
-      const uint8_t* at[kRowsOfLane];
+    // ---- fetching.  Steps are counted from the segment's first.  Tokens past the end are the last one's row again (masked).
+    const int base = t_begin * kMlaTile, steps = min((t_end - t_begin) * (kMlaTile / TT), (len - base + TT - 1) / TT);
+    const int group = w % (NW / kSharers), share = w / (NW / kSharers), first_row = kRowsOfWave * group;
+    // What follows from the lane is computed anew for every step: kept across the loop, it goes to scratch memory, and a load from there waits for the
+    // rows that are on their way.
+    auto fresh_lane = [&] {
+      int x = lane;
+      asm volatile("" : "+v"(x));
+      return x;
     };
-    auto rows_of = [&](int t) {
-      Rows rows;
+    // The pages of a step's rows go to LDS as well, some steps ahead, so that no load into a register is ever waited for.  Always made, so that
+    // loads can be counted; past the end for the last row again.
+    const int32_t* const pages_of = p.table + b * p.table_stride;
+    const uint32_t pages_to = lds_address(&pages[0][w][0]);
+    auto fetch_pages = [&](int t) {
+      const int lane = fresh_lane();
+      const uint32_t tok = min(base + t * TT + first_row + lane, len - 1);
+      if (lane < kRowsOfWave) load4_to_lds(pages_of + tok / (uint32_t)p.page_size, pages_to + (t % kPageSlots) * (NW * 64));
+    };
+    auto fetch = [&](int t, uint32_t to) {  // to: of the stage
+      const int lane = fresh_lane();
+      const uint8_t* from[kRowsOfLane];
 #pragma unroll
       for (int k = 0; k < kRowsOfLane; ++k) {
-        const int r = FP8 ? 16 * (w & 3) + (lane >> 2) : 8 * (w * kRowsOfLane + k) + (lane >> 3);
-        const int tok = min(t * kMlaTile + r, len - 1), page = tok / p.page_size;
-        const int e = min(max(p.table[b * p.table_stride + page], 0), p.pages - 1);
-        rows.at[k] = p.cache + ((int64_t)e * p.page_size + (tok - page * p.page_size)) * kRow + (FP8 ? (lane & 3) : (lane & 7) ^ mla_swizzle(r)) * 16;
+        const int r = FP8 ? lane >> 2 : 8 * k + (lane >> 3);  // of the wave's
+        const uint32_t tok = min(base + t * TT + first_row + r, len - 1), place = tok % (uint32_t)p.page_size;
+        const uint32_t page = min(max(pages[t % kPageSlots][w][r], 0), p.pages - 1);
+        from[k] = p.cache + (uint64_t)page * (uint32_t)(p.page_size * kRow) + (place * kRow + (FP8 ? (lane & 3) : (lane & 7) ^ mla_swizzle(first_row + r)) * 16);
       }
-      return rows;
-    };
-    auto fetch = [&](const Rows& rows, uint8_t* stage) {
-      if constexpr (FP8) {
-        uint8_t* const to = stage + (w & 3) * 9 * 1024;
-        if (NW == 4) load_blocks_to_lds<64, 1024, 0, 9>(rows.at[0], to);
-        else if (w < 4) load_blocks_to_lds<64, 1024, 0, 5>(rows.at[0], to);
-        else load_blocks_to_lds<64, 1024, 5, 9>(rows.at[0], to);
-      } else {
 #pragma unroll
-        for (int k = 0; k < kRowsOfLane; ++k) load_blocks_to_lds<128, kMlaBlock, 0, 9>(rows.at[k], stage + 8 * (w * kRowsOfLane + k) * 128);
+      for (int k = 0; k < kRowsOfLane; ++k) {
+        constexpr int kStep = FP8 ? 64 : 128, kToStep = FP8 ? 1024 : kBlock;
+        const uint32_t place = FP8 ? to + group * 9 * 1024 : to + (first_row + 8 * k) * 128;
+        if (kSharers == 1 || share == 0) load_blocks_to_lds<kStep, kToStep, 0, kMost>(from[k], place);
+        else if (kSharers == 2 || share == 1) load_blocks_to_lds<kStep, kToStep, kMost, kMost + kLeast>(from[k], place);
+        else if (share == 2) load_blocks_to_lds<kStep, kToStep, kMost + kLeast, kMost + 2 * kLeast>(from[k], place);
+        else load_blocks_to_lds<kStep, kToStep, kMost + 2 * kLeast, 9>(from[k], place);
       }
     };
-
-    Rows rows = rows_of(t_begin);
-    uint8_t* const stages = smem + (FP8 ? kTileBytes : 0);
-    fetch(rows, stages);
-    rows = rows_of(min(t_begin + 1, t_end - 1));
-    for (int t = t_begin; t < t_end; ++t) {
-      uint8_t* const stage = stages + ((t - t_begin) & 1) * kStageBytes;
-      uint8_t* const other = stages + ((t - t_begin + 1) & 1) * kStageBytes;
-      // this tile's rows have arrived, and nobody reads the tile before any more
-      if (WM > 1) wait_all_barrier();
-      else wait_all();
-      if (t + 1 < t_end) {
-        const Rows next = rows;
-        rows = rows_of(min(t + 2, t_end - 1));
-        fetch(next, other);
-      }
-      const uint8_t* tile = stage;
-      if (FP8) {
-        uint8_t* const to = smem + (16 * (w & 3) + (lane >> 2)) * 128;
-        const int at0 = ((2 * (lane & 3)) ^ mla_swizzle(lane >> 2)) << 4;
-        const uint8_t* const from = stage + (w & 3) * 9 * 1024 + lane * 16;
-        auto widen = [&](int j) {
-          const v4i raw = *(const v4i*)(from + j * 1024);
-          *(v4i*)(to + j * kMlaBlock + at0) = v4i{(int)fp8_to_16bit<DT, false>(raw[0]), (int)fp8_to_16bit<DT, true>(raw[0]),
-                                                  (int)fp8_to_16bit<DT, false>(raw[1]), (int)fp8_to_16bit<DT, true>(raw[1])};
-          *(v4i*)(to + j * kMlaBlock + (at0 ^ 16)) = v4i{(int)fp8_to_16bit<DT, false>(raw[2]), (int)fp8_to_16bit<DT, true>(raw[2]),
-                                                         (int)fp8_to_16bit<DT, false>(raw[3]), (int)fp8_to_16bit<DT, true>(raw[3])};
-        };
-        if (NW == 4 || w < 4) {
+    // all loads but the youngest: FETCHES steps' rows and PAGES steps' pages
+    auto wait_but = [&](auto fetches, auto page_loads) {
+      constexpr int kF = decltype(fetches)::value, kP = decltype(page_loads)::value;
+      if (kSharers == 1 || share == 0) wait_loads<kF * kMost * kRowsOfLane + kP>();
+      else wait_loads<kF * kLeast * kRowsOfLane + kP>();
+    };
+    // 8-bit rows of a stage, as this wave fetched them, to 16 bits in a tile
+    auto widen_blocks = [&](const uint8_t* stage, uint8_t* tile, auto first_block, auto last_block) {
+      constexpr int kFirst = decltype(first_block)::value, kLast = decltype(last_block)::value;
+      const int lane = fresh_lane();
+      uint8_t* const to = tile + (first_row + (lane >> 2)) * 128;
+      const int at0 = ((2 * (lane & 3)) ^ mla_swizzle(lane >> 2)) << 4;
+      const uint8_t* const from = stage + group * 9 * 1024 + lane * 16;
+      v4i raw[kLast - kFirst];
 #pragma unroll
-          for (int j = 0; j < (NW == 4 ? 9 : 5); ++j) widen(j);
+      for (int j = kFirst; j < kLast; ++j) raw[j - kFirst] = *(const v4i*)(from + j * 1024);
+#pragma unroll
+      for (int j = kFirst; j < kLast; ++j) {
+        const v4i x = raw[j - kFirst];
+        *(v4i*)(to + j * kBlock + at0) = v4i{(int)fp8_to_16bit<DT, false>(x[0]), (int)fp8_to_16bit<DT, true>(x[0]),
+                                             (int)fp8_to_16bit<DT, false>(x[1]), (int)fp8_to_16bit<DT, true>(x[1])};
+        *(v4i*)(to + j * kBlock + (at0 ^ 16)) = v4i{(int)fp8_to_16bit<DT, false>(x[2]), (int)fp8_to_16bit<DT, true>(x[2]),
+                                                    (int)fp8_to_16bit<DT, false>(x[3]), (int)fp8_to_16bit<DT, true>(x[3])};
+      }
+    };
+    auto widen = [&](const uint8_t* stage, uint8_t* tile) {
+      if constexpr (kSharers == 1) {
+        widen_blocks(stage, tile, Const<0>{}, Const<9>{});
+      } else if constexpr (kSharers == 2) {
+        if (share == 0) {
+          widen_blocks(stage, tile, Const<0>{}, Const<3>{});  // a few at a time: registers
+          widen_blocks(stage, tile, Const<3>{}, Const<5>{});
         } else {
+          widen_blocks(stage, tile, Const<5>{}, Const<7>{});
+          widen_blocks(stage, tile, Const<7>{}, Const<9>{});
+        }
+      } else {
+        if (share == 0) widen_blocks(stage, tile, Const<0>{}, Const<3>{});
+        else if (share == 1) widen_blocks(stage, tile, Const<3>{}, Const<5>{});
+        else if (share == 2) widen_blocks(stage, tile, Const<5>{}, Const<7>{});
+        else widen_blocks(stage, tile, Const<7>{}, Const<9>{});
+      }
+    };
+
+    constexpr int kStagesAt = kTiles * kTileBytes;
+    const uint32_t lds0 = lds_address(smem) + kStagesAt;
+    auto to_stage = [&](int t) { return lds0 + t % kStageCount * kStageBytes; };
+    auto stage_of = [&](int t) { return smem + kStagesAt + t % kStageCount * kStageBytes; };
+
+    // Rows are asked for kRun steps before their step, pages kPagesRun steps before the rows.
+    //   two stages:  the rows of step t + 1 (8 bits: t + 2) while step t is waited for, which takes two barriers, or none (WM = 1)
+    //   four stages: the rows of step t + 3 (8 bits: t + 5) while those of t + 1 and t + 2 (8 bits: t + 2 .. t + 4) are on their way; one barrier
+    constexpr int kRun = kStageCount - 1 + (FP8 ? (kDeep ? 2 : 1) : 0), kPagesRun = kDeep ? (FP8 ? 4 : 2) : 1;
+    auto ask = [&](int t) {  // one step's rows, and the pages of a later one's
+      fetch_pages(t + kPagesRun);
+      fetch(t, to_stage(t));
+    };
+    constexpr int kFirst = FP8 ? kStageCount : kRun;  // steps asked for at first, with pages that have come already
 #pragma unroll
-          for (int j = 5; j < 9; ++j) widen(j);
+    for (int t = 0; t < kFirst + (kDeep ? 0 : 1); ++t) fetch_pages(t);
+    wait_loads<0>();
+#pragma unroll
+    for (int t = 0; t < kFirst; ++t)
+      if (t < steps) ask(t);
+    if constexpr (FP8 && kDeep) {  // the first tile, and the rows that take its stage
+      wait_loads<0>();
+      widen(stage_of(0), smem);
+      wait_lds();
+      if (kStageCount < steps) ask(kStageCount);
+    }
+    for (int t = 0; t < steps; ++t) {
+      const int lane = fresh_lane(), l15 = lane & 15, g = lane >> 4;
+      const uint8_t* tile;
+      if constexpr (!kDeep) {
+        if (WM > 1) lds_only_barrier();  // nobody reads the step before any more
+        else wait_lds();
+        if constexpr (!FP8) {
+          if (t + 1 < steps) {
+            ask(t + 1);
+            wait_but(Const<1>{}, Const<0>{});
+          } else wait_loads<0>();
+          tile = stage_of(t);
+        } else {
+          if (t + 1 < steps) wait_but(Const<1>{}, Const<0>{});
+          else wait_loads<0>();
+          widen(stage_of(t), smem);
+          if (t + 2 < steps) {
+            wait_lds();  // the stage has been read
+            ask(t + 2);
+          }
+          tile = smem;
         }
-        if (WM > 1) {
-          asm volatile("" ::: "memory");
-          __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
-          __builtin_amdgcn_s_barrier();
-          asm volatile("" ::: "memory");
+        if (WM > 1) lds_only_barrier();  // everybody's part of the step is there
+      } else if constexpr (!FP8) {
+        if (t + 2 < steps) wait_but(Const<2>{}, Const<1>{});
+        else wait_loads<0>();
+        lds_only_barrier();  // everybody's part of the step is there, and nobody reads the step before any more
+        if (t + 3 < steps) ask(t + 3);
+        tile = stage_of(t);
+      } else {
+        lds_only_barrier();  // this step's tile is whole, and nobody reads the other any more
+        if (t + 1 < steps) {
+          if (t + 4 < steps) wait_but(Const<3>{}, Const<3>{});
+          else wait_loads<0>();
+          widen(stage_of(t + 1), smem + (t + 1) % 2 * kTileBytes);
+          if (t + 5 < steps) {
+            wait_lds();  // the stage has been read
+            ask(t + 5);
+          }
         }
-        tile = smem;
+        tile = smem + t % 2 * kTileBytes;
       }
 
-      // ---- S^T = K . Q^T
-      v4f s[NT];
+      // ---- S^T = K . Q^T: kAhead operand reads run ahead of the products.  With one tile of tokens, two sums by turns: a product waits for the
+      // one before it in its sum.
+      constexpr int kSums = NT == 1 ? 2 : NT, kAhead = NW == 8 ? 6 : 8;
+      v4f s[kSums];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt] = v4f{0, 0, 0, 0};
+      for (int i = 0; i < kSums; ++i) s[i] = v4f{0, 0, 0, 0};
+      {
+        // row l15 of a 16-token tile, chunk 4 ks + g
+        const int k_off = (wt * NT * 16 + l15) * 128 + ((g ^ mla_swizzle(l15)) << 4);
+        const uint8_t* const even = tile + k_off;
+        const uint8_t* const odd = tile + (k_off ^ 64);
+        auto read = [&](int i) {
+          const int ks = i / NT, nt = i % NT;
+          return *(const v4i*)((ks & 1 ? odd : even) + (ks >> 1) * kBlock + nt * 16 * 128);
+        };
+        v4i ring[kAhead];
 #pragma unroll
-      for (int ks = 0; ks < 18; ++ks)
+        for (int i = 0; i < kAhead; ++i) ring[i] = read(i);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          s[nt] = mfma16<DT>(*(const v4i*)(tile + ((k_off ^ ((ks & 1) << 6)) + (ks >> 1) * kMlaBlock + nt * 16 * 128)), q[ks], s[nt]);
+        for (int i = 0; i < 18 * NT; ++i) {
+          s[i % kSums] = mfma16<DT>(ring[i % kAhead], q[i / NT], s[i % kSums]);
+          if (i + kAhead < 18 * NT) ring[i % kAhead] = read(i + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if constexpr (NT == 1) s[0] += s[1];
 
       // ---- softmax: a lane's scores are those of query row l15, tokens 16 nt + 4 g + i
-      const int tok0 = t * kMlaTile + wt * NT * 16 + 4 * g;
-      const bool masked = (t + 1) * kMlaTile > len - (p.n - 1);
+      const int tok0 = base + t * TT + wt * NT * 16 + 4 * g;
+      const bool masked = base + (t + 1) * TT > len - (p.n - 1);
       float top = -INFINITY;
+      if (__builtin_expect(masked, 0)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (tok0 + nt * 16 + i >= lim) s[nt][i] = -INFINITY;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float v = s[nt][i] * c;
-          if (masked && tok0 + nt * 16 + i >= lim) v = -INFINITY;
-          s[nt][i] = v;
-          top = fmaxf(top, v);
-        }
-      top = max_across32(max_across16(top));
-      const float raised = top > m + kMaxSlack ? top : m;
-      if (__any(raised != m)) {
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, s[nt][i]);
+      // c > 0.  The row's maximum, over four lanes, is asked for only when one of them has passed the old one by far.
+      if (__builtin_expect(__any(top * c > m + kMaxSlack), 0)) {
+        top = max_across32(max_across16(top)) * c;
+        const float raised = top > m + kMaxSlack ? top : m;
         const float alpha = raised != m ? __builtin_amdgcn_exp2f(m - raised) : 1.0f;
         m = raised;
         l *= alpha;
@@ -266,7 +379,7 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
         float e[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          e[i] = __builtin_amdgcn_exp2f(s[nt][i] - shift);
+          e[i] = __builtin_amdgcn_exp2f(fmaf(s[nt][i], c, -shift));
           l += e[i];
         }
         // weights rounded to the 16-bit type, as the matrix core takes them; their sum is of the unrounded ones
@@ -274,18 +387,31 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
         pk[nt][1] = pack2<DT>(e[2], e[3]);
       }
 
-      // ---- O^T += V^T . P^T
+      // ---- O^T += V^T . P^T, reads ahead of the products likewise; columns in the inner loop, so that a product waits for no other
+      {
+        const int v_row = 4 * g + (l15 >> 2);
+        const int v_off = (wt * NT * 16 + v_row) * 128 + ((((l15 & 3) >> 1) ^ mla_swizzle(v_row)) << 4) + ((l15 & 1) << 3);
+        const uint8_t* v[4];
 #pragma unroll
-      for (int dt = 0; dt < 32; ++dt) {
-        const uint8_t* const v = tile + ((v_off ^ ((dt & 3) << 5)) + (dt >> 2) * kMlaBlock);
-        if constexpr (NT == 1) {
-          o[dt] = mfma16_half<DT>(lds_read_transposed(v), v2i{(int)pk[0][0], (int)pk[0][1]}, o[dt]);
-        } else {
+        for (int i = 0; i < 4; ++i) v[i] = tile + (v_off ^ (i << 5));
+        constexpr int kSteps = NT == 1 ? 32 : 16 * NT, kVAhead = NW == 4 ? 8 : NT == 1 ? 6 : 5;
+        v2i ring[kVAhead][2];
+        auto read = [&](int i, v2i* to) {
+          const int dt = i & 31, nt = (i >> 5) * 2;
+          const uint8_t* const at = v[dt & 3] + (dt >> 2) * kBlock + nt * 16 * 128;
+          to[0] = lds_read_transposed(at);
+          if (NT > 1) to[1] = lds_read_transposed(at + 16 * 128);
+        };
 #pragma unroll
-          for (int nt = 0; nt < NT; nt += 2) {
-            const v2i a0 = lds_read_transposed(v + nt * 16 * 128), a1 = lds_read_transposed(v + (nt + 1) * 16 * 128);
-            o[dt] = mfma16<DT>(v4i{a0[0], a0[1], a1[0], a1[1]}, v4i{(int)pk[nt][0], (int)pk[nt][1], (int)pk[nt + 1][0], (int)pk[nt + 1][1]}, o[dt]);
-          }
+        for (int i = 0; i < kVAhead; ++i) read(i, ring[i]);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const int dt = i & 31, nt = (i >> 5) * 2;
+          const v2i* const a = ring[i % kVAhead];
+          if constexpr (NT == 1) o[dt] = mfma16_half<DT>(a[0], v2i{(int)pk[0][0], (int)pk[0][1]}, o[dt]);
+          else o[dt] = mfma16<DT>(v4i{a[0][0], a[0][1], a[1][0], a[1][1]}, v4i{(int)pk[nt][0], (int)pk[nt][1], (int)pk[nt + 1][0], (int)pk[nt + 1][1]}, o[dt]);
+          if (i + kVAhead < kSteps) read(i + kVAhead, ring[i % kVAhead]);
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -298,7 +424,8 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
       join_m[w][l15] = m;
       join_l[w][l15] = l;
     }
-    __syncthreads();  // and nobody reads a tile any more
+    wait_loads<0>();     // pages that nobody needed
+    lds_only_barrier();  // and nobody reads a tile any more
     {
       float top = -INFINITY, sum = 0.0f;
 #pragma unroll
@@ -316,82 +443,126 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
         else if (p.lse) p.lse[(int64_t)b * p.M + row] = lse2 * kLn2;
       }
     }
-    // a quarter of the 512 columns at a time through LDS: [WT][R] rows of 128 floats (and 4 of padding)
-    constexpr int kLd = 132;
-    float* const buf = (float*)smem;
+    if constexpr (WT == 1) {
+      if (row < p.M) {
+        const int64_t to = (whole ? (int64_t)b * p.M + row : slot * p.M + row) * kLatent + 4 * g;
+        if (whole) {
 #pragma unroll
-    for (int quarter = 0; quarter < 4; ++quarter) {
+          for (int dt = 0; dt < 32; ++dt) *(v2i*)((u16*)p.out + to + dt * 16) = v2i{(int)pack2<DT>(o[dt][0], o[dt][1]), (int)pack2<DT>(o[dt][2], o[dt][3])};
+        } else {
 #pragma unroll
-      for (int d = 0; d < 8; ++d) *(v4f*)(buf + (wt * R + wm * 16 + l15) * kLd + d * 16 + 4 * g) = o[quarter * 8 + d];
-      __syncthreads();
-#pragma unroll
-      for (int k = 0; k < R * 16 / (NW * 64); ++k) {
-        const int row_in = (k * NW * 64 + tid) >> 4, col = (tid & 15) * 8, r = mblk * R + row_in;
-        v4f x = *(const v4f*)(buf + row_in * kLd + col), y = *(const v4f*)(buf + row_in * kLd + col + 4);
-#pragma unroll
-        for (int i = 1; i < WT; ++i) {
-          x += *(const v4f*)(buf + (i * R + row_in) * kLd + col);
-          y += *(const v4f*)(buf + (i * R + row_in) * kLd + col + 4);
+          for (int dt = 0; dt < 32; ++dt) *(v4f*)(p.part + to + dt * 16) = o[dt];
         }
-        if (r < p.M) {
-          if (whole) {
-            const v4i v = {(int)pack2<DT>(x[0], x[1]), (int)pack2<DT>(x[2], x[3]), (int)pack2<DT>(y[0], y[1]), (int)pack2<DT>(y[2], y[3])};
-            *(v4i*)((u16*)p.out + ((int64_t)b * p.M + r) * kLatent + quarter * 128 + col) = v;
-          } else {
-            float* const to = p.part + (slot * p.M + r) * kLatent + quarter * 128 + col;
-            *(v4f*)to = x;
-            *(v4f*)(to + 4) = y;
+      }
+    } else {
+      // a quarter of the 512 columns at a time through LDS: [WT][R] rows of 128 floats (and 4 of padding)
+      constexpr int kLd = 132;
+      float* const buf = (float*)smem;
+#pragma unroll
+      for (int quarter = 0; quarter < 4; ++quarter) {
+        if (quarter) lds_only_barrier();
+#pragma unroll
+        for (int d = 0; d < 8; ++d) *(v4f*)(buf + (wt * R + wm * 16 + l15) * kLd + d * 16 + 4 * g) = o[quarter * 8 + d];
+        lds_only_barrier();
+#pragma unroll
+        for (int k = 0; k < R * 16 / (NW * 64); ++k) {
+          const int row_in = (k * NW * 64 + tid) >> 4, col = (tid & 15) * 8, r = mblk * R + row_in;
+          v4f x = *(const v4f*)(buf + row_in * kLd + col), y = *(const v4f*)(buf + row_in * kLd + col + 4);
+#pragma unroll
+          for (int i = 1; i < WT; ++i) {
+            x += *(const v4f*)(buf + (i * R + row_in) * kLd + col);
+            y += *(const v4f*)(buf + (i * R + row_in) * kLd + col + 4);
+          }
+          if (r < p.M) {
+            if (whole) {
+              const v4i v = {(int)pack2<DT>(x[0], x[1]), (int)pack2<DT>(x[2], x[3]), (int)pack2<DT>(y[0], y[1]), (int)pack2<DT>(y[2], y[3])};
+              *(v4i*)((u16*)p.out + ((int64_t)b * p.M + r) * kLatent + quarter * 128 + col) = v;
+            } else {
+              float* const to = p.part + (slot * p.M + r) * kLatent + quarter * 128 + col;
+              *(v4f*)to = x;
+              *(v4f*)(to + 4) = y;
+            }
           }
         }
       }
-      __syncthreads();
     }
+    lds_only_barrier();  // before the next request's rows come
   }
 }
 
 // Adds up the partials of requests that several runs share, in the order of their tokens, and gives requests without tokens their zeros.
-// One workgroup to a row and request; 128 threads of four columns.
-template <int DT>
+// WAVES waves of a workgroup of four share a row: one where there are many rows with few partials each, four where there are few rows with many.
+// A wave takes every WAVES-th partial, eight columns to a lane.
+template <int DT, int WAVES>
 __global__ __launch_bounds__(256) void mla_join_kernel(const MlaDecodeArgs p) {
-  __shared__ int mine[2], scan4[4];
-  __shared__ float weights[256];
-  const int r = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const int per = (p.B + 255) / 256;
-  int before;
-  const int total = mla_scan<4>(p, per, before, scan4);
-  if (tid == b / per) {
-    for (int i = tid * per; i < b; ++i) before += mla_tiles(mla_len(p, i));
-    mine[0] = before;
-  }
-  __syncthreads();
-  const int tiles = mla_tiles(mla_len(p, b));
+  __shared__ v4f parts[WAVES == 1 ? 1 : 3 * 128];
+  const int lane = threadIdx.x & 63, w = (int)(threadIdx.x >> 6) % WAVES;
+  const int b = blockIdx.y, r = (int)blockIdx.x * (4 / WAVES) + (int)(threadIdx.x >> 6) / WAVES;
+  if (r >= p.M) return;  // whole workgroups, with WAVES = 4
+  const v2i span = p.spans[b];  // anything, for a request without tokens
   const int64_t row = (int64_t)b * p.M + r;
-  u16* const out = (u16*)p.out + row * kLatent;
-  if (tiles == 0) {
-    if (tid < 128) *(v2i*)(out + 4 * tid) = v2i{0, 0};
-    if (tid == 0 && p.lse) p.lse[row] = -INFINITY;
+  u16* const out = (u16*)p.out + row * kLatent + 4 * lane;
+  if (mla_len(p, b) == 0) {
+    if (w == 0) {
+      *(v2i*)out = v2i{0, 0};
+      *(v2i*)(out + 256) = v2i{0, 0};
+      if (lane == 0 && p.lse) p.lse[row] = -INFINITY;
+    }
     return;
   }
-  const int run = mla_run(total, p.walkers), w0 = mine[0] / run, w1 = (mine[0] + tiles - 1) / run, n = w1 - w0 + 1;
+  const int n = span[1];
   if (n == 1) return;
-  // n <= walkers <= 256
-  const int64_t slot = (int64_t)(w0 + b);
-  float top = -INFINITY;
-  for (int i = 0; i < n; ++i) top = fmaxf(top, p.part_lse[(slot + i) * p.M + r]);
-  const float shift = shift_of(top);
-  if (tid < n) weights[tid] = __builtin_amdgcn_exp2f(p.part_lse[(slot + tid) * p.M + r] - shift);
-  __syncthreads();
-  float sum = 0.0f;
-  for (int i = 0; i < n; ++i) sum += weights[i];
-  if (tid < 128) {
-    v4f acc = {0, 0, 0, 0};
-    const float* from = p.part + (slot * p.M + r) * kLatent + 4 * tid;
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) acc += weights[i] * *(const v4f*)(from + (int64_t)i * p.M * kLatent);
-    acc *= sum == 0.0f ? 0.0f : 1.0f / sum;
-    *(v2i*)(out + 4 * tid) = v2i{(int)pack2<DT>(acc[0], acc[1]), (int)pack2<DT>(acc[2], acc[3])};
+  const int64_t slot = span[0] + b;
+  // n <= 256: four partials' logarithms to a lane
+  float lse[4], top = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    lse[k] = k * 64 + lane < n ? p.part_lse[(slot + k * 64 + lane) * p.M + r] : -INFINITY;
+    top = fmaxf(top, lse[k]);
   }
-  if (tid == 0 && p.lse) p.lse[row] = sum == 0.0f ? -INFINITY : (__builtin_amdgcn_logf(sum) + shift) * kLn2;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+  const float shift = shift_of(top);
+  float sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    lse[k] = __builtin_amdgcn_exp2f(lse[k] - shift);  // its weight
+    sum += lse[k];
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+  v4f x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+  const float* const from = p.part + (slot * p.M + r) * kLatent + 4 * lane;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const int end = min(n - k * 64, 64);
+#pragma unroll 8
+    for (int i = w; i < end; i += WAVES) {
+      const float* const at = from + (int64_t)(k * 64 + i) * p.M * kLatent;
+      const float weight = __shfl(lse[k], i);
+      x += weight * *(const v4f*)at;
+      y += weight * *(const v4f*)(at + 256);
+    }
+  }
+  if constexpr (WAVES > 1) {
+    if (w) {
+      parts[(w - 1) * 128 + lane] = x;
+      parts[(w - 1) * 128 + 64 + lane] = y;
+    }
+    lds_only_barrier();
+    if (w) return;
+#pragma unroll
+    for (int i = 0; i < WAVES - 1; ++i) {
+      x += parts[i * 128 + lane];
+      y += parts[i * 128 + 64 + lane];
+    }
+  }
+  const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+  x *= f;
+  y *= f;
+  *(v2i*)out = v2i{(int)pack2<DT>(x[0], x[1]), (int)pack2<DT>(x[2], x[3])};
+  *(v2i*)(out + 256) = v2i{(int)pack2<DT>(y[0], y[1]), (int)pack2<DT>(y[2], y[3])};
+  if (lane == 0 && p.lse) p.lse[row] = sum == 0.0f ? -INFINITY : (__builtin_amdgcn_logf(sum) + shift) * kLn2;
 }
 
 }  // namespace fp8k

@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
   }
 
   // a wave fetches 16 rows of each part of a stage: four wave-loads of k_nope, two of k_pe, four of v
-  auto fetch = [&](int t, uint8_t* stage) {
+  auto fetch = [&](int t, uint32_t stage) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int r = w * 16 + j * 4 + (lane >> 4), at = lane & 15;
@@ -95,11 +95,13 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
 
-  if (tiles > 0) fetch(0, smem);
+  const uint32_t lds0 = lds_address(smem);
+  if (tiles > 0) fetch(0, lds0);
   for (int t = 0; t < tiles; ++t) {
-    uint8_t* const stage = smem + (t & 1) * kStage;
-    wait_all_barrier();  // this tile has arrived, and nobody reads the one before any more
-    if (t + 1 < tiles) fetch(t + 1, smem + ((t + 1) & 1) * kStage);
+    const uint8_t* const stage = smem + (t & 1) * kStage;
+    wait_loads<0>();
+    lds_only_barrier();  // this tile has arrived, and nobody reads the one before any more
+    if (t + 1 < tiles) fetch(t + 1, lds0 + ((t + 1) & 1) * kStage);
     if (t * kPreKeys >= wave_keys) continue;  // nothing that this wave's rows see
 
     v16f s[2];
@@ -117,7 +119,7 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
 
     // a lane's scores are those of query row l31, keys 32 nt + 8 (i / 4) + 4 half + i % 4
     const int key0 = t * kPreKeys + 4 * half;
-    if ((t + 1) * kPreKeys > wave_free) {
+    if (__builtin_expect((t + 1) * kPreKeys > wave_free, 0)) {
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
@@ -129,9 +131,10 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
     for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[nt][i]);
-    top = max_across32(top) * c;  // c > 0
-    const float raised = top > m + kMaxSlack ? top : m;
-    if (__any(raised != m)) {
+    // c > 0.  The row's maximum, over two lanes, is asked for only when one of them has passed the old one by far.
+    if (__builtin_expect(__any(top * c > m + kMaxSlack), 0)) {
+      top = max_across32(top) * c;
+      const float raised = top > m + kMaxSlack ? top : m;
       const float alpha = raised != m ? __builtin_amdgcn_exp2f(m - raised) : 1.0f;
       m = raised;
       l *= alpha;
