@@ -355,11 +355,11 @@ extern "C" int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t 
   p.part_lse = (float*)((uint8_t*)workspace + up_to((d.walkers + B) * M * kLatent * 4, 256));
   p.spans = (v2i*)((uint8_t*)p.part_lse + up_to((d.walkers + B) * M * 4, 256));
   p.B = (int)B; p.n = (int)n; p.H = (int)H; p.M = (int)M;
-  p.page_size = (int)page_size; p.pages = (int)pages; p.max_len = (int)max_len;
+  p.page_size = (int)page_size; p.page_shift = (page_size & (page_size - 1)) ? -1 : __builtin_ctzll(page_size); p.pages = (int)pages; p.max_len = (int)max_len;
   p.walkers = d.walkers; p.mblocks = d.mblocks; p.sm_scale = sm_scale;
   const hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)((d.walkers + 7) / 8 * 8 * d.mblocks));
-  const bool few = B * M <= 4096;  // rows to join: a CU's worth of waves for four of them
+  const bool few = B * M <= 2 * num_cu();  // rows to join: few of them have many partials each
 #define MLA_DECODE(DT, FP8)                                                          \
   do {                                                                               \
     if (d.rows == 16) mla_decode_kernel<DT, FP8, 1><<<grid, 256, 0, st>>>(p);        \

@@ -61,10 +61,10 @@ __device__ __forceinline__ uint32_t fp8_to_16bit(uint32_t w) {
 __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p; }
 // 16 bytes from every lane's own address p + OFFSET to LDS at `to` + 16 * lane (to: the wave's, one value).  In assembly, as the compiler
 // waits for all such loads that it knows of before any transposed read; this one writes no register, and whoever reads the LDS waits
-// for vmcnt himself.  The instruction's offset counts on both sides, hence the subtraction.
+// for vmcnt himself.  The instruction's offset counts on both sides, hence the subtraction.  Non-temporal, for rows that are read once.
 template <int OFFSET = 0>
 __device__ __forceinline__ void load16_to_lds(const void* p, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2" ::"v"(p), "s"(to - OFFSET), "n"(OFFSET) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2 nt" ::"v"(p), "s"(to - OFFSET), "n"(OFFSET) : "memory");
 }
 // 4 bytes likewise, to `to` + 4 * lane
 __device__ __forceinline__ void load4_to_lds(const void* p, uint32_t to) {

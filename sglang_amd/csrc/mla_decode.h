@@ -41,6 +41,7 @@ struct MlaDecodeArgs {
   v2i* spans;              // [B]: the first run that holds tokens of a request, and how many do
   int B, n, H, M;
   int page_size, pages, max_len;
+  int page_shift;  // log2 of page_size, or -1
   int walkers, mblocks;
   float sm_scale;
 };
@@ -138,10 +139,6 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
 
   const int row = mblk * R + wm * 16 + l15;  // this lane's, of the M of a request
 
-  // Waves w and w + 4 share a SIMD.  With the first one's instructions in front, it runs ahead of the other within a tile, and its softmax beside the
-  // other's products.
-  if (NW == 8 && w < 4) __builtin_amdgcn_s_setprio(1);
-
   for (int pos = first, next_len; pos < last; ++b, len = next_len) {
     next_len = b + 1 < p.B ? mla_len(p, b + 1) : 0;
     const int tiles = mla_tiles(len), t_begin = pos - at, t_end = min(last - at, tiles);
@@ -149,24 +146,6 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
     at += tiles;
     if (t_begin >= t_end) continue;
     pos += t_end - t_begin;
-
-    // ---- the rows' queries, and how many tokens each sees
-    const int r_in = min(row, p.M - 1), qi = r_in / p.H, qh = r_in - qi * p.H;
-    const int lim = len - (p.n - 1 - qi);
-    v4i q[18];
-    {
-      const u16* qn = (const u16*)p.q_nope + b * p.qn_b + qi * p.qn_n + qh * p.qn_h + 8 * g;
-      const u16* qp = (const u16*)p.q_pe + b * p.qp_b + qi * p.qp_n + qh * p.qp_h + 8 * g;
-#pragma unroll
-      for (int ks = 0; ks < 16; ++ks) q[ks] = *(const v4i*)(qn + 32 * ks);
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) q[16 + ks] = *(const v4i*)(qp + 32 * ks);
-    }
-
-    v4f o[32];
-#pragma unroll
-    for (int dt = 0; dt < 32; ++dt) o[dt] = v4f{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f;
 
     // ---- fetching.  Steps are counted from the segment's first.  Tokens past the end are the last one's row again (masked).
     const int base = t_begin * kMlaTile, steps = min((t_end - t_begin) * (kMlaTile / TT), (len - base + TT - 1) / TT);
@@ -182,10 +161,11 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
     // loads can be counted; past the end for the last row again.
     const int32_t* const pages_of = p.table + b * p.table_stride;
     const uint32_t pages_to = lds_address(&pages[0][w][0]);
+    auto page_of = [&](uint32_t tok) { return p.page_shift >= 0 ? tok >> p.page_shift : tok / (uint32_t)p.page_size; };
     auto fetch_pages = [&](int t) {
       const int lane = fresh_lane();
       const uint32_t tok = min(base + t * TT + first_row + lane, len - 1);
-      if (lane < kRowsOfWave) load4_to_lds(pages_of + tok / (uint32_t)p.page_size, pages_to + (t % kPageSlots) * (NW * 64));
+      if (lane < kRowsOfWave) load4_to_lds(pages_of + page_of(tok), pages_to + (t % kPageSlots) * (NW * 64));
     };
     auto fetch = [&](int t, uint32_t to) {  // to: of the stage
       const int lane = fresh_lane();
@@ -193,7 +173,7 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
 #pragma unroll
       for (int k = 0; k < kRowsOfLane; ++k) {
         const int r = FP8 ? lane >> 2 : 8 * k + (lane >> 3);  // of the wave's
-        const uint32_t tok = min(base + t * TT + first_row + r, len - 1), place = tok % (uint32_t)p.page_size;
+        const uint32_t tok = min(base + t * TT + first_row + r, len - 1), place = tok - page_of(tok) * (uint32_t)p.page_size;
         const uint32_t page = min(max(pages[t % kPageSlots][w][r], 0), p.pages - 1);
         from[k] = p.cache + (uint64_t)page * (uint32_t)(p.page_size * kRow) + (place * kRow + (FP8 ? (lane & 3) : (lane & 7) ^ mla_swizzle(first_row + r)) * 16);
       }
@@ -213,42 +193,32 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
       if (kSharers == 1 || share == 0) wait_loads<kF * kMost * kRowsOfLane + kP>();
       else wait_loads<kF * kLeast * kRowsOfLane + kP>();
     };
-    // 8-bit rows of a stage, as this wave fetched them, to 16 bits in a tile
-    auto widen_blocks = [&](const uint8_t* stage, uint8_t* tile, auto first_block, auto last_block) {
-      constexpr int kFirst = decltype(first_block)::value, kLast = decltype(last_block)::value;
-      const int lane = fresh_lane();
-      uint8_t* const to = tile + (first_row + (lane >> 2)) * 128;
-      const int at0 = ((2 * (lane & 3)) ^ mla_swizzle(lane >> 2)) << 4;
-      const uint8_t* const from = stage + group * 9 * 1024 + lane * 16;
-      v4i raw[kLast - kFirst];
-#pragma unroll
-      for (int j = kFirst; j < kLast; ++j) raw[j - kFirst] = *(const v4i*)(from + j * 1024);
-#pragma unroll
-      for (int j = kFirst; j < kLast; ++j) {
-        const v4i x = raw[j - kFirst];
-        *(v4i*)(to + j * kBlock + at0) = v4i{(int)fp8_to_16bit<DT, false>(x[0]), (int)fp8_to_16bit<DT, true>(x[0]),
-                                             (int)fp8_to_16bit<DT, false>(x[1]), (int)fp8_to_16bit<DT, true>(x[1])};
-        *(v4i*)(to + j * kBlock + (at0 ^ 16)) = v4i{(int)fp8_to_16bit<DT, false>(x[2]), (int)fp8_to_16bit<DT, true>(x[2]),
-                                                    (int)fp8_to_16bit<DT, false>(x[3]), (int)fp8_to_16bit<DT, true>(x[3])};
-      }
+    // 8-bit rows of a stage, as this wave fetched them: to registers, and from there as 16 bits to a tile
+    const int first_block = share == 0 ? 0 : kMost + (share - 1) * kLeast;
+    struct Raw {
+      v4i x[kMost];
     };
-    auto widen = [&](const uint8_t* stage, uint8_t* tile) {
-      if constexpr (kSharers == 1) {
-        widen_blocks(stage, tile, Const<0>{}, Const<9>{});
-      } else if constexpr (kSharers == 2) {
-        if (share == 0) {
-          widen_blocks(stage, tile, Const<0>{}, Const<3>{});  // a few at a time: registers
-          widen_blocks(stage, tile, Const<3>{}, Const<5>{});
-        } else {
-          widen_blocks(stage, tile, Const<5>{}, Const<7>{});
-          widen_blocks(stage, tile, Const<7>{}, Const<9>{});
+    auto raw_of = [&](const uint8_t* stage) {
+      const uint8_t* const from = stage + (group * 9 + first_block) * 1024 + fresh_lane() * 16;
+      Raw raw;
+#pragma unroll
+      for (int j = 0; j < kMost; ++j)
+        if (j < kLeast || share == 0) raw.x[j] = *(const v4i*)(from + j * 1024);
+      return raw;
+    };
+    auto widen = [&](const Raw& raw, uint8_t* tile) {
+      const int lane = fresh_lane();
+      uint8_t* const to = tile + first_block * kBlock + (first_row + (lane >> 2)) * 128;
+      const int at0 = ((2 * (lane & 3)) ^ mla_swizzle(lane >> 2)) << 4;
+#pragma unroll
+      for (int j = 0; j < kMost; ++j)
+        if (j < kLeast || share == 0) {
+          const v4i x = raw.x[j];
+          *(v4i*)(to + j * kBlock + at0) = v4i{(int)fp8_to_16bit<DT, false>(x[0]), (int)fp8_to_16bit<DT, true>(x[0]),
+                                               (int)fp8_to_16bit<DT, false>(x[1]), (int)fp8_to_16bit<DT, true>(x[1])};
+          *(v4i*)(to + j * kBlock + (at0 ^ 16)) = v4i{(int)fp8_to_16bit<DT, false>(x[2]), (int)fp8_to_16bit<DT, true>(x[2]),
+                                                      (int)fp8_to_16bit<DT, false>(x[3]), (int)fp8_to_16bit<DT, true>(x[3])};
         }
-      } else {
-        if (share == 0) widen_blocks(stage, tile, Const<0>{}, Const<3>{});
-        else if (share == 1) widen_blocks(stage, tile, Const<3>{}, Const<5>{});
-        else if (share == 2) widen_blocks(stage, tile, Const<5>{}, Const<7>{});
-        else widen_blocks(stage, tile, Const<7>{}, Const<9>{});
-      }
     };
 
     constexpr int kStagesAt = kTiles * kTileBytes;
@@ -267,19 +237,41 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
     constexpr int kFirst = FP8 ? kStageCount : kRun;  // steps asked for at first, with pages that have come already
 #pragma unroll
     for (int t = 0; t < kFirst + (kDeep ? 0 : 1); ++t) fetch_pages(t);
+
     wait_loads<0>();
 #pragma unroll
     for (int t = 0; t < kFirst; ++t)
       if (t < steps) ask(t);
+
+    // ---- the rows' queries, and how many tokens each sees
+    const int r_in = min(row, p.M - 1), qi = r_in / p.H, qh = r_in - qi * p.H;
+    const int lim = len - (p.n - 1 - qi);
+    v4i q[18];
+    {
+      const u16* qn = (const u16*)p.q_nope + b * p.qn_b + qi * p.qn_n + qh * p.qn_h + 8 * g;
+      const u16* qp = (const u16*)p.q_pe + b * p.qp_b + qi * p.qp_n + qh * p.qp_h + 8 * g;
+#pragma unroll
+      for (int ks = 0; ks < 16; ++ks) q[ks] = *(const v4i*)(qn + 32 * ks);
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) q[16 + ks] = *(const v4i*)(qp + 32 * ks);
+    }
+
+    v4f o[32];
+#pragma unroll
+    for (int dt = 0; dt < 32; ++dt) o[dt] = v4f{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+
     if constexpr (FP8 && kDeep) {  // the first tile, and the rows that take its stage
       wait_loads<0>();
-      widen(stage_of(0), smem);
+      widen(raw_of(stage_of(0)), smem);
       wait_lds();
       if (kStageCount < steps) ask(kStageCount);
     }
+    wait_loads<0>();  // the queries: waited for here, not in the loop
     for (int t = 0; t < steps; ++t) {
       const int lane = fresh_lane(), l15 = lane & 15, g = lane >> 4;
       const uint8_t* tile;
+      Raw raw;
       if constexpr (!kDeep) {
         if (WM > 1) lds_only_barrier();  // nobody reads the step before any more
         else wait_lds();
@@ -292,11 +284,10 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
         } else {
           if (t + 1 < steps) wait_but(Const<1>{}, Const<0>{});
           else wait_loads<0>();
-          widen(stage_of(t), smem);
-          if (t + 2 < steps) {
-            wait_lds();  // the stage has been read
-            ask(t + 2);
-          }
+          const Raw raw = raw_of(stage_of(t));
+          wait_lds();
+          if (t + 2 < steps) ask(t + 2);
+          widen(raw, smem);
           tile = smem;
         }
         if (WM > 1) lds_only_barrier();  // everybody's part of the step is there
@@ -304,25 +295,20 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
         if (t + 2 < steps) wait_but(Const<2>{}, Const<1>{});
         else wait_loads<0>();
         lds_only_barrier();  // everybody's part of the step is there, and nobody reads the step before any more
-        if (t + 3 < steps) ask(t + 3);
         tile = stage_of(t);
       } else {
         lds_only_barrier();  // this step's tile is whole, and nobody reads the other any more
         if (t + 1 < steps) {
           if (t + 4 < steps) wait_but(Const<3>{}, Const<3>{});
           else wait_loads<0>();
-          widen(stage_of(t + 1), smem + (t + 1) % 2 * kTileBytes);
-          if (t + 5 < steps) {
-            wait_lds();  // the stage has been read
-            ask(t + 5);
-          }
+          raw = raw_of(stage_of(t + 1));
         }
         tile = smem + t % 2 * kTileBytes;
       }
 
       // ---- S^T = K . Q^T: kAhead operand reads run ahead of the products.  With one tile of tokens, two sums by turns: a product waits for the
       // one before it in its sum.
-      constexpr int kSums = NT == 1 ? 2 : NT, kAhead = NW == 8 ? 6 : 8;
+      constexpr int kSums = NT == 1 ? 2 : NT, kAhead = NW == 4 ? 8 : kDeep && FP8 ? 3 : 6;
       v4f s[kSums];
 #pragma unroll
       for (int i = 0; i < kSums; ++i) s[i] = v4f{0, 0, 0, 0};
@@ -346,6 +332,17 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
         }
       }
       if constexpr (NT == 1) s[0] += s[1];
+      // what has to be done for later steps, beside the last products
+      if constexpr (kDeep && !FP8) {
+        if (t + 3 < steps) ask(t + 3);
+      }
+      if constexpr (kDeep && FP8) {
+        if (t + 1 < steps) {
+          wait_lds();  // the stage has been read
+          if (t + 5 < steps) ask(t + 5);
+          widen(raw, smem + (t + 1) % 2 * kTileBytes);
+        }
+      }
 
       // ---- softmax: a lane's scores are those of query row l15, tokens 16 nt + 4 g + i
       const int tok0 = base + t * TT + wt * NT * 16 + 4 * g;
@@ -496,7 +493,7 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
 template <int DT, int WAVES>
 __global__ __launch_bounds__(256) void mla_join_kernel(const MlaDecodeArgs p) {
   __shared__ v4f parts[WAVES == 1 ? 1 : 3 * 128];
-  const int lane = threadIdx.x & 63, w = (int)(threadIdx.x >> 6) % WAVES;
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) % WAVES);
   const int b = blockIdx.y, r = (int)blockIdx.x * (4 / WAVES) + (int)(threadIdx.x >> 6) / WAVES;
   if (r >= p.M) return;  // whole workgroups, with WAVES = 4
   const v2i span = p.spans[b];  // anything, for a request without tokens
@@ -513,37 +510,47 @@ __global__ __launch_bounds__(256) void mla_join_kernel(const MlaDecodeArgs p) {
   const int n = span[1];
   if (n == 1) return;
   const int64_t slot = span[0] + b;
-  // n <= 256: four partials' logarithms to a lane
-  float lse[4], top = -INFINITY;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    lse[k] = k * 64 + lane < n ? p.part_lse[(slot + k * 64 + lane) * p.M + r] : -INFINITY;
-    top = fmaxf(top, lse[k]);
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-  const float shift = shift_of(top);
-  float sum = 0.0f;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    lse[k] = __builtin_amdgcn_exp2f(lse[k] - shift);  // its weight
-    sum += lse[k];
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+  // The partials are asked for before their weights are known, a batch of up to 64 at a time (n <= 256): a logarithm to a lane, and
+  // kEach partials to a wave at once.
+  constexpr int kEach = WAVES == 1 ? 4 : 16;
   v4f x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+  float top = -INFINITY, sum = 0.0f;
   const float* const from = p.part + (slot * p.M + r) * kLatent + 4 * lane;
+  for (int at = 0; at < n; at += kEach * WAVES) {
+    const int count = min(n - at, kEach * WAVES);  // at most 64
+    const float lse = lane < count ? p.part_lse[(slot + at + lane) * p.M + r] : -INFINITY;
+    v4f u[kEach], v[kEach];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const int end = min(n - k * 64, 64);
-#pragma unroll 8
-    for (int i = w; i < end; i += WAVES) {
-      const float* const at = from + (int64_t)(k * 64 + i) * p.M * kLatent;
-      const float weight = __shfl(lse[k], i);
-      x += weight * *(const v4f*)at;
-      y += weight * *(const v4f*)(at + 256);
+    for (int i = 0; i < kEach; ++i) {
+      u[i] = v[i] = v4f{0, 0, 0, 0};
+      if (i * WAVES + w < count) {
+        const float* const part = from + (int64_t)(at + i * WAVES + w) * p.M * kLatent;
+        u[i] = *(const v4f*)part;
+        v[i] = *(const v4f*)(part + 256);
+      }
+    }
+    float most = lse;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) most = fmaxf(most, __shfl_xor(most, d));
+    most = fmaxf(most, top);
+    const float before = __builtin_amdgcn_exp2f(top - shift_of(most));  // 0 at first
+    const float weight = __builtin_amdgcn_exp2f(lse - shift_of(most));
+    top = most;
+    float s = weight;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
+    sum = sum * before + s;
+    x *= before;
+    y *= before;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      if (i * WAVES + w >= count) break;
+      const float f = __shfl(weight, i * WAVES + w);
+      x += f * u[i];
+      y += f * v[i];
     }
   }
+  const float shift = shift_of(top);
   if constexpr (WAVES > 1) {
     if (w) {
       parts[(w - 1) * 128 + lane] = x;
