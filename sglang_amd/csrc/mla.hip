@@ -399,6 +399,7 @@ extern "C" int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_str
                "mla prefill: operands must be 16-byte aligned");
   FP8K_REQUIRE(q_stride_t >= 0 && q_stride_h >= 0 && kn_stride_t >= 0 && kn_stride_h >= 0 && kp_stride_t >= 0 && v_stride_t >= 0 && v_stride_h >= 0,
                "mla prefill: negative stride");
+  FP8K_REQUIRE(kn_stride_t < (1 << 24) && kp_stride_t < (1 << 24) && v_stride_t < (1 << 24), "mla prefill: rows of keys further apart than 2^24");
   const int64_t blocks = (std::min(max_seqlen_q, Tq) + kPreRows - 1) / kPreRows, units = up_to(B * H, 8);
   FP8K_REQUIRE(units * blocks < (1ll << 31), "mla prefill: too many blocks of queries");
   MlaPrefillArgs p{};

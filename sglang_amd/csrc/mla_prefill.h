@@ -3,14 +3,17 @@
 //
 //   s[i, j] = scale * (q[i, :128] . k_nope[j] + q[i, 128:] . k_pe[j]),   o[i] = sum over j <= i + Lk - Lq of softmax(s[i])[j] v[j]
 //
-// A workgroup is four waves with 32 query rows each, on tiles of 64 keys; two workgroups share a CU, so that one's softmax runs beside the
-// other's products.  Scores are formed transposed, S^T = K . Q^T, in 32x32x16 products: a lane holds 32 scores of one query row, a row's maximum is
-// a lane's own and that of the lane 32 away, and what a lane holds is the operand of O^T = V^T . P^T as it lies, the order of the keys inside
-// a product being free as long as V^T, read from LDS by transposed reads, has the same.
+// A workgroup is four waves with 32 query rows each, on tiles of 64 keys; two workgroups share a CU.  Scores are formed transposed, S^T = K . Q^T, in
+// 32x32x16 products: a lane holds 32 scores of one query row, a row's maximum is a lane's own and that of the lane 32 away, and what a lane
+// holds is the operand of O^T = V^T . P^T as it lies, the order of the keys inside a product being free as long as V^T, read from LDS by
+// transposed reads, has the same.
 //
-// LDS: two stages of k_nope [64, 128], k_pe [64, 64] and v [64, 128], filled by global_load_lds; the position part is read where it lies, once for
-// each head, and never copied beside the keys.  16-byte chunks of a row are permuted by the row so that the operand reads (16 rows, one
-// chunk) and the transposed ones (8 rows, two chunks) spread over all banks.
+// The products of tile t + 1 run beside the exponentials of tile t, one instruction behind the other: a product keeps the matrix core busy for 32 clocks,
+// in which the wave issues the exponentials of two scores.
+//
+// LDS: two stages of k_nope [64, 128] and k_pe [64, 64], and two of v [64, 128], one tile behind, filled by global_load_lds; the position part is
+// read where it lies, once for each head, and never copied beside the keys.  16-byte chunks of a row are permuted by the row so that the
+// operand reads (16 rows, one chunk) and the transposed ones (8 rows, two chunks) spread over all banks.
 #pragma once
 
 #include "mla_common.h"
@@ -35,8 +38,8 @@ __device__ __forceinline__ int mla_value_swizzle(int r) { return ((r & 1) ? 12 :
 
 template <int DT>
 __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArgs p) {
-  constexpr int kN = 0, kP = kPreKeys * 256, kV = kP + kPreKeys * 128, kStage = kV + kPreKeys * 256;  // 40960 bytes
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kStage];
+  constexpr int kKey = kPreKeys * 384, kVal = kPreKeys * 256, kPe = kPreKeys * 256;  // bytes of a stage, and where k_pe begins in it
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[2 * kKey + 2 * kVal];
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, half = lane >> 5;
@@ -66,27 +69,55 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
     for (int ks = 0; ks < 12; ++ks) q[ks] = *(const v4i*)(from + 16 * ks);
   }
 
-  // a wave fetches 16 rows of each part of a stage: four wave-loads of k_nope, two of k_pe, four of v
-  auto fetch = [&](int t, uint32_t stage) {
+  // A wave fetches 16 rows of each part of a stage: four wave-loads of k_nope and of v, of four rows each, two of k_pe, of eight.  Load j is of row
+  // 4 j (8 j) + lane / 16 (lane / 8) of the wave's: the lane's offset is that row's, which j moves by a number that all lanes share, and a chunk, which j
+  // moves by an exclusive or.  Rows past the sequence's last are that row again (masked).
+  const uint32_t lds0 = lds_address(smem);
+  const int r16 = w * 16 + (lane >> 4), r8 = w * 16 + (lane >> 3);
+  const int n_chunk = (lane & 15) ^ (r16 & 15), p_chunk = (lane & 7) ^ ((r8 >> 1) & 7), v_part = (lane & 15) ^ mla_value_swizzle(r16);
+  const uint32_t n_stride = (uint32_t)p.kn_t * 2, p_stride = (uint32_t)p.kp_t * 2, v_stride = (uint32_t)p.v_t * 2;  // bytes
+  const uint8_t* const n_from = (const uint8_t*)p.k_nope + ((int64_t)k_begin * p.kn_t + h * p.kn_h) * 2;
+  const uint8_t* const p_from = (const uint8_t*)p.k_pe + (int64_t)k_begin * p.kp_t * 2;
+  const uint8_t* const v_from = (const uint8_t*)p.v + ((int64_t)k_begin * p.v_t + h * p.v_h) * 2;
+  auto fetch_keys = [&](int t) {
+    const uint32_t to = lds0 + (t & 1) * kKey + w * 16 * 256, to_pe = lds0 + (t & 1) * kKey + kPe + w * 16 * 128;
+    const uint8_t* const n_tile = n_from + (uint64_t)(uint32_t)(t * kPreKeys) * n_stride;
+    const uint8_t* const p_tile = p_from + (uint64_t)(uint32_t)(t * kPreKeys) * p_stride;
+    if ((t + 1) * kPreKeys <= lk) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int r = w * 16 + j * 4 + (lane >> 4), at = lane & 15;
-      const int64_t row = k_begin + min(t * kPreKeys + r, lk - 1);
-      load16_to_lds((const u16*)p.k_nope + row * p.kn_t + h * p.kn_h + ((at ^ (r & 15)) << 3), stage + kN + (w * 16 + j * 4) * 256);
-      load16_to_lds((const u16*)p.v + row * p.v_t + h * p.v_h + ((at ^ mla_value_swizzle(r)) << 3), stage + kV + (w * 16 + j * 4) * 256);
+      for (int j = 0; j < 4; ++j) load16_to_lds(n_tile + 4 * j * n_stride, r16 * n_stride + ((n_chunk ^ (4 * j)) << 4), to + j * 1024);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) load16_to_lds(p_tile + 8 * j * p_stride, r8 * p_stride + ((p_chunk ^ (4 * j)) << 4), to_pe + j * 1024);
+    } else {
+      const int last = lk - 1 - t * kPreKeys;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) load16_to_lds(n_tile, min(r16 + 4 * j, last) * n_stride + ((n_chunk ^ (4 * j)) << 4), to + j * 1024);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) load16_to_lds(p_tile, min(r8 + 8 * j, last) * p_stride + ((p_chunk ^ (4 * j)) << 4), to_pe + j * 1024);
     }
+  };
+  auto fetch_values = [&](int t) {
+    const uint32_t to = lds0 + 2 * kKey + (t & 1) * kVal + w * 16 * 256;
+    const uint8_t* const tile = v_from + (uint64_t)(uint32_t)(t * kPreKeys) * v_stride;
+    if ((t + 1) * kPreKeys <= lk) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int r = w * 16 + j * 8 + (lane >> 3), at = lane & 7;
-      const int64_t row = k_begin + min(t * kPreKeys + r, lk - 1);
-      load16_to_lds((const u16*)p.k_pe + row * p.kp_t + ((at ^ ((r >> 1) & 7)) << 3), stage + kP + (w * 16 + j * 8) * 128);
+      for (int j = 0; j < 4; ++j) load16_to_lds(tile + 4 * j * v_stride, r16 * v_stride + ((v_part ^ (j & 1 ? 6 : 0)) << 4), to + j * 1024);
+    } else {
+      const int last = lk - 1 - t * kPreKeys;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) load16_to_lds(tile, min(r16 + 4 * j, last) * v_stride + ((v_part ^ (j & 1 ? 6 : 0)) << 4), to + j * 1024);
     }
   };
 
-  // LDS offsets of a lane: row l31 of a 32-key tile, chunk 2 ks + half; transposed reads of v
-  const int n_off = kN + l31 * 256, n_sw = l31 & 15, p_off = kP + l31 * 128, p_sw = (l31 >> 1) & 7;
+  // LDS offsets of a lane in a stage: row l31 of a 32-key tile, chunk `half` of k_nope and of k_pe; a transposed read of v.  Other chunks differ in
+  // bits 4 .. 7 alone: an exclusive or.
+  const int n_off = l31 * 256 + ((half ^ (l31 & 15)) << 4), p_off = kPe + l31 * 128 + ((half ^ ((l31 >> 1) & 7)) << 4);
   const int v_row = 4 * half + ((lane & 15) >> 2), v_chunk = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-  const int v_off = kV + v_row * 256 + ((lane & 1) << 3), v_sw = mla_value_swizzle(v_row);
+  const int v_off = 2 * kKey + v_row * 256 + ((v_chunk ^ mla_value_swizzle(v_row)) << 4) + ((lane & 1) << 3);
+  auto anew = [](int x) {  // computed where it is used, rather than a dozen addresses kept
+    asm volatile("" : "+v"(x));
+    return x;
+  };
 
   v16f o[4];
 #pragma unroll
@@ -95,31 +126,29 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
   float m = -INFINITY, l = 0.0f;
 
-  const uint32_t lds0 = lds_address(smem);
-  if (tiles > 0) fetch(0, lds0);
-  for (int t = 0; t < tiles; ++t) {
-    const uint8_t* const stage = smem + (t & 1) * kStage;
-    wait_loads<0>();
-    lds_only_barrier();  // this tile has arrived, and nobody reads the one before any more
-    if (t + 1 < tiles) fetch(t + 1, lds0 + ((t + 1) & 1) * kStage);
-    if (t * kPreKeys >= wave_keys) continue;  // nothing that this wave's rows see
-
-    v16f s[2];
+  // operand i of a tile's scores: 24 products, the two 32-key tiles by turns
+  auto key_operand = [&](int n_at, int p_at, int i) {
+    const int ks = i >> 1, nt = i & 1;
+    return *(const v4i*)(smem + (ks < 8 ? (n_at ^ (ks << 5)) + nt * 32 * 256 : (p_at ^ ((ks - 8) << 5)) + nt * 32 * 128));
+  };
+  auto first_scores = [&](v16f* s) {
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
+    for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[nt][i] = 0.0f;
-#pragma unroll
-      for (int ks = 0; ks < 12; ++ks) {
-        const uint8_t* const at = ks < 8 ? stage + n_off + nt * 32 * 256 + (((2 * ks + half) ^ n_sw) << 4)
-                                         : stage + p_off + nt * 32 * 128 + (((2 * (ks - 8) + half) ^ p_sw) << 4);
-        s[nt] = mfma32<DT>(*(const v4i*)at, q[ks], s[nt]);
-      }
-    }
+  };
+
+  // One tile: the weights of the scores s of tile t and their product with v, and, if there are any, the scores `next` of tile t + 1.
+  auto step = [&](int t, v16f* s, v16f* next) {
+    wait_loads<0>();
+    lds_only_barrier();  // keys of t + 1 and values of t have arrived, and nobody reads those of t and t - 1 any more
+    if (t + 2 < tiles) fetch_keys(t + 2);
+    if (t + 1 < tiles) fetch_values(t + 1);
+    if (t * kPreKeys >= wave_keys) return;  // nothing that this wave's rows see
 
     // a lane's scores are those of query row l31, keys 32 nt + 8 (i / 4) + 4 half + i % 4
-    const int key0 = t * kPreKeys + 4 * half;
     if (__builtin_expect((t + 1) * kPreKeys > wave_free, 0)) {
+      const int key0 = t * kPreKeys + 4 * half;
 #pragma unroll
       for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
@@ -142,30 +171,91 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
       for (int dt = 0; dt < 4; ++dt) o[dt] *= alpha;
     }
     const float shift = shift_of(m);
-    uint32_t pk[2][8];
+    uint32_t pk[16];
+    // scores 2 j and 2 j + 1: arguments, exponentials, and one pair later sum and rounding to the 16-bit type, as the matrix core takes them; the sum is of
+    // the unrounded ones
+    auto argument = [&](int j) {
+      s[j >> 3][(2 * j) & 15] = fmaf(s[j >> 3][(2 * j) & 15], c, -shift);
+      s[j >> 3][(2 * j + 1) & 15] = fmaf(s[j >> 3][(2 * j + 1) & 15], c, -shift);
+    };
+    auto exponential = [&](int j) {
+      s[j >> 3][(2 * j) & 15] = __builtin_amdgcn_exp2f(s[j >> 3][(2 * j) & 15]);
+      s[j >> 3][(2 * j + 1) & 15] = __builtin_amdgcn_exp2f(s[j >> 3][(2 * j + 1) & 15]);
+    };
+    auto finish = [&](int j) {
+      l += s[j >> 3][(2 * j) & 15];
+      l += s[j >> 3][(2 * j + 1) & 15];
+      pk[j] = pack2<DT>(s[j >> 3][(2 * j) & 15], s[j >> 3][(2 * j + 1) & 15]);
+    };
+    argument(0);
+    argument(1);
+    exponential(0);
+    if ((t + 1) * kPreKeys < wave_keys) {
+      constexpr int kAhead = 5;
+      v4i ring[kAhead];
+      const int n_at = anew(n_off + ((t + 1) & 1) * kKey), p_at = anew(p_off + ((t + 1) & 1) * kKey);
+      first_scores(next);
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
+      for (int i = 0; i < kAhead; ++i) ring[i] = key_operand(n_at, p_at, i);
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        const float e0 = __builtin_amdgcn_exp2f(fmaf(s[nt][i], c, -shift)), e1 = __builtin_amdgcn_exp2f(fmaf(s[nt][i + 1], c, -shift));
-        l += e0;
-        l += e1;
-        // weights rounded to the 16-bit type, as the matrix core takes them; their sum is of the unrounded ones
-        pk[nt][i >> 1] = pack2<DT>(e0, e1);
-      }
-
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        const v4i pb = {(int)pk[nt][4 * ks], (int)pk[nt][4 * ks + 1], (int)pk[nt][4 * ks + 2], (int)pk[nt][4 * ks + 3]};
-#pragma unroll
-        for (int dt = 0; dt < 4; ++dt) {
-          const uint8_t* const at = stage + v_off + (nt * 32 + ks * 16) * 256 + (((4 * dt + v_chunk) ^ v_sw) << 4);
-          const v2i a0 = lds_read_transposed(at), a1 = lds_read_transposed(at + 8 * 256);
-          o[dt] = mfma32<DT>(v4i{a0[0], a0[1], a1[0], a1[1]}, pb, o[dt]);
+      for (int i = 0; i < 24; ++i) {
+        next[i & 1] = mfma32<DT>(ring[i % kAhead], q[i >> 1], next[i & 1]);
+        if (i + kAhead < 24) ring[i % kAhead] = key_operand(n_at, p_at, i + kAhead);
+        if (i % 3 != 2) {  // two pairs to three products
+          const int j = i / 3 * 2 + i % 3;
+          if (j + 2 < 16) argument(j + 2);
+          if (j + 1 < 16) exponential(j + 1);
+          finish(j);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        if (j + 2 < 16) argument(j + 2);
+        if (j + 1 < 16) exponential(j + 1);
+        finish(j);
+      }
+    }
+
+    {
+      constexpr int kAhead = 5;
+      v2i ring[kAhead][2];
+      const int v_at = anew(v_off + (t & 1) * kVal);
+      auto read = [&](int i, v2i* to) {
+        const uint8_t* const at = smem + (v_at ^ ((i & 3) << 6)) + (i >> 2) * 16 * 256;
+        to[0] = lds_read_transposed(at);
+        to[1] = lds_read_transposed(at + 8 * 256);
+      };
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) read(i, ring[i]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const v2i* const a = ring[i % kAhead];
+        const int k = i >> 2;
+        o[i & 3] = mfma32<DT>(v4i{a[0][0], a[0][1], a[1][0], a[1][1]}, v4i{(int)pk[4 * k], (int)pk[4 * k + 1], (int)pk[4 * k + 2], (int)pk[4 * k + 3]}, o[i & 3]);
+        if (i + kAhead < 16) read(i + kAhead, ring[i % kAhead]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+
+  v16f s0[2], s1[2];
+  if (tiles > 0) {
+    fetch_keys(0);
+    wait_loads<0>();
+    lds_only_barrier();
+    if (tiles > 1) fetch_keys(1);
+    fetch_values(0);
+    first_scores(s0);
+    if (wave_keys > 0) {
+#pragma unroll
+      for (int i = 0; i < 24; ++i) s0[i & 1] = mfma32<DT>(key_operand(n_off, p_off, i), q[i >> 1], s0[i & 1]);
+    }
+  }
+  for (int t = 0; t < tiles; t += 2) {
+    step(t, s0, s1);
+    if (t + 1 < tiles) step(t + 1, s1, s0);
   }
 
   l = sum_across32(l);
