@@ -576,11 +576,15 @@ int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t qn_stride_n
  * of k_nope [Tk, H, 128], k_pe [Tk, 64] (all heads') and v [Tk, H, 128] (int32 [B + 1], not decreasing).  Query i of its lq sees (causal) keys j <= i + lk - lq, else all.
  * out [Tq, H, 128] and lse (NULL or float32 [Tq, H]) contiguous; a query that sees nothing gets 0 and -inf, queries of no sequence
  * stay as they are.  max_seqlen_q: at least the longest lq.  Keys that a sequence has must be finite; whatever lies outside it may be anything.
+ * Workspace: 256-byte aligned, fp8k_mla_prefill_workspace_bytes of it (0 possible: few blocks of queries with long keys are split over the
+ * keys, and joined in float32), not initialised.
  */
+int64_t fp8k_mla_prefill_workspace_bytes(int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q);
 int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_nope, int64_t kn_stride_t,
                      int64_t kn_stride_h, const void* k_pe, int64_t kp_stride_t, const void* v, int64_t v_stride_t,
                      int64_t v_stride_h, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, void* out, float* lse, int64_t B,
-                     int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q, float sm_scale, int causal, int dtype, void* stream);
+                     int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q, float sm_scale, int causal, int dtype, void* workspace,
+                     int64_t workspace_bytes, void* stream);
 
 /*
  * Two attentions over disjoint keys as one: out = (exp(lse_a) out_a + exp(lse_b) out_b) / (exp(lse_a) + exp(lse_b)), lse = log(exp(lse_a) + exp(lse_b)),

@@ -119,9 +119,10 @@ SIGNATURES = {
         _c_int, [_c_ptr] + [_c_i64] * 3 + [_c_ptr] + [_c_i64] * 3 + [_c_ptr, _c_ptr, _c_i64, _c_i64] + [_c_ptr] * 4 + [_c_i64] * 5
         + [_c_f32, _c_int, _c_int, _c_ptr, _c_i64, _c_ptr],
     ),
+    "fp8k_mla_prefill_workspace_bytes": (_c_i64, [_c_i64] * 5),
     "fp8k_mla_prefill": (
         _c_int, [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_i64, _c_i64] + [_c_ptr] * 4 + [_c_i64] * 5
-        + [_c_f32, _c_int, _c_int, _c_ptr],
+        + [_c_f32, _c_int, _c_int, _c_ptr, _c_i64, _c_ptr],
     ),
     "fp8k_merge_attention_states": (_c_int, [_c_ptr] * 6 + [_c_i64, _c_i64, _c_int, _c_ptr]),
     "fp8k_moe_fused_gate": (

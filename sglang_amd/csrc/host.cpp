@@ -985,9 +985,11 @@ PyObject* mla_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     OBSERVED("mla_prefill", q, kn, kp, v, cu_q, cu_k);
     if (fresh) out = empty({Tq, H, kMlaValue}, dt, q.device());
     if (want_lse) lse = empty({Tq, H}, ScalarType::Float, q.device());
+    const int64_t wsb = fp8k_mla_prefill_workspace_bytes(B, H, Tq, Tk, most);
+    Scratch mem(wsb, c.stream);
     check(fp8k_mla_prefill(q.data_ptr(), q.stride(0), q.stride(1), kn.data_ptr(), kn.stride(0), kn.stride(1), kp.data_ptr(), kp.stride(0), v.data_ptr(),
                            v.stride(0), v.stride(1), cu_q.data_ptr<int32_t>(), cu_k.data_ptr<int32_t>(), out.data_ptr(), float_or_null(lse), B, H, Tq,
-                           Tk, most, (float)sm_scale, causal, code(dt), c.stream));
+                           Tk, most, (float)sm_scale, causal, code(dt), wsb ? mem.take(wsb) : nullptr, wsb, c.stream));
   }
   PyObject* const result = fresh ? THPVariable_Wrap(std::move(out)) : same(a[10]);
   return want_lse ? pair(result, THPVariable_Wrap(std::move(lse))) : result;

@@ -240,6 +240,14 @@ DecodePlan decode_plan(int64_t B, int64_t M, int64_t max_len) {
   return d;
 }
 
+// Splits of the keys of a prefill call: none, unless its blocks of queries leave CUs idle and the keys are long; then as many as give every CU its
+// two workgroups, eight tiles of keys to each on average.
+int prefill_splits(int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q) {
+  const int64_t blocks = (std::min(max_seqlen_q, Tq) + kPreRows - 1) / kPreRows, groups = B * H * blocks;
+  if (groups <= 0 || groups > num_cu()) return 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(2 * num_cu() / groups, 32), Tk / B / (8 * kPreKeys)));
+}
+
 }  // namespace
 }  // namespace fp8k
 
@@ -383,10 +391,17 @@ extern "C" int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t 
   return check_launch("mla decode");
 }
 
+extern "C" int64_t fp8k_mla_prefill_workspace_bytes(int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q) {
+  if (B <= 0 || H <= 0 || Tq <= 0 || Tk <= 0 || max_seqlen_q <= 0) return 0;
+  const int64_t splits = prefill_splits(B, H, Tq, Tk, max_seqlen_q);
+  return splits == 1 ? 0 : up_to(splits * Tq * H * kPreValue * 4, 256) + up_to(splits * Tq * H * 4, 256);
+}
+
 extern "C" int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_nope, int64_t kn_stride_t,
                                 int64_t kn_stride_h, const void* k_pe, int64_t kp_stride_t, const void* v, int64_t v_stride_t,
                                 int64_t v_stride_h, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, void* out, float* lse, int64_t B,
-                                int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q, float sm_scale, int causal, int dtype, void* stream) {
+                                int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q, float sm_scale, int causal, int dtype, void* workspace,
+                                int64_t workspace_bytes, void* stream) {
   clear_error();
   FP8K_REQUIRE(is_half_type(dtype), "mla prefill: Half or BFloat16 operands expected");
   FP8K_REQUIRE(B >= 0 && H > 0 && B < (1 << 24) && H <= (1 << 16) && Tq >= 0 && Tk >= 0 && Tq < (1ll << 31) - 1024 && Tk < (1ll << 31) - 1024 && max_seqlen_q >= 0,
@@ -407,10 +422,21 @@ extern "C" int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_str
   p.q_t = q_stride_t; p.q_h = q_stride_h; p.kn_t = kn_stride_t; p.kn_h = kn_stride_h; p.kp_t = kp_stride_t; p.v_t = v_stride_t; p.v_h = v_stride_h;
   p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.out = out; p.lse = lse;
   p.B = (int)B; p.H = (int)H; p.Tq = (int)Tq; p.Tk = (int)Tk; p.blocks = (int)blocks; p.causal = causal != 0; p.sm_scale = sm_scale;
-  const dim3 grid((unsigned)(units * blocks));
+  p.splits = prefill_splits(B, H, Tq, Tk, max_seqlen_q);
+  const int64_t need = fp8k_mla_prefill_workspace_bytes(B, H, Tq, Tk, max_seqlen_q);
+  if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
+    return fail(FP8K_ERR_WORKSPACE, "mla prefill: workspace of %lld bytes needed, 256-byte aligned", (long long)need);
+  p.part = (float*)workspace;
+  p.part_lse = (float*)((uint8_t*)workspace + up_to(p.splits * Tq * H * kPreValue * 4, 256));
+  const dim3 grid((unsigned)(units * blocks), (unsigned)p.splits), join_grid((unsigned)(units * blocks), 16);
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == FP8K_BF16) mla_prefill_kernel<FP8K_BF16><<<grid, 256, 0, st>>>(p);
   else mla_prefill_kernel<FP8K_F16><<<grid, 256, 0, st>>>(p);
+  if (p.splits > 1) {
+    if (const int rc = check_launch("mla prefill")) return rc;
+    if (dtype == FP8K_BF16) mla_prefill_join_kernel<FP8K_BF16><<<join_grid, 256, 0, st>>>(p);
+    else mla_prefill_join_kernel<FP8K_F16><<<join_grid, 256, 0, st>>>(p);
+  }
   return check_launch("mla prefill");
 }
 

@@ -26,7 +26,9 @@ struct MlaPrefillArgs {
   const int32_t *cu_q, *cu_k;
   void* out;   // [Tq, H, 128]
   float* lse;  // [Tq, H] or null
+  float *part, *part_lse;  // [splits, Tq, H, 128], [splits, Tq, H]
   int B, H, Tq, Tk, blocks;  // blocks: of 128 queries that a sequence has at most
+  int splits;              // of a block's keys, each a workgroup's
   int causal;
   float sm_scale;
 };
@@ -36,6 +38,27 @@ constexpr int kPreRows = 128, kPreKeys = 64, kPreNope = 128, kPreValue = 128;
 // position of the 16-byte chunks of a value's row of 256 bytes: c ^ swizzle(r), as the transposed reads of 16 rows x 32 bytes spread best
 __device__ __forceinline__ int mla_value_swizzle(int r) { return ((r & 1) ? 12 : 0) ^ ((r & 2) ? 10 : 0) ^ ((r & 4) ? 6 : 0); }
 
+// A workgroup's 128 queries.  The blocks of a sequence's head follow each other on one XCD (workgroup i runs on XCD i % 8): they read the same
+// keys.  Of a causal head the last queries, which have most keys, come first, in every other head the first ones: the workgroups that start
+// together, two to a CU, are long and short ones.
+struct MlaBlock {
+  int b, h, q_begin, lq, q0, rows;
+};
+__device__ __forceinline__ MlaBlock mla_block(const MlaPrefillArgs& p) {
+  MlaBlock x;
+  const int line = (int)blockIdx.x / 8, group = line / p.blocks, place = line - group * p.blocks, unit = group * 8 + (int)(blockIdx.x % 8);
+  x.rows = 0;
+  if (unit >= p.B * p.H) return x;
+  x.b = unit / p.H;
+  x.h = unit - x.b * p.H;
+  x.q_begin = min(max(p.cu_q[x.b], 0), p.Tq);
+  x.lq = min(max(p.cu_q[x.b + 1], x.q_begin), p.Tq) - x.q_begin;
+  const int groups = (int)gridDim.x / 8 / p.blocks;
+  x.q0 = ((groups - group) & 1 ? p.blocks - 1 - place : place) * kPreRows;
+  x.rows = min(kPreRows, x.lq - x.q0);
+  return x;
+}
+
 template <int DT>
 __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArgs p) {
   constexpr int kKey = kPreKeys * 384, kVal = kPreKeys * 256, kPe = kPreKeys * 256;  // bytes of a stage, and where k_pe begins in it
@@ -43,19 +66,16 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, half = lane >> 5;
-  // the blocks of a sequence's head follow each other on one XCD (workgroup i runs on XCD i % 8): they read the same keys; the last
-  // queries, which have most keys, first
-  const int unit = (int)(blockIdx.x / 8 / p.blocks) * 8 + (int)(blockIdx.x % 8);
-  if (unit >= p.B * p.H) return;
-  const int b = unit / p.H, h = unit - b * p.H, block = p.blocks - 1 - (int)(blockIdx.x / 8) % p.blocks;
-  const int q_begin = min(max(p.cu_q[b], 0), p.Tq), q_end = min(max(p.cu_q[b + 1], q_begin), p.Tq), lq = q_end - q_begin;
-  const int k_begin = min(max(p.cu_k[b], 0), p.Tk), k_end = min(max(p.cu_k[b + 1], k_begin), p.Tk), lk = k_end - k_begin;
-  const int q0 = block * kPreRows;
-  if (q0 >= lq) return;
+  const MlaBlock at = mla_block(p);
+  if (at.rows <= 0) return;
+  const int h = at.h, q_begin = at.q_begin, q0 = at.q0, lq = at.lq;
+  const int k_begin = min(max(p.cu_k[at.b], 0), p.Tk), k_end = min(max(p.cu_k[at.b + 1], k_begin), p.Tk), lk = k_end - k_begin;
   const int shift_k = lk - lq;  // query i is the key of place i + shift_k
-  const int last_row = min(q0 + kPreRows, lq) - 1;
-  const int keys = p.causal ? min(max(last_row + shift_k + 1, 0), lk) : lk;  // that any row of the workgroup sees
-  const int tiles = (keys + kPreKeys - 1) / kPreKeys;
+  const int last_row = q0 + at.rows - 1;
+  const int keys = p.causal ? min(max(last_row + shift_k + 1, 0), lk) : lk;  // that any row of the block sees
+  // this workgroup's share of their tiles
+  const int all_tiles = (keys + kPreKeys - 1) / kPreKeys, split = blockIdx.y;
+  const int first = (int)((int64_t)all_tiles * split / p.splits), tiles = (int)((int64_t)all_tiles * (split + 1) / p.splits);
 
   const int row0 = q0 + w * 32, qi = min(row0 + l31, lq - 1);
   const int lim = p.causal ? min(qi + shift_k + 1, lk) : lk;  // keys that this lane's row sees
@@ -190,7 +210,7 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
     argument(0);
     argument(1);
     exponential(0);
-    if ((t + 1) * kPreKeys < wave_keys) {
+    if (t + 1 < tiles && (t + 1) * kPreKeys < wave_keys) {
       constexpr int kAhead = 5;
       v4i ring[kAhead];
       const int n_at = anew(n_off + ((t + 1) & 1) * kKey), p_at = anew(p_off + ((t + 1) & 1) * kKey);
@@ -241,19 +261,20 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
   };
 
   v16f s0[2], s1[2];
-  if (tiles > 0) {
-    fetch_keys(0);
+  if (first < tiles) {
+    fetch_keys(first);
     wait_loads<0>();
     lds_only_barrier();
-    if (tiles > 1) fetch_keys(1);
-    fetch_values(0);
+    if (first + 1 < tiles) fetch_keys(first + 1);
+    fetch_values(first);
     first_scores(s0);
-    if (wave_keys > 0) {
+    if (first * kPreKeys < wave_keys) {
+      const int n_at = n_off + (first & 1) * kKey, p_at = p_off + (first & 1) * kKey;
 #pragma unroll
-      for (int i = 0; i < 24; ++i) s0[i & 1] = mfma32<DT>(key_operand(n_off, p_off, i), q[i >> 1], s0[i & 1]);
+      for (int i = 0; i < 24; ++i) s0[i & 1] = mfma32<DT>(key_operand(n_at, p_at, i), q[i >> 1], s0[i & 1]);
     }
   }
-  for (int t = 0; t < tiles; t += 2) {
+  for (int t = first; t < tiles; t += 2) {
     step(t, s0, s1);
     if (t + 1 < tiles) step(t + 1, s1, s0);
   }
@@ -262,13 +283,48 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
   const float f = l == 0.0f ? 0.0f : 1.0f / l;
   if (row0 + l31 < lq) {
     const int64_t row = (int64_t)(q_begin + row0 + l31) * p.H + h;
-    u16* const to = (u16*)p.out + row * kPreValue + 4 * half;
+    const float lse2 = l == 0.0f ? -INFINITY : __builtin_amdgcn_logf(l) + shift_of(m);
+    if (p.splits == 1) {
+      u16* const to = (u16*)p.out + row * kPreValue + 4 * half;
 #pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
+      for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        *(v2i*)(to + dt * 32 + k * 8) = v2i{(int)pack2<DT>(o[dt][4 * k] * f, o[dt][4 * k + 1] * f), (int)pack2<DT>(o[dt][4 * k + 2] * f, o[dt][4 * k + 3] * f)};
-    if (half == 0 && p.lse) p.lse[row] = l == 0.0f ? -INFINITY : (__builtin_amdgcn_logf(l) + shift_of(m)) * kLn2;
+        for (int k = 0; k < 4; ++k)
+          *(v2i*)(to + dt * 32 + k * 8) = v2i{(int)pack2<DT>(o[dt][4 * k] * f, o[dt][4 * k + 1] * f), (int)pack2<DT>(o[dt][4 * k + 2] * f, o[dt][4 * k + 3] * f)};
+      if (half == 0 && p.lse) p.lse[row] = lse2 * kLn2;
+    } else {
+      const int64_t place = (int64_t)split * p.Tq * p.H + row;
+      float* const to = p.part + place * kPreValue + 4 * half;
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) *(v4f*)(to + dt * 32 + k * 8) = v4f{o[dt][4 * k] * f, o[dt][4 * k + 1] * f, o[dt][4 * k + 2] * f, o[dt][4 * k + 3] * f};
+      if (half == 0) p.part_lse[place] = lse2;
+    }
+  }
+}
+
+// Adds up the splits of a block's rows, in the order of their keys: 32 lanes of four columns to a row.
+template <int DT>
+__global__ __launch_bounds__(256) void mla_prefill_join_kernel(const MlaPrefillArgs p) {
+  const MlaBlock at = mla_block(p);
+  const int col = 4 * (int)(threadIdx.x & 31);
+  for (int r = (int)blockIdx.y * 8 + (int)(threadIdx.x >> 5); r < at.rows; r += (int)gridDim.y * 8) {
+    const int64_t row = (int64_t)(at.q_begin + at.q0 + r) * p.H + at.h, step = (int64_t)p.Tq * p.H;
+    float top = -INFINITY;
+    for (int i = 0; i < p.splits; ++i) top = fmaxf(top, p.part_lse[i * step + row]);
+    const float shift = shift_of(top);
+    float sum = 0.0f;
+    v4f x = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int i = 0; i < p.splits; ++i) {
+      const float weight = __builtin_amdgcn_exp2f(p.part_lse[i * step + row] - shift);
+      sum += weight;
+      x += weight * *(const v4f*)(p.part + (i * step + row) * kPreValue + col);
+    }
+    x *= sum == 0.0f ? 0.0f : 1.0f / sum;
+    *(v2i*)((u16*)p.out + row * kPreValue + col) = v2i{(int)pack2<DT>(x[0], x[1]), (int)pack2<DT>(x[2], x[3])};
+    if (col == 0 && p.lse) p.lse[row] = sum == 0.0f ? -INFINITY : (__builtin_amdgcn_logf(sum) + shift) * kLn2;
   }
 }
 

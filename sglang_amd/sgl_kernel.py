@@ -1312,11 +1312,13 @@ def mla_prefill_attention(q: torch.Tensor, k_nope: torch.Tensor, k_pe: torch.Ten
         raise RuntimeError("sm_scale must be positive and finite")
     if B == 0 or Tq == 0:
         return
+    need = lib.fp8k_mla_prefill_workspace_bytes(B, H, Tq, Tk, int(max_seqlen_q))
     with torch.cuda.device(q.device):
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
         check(lib.fp8k_mla_prefill(
             q.data_ptr(), q.stride(0), q.stride(1), k_nope.data_ptr(), k_nope.stride(0), k_nope.stride(1), k_pe.data_ptr(), k_pe.stride(0),
             v.data_ptr(), v.stride(0), v.stride(1), cu_seqlens_q.data_ptr(), cu_seqlens_k.data_ptr(), out.data_ptr(), _ptr(lse), B, H, Tq, Tk,
-            int(max_seqlen_q), float(sm_scale), 1 if causal else 0, dtype_code(q.dtype), stream_ptr(q.device)))
+            int(max_seqlen_q), float(sm_scale), 1 if causal else 0, dtype_code(q.dtype), _ptr(ws), need, stream_ptr(q.device)))
 
 
 def merge_attention_states(out_a: torch.Tensor, lse_a: torch.Tensor, out_b: torch.Tensor, lse_b: torch.Tensor, out: torch.Tensor,

@@ -95,9 +95,9 @@ def test_c_refusals_of_the_attentions():
     _refused(decode(ws=p + 128), "workspace")
     assert lib.fp8k_mla_decode_workspace_bytes(0, 1, 16, 64) == 0
 
-    def prefill(q=p, k=p, strides=(192, 192, 256, 256, 64, 256, 256), B=1, H=1, Tq=4, Tk=4, most=4, scale=0.1, dtype=_lib.BF16):
+    def prefill(q=p, k=p, strides=(192, 192, 256, 256, 64, 256, 256), B=1, H=1, Tq=4, Tk=4, most=4, scale=0.1, dtype=_lib.BF16, ws=None):
         s = strides
-        return lib.fp8k_mla_prefill(q, s[0], s[1], k, s[2], s[3], p, s[4], p, s[5], s[6], p, p, p, None, B, H, Tq, Tk, most, scale, 1, dtype, None)
+        return lib.fp8k_mla_prefill(q, s[0], s[1], k, s[2], s[3], p, s[4], p, s[5], s[6], p, p, p, None, B, H, Tq, Tk, most, scale, 1, dtype, ws, 1 << 20, None)
 
     assert prefill(B=0) == 0 and prefill(Tq=0) == 0 and prefill(most=0) == 0
     _refused(prefill(dtype=_lib.F32), "Half or BFloat16")
@@ -107,6 +107,10 @@ def test_c_refusals_of_the_attentions():
     _refused(prefill(strides=(192, 192, 256, -256, 64, 256, 256)), "negative")
     _refused(prefill(scale=0.0), "positive")
     _refused(prefill(most=-1), "sizes")
+    _refused(prefill(strides=(192, 192, 1 << 25, 256, 64, 256, 256)), "further apart")
+    _refused(prefill(Tk=1 << 16), "workspace")
+    _refused(prefill(Tk=1 << 16, ws=p + 8), "workspace")
+    assert lib.fp8k_mla_prefill_workspace_bytes(1, 1, 4, 64, 4) == 0 and lib.fp8k_mla_prefill_workspace_bytes(1, 1, 4, 1 << 16, 4) > 0
     _refused(prefill(B=1 << 23, H=1 << 16, Tq=1 << 30, most=1 << 30), "blocks")
 
     def merge(a=p, rows=4, D=128, dtype=_lib.BF16):
