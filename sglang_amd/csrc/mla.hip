@@ -23,27 +23,30 @@ struct MlaWriteArgs {
   float eps;
 };
 
-// 16 numbers of a position part, eight pairs, rotated: pairs of neighbours (x the 16 numbers from 16 part on), or (neox) of numbers that lie
-// 32 apart (x the eight from 8 part on, then the eight from 32 + 8 part on).  table: 32 cosines, 32 sines.
-__device__ __forceinline__ void rotate16(float* x, const float* table, int part, bool neox) {
+// The cosines and sines of eight pairs: those from 8 part on of a row's 32 and 32.
+struct Angles {
   v4f co[2], si[2];
-  co[0] = *(const v4f*)(table + 8 * part);
-  co[1] = *(const v4f*)(table + 8 * part + 4);
-  si[0] = *(const v4f*)(table + 32 + 8 * part);
-  si[1] = *(const v4f*)(table + 32 + 8 * part + 4);
+};
+__device__ __forceinline__ Angles angles_of(const float* row, int part) {
+  const v4f* const at = (const v4f*)row + 2 * part;
+  return Angles{{at[0], at[1]}, {at[8], at[9]}};
+}
+// 16 numbers of a position part, eight pairs, rotated: pairs of neighbours (x the 16 numbers from 16 part on), or (neox) of numbers that lie
+// 32 apart (x the eight from 8 part on, then the eight from 32 + 8 part on).
+__device__ __forceinline__ void rotate16(float* x, const Angles& a, bool neox) {
   if (neox) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float cs = co[i >> 2][i & 3], sn = si[i >> 2][i & 3], a = x[i], b = x[8 + i];
-      x[i] = a * cs - b * sn;
-      x[8 + i] = b * cs + a * sn;
+      const float cs = a.co[i >> 2][i & 3], sn = a.si[i >> 2][i & 3], u = x[i], v = x[8 + i];
+      x[i] = u * cs - v * sn;
+      x[8 + i] = v * cs + u * sn;
     }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float cs = co[i >> 2][i & 3], sn = si[i >> 2][i & 3], a = x[2 * i], b = x[2 * i + 1];
-      x[2 * i] = a * cs - b * sn;
-      x[2 * i + 1] = b * cs + a * sn;
+      const float cs = a.co[i >> 2][i & 3], sn = a.si[i >> 2][i & 3], u = x[2 * i], v = x[2 * i + 1];
+      x[2 * i] = u * cs - v * sn;
+      x[2 * i + 1] = v * cs + u * sn;
     }
   }
 }
@@ -62,15 +65,29 @@ template <int DT>
 __device__ __forceinline__ void store8(u16* p, const float* x) {
   *(v4i*)p = v4i{(int)pack2<DT>(x[0], x[1]), (int)pack2<DT>(x[2], x[3]), (int)pack2<DT>(x[4], x[5]), (int)pack2<DT>(x[6], x[7])};
 }
-// x / scale to e4m3: nearest, ties to even, at most 448; NaN stays NaN
-__device__ __forceinline__ float to_fp8_range(float x, float scale) {
-  const float v = x / scale;
+// x / scale to e4m3: nearest, ties to even, at most 448; NaN stays NaN.  The quotient of a scale whose reciprocal is an ordinary number is the product
+// with that and one correction by its remainder, the division's own result but for the last place at times: a division is ten instructions, and
+// there are 576 to a row.
+struct Fp8Scale {
+  float scale, inverse;
+  bool ordinary;
+};
+__device__ __forceinline__ Fp8Scale fp8_scale(const float* p) {
+  Fp8Scale s{p ? *p : 1.0f, 0.0f, false};
+  s.inverse = 1.0f / s.scale;
+  s.ordinary = fabsf(s.inverse) >= 0x1p-100f && fabsf(s.inverse) <= 0x1p100f;
+  return s;
+}
+__device__ __forceinline__ float to_fp8_range(float x, const Fp8Scale& s) {
+  float v = x * s.inverse;
+  if (s.ordinary) v = fabsf(v) <= kFp8Max ? fmaf(fmaf(-v, s.scale, x), s.inverse, v) : v;
+  else v = x / s.scale;
   return v != v ? v : fminf(fmaxf(v, -kFp8Max), kFp8Max);
 }
-__device__ __forceinline__ void store8_fp8(uint8_t* p, const float* x, float scale) {
+__device__ __forceinline__ void store8_fp8(uint8_t* p, const float* x, const Fp8Scale& s) {
   float v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = to_fp8_range(x[i], scale);
+  for (int i = 0; i < 8; ++i) v[i] = to_fp8_range(x[i], s);
   *(v2i*)p = v2i{(int)cvt4_fp8(v[0], v[1], v[2], v[3]), (int)cvt4_fp8(v[4], v[5], v[6], v[7])};
 }
 
@@ -94,47 +111,67 @@ __global__ __launch_bounds__(256) void mla_write_kernel(const MlaWriteArgs p) {
     float x[16];
     load8<DT>(from + first, x);
     load8<DT>(from + second, x + 8);
-    rotate16(x, table_of(t), part, p.neox);
+    rotate16(x, angles_of(table_of(t), part), p.neox);
     store8<DT>(to + first, x);
     store8<DT>(to + second, x + 8);
     return;
   }
   const int t = (int)blockIdx.x * 4 + (tid >> 6);
   if (t >= p.T) return;
-  const int64_t slot = p.slots64 ? ((const int64_t*)p.slots)[t] : ((const int32_t*)p.slots)[t];
-  if (slot < 0 || slot >= p.num_slots) return;
+  // Everything is asked for before anything is looked at: a row is short, and what it costs is the loads that wait for others.
   const u16* const from = p.latent + t * p.ld_latent;
-  float x[8];
+  const int64_t slot = p.slots64 ? ((const int64_t*)p.slots)[t] : ((const int32_t*)p.slots)[t];
+  const Fp8Scale scale = fp8_scale(FP8 ? p.scale : nullptr);
+  float x[8], weight[8];
   load8<DT>(from + 8 * lane, x);
+  // lanes 0 .. 31: a pair of the position part each, neighbours or numbers 32 apart
+  const int pair = lane & 31, first = p.neox ? pair : 2 * pair, second = p.neox ? 32 + pair : 2 * pair + 1;
+  float u = 0.0f, v = 0.0f, cs = 1.0f, sn = 0.0f;
+  if (lane < 32) {
+    u = unpack2<DT>(from[kLatent + first])[0];
+    v = unpack2<DT>(from[kLatent + second])[0];
+    if (p.cos_sin) {
+      const float* const row = table_of(t);
+      cs = row[pair];
+      sn = row[32 + pair];
+    }
+  }
   if (p.norm_weight) {
+    if (p.weight_f32) {
+      *(v4f*)weight = *(const v4f*)((const float*)p.norm_weight + 8 * lane);
+      *(v4f*)(weight + 4) = *(const v4f*)((const float*)p.norm_weight + 8 * lane + 4);
+    } else load8<DT>((const u16*)p.norm_weight + 8 * lane, weight);
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += x[i] * x[i];
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
     const float f = 1.0f / sqrtf(sum * (1.0f / kLatent) + p.eps);
-    float weight[8];
-    if (p.weight_f32) {
-      *(v4f*)weight = *(const v4f*)((const float*)p.norm_weight + 8 * lane);
-      *(v4f*)(weight + 4) = *(const v4f*)((const float*)p.norm_weight + 8 * lane + 4);
-    } else load8<DT>((const u16*)p.norm_weight + 8 * lane, weight);
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = x[i] * f * weight[i];
   }
-  const float scale = FP8 && p.scale ? *p.scale : 1.0f;
-  auto store = [&](int at, const float* v) {
-    if (FP8) store8_fp8((uint8_t*)p.cache + slot * kLatentRow + at, v, scale);
-    else store8<DT>((u16*)p.cache + slot * kLatentRow + at, v);
-  };
-  store(8 * lane, x);
-  if (lane < 4) {
-    const int first = p.neox ? 8 * lane : 16 * lane, second = p.neox ? 32 + 8 * lane : 16 * lane + 8;
-    float y[16];
-    load8<DT>(from + kLatent + first, y);
-    load8<DT>(from + kLatent + second, y + 8);
-    if (p.cos_sin) rotate16(y, table_of(t), lane, p.neox);
-    store(kLatent + first, y);
-    store(kLatent + second, y + 8);
+  if (slot < 0 || slot >= p.num_slots) return;
+  if (p.cos_sin) {
+    const float a = u * cs - v * sn;
+    v = v * cs + u * sn;
+    u = a;
+  }
+  if (FP8) {
+    uint8_t* const to = (uint8_t*)p.cache + slot * kLatentRow;
+    store8_fp8(to + 8 * lane, x, scale);
+    const uint32_t w = cvt_pk_fp8_lo(to_fp8_range(u, scale), to_fp8_range(v, scale), 0);
+    if (lane < 32) {
+      to[kLatent + first] = (uint8_t)w;
+      to[kLatent + second] = (uint8_t)(w >> 8);
+    }
+  } else {
+    u16* const to = (u16*)p.cache + slot * kLatentRow;
+    store8<DT>(to + 8 * lane, x);
+    const uint32_t w = pack2<DT>(u, v);
+    if (lane < 32) {
+      to[kLatent + first] = (u16)w;
+      to[kLatent + second] = (u16)(w >> 16);
+    }
   }
 }
 
@@ -262,7 +299,7 @@ extern "C" int fp8k_mla_write_cache(const void* latent, int64_t ld_latent, void*
   FP8K_REQUIRE(is_half_type(dtype), "mla write: Half or BFloat16 rows expected");
   FP8K_REQUIRE(T >= 0 && T < (1ll << 30) && num_slots >= 0 && H >= 0 && H <= (1 << 16), "mla write: bad sizes");
   if (T == 0) return FP8K_OK;
-  FP8K_REQUIRE(latent && cache && slots, "mla write: null pointer");
+  FP8K_REQUIRE(latent && (cache || num_slots == 0) && slots, "mla write: null pointer");
   FP8K_REQUIRE(aligned(latent, 16) && aligned(cache, 16) && ld_latent % 8 == 0 && ld_latent >= kLatentRow, "mla write: rows must be 16-byte aligned");
   FP8K_REQUIRE(aligned(slots, slots_are_64bit ? 8 : 4), "mla write: misaligned slots");
   FP8K_REQUIRE(!norm_weight || ((norm_weight_dtype == dtype || norm_weight_dtype == FP8K_F32) && aligned(norm_weight, 16)),
@@ -348,8 +385,8 @@ extern "C" int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t 
   FP8K_REQUIRE(qn_stride_b >= 0 && qn_stride_n >= 0 && qn_stride_h >= 0 && qp_stride_b >= 0 && qp_stride_n >= 0 && qp_stride_h >= 0,
                "mla decode: negative stride");
   const int64_t max_len = table_width * page_size;
-  FP8K_REQUIRE(table_width < (1ll << 31) && max_len < (1ll << 31) - kMlaTile && B * (max_len / kMlaTile + 1) < (1ll << 31),
-               "mla decode: the page table holds more tokens than 32 bits count");
+  FP8K_REQUIRE(table_width < (1ll << 31) && max_len <= (1ll << 30) && B * (max_len / kMlaTile + 1) < (1ll << 30),
+               "mla decode: the page table holds more than 2^30 tokens to a request, or 2^36 in all");
   const int64_t need = fp8k_mla_decode_workspace_bytes(B, n, H, max_len);
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
     return fail(FP8K_ERR_WORKSPACE, "mla decode: workspace of %lld bytes needed, 256-byte aligned", (long long)need);

@@ -66,9 +66,10 @@ template <int OFFSET = 0>
 __device__ __forceinline__ void load16_to_lds(const void* p, uint32_t to) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2 nt" ::"v"(p), "s"(to - OFFSET), "n"(OFFSET) : "memory");
 }
-// the same from base + every lane's own offset, cached; base is the wave's
+// the same from base + every lane's own offset, cached; base is the wave's.  (Five wait states in front: a scalar register that a vector instruction
+// has just written - the compiler's own spills - is not ready for a vector load before.)
 __device__ __forceinline__ void load16_to_lds(const void* base, uint32_t offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to) : "memory");
 }
 // 4 bytes likewise, to `to` + 4 * lane
 __device__ __forceinline__ void load4_to_lds(const void* p, uint32_t to) {

@@ -8,8 +8,9 @@
 // holds is the operand of O^T = V^T . P^T as it lies, the order of the keys inside a product being free as long as V^T, read from LDS by
 // transposed reads, has the same.
 //
-// The products of tile t + 1 run beside the exponentials of tile t, one instruction behind the other: a product keeps the matrix core busy for 32 clocks,
-// in which the wave issues the exponentials of two scores.
+// The products of tile t + 1 with the queries run beside the exponentials of tile t, those of tile t with the values beside the exponentials' sum and the
+// maximum of tile t + 1, one instruction behind the other: a product keeps the matrix core busy for 32 clocks, in which the wave issues the exponentials
+// of two scores.
 //
 // LDS: two stages of k_nope [64, 128] and k_pe [64, 64], and two of v [64, 128], one tile behind, filled by global_load_lds; the position part is
 // read where it lies, once for each head, and never copied beside the keys.  16-byte chunks of a row are permuted by the row so that the
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
   for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
+  float m = -INFINITY, l = 0.0f, l_odd = 0.0f;  // of the odd scores: two sums that do not wait for each other
 
   // operand i of a tile's scores: 24 products, the two 32-key tiles by turns
   auto key_operand = [&](int n_at, int p_at, int i) {
@@ -158,13 +159,22 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
       for (int i = 0; i < 16; ++i) s[nt][i] = 0.0f;
   };
 
-  // One tile: the weights of the scores s of tile t and their product with v, and, if there are any, the scores `next` of tile t + 1.
-  auto step = [&](int t, v16f* s, v16f* next) {
+  auto score = [](v16f* s, int i) -> float { return s[i >> 4][i & 15]; };
+  auto top_of = [&](v16f* s) {
+    float top = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) top = fmaxf(top, score(s, i));
+    return top;
+  };
+
+  // One tile: the weights of the scores s of tile t, whose largest is top, and their product with v; and, if there are any, the scores `next` of tile
+  // t + 1, whose largest is returned.
+  auto step = [&](int t, v16f* s, float top, v16f* next) -> float {
     wait_loads<0>();
     lds_only_barrier();  // keys of t + 1 and values of t have arrived, and nobody reads those of t and t - 1 any more
     if (t + 2 < tiles) fetch_keys(t + 2);
     if (t + 1 < tiles) fetch_values(t + 1);
-    if (t * kPreKeys >= wave_keys) return;  // nothing that this wave's rows see
+    if (t * kPreKeys >= wave_keys) return top;  // nothing that this wave's rows see
 
     // a lane's scores are those of query row l31, keys 32 nt + 8 (i / 4) + 4 half + i % 4
     if (__builtin_expect((t + 1) * kPreKeys > wave_free, 0)) {
@@ -174,12 +184,8 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
 #pragma unroll
         for (int i = 0; i < 16; ++i)
           if (key0 + nt * 32 + 8 * (i >> 2) + (i & 3) >= lim) s[nt][i] = -INFINITY;
+      top = top_of(s);
     }
-    float top = -INFINITY;
-#pragma unroll
-    for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[nt][i]);
     // c > 0.  The row's maximum, over two lanes, is asked for only when one of them has passed the old one by far.
     if (__builtin_expect(__any(top * c > m + kMaxSlack), 0)) {
       top = max_across32(top) * c;
@@ -187,13 +193,13 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
       const float alpha = raised != m ? __builtin_amdgcn_exp2f(m - raised) : 1.0f;
       m = raised;
       l *= alpha;
+      l_odd *= alpha;
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) o[dt] *= alpha;
     }
     const float shift = shift_of(m);
     uint32_t pk[16];
-    // scores 2 j and 2 j + 1: arguments, exponentials, and one pair later sum and rounding to the 16-bit type, as the matrix core takes them; the sum is of
-    // the unrounded ones
+    // scores 2 j and 2 j + 1: arguments, exponentials, and their rounding to the 16-bit type, as the matrix core takes them; the sum is of the unrounded ones
     auto argument = [&](int j) {
       s[j >> 3][(2 * j) & 15] = fmaf(s[j >> 3][(2 * j) & 15], c, -shift);
       s[j >> 3][(2 * j + 1) & 15] = fmaf(s[j >> 3][(2 * j + 1) & 15], c, -shift);
@@ -202,15 +208,12 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
       s[j >> 3][(2 * j) & 15] = __builtin_amdgcn_exp2f(s[j >> 3][(2 * j) & 15]);
       s[j >> 3][(2 * j + 1) & 15] = __builtin_amdgcn_exp2f(s[j >> 3][(2 * j + 1) & 15]);
     };
-    auto finish = [&](int j) {
-      l += s[j >> 3][(2 * j) & 15];
-      l += s[j >> 3][(2 * j + 1) & 15];
-      pk[j] = pack2<DT>(s[j >> 3][(2 * j) & 15], s[j >> 3][(2 * j + 1) & 15]);
-    };
+    auto round = [&](int j) { pk[j] = pack2<DT>(score(s, 2 * j), score(s, 2 * j + 1)); };
     argument(0);
     argument(1);
     exponential(0);
-    if (t + 1 < tiles && (t + 1) * kPreKeys < wave_keys) {
+    const bool more = t + 1 < tiles && (t + 1) * kPreKeys < wave_keys;
+    if (more) {
       constexpr int kAhead = 5;
       v4i ring[kAhead];
       const int n_at = anew(n_off + ((t + 1) & 1) * kKey), p_at = anew(p_off + ((t + 1) & 1) * kKey);
@@ -225,7 +228,7 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
           const int j = i / 3 * 2 + i % 3;
           if (j + 2 < 16) argument(j + 2);
           if (j + 1 < 16) exponential(j + 1);
-          finish(j);
+          round(j);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -234,10 +237,11 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
       for (int j = 0; j < 16; ++j) {
         if (j + 2 < 16) argument(j + 2);
         if (j + 1 < 16) exponential(j + 1);
-        finish(j);
+        round(j);
       }
     }
 
+    top = -INFINITY;
     {
       constexpr int kAhead = 5;
       v2i ring[kAhead][2];
@@ -255,31 +259,38 @@ __global__ __launch_bounds__(256, 2) void mla_prefill_kernel(const MlaPrefillArg
         const int k = i >> 2;
         o[i & 3] = mfma32<DT>(v4i{a[0][0], a[0][1], a[1][0], a[1][1]}, v4i{(int)pk[4 * k], (int)pk[4 * k + 1], (int)pk[4 * k + 2], (int)pk[4 * k + 3]}, o[i & 3]);
         if (i + kAhead < 16) read(i + kAhead, ring[i % kAhead]);
+        l += score(s, 2 * i);
+        l_odd += score(s, 2 * i + 1);
+        // (stale, and not used, after the last tile)
+        top = fmaxf(fmaxf(top, score(next, 2 * i)), score(next, 2 * i + 1));
         __builtin_amdgcn_sched_barrier(0);
       }
     }
+    return top;
   };
 
   v16f s0[2], s1[2];
+  first_scores(s0);
+  first_scores(s1);
   if (first < tiles) {
     fetch_keys(first);
     wait_loads<0>();
     lds_only_barrier();
     if (first + 1 < tiles) fetch_keys(first + 1);
     fetch_values(first);
-    first_scores(s0);
     if (first * kPreKeys < wave_keys) {
       const int n_at = n_off + (first & 1) * kKey, p_at = p_off + (first & 1) * kKey;
 #pragma unroll
       for (int i = 0; i < 24; ++i) s0[i & 1] = mfma32<DT>(key_operand(n_at, p_at, i), q[i >> 1], s0[i & 1]);
     }
   }
+  float top = top_of(s0);
   for (int t = first; t < tiles; t += 2) {
-    step(t, s0, s1);
-    if (t + 1 < tiles) step(t + 1, s1, s0);
+    top = step(t, s0, top, s1);
+    if (t + 1 < tiles) top = step(t + 1, s1, top, s0);
   }
 
-  l = sum_across32(l);
+  l = sum_across32(l + l_odd);
   const float f = l == 0.0f ? 0.0f : 1.0f / l;
   if (row0 + l31 < lq) {
     const int64_t row = (int64_t)(q_begin + row0 + l31) * p.H + h;

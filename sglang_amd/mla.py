@@ -2,7 +2,7 @@
 
 A token's keys and values are one row of 576 numbers that all heads share: a latent of 512 and a part of 64 that carries the rotary
 position.  The cache holds those rows and nothing else, [pages, page_size, 576] in the operands' 16-bit type or in float8_e4m3fn with one
-scale (value = code * scale, a float32 tensor of one element; None: 1).  A request's pages are a row of an int32 page table.
+scale (value = code * scale, a float32 tensor of one positive element; None: 1).  A request's pages are a row of an int32 page table.
 
   a layer's new tokens      mla_write_cache: norm of the latent, rotation of the position part and of the queries', store
   decode (absorbed)         per_tensor_quant_mla_fp8 and bmm_fp8 fold the keys' up-projection into the queries, mla_decode_attention, then the
@@ -33,7 +33,8 @@ def mla_write_cache(latent: torch.Tensor, cache: torch.Tensor, slots: torch.Tens
                     q_pe: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None,
                     q_out: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Stores the rows of new tokens, latent [T, 576] float16 / bfloat16 (what the down-projection gives), at slots [T] (int32 or int64; slot
-    page * page_size + place) of the cache.  Slots are distinct; one that the cache does not have (-1: the padding of a batch) is skipped.
+    page * page_size + place) of the cache.  Slots are distinct (of rows that share one, each number may be any row's); one that the cache does not
+    have (-1: the padding of a batch) is skipped.
 
     norm_weight [512] (of the rows' type or float32): the latent becomes x / sqrt(mean(x^2) + eps) * norm_weight.
     cos_sin float32 [P, 64] (32 cosines, 32 sines of a position) and positions [T] (int32 or int64; held within 0 .. P - 1): the position
@@ -81,7 +82,7 @@ def mla_decode_attention(q_nope: torch.Tensor, q_pe: torch.Tensor, cache: torch.
     before it all but the last, and so on.  A query that sees nothing gets 0 and -inf.  The absorbed queries may be a transposed view.
 
     The exponentials are rounded to 16 bits for their product with the rows (their sum is not).  Lengths are held within the page table's width;
-    of each page what lies behind the last token is not used.  The cache is cut over the whole batch's tokens into equal runs, whose float32
+    of a page what lies behind the last token may hold anything, the request's own rows are finite.  The cache is cut over the whole batch's tokens into equal runs, whose float32
     partials are joined in the order of the tokens: results do not depend on timing, but on how the batch is cut."""
     if not torch.compiler.is_compiling():
         got = _host.mla_decode(q_nope, q_pe, cache, page_table, seq_lens, sm_scale, scale, return_lse, out)

@@ -89,7 +89,7 @@ def test_c_refusals_of_the_attentions():
     _refused(decode(n=513, H=128), "sizes")
     _refused(decode(pages=0), "page table")
     _refused(decode(width=0), "page table")
-    _refused(decode(width=1 << 20, page=1 << 12, ws_bytes=1 << 50), "32 bits")
+    _refused(decode(width=1 << 20, page=1 << 12, ws_bytes=1 << 50), "2^30")
     _refused(decode(ws=None), "workspace")
     _refused(decode(ws_bytes=16), "workspace")
     _refused(decode(ws=p + 128), "workspace")

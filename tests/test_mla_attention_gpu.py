@@ -45,11 +45,11 @@ def _queries(g, B, n, H, dtype):
     return q, torch.randn((B, n, H, 64), generator=g, device="cuda").to(dtype)
 
 
-def _check_decode(lens, n, H, page, dtype, fp8, seed=0, sharp=1.0):
+def _check_decode(lens, n, H, page, dtype, fp8, seed=0, sharp=1.0, width=None):
     from sglang_amd import mla
 
     g = _gen(seed)
-    cache, table, pt, scale = _filled(g, lens, page, dtype, fp8, sharp=sharp)
+    cache, table, pt, scale = _filled(g, lens, page, dtype, fp8, sharp=sharp, width=width)
     q, qp = _queries(g, len(lens), n, H, dtype)
     sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
     out, lse = mla.mla_decode_attention(q, qp, cache, pt, sl, SCALE, scale=scale, return_lse=True)
@@ -83,6 +83,31 @@ def test_decode_over_several_runs(dev, lens, n, H, fp8):
 def test_decode_of_every_block_of_rows(dev, rows, H):
     """A batch with tiles enough for every CU takes the largest block of rows that its heads fill; its runs hold parts of several requests."""
     _check_decode([333 + 7 * i for i in range(130)], 1, H, 64, BF16 if H != 64 else F16, H == 32, seed=H)
+
+
+@pytest.mark.parametrize("dtype,fp8", [(BF16, False), (F16, True), (BF16, True), (F16, False)])
+@pytest.mark.parametrize("H,width", [(128, 1), (128, 16), (128, 64), (128, 300), (64, 300), (32, 300), (70, 300), (257, 64)])
+def test_decode_of_every_cut(dev, H, width, dtype, fp8):
+    """The width of the page table bounds the lengths, and that decides how many rows a workgroup takes: from 16 to 128 of 128 heads, blocks that
+    the heads do not fill, more blocks than one.  Lengths are few, or none, or end a step before, at and behind the steps that run ahead."""
+    lens = [1, 31, 32, 33, 63, 64] if width == 1 else [0, 1, 64, 95, 96, 97, 128, 129, 160, 161, 192, 193, 257, 321, 400, 33]
+    _check_decode(lens, 1, H, 64, dtype, fp8, seed=H + width, width=width)
+
+
+@pytest.mark.parametrize("n,H,B,width", [(2, 8, 700, 4), (1, 16, 1500, 4), (3, 24, 600, 40), (1, 128, 520, 8)])
+def test_decode_of_more_requests_than_threads(dev, n, H, B, width):
+    """A thread of the prefix sum counts several requests, empty ones among them."""
+    _check_decode([(i * 37) % 250 if i % 5 else 0 for i in range(B)], n, H, 64, BF16, n == 2, seed=B, width=width)
+
+
+def test_decode_lengths_below_zero(dev):
+    from sglang_amd import mla
+
+    g = _gen(1)
+    cache, table, pt, _ = _filled(g, [70, 70], 64, BF16, False)
+    q, qp = _queries(g, 2, 1, 16, BF16)
+    out, lse = mla.mla_decode_attention(q, qp, cache, pt, torch.tensor([-3, -(1 << 31)], dtype=torch.int32, device="cuda"), SCALE, return_lse=True)
+    assert not out.any() and bool((lse == float("-inf")).all())
 
 
 @pytest.mark.parametrize("order", ["rising", "falling", "spike"])
@@ -230,6 +255,26 @@ def test_prefill_over_split_keys(dev, lq, lk, H, causal, dtype):
 def test_prefill_of_many_blocks(dev):
     """More workgroups than run at once: no splits, long and short blocks by turns."""
     _check_prefill([700, 130, 1500], [700, 400, 1500], 64, BF16, True)
+
+
+def test_prefill_of_far_keys(dev):
+    """Keys and values whose rows lie beyond 2^32 bytes, split and not."""
+    from sglang_amd import mla
+
+    g = _gen(13)
+    tk = (1 << 33) // (128 * 256 * 2) + 700
+    kv = torch.empty((tk, 128, 256), dtype=BF16, device="cuda")
+    pe = torch.randn((tk, 64), generator=g, device="cuda").to(BF16)
+    ends = [tk - 1500, tk - 700, tk]
+    for h in (0, 1):
+        kv[ends[0]:, h] = torch.randn((1500, 256), generator=g, device="cuda").to(BF16)
+    q = torch.randn((150, 2, 192), generator=g, device="cuda").to(BF16)
+    tq = torch.tensor([0, 30, 150], dtype=torch.int32, device="cuda")
+    tk_ = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    for most in (120, 1 << 15):
+        out = mla.mla_prefill_attention(q, kv[:, :2, :128], pe, kv[:, :2, 128:], tq, tk_, most, SCALE)
+        want, _, tol, _ = R.prefill(q, kv[:, :2, :128], pe, kv[:, :2, 128:], [0, 30, 150], ends, SCALE, True)
+        R.close(out, want, tol)
 
 
 def test_prefill_layouts(dev):
