@@ -9,6 +9,12 @@ namespace fp8k {
 constexpr int kLatent = 512, kRope = 64, kLatentRow = kLatent + kRope;  // numbers of a cached row
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
+// a number as an argument's type
+template <int N>
+struct Const {
+  static constexpr int value = N;
+};
+
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));

@@ -85,11 +85,6 @@ __device__ __forceinline__ int mla_scan(const MlaDecodeArgs& p, int per, int& be
 // does as well for the first alone, its rotation has half the rate there).
 __device__ __forceinline__ int mla_swizzle(int r) { return ((r & 2) ? 6 : 0) ^ ((r & 4) ? 5 : 0) ^ ((r & 8) ? 4 : 0); }
 
-template <int N>
-struct Const {
-  static constexpr int value = N;
-};
-
 template <int DT, bool FP8, int WM>
 __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const MlaDecodeArgs p) {
   constexpr int NW = WM == 1 ? 4 : 8, WT = NW / WM, R = 16 * WM;
