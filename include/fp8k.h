@@ -533,6 +533,8 @@ int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2, const void
  * type of the operands or (cache_is_fp8) in e4m3 with one device-resident scale (NULL: 1): value = code * scale.  It is [pages, page_size, 576],
  * contiguous; a page table int32 [B, width] (row stride table_stride) names a request's pages in the order of its tokens.  Entries that
  * are no page of the cache are read as the nearest one.  dtype: F16/BF16.  Strides in elements, multiples of 8; pointers 16-byte aligned.
+ * Limits beyond those named below: decode, pages of at most 2^20 tokens, page tables of at most 2^30 tokens to a request and 2^36 in all;
+ * prefill, rows of keys and of values less than 2^24 elements apart.
  *
  * fp8k_mla_write_cache: for every token t, latent[t] (row stride ld_latent) goes to row slots[t] (int32 or int64) of the num_slots rows of the
  * cache; a slot that is none of them (-1: a padded batch) is skipped.  Slots are distinct.  norm_weight (NULL: no norm; of dtype or F32): the latent
@@ -588,7 +590,7 @@ int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, cons
 
 /*
  * Two attentions over disjoint keys as one: out = (exp(lse_a) out_a + exp(lse_b) out_b) / (exp(lse_a) + exp(lse_b)), lse = log(exp(lse_a) + exp(lse_b)),
- * over rows x D numbers of dtype (F16/BF16/F32), D a multiple of 8, all contiguous; out may be out_a or out_b, lse likewise.  A part
+ * over rows x D numbers of dtype (F16/BF16/F32), D a multiple of 8, all contiguous; out may be out_a or out_b, lse is memory of its own.  A part
  * with an lse of -inf counts nothing, whatever its row holds; two of them give 0 and -inf.
  */
 int fp8k_merge_attention_states(const void* out_a, const float* lse_a, const void* out_b, const float* lse_b, void* out, float* lse,

@@ -487,6 +487,8 @@ extern "C" int fp8k_merge_attention_states(const void* out_a, const float* lse_a
   FP8K_REQUIRE(aligned(out_a, 16) && aligned(out_b, 16) && aligned(out, 16), "merge states: operands must be 16-byte aligned");
   const int64_t blocks = (rows * (D / 8) + 255) / 256;
   FP8K_REQUIRE(rows < (1ll << 40) && blocks < (1ll << 31), "merge states: too large");
+  // a row's numbers may be several workgroups', and each reads both logarithms
+  FP8K_REQUIRE(lse != lse_a && lse != lse_b, "merge states: lse must be memory of its own");
   const dim3 grid((unsigned)blocks);
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == FP8K_BF16) mla_merge_kernel<FP8K_BF16><<<grid, 256, 0, st>>>(out_a, lse_a, out_b, lse_b, out, lse, rows, (int)(D / 8));

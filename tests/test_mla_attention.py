@@ -249,3 +249,14 @@ def test_reference_is_attention():
     assert torch.allclose(R.rotate(x, table, False)[0], torch.view_as_real(pairs).reshape(3, 64))
     halves = torch.complex(x[:, :32], x[:, 32:]) * torch.polar(torch.ones_like(cs), cs)
     assert torch.allclose(R.rotate(x, table, True)[0], torch.cat((halves.real, halves.imag), 1))
+
+
+def test_the_joined_logarithm_is_memory_of_its_own():
+    """A row's numbers may be several workgroups', which all read both logarithms: none may be overwritten."""
+    from sglang_amd import _lib
+
+    keep, p = _address()
+    merge = _lib.lib.fp8k_merge_attention_states
+    _refused(merge(p, p + 1024, p, p + 2048, p, p + 1024, 2, 192, _lib.BF16, None), "memory of its own")
+    _refused(merge(p, p + 1024, p, p + 2048, p, p + 2048, 2, 192, _lib.BF16, None), "memory of its own")
+    del keep
