@@ -261,17 +261,17 @@ int64_t up_to(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 // How a decode call is cut: rows of a workgroup (16, 32, 64 or 128), and runs of tiles.  `walkers` workgroups to a block of rows, one
 // workgroup to a CU.  Few rows to a workgroup read the cache more often, but put more CUs on a row's tokens for the same number of partials, and begin
-// and end sooner: the fewest rows with which a CU meets at most 24 tiles, by the most tiles that the page table allows.  128 heads, bf16, us with
-// 16 / 32 / 64 / 128 rows: one request of 32000 tokens 41 / 42 / 43 / 49, 16 of 4000 58 / 55 / 55 / 66, 32 of 4000 97 / 79 / 75 / 82, 64 of 4000 166 / 129 / 112 /
-// 104; 64 heads, 16 of 4000 42 / 43 / 50.
+// and end sooner: the fewest rows with which a CU meets at most 12 tiles, by the most that the page table allows and with what beginning a request costs.
+// 128 heads, bf16, us with 16 / 32 / 64 / 128 rows: one request of 32000 tokens 41 / 43 / 43 / 49, 16 of up to 4000 54 / 50 / 48 / 47, 32 of 4000 91 / 74 / 71 / 66,
+// 64 of 4000 155 / 118 / 101 / 91, 256 of 200 100 / 79 / 64 / 61.  (At most 6 tiles: 31 for 27 us with 8 of 2000; at most 24: 49 for 43 with 30 of 3000, 64 heads.)
 struct DecodePlan {
   int rows, mblocks, walkers;
 };
 DecodePlan decode_plan(int64_t B, int64_t M, int64_t max_len) {
   DecodePlan d;
-  const int64_t tiles = B * ((max_len + kMlaTile - 1) / kMlaTile);
+  const int64_t tiles = B * ((max_len + kMlaTile - 1) / kMlaTile), units = tiles + B * kMlaNew;
   d.rows = 16;
-  while (d.rows < 128 && d.rows < M && tiles * ((M + d.rows - 1) / d.rows) > 24 * num_cu()) d.rows *= 2;
+  while (d.rows < 128 && d.rows < M && units * ((M + d.rows - 1) / d.rows) > 12 * num_cu()) d.rows *= 2;
   d.mblocks = (int)((M + d.rows - 1) / d.rows);
   d.walkers = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(num_cu(), 256) / d.mblocks, tiles));
   return d;

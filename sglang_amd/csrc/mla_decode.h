@@ -7,20 +7,26 @@
 // O^T = V^T . P^T as it lies: the order of the tokens inside a product is free, as long as V^T, read from LDS by transposed reads,
 // has the same.  P never goes through LDS, and the rescaling factors of O are a lane's own.
 //
-// A workgroup is eight waves (four with WM = 1) on tiles of 64 tokens.  WM of them split the R = 16 WM query rows, the other factor splits the
-// tokens of a tile; each has its own running maximum and sum, and waves that share rows are joined through LDS at the end.  A wave holds
-// its 16 rows' queries and all 512 columns of O, 200 registers.  With WM = 1 a wave reads nothing but the 16 rows that it fetched itself, and the
-// loop has no barrier.
+// A workgroup is eight waves (four with WM = 1).  WM of them split the R = 16 WM query rows, the other factor splits the tokens of a step of the
+// loop; each has its own running maximum and sum, and waves that share rows are joined through LDS at the end.  A wave holds its 16 rows' queries and
+// all 512 columns of O, 200 registers.  With WM = 1 a wave reads nothing but the 16 rows that it fetched itself, and the loop has no barrier.
 //
-// LDS: two tiles of 9 blocks of [64 rows][64 numbers], filled by global_load_lds with per-lane addresses (pages lie anywhere, beyond 4 GB
-// too).  A wave-load is 8 rows of a block, so a lane fetches from one row of a tile (WM = 1: two), at multiples of 128 bytes.  The
+// LDS: a step of T rows is 9 blocks of [T rows][64 numbers], filled by global_load_lds with per-lane addresses (pages lie anywhere, beyond 4 GB
+// too).  Few rows (WM = 1, 2) are bound by the bytes: T = 64, two stages.  Many (WM = 4, 8) by the matrix cores and LDS: T = 32, four stages, and
+// one barrier to a step.  A wave-load is 8 rows of a block, so a lane fetches from one row of a step (WM = 1: two), at multiples of 128 bytes.  The
 // 16-byte chunk c of row r of a block sits at c ^ swizzle(r), which keeps both the operand reads (16 rows, one chunk) and the transposed
-// ones (8 rows, two chunks) off each other's banks.  8-bit rows are fetched to a stage of their own, 16 rows x 64 bytes to a wave-load, and
-// widened into one 16-bit tile.
+// ones (8 rows, two chunks) off each other's banks.  8-bit rows are fetched to stages of half the size, 16 rows x 64 bytes to a wave-load, and
+// widened into one 16-bit tile (WM = 4, 8: two by turns, the next one beside the products).  The entries of the page table come the same way, some steps
+// ahead of the rows: no load into a register is waited for in the loop, which would wait for the rows behind it too.
 //
-// Work: the tiles of all requests in a row are cut into equal runs, one to a workgroup, from the lengths on the device: a captured graph
+// Work: the tiles (64 tokens) of all requests in a row are cut into equal runs, one to a workgroup, from the lengths on the device: a captured graph
 // needs no plan.  A run that holds all of a request writes its result; others write normalised float32 partials and the base-2
 // logarithm of their sums, which mla_join_kernel adds up.
+//
+// Measured (page 64, lengths from a third of the most to the most): one request of 8000 tokens, 128 heads, bf16 20 us and 4 for the join, latency; 64 of
+// 8192, 2 x 16 heads, fp16 85 + 6 us, 4.5 TB/s with everything, 6.1 TB/s in the loop (128 of 16000, 16 heads); 128 of 6000, 128 heads, 8 bits 197 + 18 us,
+// 0.67 PFLOP/s with everything, 0.90 in the loop, where the matrix cores and LDS are busy half the time each.  Of the rest the most are the partials: 100 MB
+// written at the end of all runs at once, and read by the join.
 #pragma once
 
 #include "mla_common.h"
@@ -48,19 +54,27 @@ struct MlaDecodeArgs {
 
 constexpr int kMlaTile = 64;         // tokens of a tile
 constexpr int kMlaMinRun = 2;        // tiles that a run has at least
+// What beginning a request costs beside its tiles (pages, then rows, then queries to be waited for, and a result to be written), in tiles: a run with a new
+// request in it gets as many fewer.  us with 0 / 4 / 8: 64 requests of up to 4000 tokens, 128 heads 102 / 91 / 92; 200 of 300, 16 heads 30 / 25.5 / 24;
+// 64 of 8192, 2 x 16 heads 96 / 92 / 94; one of 32000, 128 heads 42.6 / 43 / 43.
+constexpr int kMlaNew = 4;
 
 __device__ __forceinline__ int mla_len(const MlaDecodeArgs& p, int b) { return min(max(p.lens[b], 0), p.max_len); }
 __device__ __forceinline__ int mla_tiles(int len) { return (len + kMlaTile - 1) / kMlaTile; }
-// tiles of a run, from all requests' tiles
+__device__ __forceinline__ int mla_units(int tiles) { return tiles ? tiles + kMlaNew : 0; }
+// units of a run, from all requests' units
 __device__ __forceinline__ int mla_run(int total, int walkers) { return max((total + walkers - 1) / walkers, kMlaMinRun); }
-
-// Tiles of all requests, by a workgroup of NW waves; every thread returns the total.  Thread t counts requests [t * per, + per): `before`
-// is what lies in front of them, `mine` their own.
+// Units of all requests, by a workgroup of NW waves; every thread returns the total.  Thread t counts requests [t * per, + per): `before`
+// is what lies in front of them, `mine` their own, `len` the last one's tokens.
 template <int NW>
-__device__ __forceinline__ int mla_scan(const MlaDecodeArgs& p, int per, int& before, int& mine, int* lds) {
+__device__ __forceinline__ int mla_scan(const MlaDecodeArgs& p, int per, int& before, int& mine, int& len, int* lds) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   int sum = 0;
-  for (int b = tid * per; b < min((tid + 1) * per, p.B); ++b) sum += mla_tiles(mla_len(p, b));
+  len = 0;
+  for (int b = tid * per; b < min((tid + 1) * per, p.B); ++b) {
+    len = mla_len(p, b);
+    sum += mla_units(mla_tiles(len));
+  }
   int run = sum;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -111,14 +125,14 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
   if (walker >= p.walkers) return;
 
   const int per = (p.B + NW * 64 - 1) / (NW * 64);
-  int before, mine;
-  const int total = mla_scan<NW>(p, per, before, mine, scan);
+  int before, mine, mine_len;
+  const int total = mla_scan<NW>(p, per, before, mine, mine_len, scan);
   const int run = mla_run(total, p.walkers);
   if ((int64_t)walker * run >= total) return;
   const int first = walker * run, last = min(first + run, total);
   if (first >= before && first < before + mine) {  // this thread counted the request that the run begins in
-    int b = tid * per, at = before, len = mla_len(p, b);
-    for (int t = mla_tiles(len); per > 1 && first >= at + t; t = mla_tiles(len)) {
+    int b = tid * per, at = before, len = per > 1 ? mla_len(p, b) : mine_len;
+    for (int t = mla_units(mla_tiles(len)); per > 1 && first >= at + t; t = mla_units(mla_tiles(len))) {
       at += t;
       len = mla_len(p, ++b);
     }
@@ -134,13 +148,12 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
 
   const int row = mblk * R + wm * 16 + l15;  // this lane's, of the M of a request
 
-  for (int pos = first, next_len; pos < last; ++b, len = next_len) {
+  for (int next_len; at < last; ++b, len = next_len) {
     next_len = b + 1 < p.B ? mla_len(p, b + 1) : 0;
-    const int tiles = mla_tiles(len), t_begin = pos - at, t_end = min(last - at, tiles);
-    if (t_begin == 0 && mblk == 0 && tid == 0 && tiles > 0) p.spans[b] = v2i{walker, (at + tiles - 1) / run - walker + 1};
-    at += tiles;
+    const int tiles = mla_tiles(len), tiles_at = at + kMlaNew, t_begin = max(first - tiles_at, 0), t_end = min(last - tiles_at, tiles);
+    at += mla_units(tiles);
     if (t_begin >= t_end) continue;
-    pos += t_end - t_begin;
+    if (t_begin == 0 && mblk == 0 && tid == 0) p.spans[b] = v2i{walker, (at - 1) / run - walker + 1};
 
     // ---- fetching.  Steps are counted from the segment's first.  Tokens past the end are the last one's row again (masked).
     const int base = t_begin * kMlaTile, steps = min((t_end - t_begin) * (kMlaTile / TT), (len - base + TT - 1) / TT);

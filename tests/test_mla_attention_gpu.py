@@ -100,6 +100,14 @@ def test_decode_of_more_requests_than_threads(dev, n, H, B, width):
     _check_decode([(i * 37) % 250 if i % 5 else 0 for i in range(B)], n, H, 64, BF16, n == 2, seed=B, width=width)
 
 
+@pytest.mark.parametrize("B,H,width", [(200, 16, 5), (40, 128, 6), (90, 64, 8), (257, 128, 4), (16, 128, 36), (1, 128, 129)])
+@pytest.mark.parametrize("fp8", [False, True])
+def test_decode_of_short_requests(dev, B, H, width, fp8):
+    """A run counts a new request as some tiles more: its borders may lie in front of a request's tiles, in them or behind them, and a run may hold
+    no tile at all; 16 to 128 rows to a workgroup."""
+    _check_decode([(64 * width - 79 * i) % (64 * width + 1) for i in range(B)], 1, H, 64, BF16, fp8, seed=B, width=width)
+
+
 def test_decode_lengths_below_zero(dev):
     from sglang_amd import mla
 
