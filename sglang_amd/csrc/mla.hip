@@ -277,12 +277,28 @@ DecodePlan decode_plan(int64_t B, int64_t M, int64_t max_len) {
   return d;
 }
 
-// Splits of the keys of a prefill call: none, unless its blocks of queries leave CUs idle and the keys are long; then as many as give every CU its
-// two workgroups, eight tiles of keys to each on average.
-int prefill_splits(int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q) {
-  const int64_t blocks = (std::min(max_seqlen_q, Tq) + kPreRows - 1) / kPreRows, groups = B * H * blocks;
-  if (groups <= 0 || groups > num_cu()) return 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(2 * num_cu() / groups, 32), Tk / B / (8 * kPreKeys)));
+// How a prefill call is cut.  Workgroups of four waves (128 queries), two to a CU, or of eight (256), one to a CU.  Eight fetch the keys half as often, four
+// waste less on sequences' last blocks and on the diagonal, and two workgroups do not wait at each other's barriers.  Eight where the queries fill
+// their blocks by seven eighths and there are many keys to a query: all are seen and as many as there are queries, or (causal) four times as many.  us with four /
+// eight: 2000 queries of 32 heads with 18000 keys causal 641 / 608, all 656 / 621; 1000 with 4000 keys 106 / 105, 115 / 107; 8192 of 16 heads with 16384 keys 875 / 852,
+// 1160 / 1116; but 2048 of 128 heads with their own keys, causal, 200 / 210, 4 x 512 66 / 77, and 384 of 64 heads with 8384 keys 155 / 168.
+//
+// Splits of the keys: none, unless the blocks of queries leave CUs idle and the keys are long; then as many as give every CU its workgroups,
+// eight tiles of keys to each on average.
+struct PrefillPlan {
+  int waves, splits;
+  int64_t blocks;
+};
+PrefillPlan prefill_cut(int waves, int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q) {
+  const int64_t rows = 32 * waves, blocks = (std::min(max_seqlen_q, Tq) + rows - 1) / rows, groups = B * H * blocks;
+  PrefillPlan d{waves, 1, blocks};
+  if (groups > 0 && groups <= num_cu())
+    d.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(num_cu() * 8 / waves / groups, 32), Tk / B / (8 * kPreKeys)));
+  return d;
+}
+PrefillPlan prefill_plan(int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q, bool causal) {
+  const PrefillPlan d = prefill_cut(8, B, H, Tq, Tk, max_seqlen_q);
+  return Tk >= (causal ? 4 : 1) * Tq && Tq * 8 >= B * d.blocks * 256 * 7 ? d : prefill_cut(4, B, H, Tq, Tk, max_seqlen_q);
 }
 
 }  // namespace
@@ -430,7 +446,7 @@ extern "C" int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t 
 
 extern "C" int64_t fp8k_mla_prefill_workspace_bytes(int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q) {
   if (B <= 0 || H <= 0 || Tq <= 0 || Tk <= 0 || max_seqlen_q <= 0) return 0;
-  const int64_t splits = prefill_splits(B, H, Tq, Tk, max_seqlen_q);
+  const int64_t splits = std::max(prefill_cut(4, B, H, Tq, Tk, max_seqlen_q).splits, prefill_cut(8, B, H, Tq, Tk, max_seqlen_q).splits);
   return splits == 1 ? 0 : up_to(splits * Tq * H * kPreValue * 4, 256) + up_to(splits * Tq * H * 4, 256);
 }
 
@@ -452,28 +468,38 @@ extern "C" int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_str
   FP8K_REQUIRE(q_stride_t >= 0 && q_stride_h >= 0 && kn_stride_t >= 0 && kn_stride_h >= 0 && kp_stride_t >= 0 && v_stride_t >= 0 && v_stride_h >= 0,
                "mla prefill: negative stride");
   FP8K_REQUIRE(kn_stride_t < (1 << 24) && kp_stride_t < (1 << 24) && v_stride_t < (1 << 24), "mla prefill: rows of keys further apart than 2^24");
-  const int64_t blocks = (std::min(max_seqlen_q, Tq) + kPreRows - 1) / kPreRows, units = up_to(B * H, 8);
-  FP8K_REQUIRE(units * blocks < (1ll << 31), "mla prefill: too many blocks of queries");
+  const PrefillPlan d = prefill_plan(B, H, Tq, Tk, max_seqlen_q, causal != 0);
+  const int64_t units = up_to(B * H, 8);
+  FP8K_REQUIRE(units * d.blocks < (1ll << 31), "mla prefill: too many blocks of queries");
   MlaPrefillArgs p{};
   p.q = q; p.k_nope = k_nope; p.k_pe = k_pe; p.v = v;
   p.q_t = q_stride_t; p.q_h = q_stride_h; p.kn_t = kn_stride_t; p.kn_h = kn_stride_h; p.kp_t = kp_stride_t; p.v_t = v_stride_t; p.v_h = v_stride_h;
   p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.out = out; p.lse = lse;
-  p.B = (int)B; p.H = (int)H; p.Tq = (int)Tq; p.Tk = (int)Tk; p.blocks = (int)blocks; p.causal = causal != 0; p.sm_scale = sm_scale;
-  p.splits = prefill_splits(B, H, Tq, Tk, max_seqlen_q);
+  p.B = (int)B; p.H = (int)H; p.Tq = (int)Tq; p.Tk = (int)Tk; p.blocks = (int)d.blocks; p.causal = causal != 0; p.sm_scale = sm_scale;
+  p.splits = d.splits;
   const int64_t need = fp8k_mla_prefill_workspace_bytes(B, H, Tq, Tk, max_seqlen_q);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
     return fail(FP8K_ERR_WORKSPACE, "mla prefill: workspace of %lld bytes needed, 256-byte aligned", (long long)need);
   p.part = (float*)workspace;
   p.part_lse = (float*)((uint8_t*)workspace + up_to(p.splits * Tq * H * kPreValue * 4, 256));
-  const dim3 grid((unsigned)(units * blocks), (unsigned)p.splits), join_grid((unsigned)(units * blocks), 16);
+  const dim3 grid((unsigned)(units * d.blocks), (unsigned)p.splits), join_grid((unsigned)(units * d.blocks), 16);
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == FP8K_BF16) mla_prefill_kernel<FP8K_BF16><<<grid, 256, 0, st>>>(p);
-  else mla_prefill_kernel<FP8K_F16><<<grid, 256, 0, st>>>(p);
-  if (p.splits > 1) {
-    if (const int rc = check_launch("mla prefill")) return rc;
-    if (dtype == FP8K_BF16) mla_prefill_join_kernel<FP8K_BF16><<<join_grid, 256, 0, st>>>(p);
-    else mla_prefill_join_kernel<FP8K_F16><<<join_grid, 256, 0, st>>>(p);
+#define MLA_PREFILL(DT, NW)                                                       \
+  do {                                                                            \
+    mla_prefill_kernel<DT, NW><<<grid, 64 * NW, 0, st>>>(p);                      \
+    if (p.splits > 1) {                                                           \
+      if (const int rc = check_launch("mla prefill")) return rc;                  \
+      mla_prefill_join_kernel<DT, NW><<<join_grid, 256, 0, st>>>(p);              \
+    }                                                                             \
+  } while (0)
+  if (dtype == FP8K_BF16) {
+    if (d.waves == 4) MLA_PREFILL(FP8K_BF16, 4);
+    else MLA_PREFILL(FP8K_BF16, 8);
+  } else {
+    if (d.waves == 4) MLA_PREFILL(FP8K_F16, 4);
+    else MLA_PREFILL(FP8K_F16, 8);
   }
+#undef MLA_PREFILL
   return check_launch("mla prefill");
 }
 

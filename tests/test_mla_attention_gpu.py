@@ -260,6 +260,14 @@ def test_prefill_over_split_keys(dev, lq, lk, H, causal, dtype):
     _check_prefill(lq, lk, H, dtype, causal, seed=H)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lq,lk,H,causal", [([256], [256], 3, False), ([256], [1100], 3, True), ([251, 256], [1600, 650], 2, True), ([480], [480], 150, False),
+                                            ([1000], [4100], 40, True), ([230, 256, 250], [0, 900, 7], 2, False), ([512, 512], [4000, 97], 1, True)], ids=str)
+def test_prefill_in_large_blocks(dev, lq, lk, H, causal, dtype):
+    """Queries that fill blocks of 256 and have many keys: eight waves to a workgroup, the keys split and not; sequences without keys, and with few, among them."""
+    _check_prefill(lq, lk, H, dtype, causal, seed=H)
+
+
 def test_prefill_of_many_blocks(dev):
     """More workgroups than run at once: no splits, long and short blocks by turns."""
     _check_prefill([700, 130, 1500], [700, 400, 1500], 64, BF16, True)
