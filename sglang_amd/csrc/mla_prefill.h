@@ -18,7 +18,7 @@
 //
 // Measured, bf16: 8192 queries of 128 heads with their own keys, causal, 2.5 ms or 1.07 PFLOP/s, where a library's matrix product of 8192^3 reaches 1.55; the
 // matrix cores are busy 57 % of the time at the 1.8 GHz that the power limit leaves, LDS (1160 clocks of reads and fills to the products' 1280, four
-// waves) and the vector instructions (1020) nearly as long.  1000 queries of 32 heads with 10000 keys, float16, 207 us or 0.94 PFLOP/s, the join 8 us of it.  17
+// waves) and the vector instructions (1020) nearly as long.  1000 queries of 32 heads with 10000 keys, float16, 207 us or 0.94 PFLOP/s, the join 9 us of it.  17
 // prompts of 100 to 300 tokens, 16 heads, 25 us: 2.7 TB/s, latency (a workgroup alone takes 6 to 11 us).
 #pragma once
 
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mla_prefill_kernel(const MlaPrefil
     for (int ks = 0; ks < 12; ++ks) q[ks] = *(const v4i*)(from + 16 * ks);
   }
 
-  // A wave fetches 16 rows of each part of a stage: four wave-loads of k_nope and of v, of four rows each, two of k_pe, of eight.  Load j is of row
+  // A wave fetches 16 rows (of eight waves: 8) of each part of a stage: four wave-loads of k_nope and of v, of four rows each, two of k_pe, of eight.  Load j is of row
   // 4 j (8 j) + lane / 16 (lane / 8) of the wave's: the lane's offset is that row's, which j moves by a number that all lanes share, and a chunk, which j
   // moves by an exclusive or.  Rows past the sequence's last are that row again (masked).
   const uint32_t lds0 = lds_address(smem);
