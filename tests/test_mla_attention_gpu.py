@@ -573,6 +573,98 @@ def test_whole_step_in_a_graph_and_on_another_stream(dev):
     assert first.shape == (B, H, 512)
 
 
+def test_prefill_in_graphs(dev):
+    """Two captured chains, each a prompt's chunk over split keys and its cached prefix's rows, joined; lengths change between replays on two streams."""
+    from sglang_amd import mla
+
+    g = _gen(33)
+    to = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    cases = []
+    for H, dtype in ((3, BF16), (2, F16)):
+        cache, table, pt, _ = _filled(g, [1900], 64, dtype, False)
+        rand = lambda *shape: torch.randn(shape, generator=g, device="cuda").to(dtype)  # noqa: E731, B023
+        cases.append([rand(256, H, 192), rand(3000, H, 128), rand(3000, 64), rand(3000, H, 128), to(0, 256), to(0, 3000), cache, pt, to(0, 1900)])
+
+    def chain(q, kn, kp, v, cu_q, cu_k, cache, pt, cu_p):
+        own, s = mla.mla_prefill_attention(q, kn, kp, v, cu_q, cu_k, 256, SCALE, return_lse=True)
+        rows = mla.mla_gather_cache(cache, pt, cu_p, 1900, dtype=q.dtype)
+        keys = rows[:, None, :128].expand(-1, q.shape[1], -1).contiguous()
+        pre, ps = mla.mla_prefill_attention(q, keys, rows[:, 512:], keys, cu_q, cu_p, 256, SCALE, causal=False, return_lse=True)
+        return mla.merge_attention_states(own, s, pre, ps)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    for c in cases:
+        with torch.cuda.stream(side):
+            chain(*c)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            res = chain(*c)
+        graphs.append((graph, res))
+    for turn in range(4):
+        for i, c in enumerate(cases):
+            c[0].normal_(generator=g)
+            c[4].copy_(to(0, 256 - 50 * turn))
+            c[5].copy_(to(0, 3000 - 700 * turn * i))
+            c[8].copy_(to(0, (1900, 64, 0, 1000)[turn]))
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in cases]
+        for s, (graph, _) in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for c, (_, got) in zip(cases, graphs):
+            n = 256 - 50 * turn
+            for a, b in zip(got, chain(*c)):
+                assert torch.equal(a[:n], b[:n]) and bool(torch.isfinite(a[:n]).all()), turn
+
+
+def test_calls_of_two_threads(dev):
+    """Two threads, a stream each, make calls at once; every result is that of a call alone."""
+    import threading
+
+    from sglang_amd import mla
+
+    g = _gen(35)
+    work = []
+    for lens, H in (([1200, 30, 500], 128), ([90] * 20, 16)):
+        cache, table, pt, _ = _filled(g, lens, 64, BF16, False)
+        q, qp = _queries(g, len(lens), 1, H, BF16)
+        sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        pq, kn, kp, v, cu_q, cu_k, tq, tk = _prefill_inputs(g, [40], [2000 + H], 2, BF16, slack=0)
+        work.append(lambda a=(q, qp, cache, pt, sl, SCALE), b=(pq, kn, kp, v, tq, tk, 40, SCALE): (mla.mla_decode_attention(*a), mla.mla_prefill_attention(*b)))
+    want = [fn() for fn in work]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def run(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] += [work[i]() for _ in range(10)]
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    for w, results in zip(want, got):
+        assert len(results) == 10 and all(torch.equal(x, y) for r in results for x, y in zip(w, r))
+
+
+def test_decode_of_a_shared_row_of_pages(dev):
+    """Requests that share one row of the page table, which is expanded rather than copied; one request twice."""
+    from sglang_amd import mla
+
+    g = _gen(37)
+    cache, table, pt, _ = _filled(g, [700], 16, BF16, False)
+    q, qp = _queries(g, 4, 2, 16, BF16)
+    q[3], qp[3] = q[1], qp[1]
+    sl = torch.tensor([700, 65, 1, 65], dtype=torch.int32, device="cuda")
+    out = mla.mla_decode_attention(q, qp, cache, pt.expand(4, -1), sl, SCALE)
+    assert torch.equal(out, mla.mla_decode_attention(q, qp, cache, pt.repeat(4, 1), sl, SCALE))
+    want, _, tol, _ = R.decode(q, qp, cache, table * 4, sl.tolist(), SCALE, None)
+    R.close(out, want, tol, "out")
+
+
 def test_compiled(dev):
     from sglang_amd import mla
 
