@@ -331,6 +331,10 @@ extern "C" int fp8k_mla_write_cache(const void* latent, int64_t ld_latent, void*
     FP8K_REQUIRE(aligned(q_pe, 16) && aligned(q_out, 16) && q_stride_t % 8 == 0 && q_stride_h % 8 == 0 && o_stride_t % 8 == 0 && o_stride_h % 8 == 0,
                  "mla write: queries must be 16-byte aligned");
     FP8K_REQUIRE(q_stride_t >= 0 && q_stride_h >= 0 && o_stride_t >= 0 && o_stride_h >= 0, "mla write: negative stride");
+    const auto apart = [](int64_t inner, int64_t n, int64_t outer, int64_t m) {
+      return (n == 1 || inner >= kRope) && (m == 1 || outer >= (n - 1) * inner + kRope);
+    };
+    FP8K_REQUIRE(apart(o_stride_h, H, o_stride_t, T) || apart(o_stride_t, T, o_stride_h, H), "mla write: the rotated queries' places overlap each other");
   }
   MlaWriteArgs p{};
   p.latent = (const u16*)latent; p.q_pe = (const u16*)q_pe; p.cache = cache; p.q_out = (u16*)q_out;

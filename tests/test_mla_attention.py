@@ -260,3 +260,19 @@ def test_the_joined_logarithm_is_memory_of_its_own():
     _refused(merge(p, p + 1024, p, p + 2048, p, p + 1024, 2, 192, _lib.BF16, None), "memory of its own")
     _refused(merge(p, p + 1024, p, p + 2048, p, p + 2048, 2, 192, _lib.BF16, None), "memory of its own")
     del keep
+
+
+def test_places_of_rotated_queries_do_not_overlap():
+    """An expanded or otherwise overlapping output of the writer is refused."""
+    from sglang_amd import _lib
+
+    keep, p = _address()
+
+    def write(ot, oh, T=4, H=3):
+        return _lib.lib.fp8k_mla_write_cache(p, 576, p, p, 1, None, 0, 1e-6, p, 10, p, 1, 0, p, 192, 64, p, ot, oh, None, T, H, 100, _lib.BF16, 0, None)
+
+    for ot, oh in ((0, 64), (64, 64), (192, 0), (128, 64), (64, 192), (184, 64), (32, 256)):
+        _refused(write(ot, oh), "overlap")
+    _refused(write(0, 64, H=1), "overlap")
+    _refused(write(192, 0, T=1), "overlap")
+    del keep
