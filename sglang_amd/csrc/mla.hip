@@ -287,8 +287,9 @@ DecodePlan decode_plan(int64_t B, int64_t M, int64_t max_len) {
 // eight: 2000 queries of 32 heads with 18000 keys causal 641 / 608, all 656 / 621; 1000 with 4000 keys 106 / 105, 115 / 107; 8192 of 16 heads with 16384 keys 875 / 852,
 // 1160 / 1116; but 2048 of 128 heads with their own keys, causal, 200 / 210, 4 x 512 66 / 77, and 384 of 64 heads with 8384 keys 155 / 168.
 //
-// Splits of the keys: none, unless the blocks of queries leave CUs idle and the keys are long; then as many as give every CU its workgroups,
-// eight tiles of keys to each on average.
+// Splits of the keys, where the blocks of queries leave CUs idle: as many as a model of the call's time has fewest us for, at least two tiles of keys to
+// each.  A tile of a workgroup of four waves takes 1.25 us alone on a CU, 2.5 beside another, of eight 2.2; a join 5 and its partials, written and read at 4.5 TB/s.  us,
+// causal: 1024 queries of 32 heads 30 whole, 41 in two; 2048 of 16 48, 56 in two; of 8 44, 35 in two, 40 in four; 16 with 2016 keys of 16 heads 42 whole, 21 in three, 15 so.
 struct PrefillPlan {
   int waves, splits;
   int64_t blocks;
@@ -296,8 +297,16 @@ struct PrefillPlan {
 PrefillPlan prefill_cut(int waves, int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q) {
   const int64_t rows = 32 * waves, blocks = (std::min(max_seqlen_q, Tq) + rows - 1) / rows, groups = B * H * blocks;
   PrefillPlan d{waves, 1, blocks};
-  if (groups > 0 && groups <= num_cu())
-    d.splits = (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(num_cu() * 8 / waves / groups, 32), Tk / B / (8 * kPreKeys)));
+  if (groups <= 0 || groups > num_cu()) return d;
+  const int64_t tiles = (Tk / B + kPreKeys - 1) / kPreKeys, most = std::min<int64_t>(std::min<int64_t>(num_cu() * 8 / waves / groups, 32), tiles / 2);
+  const double partials = (double)(Tq * H) * (2 * 4 * kPreValue) / 4.5e6;
+  double least = 0;
+  for (int64_t n = 1; n <= most; ++n) {
+    const double us = (waves == 8 ? 2.2 : groups * n > num_cu() ? 2.5 : 1.25) * (double)((tiles + n - 1) / n) + (n > 1 ? 5 + n * (partials + 0.25) : 0);
+    if (n > 1 && us >= least) continue;
+    least = us;
+    d.splits = (int)n;
+  }
   return d;
 }
 PrefillPlan prefill_plan(int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q, bool causal) {
@@ -485,12 +494,15 @@ extern "C" int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_str
   p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.out = out; p.lse = lse;
   p.B = (int)B; p.H = (int)H; p.Tq = (int)Tq; p.Tk = (int)Tk; p.blocks = (int)d.blocks; p.causal = causal != 0; p.sm_scale = sm_scale;
   p.splits = d.splits;
+  // Heads by XCDs, unless that leaves more than an eighth of them idle (1000 queries of 4 heads with 10000 keys 79 us by XCDs, 49 over all)
+  p.xcds = units * 8 > B * H * 9 ? 1 : 8;
+  const int64_t lines = p.xcds == 8 ? units : B * H;
   const int64_t need = fp8k_mla_prefill_workspace_bytes(B, H, Tq, Tk, max_seqlen_q);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
     return fail(FP8K_ERR_WORKSPACE, "mla prefill: workspace of %lld bytes needed, 256-byte aligned", (long long)need);
   p.part = (float*)workspace;
   p.part_lse = (float*)((uint8_t*)workspace + up_to(p.splits * Tq * H * kPreValue * 4, 256));
-  const dim3 grid((unsigned)(units * d.blocks), (unsigned)p.splits), join_grid((unsigned)(units * d.blocks), 16);
+  const dim3 grid((unsigned)(lines * d.blocks), (unsigned)p.splits), join_grid((unsigned)(lines * d.blocks), 16);
   const hipStream_t st = (hipStream_t)stream;
 #define MLA_PREFILL(DT, NW)                                                       \
   do {                                                                            \

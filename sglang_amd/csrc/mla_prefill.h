@@ -35,6 +35,7 @@ struct MlaPrefillArgs {
   float *part, *part_lse;  // [splits, Tq, H, 128], [splits, Tq, H]
   int B, H, Tq, Tk, blocks;  // blocks: of a workgroup's queries, that a sequence has at most
   int splits;              // of a block's keys, each a workgroup's
+  int xcds;                // heads side by side: 8, one to an XCD, or 1
   int causal;
   float sm_scale;
 };
@@ -45,7 +46,7 @@ constexpr int kPreKeys = 64, kPreNope = 128, kPreValue = 128;
 __device__ __forceinline__ int mla_value_swizzle(int r) { return ((r & 1) ? 12 : 0) ^ ((r & 2) ? 10 : 0) ^ ((r & 4) ? 6 : 0); }
 
 // A workgroup's 128 (256) queries.  The blocks of a sequence's head follow each other on one XCD (workgroup i runs on XCD i % 8): they read the same
-// keys.  Of a causal head the last queries, which have most keys, come first, in every other head the first ones: the workgroups that start
+// keys.  (Few heads, or some more than a multiple of 8, would leave XCDs idle: their blocks go to all of them.)  Of a causal head the last queries, which have most keys, come first, in every other head the first ones: the workgroups that start
 // together, two to a CU, are long and short ones.
 struct MlaBlock {
   int b, h, q_begin, lq, q0, rows;
@@ -53,14 +54,14 @@ struct MlaBlock {
 template <int ROWS>
 __device__ __forceinline__ MlaBlock mla_block(const MlaPrefillArgs& p) {
   MlaBlock x;
-  const int line = (int)blockIdx.x / 8, group = line / p.blocks, place = line - group * p.blocks, unit = group * 8 + (int)(blockIdx.x % 8);
+  const int line = (int)blockIdx.x / p.xcds, group = line / p.blocks, place = line - group * p.blocks, unit = group * p.xcds + (int)blockIdx.x % p.xcds;
   x.rows = 0;
   if (unit >= p.B * p.H) return x;
   x.b = unit / p.H;
   x.h = unit - x.b * p.H;
   x.q_begin = min(max(p.cu_q[x.b], 0), p.Tq);
   x.lq = min(max(p.cu_q[x.b + 1], x.q_begin), p.Tq) - x.q_begin;
-  const int groups = (int)gridDim.x / 8 / p.blocks;
+  const int groups = (int)gridDim.x / p.xcds / p.blocks;
   x.q0 = ((groups - group) & 1 ? p.blocks - 1 - place : place) * ROWS;
   x.rows = min(ROWS, x.lq - x.q0);
   return x;
