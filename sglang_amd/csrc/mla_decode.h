@@ -144,7 +144,8 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
   int b = __builtin_amdgcn_readfirstlane(found[0]), at = __builtin_amdgcn_readfirstlane(found[1]), len = __builtin_amdgcn_readfirstlane(found[2]);
 
   const float kscale = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(FP8 && p.scale ? *p.scale : 1.0f)));
-  const float c = p.sm_scale * kLog2e * kscale;
+  // at least the smallest number: with a product that is no number above zero any more, what is masked would be 0 times -inf
+  const float c = fmaxf(p.sm_scale * kLog2e * kscale, 0x1p-149f);
 
   const int row = mblk * R + wm * 16 + l15;  // this lane's, of the M of a request
 
