@@ -396,7 +396,7 @@ extern "C" int fp8k_mla_gather_cache(const void* cache, const int32_t* page_tabl
 
 extern "C" int64_t fp8k_mla_decode_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t max_len) {
   if (B <= 0 || n <= 0 || H <= 0 || max_len <= 0) return 0;
-  const int64_t M = n * H, slots = decode_plan(B, M, max_len).walkers + B;
+  const int64_t M = n * H, slots = mla_slots(B, decode_plan(B, M, max_len).walkers);
   return up_to(slots * M * kLatent * 4, 256) + up_to(slots * M * 4, 256) + up_to(B * 8, 256);
 }
 
@@ -425,6 +425,7 @@ extern "C" int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t 
     return fail(FP8K_ERR_WORKSPACE, "mla decode: workspace of %lld bytes needed, 256-byte aligned", (long long)need);
   const int64_t M = n * H;
   const DecodePlan d = decode_plan(B, M, max_len);
+  const int64_t slots = mla_slots(B, d.walkers);
   MlaDecodeArgs p{};
   p.q_nope = q_nope; p.q_pe = q_pe;
   p.qn_b = qn_stride_b; p.qn_n = qn_stride_n; p.qn_h = qn_stride_h;
@@ -432,8 +433,8 @@ extern "C" int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t 
   p.cache = (const uint8_t*)cache; p.table = page_table; p.table_stride = table_stride; p.lens = seq_lens; p.scale = scale;
   p.out = out; p.lse = lse;
   p.part = (float*)workspace;
-  p.part_lse = (float*)((uint8_t*)workspace + up_to((d.walkers + B) * M * kLatent * 4, 256));
-  p.spans = (v2i*)((uint8_t*)p.part_lse + up_to((d.walkers + B) * M * 4, 256));
+  p.part_lse = (float*)((uint8_t*)workspace + up_to(slots * M * kLatent * 4, 256));
+  p.spans = (v2i*)((uint8_t*)p.part_lse + up_to(slots * M * 4, 256));
   p.B = (int)B; p.n = (int)n; p.H = (int)H; p.M = (int)M;
   p.page_size = (int)page_size; p.page_shift = (page_size & (page_size - 1)) ? -1 : __builtin_ctzll(page_size); p.pages = (int)pages; p.max_len = (int)max_len;
   p.walkers = d.walkers; p.mblocks = d.mblocks; p.sm_scale = sm_scale;

@@ -43,7 +43,7 @@ struct MlaDecodeArgs {
   const float* scale;  // of the 8-bit cache, or null
   void* out;           // [B, n, H, 512]
   float* lse;          // [B, n, H] or null
-  float *part, *part_lse;  // [walkers + B, M, 512], [walkers + B, M]
+  float *part, *part_lse;  // [slots, M, 512], [slots, M]: mla_slots(B, walkers) of them
   v2i* spans;              // [B]: the first run that holds tokens of a request, and how many do
   int B, n, H, M;
   int page_size, pages, max_len;
@@ -58,6 +58,13 @@ constexpr int kMlaMinRun = 2;        // tiles that a run has at least
 // request in it gets as many fewer.  us with 0 / 4 / 8: 64 requests of up to 4000 tokens, 128 heads 102 / 91 / 92; 200 of 300, 16 heads 30 / 25.5 / 24;
 // 64 of 8192, 2 x 16 heads 96 / 92 / 94; one of 32000, 128 heads 42.6 / 43 / 43.
 constexpr int kMlaNew = 4;
+
+// Places of partials.  A run leaves at most two: of the request that it goes on with, at the run's number, and of one that begins in it and does not
+// end in it, behind those, at the request's number or the run's, whichever are fewer.
+__host__ __device__ __forceinline__ int64_t mla_slots(int64_t B, int64_t walkers) { return walkers + (B < walkers ? B : walkers); }
+__device__ __forceinline__ int mla_slot(const MlaDecodeArgs& p, int walker, int b, bool begins) {
+  return begins ? p.walkers + (p.B < p.walkers ? b : walker) : walker;
+}
 
 __device__ __forceinline__ int mla_len(const MlaDecodeArgs& p, int b) { return min(max(p.lens[b], 0), p.max_len); }
 __device__ __forceinline__ int mla_tiles(int len) { return (len + kMlaTile - 1) / kMlaTile; }
@@ -424,7 +431,7 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
 
     // ---- join the waves that share rows, normalise, write
     const bool whole = t_end - t_begin == tiles;
-    const int64_t slot = walker + b;
+    const int64_t slot = mla_slot(p, walker, b, t_begin == 0);
     l = sum_across32(sum_across16(l));
     if (g == 0) {
       join_m[w][l15] = m;
@@ -518,22 +525,23 @@ __global__ __launch_bounds__(256) void mla_join_kernel(const MlaDecodeArgs p) {
   }
   const int n = span[1];
   if (n == 1) return;
-  const int64_t slot = span[0] + b;
+  const int beginning = mla_slot(p, span[0], b, true);
+  auto slot_of = [&](int i) -> int64_t { return i ? span[0] + i : beginning; };
   // The partials are asked for before their weights are known, a batch of up to 64 at a time (n <= 256): a logarithm to a lane, and
   // kEach partials to a wave at once.
   constexpr int kEach = WAVES == 1 ? 4 : 16;
   v4f x = {0, 0, 0, 0}, y = {0, 0, 0, 0};
   float top = -INFINITY, sum = 0.0f;
-  const float* const from = p.part + (slot * p.M + r) * kLatent + 4 * lane;
+  const float* const from = p.part + (int64_t)r * kLatent + 4 * lane;
   for (int at = 0; at < n; at += kEach * WAVES) {
     const int count = min(n - at, kEach * WAVES);  // at most 64
-    const float lse = lane < count ? p.part_lse[(slot + at + lane) * p.M + r] : -INFINITY;
+    const float lse = lane < count ? p.part_lse[slot_of(at + lane) * p.M + r] : -INFINITY;
     v4f u[kEach], v[kEach];
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
       u[i] = v[i] = v4f{0, 0, 0, 0};
       if (i * WAVES + w < count) {
-        const float* const part = from + (int64_t)(at + i * WAVES + w) * p.M * kLatent;
+        const float* const part = from + slot_of(at + i * WAVES + w) * p.M * kLatent;
         u[i] = *(const v4f*)part;
         v[i] = *(const v4f*)(part + 256);
       }

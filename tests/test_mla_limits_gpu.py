@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from tests import mla_reference as R
-from tests.test_mla_attention_gpu import BF16, F16, _filled, _gen, _prefill_inputs, _queries
+from tests.test_mla_attention_gpu import BF16, F16, SCALE, _filled, _gen, _prefill_inputs, _queries
 
 pytestmark = pytest.mark.gpu
 
@@ -34,5 +34,35 @@ def test_prefill_of_scores_scaled_to_nothing(dev, causal, dtype):
     q, kn, kp, v, cu_q, cu_k, tq, tk = _prefill_inputs(_gen(3), [70, 5], [70, 130], 2, dtype, slack=0)
     out, lse = mla.mla_prefill_attention(q, kn, kp, v, tq, tk, 70, 1e-45, causal=causal, return_lse=True)
     want, want_lse, tol, lse_tol = R.prefill(q, kn, kp, v, cu_q, cu_k, 1e-45, causal)
+    R.close(out, want, tol, "out")
+    R.close(lse, want_lse, lse_tol, "lse")
+
+
+def _decode_by_abi(q, qp, cache, pt, sl, guard=4096):
+    """fp8k_mla_decode with just the workspace that it asks for, full of ones, and bytes behind it that must stay as they are."""
+    from sglang_amd._lib import BF16 as CODE, check, lib, stream_ptr
+
+    B, n, H, _ = q.shape
+    out = torch.full((B, n, H, 512), 9.0, dtype=q.dtype, device="cuda")
+    lse = torch.full((B, n, H), 9.0, device="cuda")
+    need = lib.fp8k_mla_decode_workspace_bytes(B, n, H, pt.shape[1] * cache.shape[1])
+    ws = torch.full((need + guard,), 255, dtype=torch.uint8, device="cuda")
+    check(lib.fp8k_mla_decode(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), qp.data_ptr(), qp.stride(0), qp.stride(1), qp.stride(2), cache.data_ptr(),
+                              pt.data_ptr(), pt.stride(0), pt.shape[1], sl.data_ptr(), None, out.data_ptr(), lse.data_ptr(), B, n, H, cache.shape[0],
+                              cache.shape[1], SCALE, CODE, 0, ws.data_ptr(), need, stream_ptr(q.device)))
+    assert bool((ws[need:] == 255).all())
+    return out, lse
+
+
+@pytest.mark.parametrize("n,H,lens,width", [(1, 128, [64 * 40, 100, 0, 64 * 33], 40), (1, 16, [(i * 53) % 900 for i in range(300)], 16),
+                                            (2, 32, [(i * 37) % 250 if i % 5 else 0 for i in range(700)], 4), (1, 128, [0, 0, 0], 2),
+                                            (1, 8, [0] * 600, 2), (1, 128, [130] * 256, 3), (1, 16, [700] * 257, 11)], ids=lambda x: None if isinstance(x, list) else str(x))
+def test_decode_stays_in_its_workspace(dev, n, H, lens, width):
+    """Batches with fewer requests than runs and with more, with and without empty ones, in a workspace that held something else."""
+    g = _gen(len(lens) + H)
+    cache, table, pt, _ = _filled(g, lens, 64, BF16, False, width=width)
+    q, qp = _queries(g, len(lens), n, H, BF16)
+    out, lse = _decode_by_abi(q, qp, cache, pt, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    want, want_lse, tol, lse_tol = R.decode(q, qp, cache, table, lens, SCALE, None)
     R.close(out, want, tol, "out")
     R.close(lse, want_lse, lse_tol, "lse")
