@@ -44,7 +44,7 @@ struct MlaDecodeArgs {
   void* out;           // [B, n, H, 512]
   float* lse;          // [B, n, H] or null
   float *part, *part_lse;  // [slots, M, 512], [slots, M]: mla_slots(B, walkers) of them
-  v2i* spans;              // [B]: the first run that holds tokens of a request, and how many do
+  v2i* spans;              // [B]: the first run that holds tokens of a request, and how many do (none: it has no tokens)
   int B, n, H, M;
   int page_size, pages, max_len;
   int page_shift;  // log2 of page_size, or -1
@@ -72,14 +72,15 @@ __device__ __forceinline__ int mla_units(int tiles) { return tiles ? tiles + kMl
 // units of a run, from all requests' units
 __device__ __forceinline__ int mla_run(int total, int walkers) { return max((total + walkers - 1) / walkers, kMlaMinRun); }
 // Units of all requests, by a workgroup of NW waves; every thread returns the total.  Thread t counts requests [t * per, + per): `before`
-// is what lies in front of them, `mine` their own, `len` the last one's tokens.
+// is what lies in front of them, `mine` their own, `len` the last one's tokens.  `note`: requests without tokens, which no run meets, get their spans.
 template <int NW>
-__device__ __forceinline__ int mla_scan(const MlaDecodeArgs& p, int per, int& before, int& mine, int& len, int* lds) {
+__device__ __forceinline__ int mla_scan(const MlaDecodeArgs& p, int per, int& before, int& mine, int& len, int* lds, bool note) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   int sum = 0;
   len = 0;
   for (int b = tid * per; b < min((tid + 1) * per, p.B); ++b) {
     len = mla_len(p, b);
+    if (note && len == 0) p.spans[b] = v2i{0, 0};
     sum += mla_units(mla_tiles(len));
   }
   int run = sum;
@@ -133,13 +134,16 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
 
   const int per = (p.B + NW * 64 - 1) / (NW * 64);
   int before, mine, mine_len;
-  const int total = mla_scan<NW>(p, per, before, mine, mine_len, scan);
+  const int total = mla_scan<NW>(p, per, before, mine, mine_len, scan, walker == 0 && mblk == 0);
   const int run = mla_run(total, p.walkers);
   if ((int64_t)walker * run >= total) return;
   const int first = walker * run, last = min(first + run, total);
+  // Lengths are read again from here on.  Should they have changed (a caller that overwrites them under the call gets no result to rely on), both walks over
+  // the requests still end at the last one.
   if (first >= before && first < before + mine) {  // this thread counted the request that the run begins in
     int b = tid * per, at = before, len = per > 1 ? mla_len(p, b) : mine_len;
-    for (int t = mla_units(mla_tiles(len)); per > 1 && first >= at + t; t = mla_units(mla_tiles(len))) {
+    const int end = min((tid + 1) * per, p.B) - 1;
+    for (int t = mla_units(mla_tiles(len)); b < end && first >= at + t; t = mla_units(mla_tiles(len))) {
       at += t;
       len = mla_len(p, ++b);
     }
@@ -156,7 +160,7 @@ __global__ __launch_bounds__(WM == 1 ? 256 : 512) void mla_decode_kernel(const M
 
   const int row = mblk * R + wm * 16 + l15;  // this lane's, of the M of a request
 
-  for (int next_len; at < last; ++b, len = next_len) {
+  for (int next_len; at < last && b < p.B; ++b, len = next_len) {
     next_len = b + 1 < p.B ? mla_len(p, b + 1) : 0;
     const int tiles = mla_tiles(len), tiles_at = at + kMlaNew, t_begin = max(first - tiles_at, 0), t_end = min(last - tiles_at, tiles);
     at += mla_units(tiles);
@@ -512,10 +516,14 @@ __global__ __launch_bounds__(256) void mla_join_kernel(const MlaDecodeArgs p) {
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6) % WAVES);
   const int b = blockIdx.y, r = (int)blockIdx.x * (4 / WAVES) + (int)(threadIdx.x >> 6) / WAVES;
   if (r >= p.M) return;  // whole workgroups, with WAVES = 4
-  const v2i span = p.spans[b];  // anything, for a request without tokens
+  // The cut is that of the first launch, whatever becomes of the lengths meanwhile; held within the runs, so that no partial outside the workspace is
+  // read even if lengths that changed under that launch left a span that nobody wrote.
+  v2i span = p.spans[b];
+  span[0] = min(max(span[0], 0), p.walkers - 1);
+  const int n = min(span[1], p.walkers - span[0]);
   const int64_t row = (int64_t)b * p.M + r;
   u16* const out = (u16*)p.out + row * kLatent + 4 * lane;
-  if (mla_len(p, b) == 0) {
+  if (n <= 0) {
     if (w == 0) {
       *(v2i*)out = v2i{0, 0};
       *(v2i*)(out + 256) = v2i{0, 0};
@@ -523,7 +531,6 @@ __global__ __launch_bounds__(256) void mla_join_kernel(const MlaDecodeArgs p) {
     }
     return;
   }
-  const int n = span[1];
   if (n == 1) return;
   const int beginning = mla_slot(p, span[0], b, true);
   auto slot_of = [&](int i) -> int64_t { return i ? span[0] + i : beginning; };

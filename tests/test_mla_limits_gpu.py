@@ -66,3 +66,26 @@ def test_decode_stays_in_its_workspace(dev, n, H, lens, width):
     want, want_lse, tol, lse_tol = R.decode(q, qp, cache, table, lens, SCALE, None)
     R.close(out, want, tol, "out")
     R.close(lse, want_lse, lse_tol, "lse")
+
+
+@pytest.mark.parametrize("n,H,B,width", [(1, 16, 5, 4), (1, 128, 300, 3), (2, 40, 1100, 2)])
+def test_decode_cuts_by_one_reading_of_the_lengths(dev, n, H, B, width):
+    """Calls one behind the other in one workspace, each with other lengths: what one has left there - which runs hold a request, partials - never
+    reaches the next, requests that have lost all their tokens among them."""
+    from sglang_amd._lib import BF16 as CODE, check, lib, stream_ptr
+
+    g = _gen(B)
+    most = [64 * width] * B
+    cache, table, pt, _ = _filled(g, most, 64, BF16, False, width=width)
+    q, qp = _queries(g, B, n, H, BF16)
+    need = lib.fp8k_mla_decode_workspace_bytes(B, n, H, 64 * width)
+    ws = torch.full((need,), 255, dtype=torch.uint8, device="cuda")
+    out, lse = torch.empty((B, n, H, 512), dtype=BF16, device="cuda"), torch.empty((B, n, H), device="cuda")
+    for turn, lens in enumerate((most, [0] * B, [(29 * i) % (64 * width + 1) if i % 3 else 0 for i in range(B)], [0] * (B - 1) + [64 * width], [1] + [0] * (B - 1))):
+        sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        check(lib.fp8k_mla_decode(q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), qp.data_ptr(), qp.stride(0), qp.stride(1), qp.stride(2), cache.data_ptr(),
+                                  pt.data_ptr(), pt.stride(0), width, sl.data_ptr(), None, out.data_ptr(), lse.data_ptr(), B, n, H, cache.shape[0], 64, SCALE,
+                                  CODE, 0, ws.data_ptr(), need, stream_ptr(q.device)))
+        want, want_lse, tol, lse_tol = R.decode(q, qp, cache, table, lens, SCALE, None)
+        R.close(out, want, tol, "out %d" % turn)
+        R.close(lse, want_lse, lse_tol, "lse %d" % turn)
