@@ -70,16 +70,16 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) { return (uint32_
 // for vmcnt himself.  The instruction's offset counts on both sides, hence the subtraction.  Non-temporal, for rows that are read once.
 template <int OFFSET = 0>
 __device__ __forceinline__ void load16_to_lds(const void* p, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2 nt" ::"v"(p), "s"(to - OFFSET), "n"(OFFSET) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%2 nt" ::"v"(p), "s"(to - OFFSET), "n"(OFFSET) : "m0", "memory");
 }
 // the same from base + every lane's own offset, cached; base is the wave's.  (Five wait states in front: a scalar register that a vector instruction
 // has just written - the compiler's own spills - is not ready for a vector load before.)
 __device__ __forceinline__ void load16_to_lds(const void* base, uint32_t offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to) : "m0", "memory");
 }
 // 4 bytes likewise, to `to` + 4 * lane
 __device__ __forceinline__ void load4_to_lds(const void* p, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(p), "s"(to) : "m0", "memory");
 }
 // FIRST .. LAST - 1 of a row of such loads: the lanes' addresses p + STEP * j to `to` + TO_STEP * j + 16 * lane
 template <int STEP, int TO_STEP, int FIRST, int LAST>

@@ -14,3 +14,19 @@ def test_decode_workspace_goes_by_runs(n, H, max_len):
         assert size(B) <= min(512, 256 + B) * n * H * (512 + 1) * 4 + 8 * B + 3 * 256
     if 65535 * (max_len // 64 + 1) < 1 << 30:
         assert size(65535) - size(4096) <= 8 * (65535 - 4096) + 256
+
+
+def test_assembly_names_the_registers_that_it_sets():
+    """An asm statement that sets m0 says so, or the compiler may keep something of its own there across it."""
+    import pathlib
+    import re
+
+    import sglang_amd
+
+    found = 0
+    for path in (pathlib.Path(sglang_amd.__file__).parent / "csrc").glob("*.h*"):
+        for text in re.findall(r"\basm\b[^;]*;", path.read_text()):
+            if re.search(r"s_mov_b32 m0", text):
+                found += 1
+                assert '"m0"' in text, (path.name, text)
+    assert found == 3
