@@ -590,7 +590,7 @@ int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, cons
 
 /*
  * Two attentions over disjoint keys as one: out = (exp(lse_a) out_a + exp(lse_b) out_b) / (exp(lse_a) + exp(lse_b)), lse = log(exp(lse_a) + exp(lse_b)),
- * over rows x D numbers of dtype (F16/BF16/F32), D a multiple of 8, all contiguous; out may be out_a or out_b, lse is memory of its own.  A part
+ * over rows x D numbers of dtype (F16/BF16/F32), D a multiple of 8, all contiguous; out is out_a, out_b or memory of its own, lse memory of its own.  A part
  * with an lse of -inf counts nothing, whatever its row holds; two of them give 0 and -inf.
  */
 int fp8k_merge_attention_states(const void* out_a, const float* lse_a, const void* out_b, const float* lse_b, void* out, float* lse,

@@ -10,6 +10,12 @@ namespace {
 
 bool is_half_type(int dtype) { return dtype == FP8K_BF16 || dtype == FP8K_F16; }
 
+// whether two pieces of memory share a byte
+bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
+  const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
+  return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
+
 // ---------------------------------------------------------------------------------------------- cache
 struct MlaWriteArgs {
   const u16 *latent, *q_pe;
@@ -534,8 +540,16 @@ extern "C" int fp8k_merge_attention_states(const void* out_a, const float* lse_a
   FP8K_REQUIRE(aligned(out_a, 16) && aligned(out_b, 16) && aligned(out, 16), "merge states: operands must be 16-byte aligned");
   const int64_t blocks = (rows * (D / 8) + 255) / 256;
   FP8K_REQUIRE(rows < (1ll << 40) && blocks < (1ll << 31), "merge states: too large");
-  // a row's numbers may be several workgroups', and each reads both logarithms
-  FP8K_REQUIRE(lse != lse_a && lse != lse_b, "merge states: lse must be memory of its own");
+  // a row's numbers may be several workgroups', and each reads both logarithms; of the rows a thread reads what it overwrites, and nothing else
+  const int64_t bytes = rows * D * (dtype == FP8K_F32 ? 4 : 2), lse_bytes = rows * 4;
+  const void* const parts[2] = {out_a, out_b};
+  const void* const logs[2] = {lse_a, lse_b};
+  for (int i = 0; i < 2; ++i) {
+    FP8K_REQUIRE(!overlap(lse, lse_bytes, logs[i], lse_bytes) && !overlap(lse, lse_bytes, parts[i], bytes), "merge states: lse must be memory of its own");
+    FP8K_REQUIRE((out == parts[i] || !overlap(out, bytes, parts[i], bytes)) && !overlap(out, bytes, logs[i], lse_bytes),
+                 "merge states: out must be out_a, out_b or memory of its own");
+  }
+  FP8K_REQUIRE(!overlap(out, bytes, lse, lse_bytes), "merge states: lse must be memory of its own");
   const dim3 grid((unsigned)blocks);
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == FP8K_BF16) mla_merge_kernel<FP8K_BF16><<<grid, 256, 0, st>>>(out_a, lse_a, out_b, lse_b, out, lse, rows, (int)(D / 8));

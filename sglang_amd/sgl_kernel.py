@@ -1323,7 +1323,8 @@ def mla_prefill_attention(q: torch.Tensor, k_nope: torch.Tensor, k_pe: torch.Ten
 
 def merge_attention_states(out_a: torch.Tensor, lse_a: torch.Tensor, out_b: torch.Tensor, lse_b: torch.Tensor, out: torch.Tensor,
                            lse: torch.Tensor) -> None:
-    """Two attentions over disjoint keys as one (include/fp8k.h: fp8k_merge_attention_states)."""
+    """Two attentions over disjoint keys as one (include/fp8k.h: fp8k_merge_attention_states).  out is out_a, out_b or memory of its own, lse memory
+    of its own."""
     _same_device(out_a, lse_a, out_b, lse_b, out, lse)
     if out_a.dtype not in _HALVES + (torch.float32,) or out_a.dim() < 1:
         raise RuntimeError("out_a must be float32, float16 or bfloat16")

@@ -89,3 +89,23 @@ def test_decode_cuts_by_one_reading_of_the_lengths(dev, n, H, B, width):
         want, want_lse, tol, lse_tol = R.decode(q, qp, cache, table, lens, SCALE, None)
         R.close(out, want, tol, "out %d" % turn)
         R.close(lse, want_lse, lse_tol, "lse %d" % turn)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, torch.float32])
+@pytest.mark.parametrize("rows,D", [(5, 8), (37, 192), (3, 8192)])
+def test_merge_in_place(dev, rows, D, dtype):
+    """The result may take the place of either operand, rows of several workgroups among them."""
+    from sglang_amd import mla, sgl_kernel
+
+    g = _gen(D)
+    a, b = (torch.randn((rows, D), generator=g, device="cuda").to(dtype) for _ in range(2))
+    la, lb = (torch.randn((rows,), generator=g, device="cuda") * 3 for _ in range(2))
+    la[0] = lb[1] = float("-inf")
+    want, want_lse = mla.merge_attention_states(a, la, b, lb)
+    for which in (0, 1):
+        x, y, lse = a.clone(), b.clone(), torch.empty_like(la)
+        sgl_kernel.merge_attention_states(x, la, y, lb, (x, y)[which], lse)
+        assert torch.equal((x, y)[which], want) and torch.equal((y, x)[which], (b, a)[which]) and torch.equal(lse, want_lse)
+    both = torch.cat((a, a))
+    with pytest.raises(RuntimeError, match="out must be"):
+        sgl_kernel.merge_attention_states(both[:rows], la, b, lb, both[1:rows + 1], torch.empty_like(la))
