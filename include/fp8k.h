@@ -540,7 +540,8 @@ int fp8k_mxfp4_experts(const void* x, const void* w1, const void* w2, const void
  * cache; a slot that is none of them (-1: a padded batch) is skipped.  Slots are distinct.  norm_weight (NULL: no norm; of dtype or F32): the latent
  * becomes x / sqrt(mean(x^2) + eps) * weight.  cos_sin (NULL: no rotation), float32 [max_pos, 64], 32 cosines then 32 sines, row
  * positions[t] (int32 or int64, held within the table): the position part is rotated, pairs of neighbours, or (neox) of numbers 32 apart.
- * q_pe (NULL: none) [T, H, 64]: rotated likewise into q_out, which may be q_pe itself.  Float32 throughout, one rounding; e4m3 by
+ * q_pe (NULL: none) [T, H, 64]: rotated likewise into q_out, which is q_pe itself (its strides too) or shares none of its numbers (places that lie
+ * between q_pe's with other strides, and with neither a common divisor nor a period that tells them apart, are refused).  Float32 throughout, one rounding; e4m3 by
  * x / scale, to nearest, at most 448 (NaN stays NaN).
  */
 int fp8k_mla_write_cache(const void* latent, int64_t ld_latent, void* cache, const void* slots, int slots_are_64bit,

@@ -267,6 +267,46 @@ __global__ __launch_bounds__(256) void mla_merge_kernel(const void* a, const flo
   } else store8<DT>((u16*)out + 8 * i, u);
 }
 
+// T x H rows of kRope numbers, `t` and `h` apart (0 where there is one alone).
+struct QueryRows {
+  int64_t t, h;
+};
+// Whether rows o, at `delta` numbers from rows q, share no number with them; o's lie apart from each other.  Exact where the strides are q's; else what the ends,
+// the strides' common divisor, or a period that the outer rows of both have tell: that finds slices of one buffer apart, and takes for a collision what it cannot tell.
+bool queries_apart(int64_t delta, QueryRows q, QueryRows o, int64_t T, int64_t H) {
+  const auto extent = [&](QueryRows r) { return (T - 1) * r.t + (H - 1) * r.h + kRope; };
+  if (delta >= extent(q) || -delta >= extent(o)) return true;
+  const auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b != 0 && (a < 0) != (b < 0)); };
+  const auto mod = [&](int64_t a, int64_t b) { return a - floor_div(a, b) * b; };
+  if (q.t == o.t && q.h == o.h) {
+    // Rows of differences a inner + b outer, |a| < n, |b| < m.  The outer stride is more than the inner rows' extent, so that only its two
+    // multiples around delta come near, and then the inner one's two around the rest.
+    const bool h_inner = H > 1 && (T == 1 || q.h < q.t);
+    const int64_t inner = h_inner ? q.h : q.t, n = h_inner ? H : T, outer = h_inner ? q.t : q.h, m = h_inner ? T : H;
+    for (int64_t i = 0; i < 2; ++i) {
+      const int64_t b = m == 1 ? 0 : std::min(std::max(floor_div(delta, outer) + i, 1 - m), m - 1), rest = delta - b * outer;
+      for (int64_t j = 0; j < 2; ++j) {
+        const int64_t a = n == 1 ? 0 : std::min(std::max(floor_div(rest, inner) + j, 1 - n), n - 1), gap = rest - a * inner;
+        if (gap > -kRope && gap < kRope) return false;
+      }
+    }
+    return true;
+  }
+  int64_t common = 0;
+  for (int64_t x : {q.t, q.h, o.t, o.h})
+    while (x) {
+      const int64_t y = common % x;
+      common = x;
+      x = y;
+    }
+  if (common && mod(delta, common) >= kRope && mod(delta, common) <= common - kRope) return true;
+  const auto in_period = [&](int64_t period, int64_t q_inner, int64_t o_inner, int64_t n) {
+    const int64_t q_size = (n - 1) * q_inner + kRope, o_size = (n - 1) * o_inner + kRope;
+    return mod(delta, period) >= q_size && mod(delta, period) + o_size <= period;
+  };
+  return (q.t == o.t && q.t > 0 && in_period(q.t, q.h, o.h, H)) || (q.h == o.h && q.h > 0 && in_period(q.h, q.t, o.t, T));
+}
+
 int64_t up_to(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
 
 // How a decode call is cut: rows of a workgroup (16, 32, 64 or 128), and runs of tiles.  `walkers` workgroups to a block of rows, one
@@ -337,8 +377,6 @@ extern "C" int fp8k_mla_write_cache(const void* latent, int64_t ld_latent, void*
   FP8K_REQUIRE(latent && (cache || num_slots == 0) && slots, "mla write: null pointer");
   FP8K_REQUIRE(aligned(latent, 16) && aligned(cache, 16) && ld_latent % 8 == 0 && ld_latent >= kLatentRow, "mla write: rows must be 16-byte aligned");
   FP8K_REQUIRE(aligned(slots, slots_are_64bit ? 8 : 4), "mla write: misaligned slots");
-  FP8K_REQUIRE(!norm_weight || ((norm_weight_dtype == dtype || norm_weight_dtype == FP8K_F32) && aligned(norm_weight, 16)),
-               "mla write: the norm's weight must be of the rows' type or float32, 16-byte aligned");
   FP8K_REQUIRE(!cos_sin || (positions && max_pos > 0 && aligned(cos_sin, 16) && aligned(positions, positions_are_64bit ? 8 : 4)),
                "mla write: the rotation needs positions and a 16-byte aligned table");
   FP8K_REQUIRE(!q_pe || (cos_sin && q_out && H > 0), "mla write: queries need a table of cosines and sines, and a place");
@@ -350,7 +388,13 @@ extern "C" int fp8k_mla_write_cache(const void* latent, int64_t ld_latent, void*
       return (n == 1 || inner >= kRope) && (m == 1 || outer >= (n - 1) * inner + kRope);
     };
     FP8K_REQUIRE(apart(o_stride_h, H, o_stride_t, T) || apart(o_stride_t, T, o_stride_h, H), "mla write: the rotated queries' places overlap each other");
+    const QueryRows q{T > 1 ? q_stride_t : 0, H > 1 ? q_stride_h : 0}, o{T > 1 ? o_stride_t : 0, H > 1 ? o_stride_h : 0};
+    const int64_t delta = ((intptr_t)q_out - (intptr_t)q_pe) / 2;
+    FP8K_REQUIRE((delta == 0 && q.t == o.t && q.h == o.h) || queries_apart(delta, q, o, T, H),
+                 "mla write: the rotated queries' places overlap queries other than their own");
   }
+  FP8K_REQUIRE(!norm_weight || ((norm_weight_dtype == dtype || norm_weight_dtype == FP8K_F32) && aligned(norm_weight, 16)),
+               "mla write: the norm's weight must be of the rows' type or float32, 16-byte aligned");
   MlaWriteArgs p{};
   p.latent = (const u16*)latent; p.q_pe = (const u16*)q_pe; p.cache = cache; p.q_out = (u16*)q_out;
   p.slots = slots; p.norm_weight = norm_weight; p.positions = positions; p.cos_sin = cos_sin; p.scale = scale;

@@ -39,7 +39,7 @@ def mla_write_cache(latent: torch.Tensor, cache: torch.Tensor, slots: torch.Tens
     norm_weight [512] (of the rows' type or float32): the latent becomes x / sqrt(mean(x^2) + eps) * norm_weight.
     cos_sin float32 [P, 64] (32 cosines, 32 sines of a position) and positions [T] (int32 or int64; held within 0 .. P - 1): the position
     part is rotated, by pairs of neighbours, or with neox of numbers that lie 32 apart.
-    q_pe [T, heads, 64]: rotated likewise; returned as a fresh tensor, or in q_out, which may be q_pe itself (but must not overlap it otherwise).
+    q_pe [T, heads, 64]: rotated likewise; returned as a fresh tensor, or in q_out, which may be q_pe itself; one that overlaps it otherwise is refused.
 
     A float8_e4m3fn cache takes x / scale, to nearest, ties to even, values beyond 448 as 448; NaN stays NaN."""
     if not torch.compiler.is_compiling():

@@ -1177,7 +1177,7 @@ def _ints(t: torch.Tensor, shape: tuple, what: str, types=(torch.int32,)) -> Non
 def mla_write_cache(latent: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor, norm_weight: Optional[torch.Tensor], eps: float,
                     cos_sin: Optional[torch.Tensor], positions: Optional[torch.Tensor], neox: bool, q_pe: Optional[torch.Tensor],
                     q_out: Optional[torch.Tensor], scale: Optional[torch.Tensor]) -> None:
-    """Norm, rotation and store of tokens' rows (include/fp8k.h: fp8k_mla_write_cache).  q_out may be q_pe."""
+    """Norm, rotation and store of tokens' rows (include/fp8k.h: fp8k_mla_write_cache).  q_out is q_pe, or shares no memory with it."""
     _same_device(latent, cache, slots, norm_weight, cos_sin, positions, q_pe, q_out, scale)
     if latent.dtype not in _HALVES or latent.dim() != 2 or latent.shape[1] != MLA_ROW or latent.stride(1) != 1:
         raise RuntimeError("latent must be float16 or bfloat16 [tokens, 576] with contiguous rows")

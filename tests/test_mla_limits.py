@@ -69,3 +69,53 @@ def test_joined_rows_and_logarithms_are_memory_of_their_own():
     _refused(merge(la=out + 1144), "out must be")
     _refused(merge(lb=out - 8), "out must be")
     del keep
+
+
+def _write_with_bad_weight(q, qt, qh, out, ot, oh, T, H):
+    """What the writer says of these queries and their places.  Nothing is ever launched: the norm's weight is of a wrong type, and looked at last."""
+    from sglang_amd import _lib
+
+    p = 1 << 20
+    rc = _lib.lib.fp8k_mla_write_cache(p, 576, p, p, 1, p, _lib.F16, 1e-6, p, 10, p, 1, 0, q, qt, qh, out, ot, oh, None, T, H, 100, _lib.BF16, 0, None)
+    text = _lib.lib.fp8k_last_error().decode()
+    assert rc != 0 and ("weight" in text or "overlap" in text), text
+    return "overlap" in text
+
+
+def test_rotated_queries_share_no_memory_with_others():
+    """Every place among some thousand random ones against the numbers that it holds: what overlaps is refused, the queries' own place and places with their
+    strides are taken whenever they may be."""
+    import random
+
+    rng = random.Random(3)
+    base = 1 << 30
+    seen = {"overlap": 0, "apart": 0, "in place": 0, "other strides": 0}
+    for _ in range(4000):
+        T, H = rng.choice([(1, 1), (1, 5), (4, 1), (3, 4), (2, 7), (6, 3)])
+        nest = lambda: rng.choice([(64 * H, 64), (192 * H, 192), (192 * H + 64, 192), (64, 64 * T), (72, 72 * T), (192 * H + 576, 192), (64 * H + 8, 64)])  # noqa: E731
+        (qt, qh), (ot, oh) = nest(), nest()
+        if rng.random() < 0.6:
+            ot, oh = qt, qh
+        if rng.random() < 0.1:
+            qh = 0
+        delta = rng.choice([0, 0, 64, -64, 128, 8 * rng.randint(-300, 300), rng.choice([1, -1]) * (ot * rng.randint(0, 3) + oh * rng.randint(0, 3)), qt * rng.randint(-2, 2) + 64])
+        rows = lambda st, sh, at: {at + t * st + h * sh + i for t in range(T) for h in range(H) for i in range(64)}  # noqa: E731
+        own = delta == 0 and (T == 1 or qt == ot) and (H == 1 or qh == oh)
+        if len(rows(ot, oh, 0)) < T * H * 64:
+            continue  # places that overlap each other are another refusal
+        refused = _write_with_bad_weight(base, qt, qh, base + 2 * delta, ot, oh, T, H)
+        collide = bool(rows(qt, qh, 0) & rows(ot, oh, delta)) and not own
+        what = (T, H, qt, qh, ot, oh, delta)
+        if collide:
+            assert refused, what
+        elif (T == 1 or qt == ot) and (H == 1 or qh == oh):
+            assert not refused, what
+        seen["overlap" if collide else "in place" if own else "apart" if (qt, qh) == (ot, oh) else "other strides"] += 1
+    assert min(seen.values()) > 50, seen
+    # slices of one buffer: heads' 64 of 192, tokens of 8 heads and 576 more; the result behind the heads, or between them
+    assert not _write_with_bad_weight(base + 256, 8 * 192 + 576, 192, base + 2 * 8 * 192, 8 * 192 + 576, 64, 30, 8)
+    assert not _write_with_bad_weight(base + 256, 8 * 192, 192, base, 8 * 192, 192, 30, 8)
+    assert not _write_with_bad_weight(base, 8 * 192, 192, base + 2 * 64, 64 * 192, 192, 30, 8)  # other strides, a common divisor
+    assert _write_with_bad_weight(base, 8 * 192, 192, base + 2 * 192, 8 * 192, 192, 30, 8)  # one head on
+    assert _write_with_bad_weight(base, 8 * 192, 192, base + 2 * 8 * 192, 8 * 192, 192, 30, 8)  # one token on
+    assert _write_with_bad_weight(base, 8 * 64, 64, base + 16, 8 * 64, 64, 1, 1)

@@ -109,3 +109,32 @@ def test_merge_in_place(dev, rows, D, dtype):
     both = torch.cat((a, a))
     with pytest.raises(RuntimeError, match="out must be"):
         sgl_kernel.merge_attention_states(both[:rows], la, b, lb, both[1:rows + 1], torch.empty_like(la))
+
+
+@pytest.mark.parametrize("T,H", [(1, 1), (5, 16), (30, 8), (1, 128)])
+def test_rotated_queries_in_slices_of_one_buffer(dev, T, H):
+    """Queries and their place as slices of one buffer: the part of a head in front of its queries, a block behind a token's heads, another order of rows."""
+    from sglang_amd import mla
+    from tests.test_mla_attention_gpu import _table_of_angles
+
+    g = _gen(T * H)
+    latent = torch.randn((T, 576), generator=g, device="cuda").to(BF16)
+    cache, slots = torch.zeros((2, 64, 576), dtype=BF16, device="cuda"), torch.arange(T, device="cuda")
+    rest = dict(cos_sin=_table_of_angles(64), positions=torch.arange(T, device="cuda"))
+    width = H * 192 + H * 64 + 576
+    for place in (lambda b: b[:, :H * 192].view(T, H, 192)[..., :64], lambda b: b[:, H * 192:H * 256].view(T, H, 64)):
+        buffer = torch.randn((T, width), generator=g, device="cuda").to(BF16)
+        q, out = buffer[:, :H * 192].view(T, H, 192)[..., 128:], place(buffer)
+        before, kept = buffer.clone(), q.clone()
+        want = mla.mla_write_cache(latent, cache, slots, q_pe=kept, **rest)
+        assert mla.mla_write_cache(latent, cache, slots, q_pe=q, q_out=out, **rest) is out
+        assert torch.equal(out, want) and torch.equal(q, kept)
+        place(before).copy_(want)
+        assert torch.equal(buffer, before)
+    if T > 1:
+        buffer = torch.randn((T * H + H, 64), generator=g, device="cuda").to(BF16)
+        with pytest.raises(RuntimeError, match="overlap"):
+            mla.mla_write_cache(latent, cache, slots, q_pe=buffer[:T * H].view(T, H, 64), q_out=buffer[H:].view(T, H, 64), **rest)
+        with pytest.raises(RuntimeError, match="overlap"):
+            torch.ops.fp8k.mla_write_cache(latent, cache, slots, None, 1e-6, rest["cos_sin"], rest["positions"], False, buffer[:T * H].view(T, H, 64),
+                                           buffer[H:].view(T, H, 64), None)
