@@ -553,6 +553,7 @@ int fp8k_mla_write_cache(const void* latent, int64_t ld_latent, void* cache, con
 /*
  * Row cu_seqlens[b] + i of out (row stride ld_out) becomes token starts[b] + i (starts NULL: i) of request b, for the rows up to
  * cu_seqlens[b + 1] (int32 [B + 1], not decreasing) and num_tokens, which out has; rows of no request stay as they are.  Tokens are held within the page table.
+ * out shares no memory with the cache.
  */
 int fp8k_mla_gather_cache(const void* cache, const int32_t* page_table, int64_t table_stride, int64_t table_width,
                           const int32_t* cu_seqlens, const int32_t* starts, const float* scale, void* out, int64_t ld_out, int64_t B,
@@ -564,7 +565,7 @@ int fp8k_mla_gather_cache(const void* cache, const int32_t* page_table, int64_t 
  *   s[r] = sm_scale * (q_nope[b, i, h] . row[:512] + q_pe[b, i, h] . row[512:]),  r < seq_lens[b] - (n - 1 - i)
  *   out[b, i, h] = softmax(s) . row[:512],  lse[b, i, h] = log(sum exp(s))   (lse: NULL or float32)
  * Float32 sums; the exponentials are rounded to dtype for their product with the rows.  A query that sees nothing gets 0 and -inf.
- * out [B, n, H, 512], lse [B, n, H] contiguous.  sm_scale > 0; B <= 65535, n * H <= 65536.  Workspace: 256-byte aligned,
+ * out [B, n, H, 512], lse [B, n, H] contiguous, no part of an operand (out may be contiguous q_nope itself).  sm_scale > 0; B <= 65535, n * H <= 65536.  Workspace: 256-byte aligned,
  * fp8k_mla_decode_workspace_bytes of it (max_len: table_width * page_size), not initialised.
  */
 int64_t fp8k_mla_decode_workspace_bytes(int64_t B, int64_t n, int64_t H, int64_t max_len);
@@ -577,7 +578,7 @@ int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t qn_stride_n
 /*
  * Expanded attention over ragged sequences: sequence b has queries cu_seqlens_q[b] .. [b + 1] of q [Tq, H, 192] and keys cu_seqlens_k[b] .. [b + 1]
  * of k_nope [Tk, H, 128], k_pe [Tk, 64] (all heads') and v [Tk, H, 128] (int32 [B + 1], not decreasing).  Query i of its lq sees (causal) keys j <= i + lk - lq, else all.
- * out [Tq, H, 128] and lse (NULL or float32 [Tq, H]) contiguous; a query that sees nothing gets 0 and -inf, queries of no sequence
+ * out [Tq, H, 128] and lse (NULL or float32 [Tq, H]) contiguous, no part of an operand; a query that sees nothing gets 0 and -inf, queries of no sequence
  * stay as they are.  max_seqlen_q: at least the longest lq.  Keys that a sequence has must be finite; whatever lies outside it may be anything.
  * Workspace: 256-byte aligned, fp8k_mla_prefill_workspace_bytes of it (0 possible: few blocks of queries with long keys are split over the
  * keys, and joined in float32), not initialised.

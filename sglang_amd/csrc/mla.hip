@@ -1,6 +1,8 @@
 // Latent attention: C entry points, the cache's writer and reader, and the join of two attentions.  The attention kernels are in
 // mla_decode.h and mla_prefill.h.
 #include <algorithm>
+#include <initializer_list>
+#include <utility>
 
 #include "mla_decode.h"
 #include "mla_prefill.h"
@@ -13,7 +15,27 @@ bool is_half_type(int dtype) { return dtype == FP8K_BF16 || dtype == FP8K_F16; }
 // whether two pieces of memory share a byte
 bool overlap(const void* a, int64_t a_bytes, const void* b, int64_t b_bytes) {
   const uintptr_t x = (uintptr_t)a, y = (uintptr_t)b;
-  return x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+  return a_bytes > 0 && b_bytes > 0 && x < y + (uintptr_t)b_bytes && y < x + (uintptr_t)a_bytes;
+}
+// Memory from its first byte to its last.
+struct Piece {
+  const void* at;
+  int64_t bytes;
+};
+// rows of `last` 16-bit numbers, their sizes and strides from the outer dimension in
+Piece rows_of(const void* at, std::initializer_list<std::pair<int64_t, int64_t>> dims, int64_t last) {
+  int64_t n = last;
+  for (const auto& d : dims) {
+    if (d.first <= 0) return {at, 0};
+    n += (d.first - 1) * d.second;
+  }
+  return {at, 2 * n};
+}
+// An attention's results are written while other workgroups still read its operands, and its two results by different threads.
+bool results_apart(Piece out, Piece lse, std::initializer_list<Piece> operands) {
+  for (const Piece& x : operands)
+    if (x.at && (overlap(out.at, out.bytes, x.at, x.bytes) || (lse.at && overlap(lse.at, lse.bytes, x.at, x.bytes)))) return false;
+  return !lse.at || !overlap(out.at, out.bytes, lse.at, lse.bytes);
 }
 
 // ---------------------------------------------------------------------------------------------- cache
@@ -428,6 +450,8 @@ extern "C" int fp8k_mla_gather_cache(const void* cache, const int32_t* page_tabl
                "mla gather: bad sizes of the cache or the page table");
   FP8K_REQUIRE(cache && page_table && cu_seqlens && out, "mla gather: null pointer");
   FP8K_REQUIRE(aligned(cache, 16) && aligned(out, 16) && ld_out % 8 == 0 && ld_out >= kLatentRow, "mla gather: rows must be 16-byte aligned");
+  const Piece rows = rows_of(out, {{num_tokens, ld_out}}, kLatentRow);
+  FP8K_REQUIRE(!overlap(rows.at, rows.bytes, cache, pages * page_size * kLatentRow * (cache_is_fp8 ? 1 : 2)), "mla gather: out overlaps the cache");
   MlaGatherArgs p{};
   p.cache = (const uint8_t*)cache; p.table = page_table; p.cu = cu_seqlens; p.starts = starts; p.scale = scale; p.out = (u16*)out;
   p.table_stride = table_stride; p.ld_out = ld_out;
@@ -474,6 +498,13 @@ extern "C" int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t 
   if (!workspace || workspace_bytes < need || !aligned(workspace, 256))
     return fail(FP8K_ERR_WORKSPACE, "mla decode: workspace of %lld bytes needed, 256-byte aligned", (long long)need);
   const int64_t M = n * H;
+  const Piece out_rows = rows_of(out, {}, B * M * kLatent), lse_rows{lse, B * M * 4};
+  // In the queries' own place: a workgroup has read the rows of a request that it writes, and nobody else reads them.
+  const bool in_place = out == q_nope && (H == 1 || qn_stride_h == kLatent) && (n == 1 || qn_stride_n == H * kLatent) && (B == 1 || qn_stride_b == M * kLatent);
+  const Piece queries = rows_of(q_nope, {{B, qn_stride_b}, {n, qn_stride_n}, {H, qn_stride_h}}, kLatent);
+  FP8K_REQUIRE(results_apart(out_rows, lse_rows, {rows_of(q_pe, {{B, qp_stride_b}, {n, qp_stride_n}, {H, qp_stride_h}}, kRope),
+                                                  Piece{cache, pages * page_size * kLatentRow * (cache_is_fp8 ? 1 : 2)}, in_place ? Piece{} : queries}),
+               "mla decode: out or lse overlaps an operand");
   const DecodePlan d = decode_plan(B, M, max_len);
   const int64_t slots = mla_slots(B, d.walkers);
   MlaDecodeArgs p{};
@@ -551,6 +582,10 @@ extern "C" int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_str
   const int64_t need = fp8k_mla_prefill_workspace_bytes(B, H, Tq, Tk, max_seqlen_q);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
     return fail(FP8K_ERR_WORKSPACE, "mla prefill: workspace of %lld bytes needed, 256-byte aligned", (long long)need);
+  FP8K_REQUIRE(results_apart(rows_of(out, {}, Tq * H * kPreValue), Piece{lse, Tq * H * 4},
+                             {rows_of(q, {{Tq, q_stride_t}, {H, q_stride_h}}, kPreNope + kRope), rows_of(k_nope, {{Tk, kn_stride_t}, {H, kn_stride_h}}, kPreNope),
+                              rows_of(k_pe, {{Tk, kp_stride_t}}, kRope), rows_of(v, {{Tk, v_stride_t}, {H, v_stride_h}}, kPreValue)}),
+               "mla prefill: out or lse overlaps an operand");
   p.part = (float*)workspace;
   p.part_lse = (float*)((uint8_t*)workspace + up_to(p.splits * Tq * H * kPreValue * 4, 256));
   const dim3 grid((unsigned)(lines * d.blocks), (unsigned)p.splits), join_grid((unsigned)(lines * d.blocks), 16);

@@ -57,7 +57,7 @@ def mla_gather_cache(cache: torch.Tensor, page_table: torch.Tensor, cu_seqlens: 
                      out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Cached rows one after the other, [num_tokens, 576] of dtype (a 16-bit cache's own): row cu_seqlens[b] + i is token starts[b] + i (None: i) of
     request b.  cu_seqlens int32 [B + 1] does not decrease; starts int32 [B].  Rows of no request - behind cu_seqlens[B] - are not written:
-    those of `out` stay as they were.  Tokens beyond a request's row of the table are read as its last one."""
+    those of `out`, which is no part of the cache, stay as they were.  Tokens beyond a request's row of the table are read as its last one."""
     if not torch.compiler.is_compiling():
         got = _host.mla_gather(cache, page_table, cu_seqlens, num_tokens, starts, dtype, scale, out)
         if got is not None:
@@ -78,8 +78,8 @@ def mla_decode_attention(q_nope: torch.Tensor, q_pe: torch.Tensor, cache: torch.
 
       s[r] = sm_scale * (q_nope . row[r][:512] + q_pe . row[r][512:]),   result = softmax(s) . rows[:, :512]
 
-    of q_nope's type and shape; with return_lse also log(sum exp(s)), float32.  The last query of a request sees all its tokens, the one
-    before it all but the last, and so on.  A query that sees nothing gets 0 and -inf.  The absorbed queries may be a transposed view.
+    of q_nope's type and shape; with return_lse also log(sum exp(s)), float32.  out may be q_nope itself, else no part of an operand.  The last
+    query of a request sees all its tokens, the one before it all but the last, and so on.  A query that sees nothing gets 0 and -inf.  The absorbed queries may be a transposed view.
 
     The exponentials are rounded to 16 bits for their product with the rows (their sum is not).  Lengths are held within the page table's width, and that
     bound decides how a batch is cut: pass the columns that the longest request needs, page_table[:, :n] (one request of 4000 tokens, 128 heads, takes
@@ -109,7 +109,7 @@ def mla_prefill_attention(q: torch.Tensor, k_nope: torch.Tensor, k_pe: torch.Ten
     most queries that one has (more are left out).
 
     causal: of lq queries and lk keys, query i sees the keys j <= i + lk - lq (the queries are the last of the keys); else all.  Returns [Tq, heads, 128]
-    of q's type, with return_lse also log(sum exp(s)), float32 [Tq, heads].  A query that sees nothing gets 0 and -inf; those of no sequence are not
+    of q's type, with return_lse also log(sum exp(s)), float32 [Tq, heads]; out is no part of an operand.  A query that sees nothing gets 0 and -inf; those of no sequence are not
     written.  What lies between and behind the sequences' keys may hold anything; a sequence's own keys and values are finite.
 
     The exponentials are rounded to 16 bits for their product with the values (their sum is not)."""

@@ -119,3 +119,49 @@ def test_rotated_queries_share_no_memory_with_others():
     assert _write_with_bad_weight(base, 8 * 192, 192, base + 2 * 192, 8 * 192, 192, 30, 8)  # one head on
     assert _write_with_bad_weight(base, 8 * 192, 192, base + 2 * 8 * 192, 8 * 192, 192, 30, 8)  # one token on
     assert _write_with_bad_weight(base, 8 * 64, 64, base + 16, 8 * 64, 64, 1, 1)
+
+
+def test_results_of_attentions_are_no_part_of_their_operands():
+    """Addresses of an imagined layout, each refused before anything is launched: results that begin or end inside an operand or each other."""
+    from sglang_amd import _lib
+
+    lib, M = _lib.lib, 1 << 20
+    B, n, H, pages, page = 3, 2, 16, 4, 64
+    at = {k: (i + 1) * (M << 4) for i, k in enumerate(("q", "qp", "cache", "table", "lens", "out", "lse", "ws", "k", "kp", "v", "cu"))}
+    size = dict(q=B * n * H * 1024, qp=B * n * H * 128, cache=pages * page * 1152, out=B * n * H * 1024, lse=B * n * H * 4)
+
+    def decode(out=at["out"], lse=at["lse"], heads_first=False):
+        strides = (n * 512, 512, B * n * 512) if heads_first else (n * H * 512, H * 512, 512)
+        return lib.fp8k_mla_decode(at["q"], *strides, at["qp"], n * H * 64, H * 64, 64, at["cache"], at["table"], 4, 4, at["lens"], None, out, lse, B, n, H, pages, page,
+                                   0.1, _lib.BF16, 0, at["ws"], 1 << 40, None)
+
+    for k in ("q", "qp", "cache"):
+        _refused(decode(out=at[k] + size[k] - 16), "overlaps")
+        _refused(decode(out=at[k] - size["out"] + 16), "overlaps")
+        _refused(decode(lse=at[k] + size[k] - 4), "overlaps")
+        _refused(decode(lse=at[k] - size["lse"] + 4), "overlaps")
+    _refused(decode(lse=at["out"] + size["out"] - 4), "overlaps")
+    _refused(decode(out=at["q"], heads_first=True), "overlaps")
+    _refused(decode(out=at["q"] + 16), "overlaps")
+    _refused(decode(out=at["q"], lse=at["q"]), "overlaps")
+
+    Tq, Tk = 5, 7
+    size = dict(q=Tq * H * 384, k=(Tk - 1) * H * 512 + (H - 1) * 512 + 256, v=(Tk - 1) * H * 512 + (H - 1) * 512 + 256, kp=Tk * 128, out=Tq * H * 256, lse=Tq * H * 4)
+
+    def prefill(out=at["out"], lse=at["lse"]):
+        return lib.fp8k_mla_prefill(at["q"], H * 192, 192, at["k"], H * 256, 256, at["kp"], 64, at["v"], H * 256, 256, at["cu"], at["cu"], out, lse, 1, H, Tq, Tk, Tq, 0.1,
+                                    1, _lib.BF16, None, 0, None)
+
+    for k in ("q", "k", "kp", "v"):
+        _refused(prefill(out=at[k] + size[k] - 16), "overlaps")
+        _refused(prefill(out=at[k] - size["out"] + 16), "overlaps")
+        _refused(prefill(lse=at[k] + size[k] - 4), "overlaps")
+        _refused(prefill(lse=at[k] - size["lse"] + 4), "overlaps")
+    _refused(prefill(out=at["q"]), "overlaps")
+    _refused(prefill(lse=at["out"] + size["out"] - 4), "overlaps")
+
+    def gather(out):
+        return lib.fp8k_mla_gather_cache(at["cache"], at["table"], 4, 4, at["cu"], None, None, out, 640, 2, 9, pages, page, _lib.BF16, 0, None)
+
+    _refused(gather(at["cache"] + pages * page * 1152 - 16), "overlaps")
+    _refused(gather(at["cache"] - (8 * 640 + 576) * 2 + 16), "overlaps")

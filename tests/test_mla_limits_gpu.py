@@ -138,3 +138,46 @@ def test_rotated_queries_in_slices_of_one_buffer(dev, T, H):
         with pytest.raises(RuntimeError, match="overlap"):
             torch.ops.fp8k.mla_write_cache(latent, cache, slots, None, 1e-6, rest["cos_sin"], rest["positions"], False, buffer[:T * H].view(T, H, 64),
                                            buffer[H:].view(T, H, 64), None)
+
+
+@pytest.mark.parametrize("n,H,lens,width", [(1, 16, [70, 0, 300], 5), (2, 32, [5000, 1, 64], 800), (1, 128, [(97 * i) % 700 for i in range(90)], 11),
+                                            (1, 128, [4000], 63), (3, 50, [200] * 300, 4)], ids=lambda x: None if isinstance(x, list) else str(x))
+def test_decode_in_the_queries_place(dev, n, H, lens, width):
+    """The result may take the queries' place, in requests that one run holds and in those that several share, in every block of rows."""
+    from sglang_amd import mla
+
+    g = _gen(H)
+    cache, table, pt, _ = _filled(g, lens, 64, BF16, False, width=width)
+    q, qp = _queries(g, len(lens), n, H, BF16)
+    q = q.contiguous()
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = mla.mla_decode_attention(q, qp, cache, pt, sl, SCALE)
+    for _ in range(3):
+        place = q.clone()
+        assert mla.mla_decode_attention(place, qp, cache, pt, sl, SCALE, out=place) is place
+        assert torch.equal(place, want)
+    whole = torch.cat((q.view(-1), q.view(-1)))
+    with pytest.raises(RuntimeError, match="overlaps"):
+        mla.mla_decode_attention(whole[:q.numel()].view(q.shape), qp, cache, pt, sl, SCALE, out=whole[512:512 + q.numel()].view(q.shape))
+    assert torch.equal(whole, torch.cat((q.view(-1), q.view(-1))))
+
+
+def test_results_beside_their_operands(dev):
+    """Results and operands as pieces of one buffer, each beginning where another ends."""
+    from sglang_amd import mla
+
+    g = _gen(8)
+    q, kn, kp, v, cu_q, cu_k, tq, tk = _prefill_inputs(g, [70, 5], [70, 130], 2, BF16, slack=0)
+    want = mla.mla_prefill_attention(q, kn, kp, v, tq, tk, 70, SCALE)
+    buffer = torch.empty((q.numel() + want.numel() + kp.numel(),), dtype=BF16, device="cuda")
+    q2, out, kp2 = (x.view(s) for x, s in zip(buffer.split((q.numel(), want.numel(), kp.numel())), (q.shape, want.shape, kp.shape)))
+    q2.copy_(q), kp2.copy_(kp)
+    assert mla.mla_prefill_attention(q2, kn, kp2, v, tq, tk, 70, SCALE, out=out) is out and torch.equal(out, want)
+    cache, table, pt, _ = _filled(g, [70, 33], 64, BF16, False)
+    buffer = torch.empty((cache.numel() + 103 * 576,), dtype=BF16, device="cuda")
+    cache2, rows = buffer[:cache.numel()].view(cache.shape), buffer[cache.numel():].view(103, 576)
+    cache2.copy_(cache)
+    cu = torch.tensor([0, 70, 103], dtype=torch.int32, device="cuda")
+    assert torch.equal(mla.mla_gather_cache(cache2, pt, cu, 103, out=rows), mla.mla_gather_cache(cache, pt, cu, 103))
+    with pytest.raises(RuntimeError, match="overlaps"):
+        mla.mla_gather_cache(cache2, pt, cu, 103, out=buffer[cache.numel() - 576:-576].view(103, 576))
