@@ -579,7 +579,8 @@ int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t qn_stride_n
  * Expanded attention over ragged sequences: sequence b has queries cu_seqlens_q[b] .. [b + 1] of q [Tq, H, 192] and keys cu_seqlens_k[b] .. [b + 1]
  * of k_nope [Tk, H, 128], k_pe [Tk, 64] (all heads') and v [Tk, H, 128] (int32 [B + 1], not decreasing).  Query i of its lq sees (causal) keys j <= i + lk - lq, else all.
  * out [Tq, H, 128] and lse (NULL or float32 [Tq, H]) contiguous, no part of an operand; a query that sees nothing gets 0 and -inf, queries of no sequence
- * stay as they are.  max_seqlen_q: at least the longest lq.  Keys that a sequence has must be finite; whatever lies outside it may be anything.
+ * stay as they are.  max_seqlen_q: at least the longest lq; it is rounded up to a block of 128 or 256
+ * queries, and those of a longer sequence behind it stay as they are.  Keys that a sequence has must be finite; whatever lies outside it may be anything.
  * Workspace: 256-byte aligned, fp8k_mla_prefill_workspace_bytes of it (0 possible: few blocks of queries with long keys are split over the
  * keys, and joined in float32), not initialised.
  */

@@ -106,7 +106,7 @@ def mla_prefill_attention(q: torch.Tensor, k_nope: torch.Tensor, k_pe: torch.Ten
     """Expanded attention over ragged sequences.  q [Tq, heads, 192], a head's 128 numbers and its 64 rotated ones; k_nope and v
     [Tk, heads, 128], as a rule the two halves of what the up-projection gives; k_pe [Tk, 64] (or [Tk, 1, 64]), read by all heads.  Sequence b has the queries
     cu_seqlens_q[b] .. cu_seqlens_q[b + 1] and the keys cu_seqlens_k[b] .. cu_seqlens_k[b + 1] (int32 [B + 1], not decreasing); max_seqlen_q is at least the
-    most queries that one has (more are left out).
+    most queries that one has: of a longer one, queries behind the bound's block (128 or 256 queries, by the call's cut) are not computed, their rows not written.
 
     causal: of lq queries and lk keys, query i sees the keys j <= i + lk - lq (the queries are the last of the keys); else all.  Returns [Tq, heads, 128]
     of q's type, with return_lse also log(sum exp(s)), float32 [Tq, heads]; out is no part of an operand.  A query that sees nothing gets 0 and -inf; those of no sequence are not

@@ -181,3 +181,23 @@ def test_results_beside_their_operands(dev):
     assert torch.equal(mla.mla_gather_cache(cache2, pt, cu, 103, out=rows), mla.mla_gather_cache(cache, pt, cu, 103))
     with pytest.raises(RuntimeError, match="overlaps"):
         mla.mla_gather_cache(cache2, pt, cu, 103, out=buffer[cache.numel() - 576:-576].view(103, 576))
+
+
+@pytest.mark.parametrize("lq,lk,H,most", [([300], [300], 3, 100), ([300, 600], [300, 900], 2, 128), ([700], [9000], 2, 250), ([1024, 1000], [5000, 8000], 1, 512),
+                                          ([700, 20], [700, 700], 64, 1)], ids=str)
+@pytest.mark.parametrize("causal", [True, False])
+def test_prefill_of_more_queries_than_stated(dev, lq, lk, H, most, causal):
+    """A bound below the longest sequence: its queries up to the bound are as they are, those behind the bound's block are not written; keys split and not, blocks
+    of 128 and of 256."""
+    from sglang_amd import mla
+
+    q, kn, kp, v, cu_q, cu_k, tq, tk = _prefill_inputs(_gen(most), lq, lk, H, BF16)
+    out = torch.full((q.shape[0], H, 128), 7.0, dtype=BF16, device="cuda")
+    _, lse = mla.mla_prefill_attention(q, kn, kp, v, tq, tk, most, SCALE, causal=causal, return_lse=True, out=out)
+    want, want_lse, tol, lse_tol = R.prefill(q, kn, kp, v, cu_q, cu_k, SCALE, causal)
+    for at, n in zip(cu_q, lq):
+        first = slice(at, at + min(n, most))
+        R.close(out[first], want[first], tol[first], "out")
+        R.close(lse[first], want_lse[first], lse_tol[first], "lse")
+        assert bool((out[at + min(n, -(-most // 256) * 256):at + n] == 7.0).all())
+    assert bool((out[cu_q[-1]:] == 7.0).all())
