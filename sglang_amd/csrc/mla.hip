@@ -577,8 +577,9 @@ extern "C" int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_str
   p.B = (int)B; p.H = (int)H; p.Tq = (int)Tq; p.Tk = (int)Tk; p.blocks = (int)d.blocks; p.causal = causal != 0; p.sm_scale = sm_scale;
   p.splits = d.splits;
   // Heads by XCDs, unless that leaves more than an eighth of them idle (1000 queries of 4 heads with 10000 keys 79 us by XCDs, 49 over all)
-  p.xcds = units * 8 > B * H * 9 ? 1 : 8;
-  const int64_t lines = p.xcds == 8 ? units : B * H;
+  p.xcd_bits = units * 8 > B * H * 9 ? 0 : 3;
+  const int64_t lines = p.xcd_bits ? units : B * H;
+  p.groups = (int)(lines >> p.xcd_bits);
   const int64_t need = fp8k_mla_prefill_workspace_bytes(B, H, Tq, Tk, max_seqlen_q);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
     return fail(FP8K_ERR_WORKSPACE, "mla prefill: workspace of %lld bytes needed, 256-byte aligned", (long long)need);

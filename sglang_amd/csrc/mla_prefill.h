@@ -35,7 +35,8 @@ struct MlaPrefillArgs {
   float *part, *part_lse;  // [splits, Tq, H, 128], [splits, Tq, H]
   int B, H, Tq, Tk, blocks;  // blocks: of a workgroup's queries, that a sequence has at most
   int splits;              // of a block's keys, each a workgroup's
-  int xcds;                // heads side by side: 8, one to an XCD, or 1
+  int xcd_bits;            // of the number of heads side by side: 8, one to an XCD, or 1
+  int groups;              // of them
   int causal;
   float sm_scale;
 };
@@ -54,15 +55,15 @@ struct MlaBlock {
 template <int ROWS>
 __device__ __forceinline__ MlaBlock mla_block(const MlaPrefillArgs& p) {
   MlaBlock x;
-  const int line = (int)blockIdx.x / p.xcds, group = line / p.blocks, place = line - group * p.blocks, unit = group * p.xcds + (int)blockIdx.x % p.xcds;
+  const int line = (int)blockIdx.x >> p.xcd_bits, group = p.blocks == 1 ? line : line / p.blocks, place = line - group * p.blocks;
+  const int unit = (group << p.xcd_bits) + ((int)blockIdx.x & ((1 << p.xcd_bits) - 1));
   x.rows = 0;
   if (unit >= p.B * p.H) return x;
   x.b = unit / p.H;
   x.h = unit - x.b * p.H;
   x.q_begin = min(max(p.cu_q[x.b], 0), p.Tq);
   x.lq = min(max(p.cu_q[x.b + 1], x.q_begin), p.Tq) - x.q_begin;
-  const int groups = (int)gridDim.x / p.xcds / p.blocks;
-  x.q0 = ((groups - group) & 1 ? p.blocks - 1 - place : place) * ROWS;
+  x.q0 = ((p.groups - group) & 1 ? p.blocks - 1 - place : place) * ROWS;
   x.rows = min(ROWS, x.lq - x.q0);
   return x;
 }
@@ -84,7 +85,11 @@ __global__ __launch_bounds__(64 * NW, 2) void mla_prefill_kernel(const MlaPrefil
   const int keys = p.causal ? min(max(last_row + shift_k + 1, 0), lk) : lk;  // that any row of the block sees
   // this workgroup's share of their tiles
   const int all_tiles = (keys + kPreKeys - 1) / kPreKeys, split = blockIdx.y;
-  const int first = (int)((int64_t)all_tiles * split / p.splits), tiles = (int)((int64_t)all_tiles * (split + 1) / p.splits);
+  int first = 0, tiles = all_tiles;
+  if (p.splits > 1) {  // at most 2^25 tiles and 32 splits
+    first = (uint32_t)all_tiles * split / p.splits;
+    tiles = (uint32_t)all_tiles * (split + 1) / p.splits;
+  }
 
   const int row0 = q0 + w * 32, qi = min(row0 + l31, lq - 1);
   const int lim = p.causal ? min(qi + shift_k + 1, lk) : lk;  // keys that this lane's row sees
@@ -281,11 +286,12 @@ __global__ __launch_bounds__(64 * NW, 2) void mla_prefill_kernel(const MlaPrefil
   first_scores(s0);
   first_scores(s1);
   if (first < tiles) {
+    // all that the first tile takes, and the next keys, asked for at once: a short sequence waits for memory once
     fetch_keys(first);
+    fetch_values(first);
+    if (first + 1 < tiles) fetch_keys(first + 1);
     wait_loads<0>();
     lds_only_barrier();
-    if (first + 1 < tiles) fetch_keys(first + 1);
-    fetch_values(first);
     if (first * kPreKeys < wave_keys) {
       const int n_at = n_off + (first & 1) * kKey, p_at = p_off + (first & 1) * kKey;
 #pragma unroll
