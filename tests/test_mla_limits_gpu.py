@@ -201,3 +201,34 @@ def test_prefill_of_more_queries_than_stated(dev, lq, lk, H, most, causal):
         R.close(lse[first], want_lse[first], lse_tol[first], "lse")
         assert bool((out[at + min(n, -(-most // 256) * 256):at + n] == 7.0).all())
     assert bool((out[cu_q[-1]:] == 7.0).all())
+
+
+def test_decode_of_the_most_requests(dev):
+    """65535 requests of one token or none: a single token's weight is 1, its result the row itself."""
+    from sglang_amd import mla
+
+    g = _gen(65535)
+    B = 65535
+    cache = torch.randn((700, 2, 576), generator=g, device="cuda").to(BF16)
+    table = torch.randint(0, 700, (B, 1), generator=g, device="cuda", dtype=torch.int32)
+    lens = torch.randint(0, 2, (B,), generator=g, device="cuda", dtype=torch.int32)
+    q, qp = _queries(g, B, 1, 1, BF16)
+    out, lse = mla.mla_decode_attention(q[:, 0], qp[:, 0], cache, table, lens, SCALE, return_lse=True)
+    rows = cache[table[:, 0].long(), 0, :512]
+    assert torch.equal(out[:, 0], torch.where((lens > 0)[:, None], rows, torch.zeros_like(rows)))
+    assert torch.equal(torch.isinf(lse[:, 0]), lens == 0)
+
+
+@pytest.mark.parametrize("n,H", [(512, 128), (1, 65536), (65536, 1)])
+def test_decode_of_the_most_rows(dev, n, H):
+    """65536 rows to a request, new tokens by heads; more new tokens than the request has among them."""
+    g = _gen(n)
+    lens = [300, 0]
+    cache, table, pt, _ = _filled(g, lens, 64, BF16, False)
+    q, qp = _queries(g, 2, n, H, BF16)
+    from sglang_amd import mla
+
+    out, lse = mla.mla_decode_attention(q, qp, cache, pt, torch.tensor(lens, dtype=torch.int32, device="cuda"), SCALE, return_lse=True)
+    want, want_lse, tol, lse_tol = R.decode(q, qp, cache, table, lens, SCALE, None)
+    R.close(out, want, tol, "out")
+    R.close(lse, want_lse, lse_tol, "lse")
