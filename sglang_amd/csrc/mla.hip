@@ -367,7 +367,7 @@ PrefillPlan prefill_cut(int waves, int64_t B, int64_t H, int64_t Tq, int64_t Tk,
   PrefillPlan d{waves, 1, blocks};
   if (groups <= 0 || groups > num_cu()) return d;
   const int64_t tiles = (Tk / B + kPreKeys - 1) / kPreKeys, most = std::min<int64_t>(std::min<int64_t>(num_cu() * 8 / waves / groups, 32), tiles / 2);
-  const double partials = (double)(Tq * H) * (2 * 4 * kPreValue) / 4.5e6;
+  const double partials = (double)std::min(Tq * H, groups * rows) * (2 * 4 * kPreValue) / 4.5e6;
   double least = 0;
   for (int64_t n = 1; n <= most; ++n) {
     const double us = (waves == 8 ? 2.2 : groups * n > num_cu() ? 2.5 : 1.25) * (double)((tiles + n - 1) / n) + (n > 1 ? 5 + n * (partials + 0.25) : 0);
@@ -377,6 +377,12 @@ PrefillPlan prefill_cut(int waves, int64_t B, int64_t H, int64_t Tq, int64_t Tk,
   }
   return d;
 }
+// Heads by XCDs, unless that leaves more than an eighth of them idle (1000 queries of 4 heads with 10000 keys 79 us by XCDs, 49 over all)
+int prefill_xcd_bits(int64_t B, int64_t H) { return up_to(B * H, 8) * 8 > B * H * 9 ? 0 : 3; }
+int64_t prefill_workgroups(const PrefillPlan& d, int64_t B, int64_t H) { return (prefill_xcd_bits(B, H) ? up_to(B * H, 8) : B * H) * d.blocks; }
+// Of the splits' partials and their logarithms.  Splits are made of few blocks alone: at most two workgroups to a CU, 38 MB in all, however many rows q has.
+int64_t prefill_rows(const PrefillPlan& d, int64_t B, int64_t H) { return d.splits == 1 ? 0 : d.splits * prefill_workgroups(d, B, H) * 32 * d.waves; }
+int64_t prefill_workspace(int64_t rows) { return up_to(rows * kPreValue * 4, 256) + up_to(rows * 4, 256); }
 PrefillPlan prefill_plan(int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q, bool causal) {
   const PrefillPlan d = prefill_cut(8, B, H, Tq, Tk, max_seqlen_q);
   return Tk >= (causal ? 4 : 1) * Tq && Tq * 8 >= B * d.blocks * 256 * 7 ? d : prefill_cut(4, B, H, Tq, Tk, max_seqlen_q);
@@ -545,8 +551,7 @@ extern "C" int fp8k_mla_decode(const void* q_nope, int64_t qn_stride_b, int64_t 
 
 extern "C" int64_t fp8k_mla_prefill_workspace_bytes(int64_t B, int64_t H, int64_t Tq, int64_t Tk, int64_t max_seqlen_q) {
   if (B <= 0 || H <= 0 || Tq <= 0 || Tk <= 0 || max_seqlen_q <= 0) return 0;
-  const int64_t splits = std::max(prefill_cut(4, B, H, Tq, Tk, max_seqlen_q).splits, prefill_cut(8, B, H, Tq, Tk, max_seqlen_q).splits);
-  return splits == 1 ? 0 : up_to(splits * Tq * H * kPreValue * 4, 256) + up_to(splits * Tq * H * 4, 256);
+  return prefill_workspace(std::max(prefill_rows(prefill_cut(4, B, H, Tq, Tk, max_seqlen_q), B, H), prefill_rows(prefill_cut(8, B, H, Tq, Tk, max_seqlen_q), B, H)));
 }
 
 extern "C" int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k_nope, int64_t kn_stride_t,
@@ -576,10 +581,9 @@ extern "C" int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_str
   p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.out = out; p.lse = lse;
   p.B = (int)B; p.H = (int)H; p.Tq = (int)Tq; p.Tk = (int)Tk; p.blocks = (int)d.blocks; p.causal = causal != 0; p.sm_scale = sm_scale;
   p.splits = d.splits;
-  // Heads by XCDs, unless that leaves more than an eighth of them idle (1000 queries of 4 heads with 10000 keys 79 us by XCDs, 49 over all)
-  p.xcd_bits = units * 8 > B * H * 9 ? 0 : 3;
-  const int64_t lines = p.xcd_bits ? units : B * H;
-  p.groups = (int)(lines >> p.xcd_bits);
+  p.xcd_bits = prefill_xcd_bits(B, H);
+  const int64_t workgroups = prefill_workgroups(d, B, H);
+  p.groups = (int)((workgroups / d.blocks) >> p.xcd_bits);
   const int64_t need = fp8k_mla_prefill_workspace_bytes(B, H, Tq, Tk, max_seqlen_q);
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
     return fail(FP8K_ERR_WORKSPACE, "mla prefill: workspace of %lld bytes needed, 256-byte aligned", (long long)need);
@@ -588,8 +592,8 @@ extern "C" int fp8k_mla_prefill(const void* q, int64_t q_stride_t, int64_t q_str
                               rows_of(k_pe, {{Tk, kp_stride_t}}, kRope), rows_of(v, {{Tk, v_stride_t}, {H, v_stride_h}}, kPreValue)}),
                "mla prefill: out or lse overlaps an operand");
   p.part = (float*)workspace;
-  p.part_lse = (float*)((uint8_t*)workspace + up_to(p.splits * Tq * H * kPreValue * 4, 256));
-  const dim3 grid((unsigned)(lines * d.blocks), (unsigned)p.splits), join_grid((unsigned)(lines * d.blocks), 16);
+  p.part_lse = (float*)((uint8_t*)workspace + up_to(prefill_rows(d, B, H) * kPreValue * 4, 256));
+  const dim3 grid((unsigned)workgroups, (unsigned)p.splits), join_grid((unsigned)workgroups, 16);
   const hipStream_t st = (hipStream_t)stream;
 #define MLA_PREFILL(DT, NW)                                                       \
   do {                                                                            \

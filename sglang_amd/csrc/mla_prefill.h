@@ -32,7 +32,7 @@ struct MlaPrefillArgs {
   const int32_t *cu_q, *cu_k;
   void* out;   // [Tq, H, 128]
   float* lse;  // [Tq, H] or null
-  float *part, *part_lse;  // [splits, Tq, H, 128], [splits, Tq, H]
+  float *part, *part_lse;  // of split keys: [splits, gridDim.x, rows of a workgroup, 128], [splits, gridDim.x, rows]
   int B, H, Tq, Tk, blocks;  // blocks: of a workgroup's queries, that a sequence has at most
   int splits;              // of a block's keys, each a workgroup's
   int xcd_bits;            // of the number of heads side by side: 8, one to an XCD, or 1
@@ -66,6 +66,12 @@ __device__ __forceinline__ MlaBlock mla_block(const MlaPrefillArgs& p) {
   x.q0 = ((p.groups - group) & 1 ? p.blocks - 1 - place : place) * ROWS;
   x.rows = min(ROWS, x.lq - x.q0);
   return x;
+}
+
+// Where a split's rows of this workgroup's block begin, among those of all.
+template <int ROWS>
+__device__ __forceinline__ int64_t mla_split_row(int split) {
+  return ((int64_t)split * gridDim.x + blockIdx.x) * ROWS;
 }
 
 template <int DT, int NW>
@@ -318,7 +324,7 @@ __global__ __launch_bounds__(64 * NW, 2) void mla_prefill_kernel(const MlaPrefil
           *(v2i*)(to + dt * 32 + k * 8) = v2i{(int)pack2<DT>(o[dt][4 * k] * f, o[dt][4 * k + 1] * f), (int)pack2<DT>(o[dt][4 * k + 2] * f, o[dt][4 * k + 3] * f)};
       if (half == 0 && p.lse) p.lse[row] = lse2 * kLn2;
     } else {
-      const int64_t place = (int64_t)split * p.Tq * p.H + row;
+      const int64_t place = mla_split_row<32 * NW>(split) + w * 32 + l31;
       float* const to = p.part + place * kPreValue + 4 * half;
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt)
@@ -335,17 +341,17 @@ __global__ __launch_bounds__(256) void mla_prefill_join_kernel(const MlaPrefillA
   const MlaBlock at = mla_block<32 * NW>(p);
   const int col = 4 * (int)(threadIdx.x & 31);
   for (int r = (int)blockIdx.y * 8 + (int)(threadIdx.x >> 5); r < at.rows; r += (int)gridDim.y * 8) {
-    const int64_t row = (int64_t)(at.q_begin + at.q0 + r) * p.H + at.h, step = (int64_t)p.Tq * p.H;
+    const int64_t row = (int64_t)(at.q_begin + at.q0 + r) * p.H + at.h, from = mla_split_row<32 * NW>(0) + r, step = mla_split_row<32 * NW>(1) - mla_split_row<32 * NW>(0);
     float top = -INFINITY;
-    for (int i = 0; i < p.splits; ++i) top = fmaxf(top, p.part_lse[i * step + row]);
+    for (int i = 0; i < p.splits; ++i) top = fmaxf(top, p.part_lse[from + i * step]);
     const float shift = shift_of(top);
     float sum = 0.0f;
     v4f x = {0, 0, 0, 0};
 #pragma unroll 4
     for (int i = 0; i < p.splits; ++i) {
-      const float weight = __builtin_amdgcn_exp2f(p.part_lse[i * step + row] - shift);
+      const float weight = __builtin_amdgcn_exp2f(p.part_lse[from + i * step] - shift);
       sum += weight;
-      x += weight * *(const v4f*)(p.part + (i * step + row) * kPreValue + col);
+      x += weight * *(const v4f*)(p.part + (from + i * step) * kPreValue + col);
     }
     x *= sum == 0.0f ? 0.0f : 1.0f / sum;
     *(v2i*)((u16*)p.out + row * kPreValue + col) = v2i{(int)pack2<DT>(x[0], x[1]), (int)pack2<DT>(x[2], x[3])};

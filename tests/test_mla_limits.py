@@ -165,3 +165,26 @@ def test_results_of_attentions_are_no_part_of_their_operands():
 
     _refused(gather(at["cache"] + pages * page * 1152 - 16), "overlaps")
     _refused(gather(at["cache"] - (8 * 640 + 576) * 2 + 16), "overlaps")
+
+
+def test_prefill_workspace_goes_by_blocks():
+    """Keys are split where there are fewer blocks of queries than CUs: at most two workgroups of 128 rows to each of 256 CUs (and an eighth more, where heads go by XCDs), 516 bytes to
+    a row.  Rows of q that no sequence has, as a padded call's, take no memory."""
+    import random
+
+    from sglang_amd._lib import lib
+
+    size = lib.fp8k_mla_prefill_workspace_bytes
+    most = 2 * 256 * 128 * 516 * 9 // 8 + 512
+    rng = random.Random(5)
+    some = 0
+    for _ in range(3000):
+        B, H = rng.choice([1, 2, 5, 16, 64]), rng.choice([1, 4, 16, 17, 33, 128])
+        longest = int(2 ** rng.uniform(0, 13))
+        Tq, Tk = rng.choice([B * longest, rng.randint(longest, B * longest), 8192 + B * longest]), int(2 ** rng.uniform(0, 21))
+        need = size(B, H, Tq, Tk, longest)
+        assert 0 <= need <= most, (B, H, Tq, Tk, longest, need)
+        some += need > 0
+        assert size(B, H, (1 << 30) + Tq, Tk, longest) <= most
+    assert some > 300
+    assert size(1, 16, 8192, 1 << 17, 16) == size(1, 16, 16384, 1 << 17, 16) > 0

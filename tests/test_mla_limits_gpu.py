@@ -232,3 +232,26 @@ def test_decode_of_the_most_rows(dev, n, H):
     want, want_lse, tol, lse_tol = R.decode(q, qp, cache, table, lens, SCALE, None)
     R.close(out, want, tol, "out")
     R.close(lse, want_lse, lse_tol, "lse")
+
+
+@pytest.mark.parametrize("lq,lk,H,slack", [([16], [9000], 4, 4000), ([16], [9000], 8, 0), ([130, 0, 5], [5000, 3000, 0], 2, 700), ([256], [4000], 3, 9), ([512, 512], [4000, 97], 8, 0),
+                                           ([40] * 12, [700 + 100 * i for i in range(12)], 1, 2000)], ids=str)
+@pytest.mark.parametrize("causal", [True, False])
+def test_prefill_stays_in_its_workspace(dev, lq, lk, H, slack, causal):
+    """Split keys with just the workspace asked for, full of ones, and bytes behind it that must stay as they are; queries with many more rows than the sequences have."""
+    from sglang_amd._lib import BF16 as CODE, check, lib, stream_ptr
+
+    q, kn, kp, v, cu_q, cu_k, tq, tk = _prefill_inputs(_gen(H), lq, lk, H, BF16, slack=slack)
+    Tq, Tk, B = q.shape[0], kn.shape[0], len(lq)
+    out, lse = torch.full((Tq, H, 128), 7.0, dtype=BF16, device="cuda"), torch.full((Tq, H), 7.0, device="cuda")
+    need = lib.fp8k_mla_prefill_workspace_bytes(B, H, Tq, Tk, max(lq))
+    assert need > 0
+    ws = torch.full((need + 4096,), 255, dtype=torch.uint8, device="cuda")
+    check(lib.fp8k_mla_prefill(q.data_ptr(), q.stride(0), q.stride(1), kn.data_ptr(), kn.stride(0), kn.stride(1), kp.data_ptr(), kp.stride(0), v.data_ptr(), v.stride(0),
+                               v.stride(1), tq.data_ptr(), tk.data_ptr(), out.data_ptr(), lse.data_ptr(), B, H, Tq, Tk, max(lq), SCALE, 1 if causal else 0, CODE, ws.data_ptr(),
+                               need, stream_ptr(q.device)))
+    n = cu_q[-1]
+    assert bool((ws[need:] == 255).all()) and bool((out[n:] == 7.0).all()) and bool((lse[n:] == 7.0).all())
+    want, want_lse, tol, lse_tol = R.prefill(q, kn, kp, v, cu_q, cu_k, SCALE, causal)
+    R.close(out[:n], want, tol, "out")
+    R.close(lse[:n], want_lse, lse_tol, "lse")
