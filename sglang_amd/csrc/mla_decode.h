@@ -23,8 +23,8 @@
 // needs no plan.  A run that holds all of a request writes its result; others write normalised float32 partials and the base-2
 // logarithm of their sums, which mla_join_kernel adds up.
 //
-// Measured (page 64, lengths from a third of the most to the most): one request of 8000 tokens, 128 heads, bf16 20 us and 4 for the join, latency; 64 of
-// 8192, 2 x 16 heads, fp16 85 + 6 us, 4.5 TB/s with everything, 6.1 TB/s in the loop (128 of 16000, 16 heads); 128 of 6000, 128 heads, 8 bits 197 + 18 us,
+// Measured (page 64, lengths from a third of the most to the most): one request of 8000 tokens, 128 heads, bf16 19 us and 4 for the join, latency; 64 of
+// 8192, 2 x 16 heads, fp16 85 + 6 us, 4.5 TB/s with everything, 6.1 TB/s in the loop (128 of 16000, 16 heads); 128 of 6000, 128 heads, 8 bits 193 + 18 us back to back,
 // 0.67 PFLOP/s with everything, 0.90 in the loop, where the matrix cores and LDS are busy half the time each.  Of the rest the most are the partials: 100 MB
 // written at the end of all runs at once, and read by the join.
 #pragma once

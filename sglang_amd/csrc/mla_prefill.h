@@ -16,10 +16,12 @@
 // read where it lies, once for each head, and never copied beside the keys.  16-byte chunks of a row are permuted by the row so that the
 // operand reads (16 rows, one chunk) and the transposed ones (8 rows, two chunks) spread over all banks.
 //
+// The loop is 20 KB of instructions, which a short sequence runs through once: one tile of keys takes 6.4 us, where a loop without that overlap, 7 KB, takes 5.2.
+//
 // Measured, bf16: 8192 queries of 128 heads with their own keys, causal, 2.5 - 2.65 ms by the card or 1.04 - 1.1 PFLOP/s, where a library's matrix product of 8192^3 reaches 1.55; the
 // matrix cores are busy 65 % of the clocks, at the 1.6 GHz that the power limit leaves; a tile of four waves costs LDS some 1160 clocks (at the rates that its
 // reads and fills reach alone) and the vector instructions 1020, beside the products' 1280.  1000 queries of 32 heads with 10000 keys, float16, 207 us or 0.94 PFLOP/s, the join 9 us of it.  17
-// prompts of 100 to 300 tokens, 16 heads, 25 us: 2.7 TB/s, latency (a workgroup alone takes 6 to 11 us).
+// prompts of 100 to 300 tokens, 16 heads, 24 - 25 us: 2.8 TB/s, latency (a workgroup alone takes 6 to 9 us).
 #pragma once
 
 #include "mla_common.h"

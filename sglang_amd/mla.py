@@ -83,7 +83,7 @@ def mla_decode_attention(q_nope: torch.Tensor, q_pe: torch.Tensor, cache: torch.
 
     The exponentials are rounded to 16 bits for their product with the rows (their sum is not).  Lengths are held within the page table's width, and that
     bound decides how a batch is cut: pass the columns that the longest request needs, page_table[:, :n] (one request of 4000 tokens, 128 heads, takes
-    31 us rather than 20 with a table for 131072).  Of a page what lies behind the last token may hold anything, the request's own rows are finite.  The whole batch's tokens are cut into equal runs, whose float32 partials
+    30 us rather than 20 with a table for 131072).  Of a page what lies behind the last token may hold anything, the request's own rows are finite.  The whole batch's tokens are cut into equal runs, whose float32 partials
     are joined in the order of the tokens: results do not depend on timing, but on how the batch is cut."""
     if not torch.compiler.is_compiling():
         got = _host.mla_decode(q_nope, q_pe, cache, page_table, seq_lens, sm_scale, scale, return_lse, out)
